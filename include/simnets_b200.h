@@ -381,6 +381,60 @@ SIMNETS_API int simnets_mixture_statistics(const simnets_sim_desc* desc, const v
 SIMNETS_API int simnets_mixture_parameters(int32_t k, int32_t taps, float min_var, const float* stats, const float* means,
                                            float* new_means, float* new_covs, void* stream);
 
+/* ---- activations in 8 bits ------------------------------------------------ */
+/* What a layer keeps of its input for the backward pass (no counterpart in the reference, whose graphs keep whole
+ * tensors).  `count` values of `dtype`, in memory order, in groups of `group` (32, 64, 128 or 256; the last one may be
+ * short); codes: one byte per value; ranges: { base, step } per group in the values' type,
+ * simnets_checkpoint_groups(count, group) of them.
+ *   base = the group's lowest finite value (0 if there is none)
+ *   step = (highest / 2 - base / 2) / 126, or 0 where that is below the type's smallest normal number
+ *   code = rint((x / 2 - base / 2) * (2 / step)), 0 where step is 0; 253, 254, 255 for -infinity, infinity, NaN
+ * with the halves' difference and 2 / step rounded to the type and their product exact.  The value of a code below 253 is
+ * base + code * step, rounded once, at most the largest finite number: at most step / 2 (and a rounding) from x. */
+SIMNETS_API int64_t simnets_checkpoint_groups(int64_t count, int32_t group);
+SIMNETS_API int simnets_checkpoint_pack(int32_t dtype, int64_t count, int32_t group, const void* x, void* codes, void* ranges, void* stream);
+SIMNETS_API int simnets_checkpoint_unpack(int32_t dtype, int64_t count, int32_t group, const void* codes, const void* ranges, void* x, void* stream);
+
+/* Gradients of a layer at a checkpoint of its input: those of the op at the values that the codes stand for.
+ * MEX: y is computed again from them instead of being kept; a NULL dx or doffsets is not computed; d->flags as for
+ * simnets_mex_gradients, without SIMNETS_FLAG_MEX_WORKSPACE_PRIMED and SIMNETS_FLAG_MEX_MAXIMA_GIVEN
+ * (SIMNETS_E_UNSUPPORTED).  Similarity: a NULL dx is not computed, nor are dtemplates and dweights where both are NULL. */
+SIMNETS_API size_t simnets_mex_checkpoint_workspace_bytes(const simnets_mex_desc* d);
+SIMNETS_API int simnets_mex_checkpoint_gradients(const simnets_mex_desc* d, int32_t group, const void* codes, const void* ranges,
+                                                 const void* offsets, const void* dy, void* dx, void* doffsets,
+                                                 void* workspace, size_t workspace_bytes, void* stream);
+SIMNETS_API size_t simnets_similarity_checkpoint_workspace_bytes(const simnets_sim_desc* d);
+SIMNETS_API int simnets_similarity_checkpoint_gradients(const simnets_sim_desc* d, int32_t group, const void* codes, const void* ranges,
+                                                        const void* templates, const void* weights, const void* dy,
+                                                        void* dx, void* dtemplates, void* dweights,
+                                                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- routing of positions to components ----------------------------------- */
+/* scores[batch, components, positions]: of every position's components the top_k largest v = l + bias, ties to the lowest
+ * index, with l = score + prior (prior, bias: [components] or NULL; additions in the type of the scores); only those
+ * of the top_groups groups (of components / groups consecutive ones) with the largest v.  A component whose v is NaN or
+ * -infinity is not chosen.  Weights: scale times exp(l) (sigmoid != 0: sigmoid(l)) over its sum over the chosen; chosen
+ * ones with l = infinity share alike.
+ *   index[batch, top_k, positions] (-1 where nothing is left), weights likewise, by falling v; either may be NULL
+ *   dense[batch, components, positions]: weights of the chosen, 0 elsewhere; may be NULL
+ *   load[components]: number of positions that chose it; mass[components]: sum of dense (NULL if dense is)
+ * components <= 4096, top_k <= 16, groups <= 64, top_groups <= 16.  simnets_route_gradient: dscores[batch, components,
+ * positions] of `grad`, the gradient of weights.  The unsupervised initialisation assigns patches with it. */
+typedef struct simnets_route_desc {
+    int32_t dtype;
+    int32_t batch, components;
+    int32_t top_k, groups, top_groups;
+    int32_t sigmoid;
+    int32_t reserved;                   /* 0 */
+    int64_t positions;
+    double  scale;
+} simnets_route_desc;
+SIMNETS_API size_t simnets_route_workspace_bytes(const simnets_route_desc* d);
+SIMNETS_API int simnets_route(const simnets_route_desc* d, const void* scores, const void* prior, const void* bias, int32_t* index, void* weights,
+                              void* dense, int64_t* load, void* mass, void* workspace, size_t workspace_bytes, void* stream);
+SIMNETS_API int simnets_route_gradient(const simnets_route_desc* d, const void* scores, const void* prior, const int32_t* index, const void* weights,
+                                       const void* grad, void* dscores, void* stream);
+
 /* ---- sum pooling ----------------------------------------------------------- */
 /* y[p, h, w] = x[p, 2h, 2w] + x[p, 2h, 2w+1] + x[p, 2h+1, 2w] + x[p, 2h+1, 2w+1] over a dense float32 tensor
  * [planes, height, width] (planes = batch * channels); height and width even, else SIMNETS_E_UNSUPPORTED.

@@ -63,6 +63,19 @@ def lib():
         l.simnets_normalize_offsets_forward.argtypes = [C.c_int64, C.c_int32, _P, _P, _P]
         l.simnets_normalize_offsets_backward.argtypes = [C.c_int64, C.c_int32, _P, _P, _P, _P]
         l.simnets_sum_pool2x2_forward.argtypes = [C.c_int64, C.c_int32, C.c_int32, _P, _P, _P]
+        l.simnets_checkpoint_groups.restype = C.c_int64
+        l.simnets_checkpoint_groups.argtypes = [C.c_int64, C.c_int32]
+        for f in (l.simnets_checkpoint_pack, l.simnets_checkpoint_unpack):
+            f.argtypes = [C.c_int32, C.c_int64, C.c_int32, _P, _P, _P, _P]
+        for f, d in ((l.simnets_mex_checkpoint_workspace_bytes, md), (l.simnets_similarity_checkpoint_workspace_bytes, sd)):
+            f.restype, f.argtypes = C.c_size_t, [d]
+        l.simnets_mex_checkpoint_gradients.argtypes = [md, C.c_int32, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]
+        l.simnets_similarity_checkpoint_gradients.argtypes = [sd, C.c_int32, _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]
+        rd = C.POINTER(abi.RouteDesc)
+        l.simnets_route_workspace_bytes.restype = C.c_size_t
+        l.simnets_route_workspace_bytes.argtypes = [rd]
+        l.simnets_route.argtypes = [rd, _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]
+        l.simnets_route_gradient.argtypes = [rd, _P, _P, _P, _P, _P, _P, _P]
         l.simnets_fp32_fma_probe.restype = C.c_int64
         l.simnets_fp32_fma_probe.argtypes = [C.c_int32, C.c_int32, _P, _P]
         l.get_mex_offsets_nregions.restype = C.c_int

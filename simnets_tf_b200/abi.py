@@ -64,6 +64,18 @@ class MexDesc(C.Structure):
     ]
 
 
+class RouteDesc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("batch", C.c_int32), ("components", C.c_int32),
+        ("top_k", C.c_int32), ("groups", C.c_int32), ("top_groups", C.c_int32),
+        ("sigmoid", C.c_int32),
+        ("reserved", C.c_int32),
+        ("positions", C.c_int64),
+        ("scale", C.c_double),
+    ]
+
+
 class MexGeometry(C.Structure):
     _fields_ = [(n, C.c_int32) for n in (
         "block_c", "block_h", "block_w", "stride_c", "stride_h", "stride_w", "pad_c", "pad_h", "pad_w",

@@ -62,6 +62,55 @@ int mex_gradients_in(const MexGeo& g, const simnets_mex_desc* d, const void* x, 
     const bool more = ws && ws_bytes > kept;
     return mex_gradients(g, d, x, off, y, dy, dx, doff, ws, ws_bytes, more ? static_cast<char*>(ws) + kept : nullptr, more ? ws_bytes - kept : 0, s);
 }
+
+// ---- 8-bit checkpoints and routing
+int checkpoint_check(int32_t dtype, int64_t count, int32_t group) {
+    if (dtype != SIMNETS_F32 && dtype != SIMNETS_F64) return SIMNETS_E_DTYPE;
+    return count < 0 || (group != 32 && group != 64 && group != 128 && group != 256) ? SIMNETS_E_DESC : SIMNETS_OK;
+}
+
+// Sums in FP32: the tensor-core kernels truncate what they add, and here y goes through them as well (a 64-tap layer of 128 instances over
+// 524288 positions: gradients 1.2e-5 of their norm off, with FP32 sums 1.3e-6).
+uint32_t checkpoint_route(const MexGeo& g, const simnets_mex_desc& d) {
+    const bool f64 = d.dtype == SIMNETS_F64;
+    return mex_use_gemm(g, f64, d.flags) || mex_gradients_by_gemm(g, f64, d.flags) ? 0u : uint32_t(SIMNETS_FLAG_MEX_NO_TENSORCORE);
+}
+
+// the values of the checkpoint, y again from them, the layer's workspace, the products of overlapping blocks
+struct MexCheckpointWs { void *x, *y, *layer, *products; size_t layer_bytes, products_bytes, bytes; };
+MexCheckpointWs mex_checkpoint_carve(const MexGeo& g, const simnets_mex_desc& d, void* base) {
+    MexCheckpointWs w;
+    const size_t size = d.dtype == SIMNETS_F64 ? 8 : 4;
+    size_t off = 0;
+    auto take = [&](size_t bytes) { void* p = base ? static_cast<char*>(base) + off : nullptr; off += (bytes + 255) & ~size_t(255); return p; };
+    simnets_mex_desc f = d, q = d;
+    f.flags = (f.flags | checkpoint_route(g, d)) & ~uint32_t(SIMNETS_FLAG_MEX_DY_POOLED2);
+    q.flags |= checkpoint_route(g, d);
+    w.x = take(size * g.B * g.C * g.H * g.W);
+    w.y = take(size * g.B * g.M * g.N);
+    w.layer_bytes = std::max<size_t>(std::max(simnets_mex_forward_workspace_bytes(&f), simnets_mex_forward_workspace_bytes(&q)), 256);
+    w.layer = take(w.layer_bytes);
+    w.products_bytes = simnets_mex_products_bytes(&q);
+    w.products = take(w.products_bytes);
+    w.bytes = off;
+    return w;
+}
+
+size_t sim_checkpoint_values(const SimGeo& g, const simnets_sim_desc& d) {
+    return ((d.dtype == SIMNETS_F64 ? 8 : 4) * (size_t)g.B * g.C * g.H * g.W + 255) & ~size_t(255);
+}
+
+int route_check(const simnets_route_desc* d) {
+    if (!d) return SIMNETS_E_NULL;
+    if (d->dtype != SIMNETS_F32 && d->dtype != SIMNETS_F64) return SIMNETS_E_DTYPE;
+    if (d->batch < 0 || d->positions < 0 || d->components < 1 || d->top_k < 1 || d->groups < 1 || d->top_groups < 1 || d->reserved != 0) return SIMNETS_E_DESC;
+    if (d->components % d->groups || d->top_groups > d->groups || d->top_k > (long long)d->top_groups * (d->components / d->groups)) return SIMNETS_E_DESC;
+    if (!std::isfinite(d->scale) || d->scale == 0.0) return SIMNETS_E_DESC;
+    const bool all = d->top_groups == d->groups;        // (then there is no choice of groups)
+    if (d->components > 4096 || d->top_k > 16 || (!all && (d->groups > 64 || d->top_groups > 16))) return SIMNETS_E_UNSUPPORTED;
+    // (a load is counted in 32 bits by every CTA)
+    return d->batch > 0 && d->positions > ((1LL << 40) / d->batch) ? SIMNETS_E_UNSUPPORTED : SIMNETS_OK;
+}
 }  // namespace
 
 extern "C" {
@@ -377,6 +426,89 @@ int simnets_mixture_parameters(int32_t k, int32_t taps, float min_var, const flo
     if (k < 1 || taps < 1 || (long long)k * taps > (1LL << 30)) return SIMNETS_E_DESC;
     if (!stats || !means || !new_means || !new_covs) return SIMNETS_E_NULL;
     return from_cuda(launch_mixture_parameters(k, taps, min_var, stats, means, new_means, new_covs, as_stream(stream)));
+}
+
+int64_t simnets_checkpoint_groups(int64_t count, int32_t group) { return count < 0 || group < 1 ? 0 : (count + group - 1) / group; }
+
+int simnets_checkpoint_pack(int32_t dtype, int64_t count, int32_t group, const void* x, void* codes, void* ranges, void* stream) {
+    const int rc = checkpoint_check(dtype, count, group);
+    if (rc) return rc;
+    if (count > 0 && (!x || !codes || !ranges)) return SIMNETS_E_NULL;
+    return from_cuda(launch_checkpoint_pack(dtype == SIMNETS_F64, count, group, x, codes, ranges, as_stream(stream)));
+}
+
+int simnets_checkpoint_unpack(int32_t dtype, int64_t count, int32_t group, const void* codes, const void* ranges, void* x, void* stream) {
+    const int rc = checkpoint_check(dtype, count, group);
+    if (rc) return rc;
+    if (count > 0 && (!x || !codes || !ranges)) return SIMNETS_E_NULL;
+    return from_cuda(launch_checkpoint_unpack(dtype == SIMNETS_F64, 0, count, group, codes, ranges, x, as_stream(stream)));
+}
+
+size_t simnets_mex_checkpoint_workspace_bytes(const simnets_mex_desc* d) {
+    MexGeo g;
+    return mex_geometry(d, nullptr, &g) ? 0 : mex_checkpoint_carve(g, *d, nullptr).bytes;
+}
+
+int simnets_mex_checkpoint_gradients(const simnets_mex_desc* d, int32_t group, const void* codes, const void* ranges, const void* off, const void* dy, void* dx,
+                                     void* doff, void* ws, size_t ws_bytes, void* stream) {
+    MexGeo g;
+    int rc = mex_geometry(d, nullptr, &g);
+    if (rc) return rc;
+    if ((rc = checkpoint_check(d->dtype, 1, group))) return rc;
+    if (d->flags & (SIMNETS_FLAG_MEX_WORKSPACE_PRIMED | SIMNETS_FLAG_MEX_MAXIMA_GIVEN)) return SIMNETS_E_UNSUPPORTED;
+    if (!off || (g.B > 0 && (!codes || !ranges || !dy || (!dx && !doff)))) return SIMNETS_E_NULL;
+    if (g.B == 0) return mex_gradients(g, d, nullptr, off, nullptr, nullptr, nullptr, doff, ws, ws_bytes, nullptr, 0, as_stream(stream));
+    const MexCheckpointWs w = mex_checkpoint_carve(g, *d, ws);
+    if (!ws || ws_bytes < w.bytes) return SIMNETS_E_WORKSPACE;
+    const cudaError_t e = launch_checkpoint_unpack(d->dtype == SIMNETS_F64, 0, (long long)g.B * g.C * g.H * g.W, group, codes, ranges, w.x, as_stream(stream));
+    if (e != cudaSuccess) return from_cuda(e);
+    simnets_mex_desc f = *d;
+    const uint32_t route = checkpoint_route(g, *d);
+    f.flags = (d->flags | route) & ~uint32_t(SIMNETS_FLAG_MEX_DY_POOLED2 | SIMNETS_FLAG_ACCUMULATE);
+    rc = simnets_mex_forward(&f, w.x, off, w.y, w.layer, w.layer_bytes, stream);
+    if (rc) return rc;
+    f.flags = d->flags | route | SIMNETS_FLAG_MEX_WORKSPACE_PRIMED;
+    return mex_gradients(g, &f, w.x, off, w.y, dy, dx, doff, w.layer, w.layer_bytes, w.products, w.products_bytes, as_stream(stream));
+}
+
+size_t simnets_similarity_checkpoint_workspace_bytes(const simnets_sim_desc* d) {
+    SimGeo g;
+    return sim_geometry(d, &g) ? 0 : sim_checkpoint_values(g, *d) + std::max<size_t>(sim_workspace_bytes(g, d->dtype == SIMNETS_F64, d->flags), 256);
+}
+
+int simnets_similarity_checkpoint_gradients(const simnets_sim_desc* d, int32_t group, const void* codes, const void* ranges, const void* t, const void* w,
+                                            const void* dy, void* dx, void* dt, void* dw, void* ws, size_t ws_bytes, void* stream) {
+    SimGeo g;
+    int rc = sim_geometry(d, &g);
+    if (rc) return rc;
+    if ((rc = checkpoint_check(d->dtype, 1, group))) return rc;
+    if (!t || !w || (dt == nullptr) != (dw == nullptr) || (!dx && !dt && g.B > 0) || (g.B > 0 && (!codes || !ranges || !dy))) return SIMNETS_E_NULL;
+    if (!ws || ws_bytes < simnets_similarity_checkpoint_workspace_bytes(d)) return SIMNETS_E_WORKSPACE;
+    const cudaError_t e = launch_checkpoint_unpack(d->dtype == SIMNETS_F64, 0, (long long)g.B * g.C * g.H * g.W, group, codes, ranges, ws, as_stream(stream));
+    if (e != cudaSuccess) return from_cuda(e);
+    const size_t values = sim_checkpoint_values(g, *d);
+    void* rest = static_cast<char*>(ws) + values;
+    if (dx && g.B > 0 && (rc = simnets_similarity_input_grad(d, ws, t, w, dy, dx, rest, ws_bytes - values, stream))) return rc;
+    return dt ? simnets_similarity_params_grad(d, ws, t, w, dy, dt, dw, rest, ws_bytes - values, stream) : SIMNETS_OK;
+}
+
+size_t simnets_route_workspace_bytes(const simnets_route_desc* d) { return route_check(d) ? 0 : std::max<size_t>(route_workspace_bytes(*d), 256); }
+
+int simnets_route(const simnets_route_desc* d, const void* scores, const void* prior, const void* bias, int32_t* index, void* weights, void* dense, int64_t* load,
+                  void* mass, void* ws, size_t ws_bytes, void* stream) {
+    const int rc = route_check(d);
+    if (rc) return rc;
+    if (!load || (d->batch > 0 && d->positions > 0 && ((mass && !dense) || !scores || (!index && !weights && !dense)))) return SIMNETS_E_NULL;
+    if (!ws || ws_bytes < route_workspace_bytes(*d)) return SIMNETS_E_WORKSPACE;
+    return from_cuda(launch_route(*d, scores, prior, bias, index, weights, dense, reinterpret_cast<long long*>(load), mass, ws, as_stream(stream)));
+}
+
+int simnets_route_gradient(const simnets_route_desc* d, const void* scores, const void* prior, const int32_t* index, const void* weights, const void* grad,
+                           void* dscores, void* stream) {
+    const int rc = route_check(d);
+    if (rc) return rc;
+    if (d->batch > 0 && d->positions > 0 && (!scores || !index || !weights || !grad || !dscores)) return SIMNETS_E_NULL;
+    return from_cuda(launch_route_gradient(*d, scores, prior, index, weights, grad, dscores, as_stream(stream)));
 }
 
 int64_t simnets_fp32_fma_probe(int32_t packed, int32_t iters, void* scratch, void* stream) {

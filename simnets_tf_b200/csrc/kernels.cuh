@@ -160,6 +160,16 @@ cudaError_t launch_mex_bwd_gemm(const MexGeo&, bool f64, const void* x, const vo
 // number of multiprocessors of the current device (148 when no device answers)
 int device_sm_count();
 
+// checkpoint.cu -- activations in 8 bits; unpack: values first .. first + n of a checkpoint
+cudaError_t launch_checkpoint_pack(bool f64, long long n, int group, const void* x, void* codes, void* ranges, cudaStream_t);
+cudaError_t launch_checkpoint_unpack(bool f64, long long first, long long n, int group, const void* codes, const void* ranges, void* x, cudaStream_t);
+// routing.cu -- positions to components; index and weights, or dense and mass, may be null
+size_t route_workspace_bytes(const simnets_route_desc&);
+cudaError_t launch_route(const simnets_route_desc&, const void* scores, const void* prior, const void* bias, int* index, void* weights, void* dense,
+                         long long* load, void* mass, void* ws, cudaStream_t);
+cudaError_t launch_route_gradient(const simnets_route_desc&, const void* scores, const void* prior, const int* index, const void* weights, const void* grad,
+                                  void* dscores, cudaStream_t);
+
 size_t softmax_xent_workspace_bytes(int batch);
 cudaError_t launch_softmax_xent(int batch, int classes, float scale, const float* logits, const long long* labels, float* loss,
                                 float* dlogits, void* ws, cudaStream_t);

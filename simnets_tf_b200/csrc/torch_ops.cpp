@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstring>
+#include <limits>
 #include <memory>
 #include <mutex>
 #include <string>
@@ -187,6 +188,9 @@ struct SimPlan {
         if (x.dim() != 4 || x.size(0) != d.batch || x.size(1) != d.channels || x.size(2) != d.height || x.size(3) != d.width)
             throw std::invalid_argument("input does not have the planned shape");
         if ((x.scalar_type() == at::kDouble) != (d.dtype == SIMNETS_F64)) throw py::type_error("input does not have the planned dtype");
+        check_params(t, w);
+    }
+    void check_params(const Tensor& t, const Tensor& w) const {
         if (t.dim() != 4 || t.size(0) != d.num_instances || t.size(1) != d.channels || t.size(2) != d.block_h || t.size(3) != d.block_w || t.sizes() != w.sizes())
             throw std::invalid_argument("templates and weights must have the planned shape");
     }
@@ -478,6 +482,308 @@ std::pair<Tensor, Tensor> mixture_parameters(const Tensor& stats, const Tensor& 
     return {new_means, new_covs};
 }
 
+// ------------------------------------------------------------------------------------------------- activations in 8 bits
+struct Kept { Tensor codes, ranges; };
+
+Kept checkpoint_pack(const Tensor& x_in, int64_t group) {
+    require_cuda_all(x_in);
+    if (x_in.scalar_type() != at::kFloat && x_in.scalar_type() != at::kDouble) throw py::type_error("simnets ops are registered for float32 and float64 only");
+    const Tensor x = x_in.contiguous();
+    const c10::cuda::CUDAGuard guard(x.device());
+    Kept kept{at::empty({x.numel()}, x.options().dtype(at::kByte)), at::empty({simnets_checkpoint_groups(x.numel(), int32_t(group)), 2}, x.options())};
+    check(simnets_checkpoint_pack(x.scalar_type() == at::kDouble, x.numel(), int32_t(group), ptr(x), ptr(kept.codes), ptr(kept.ranges), stream_of(x)));
+    return kept;
+}
+
+// the bytes and ranges of a checkpoint of `count` values, as every entry point below takes them
+void check_checkpoint(const Tensor& codes, const Tensor& ranges, int64_t group, int64_t count) {
+    if (!codes.is_cuda() || !ranges.is_cuda()) throw std::runtime_error("simnets_b200 has no CPU kernels: every tensor must live on a CUDA device");
+    if (codes.device() != ranges.device()) throw std::runtime_error("all tensors of one op call must be on the same device");
+    if (codes.scalar_type() != at::kByte || !codes.is_contiguous() || codes.numel() != count || !ranges.is_contiguous() || ranges.dim() != 2 ||
+        ranges.size(0) != simnets_checkpoint_groups(count, int32_t(group)) || ranges.size(1) != 2)
+        throw std::invalid_argument("checkpoint: codes and ranges do not belong to the planned shape");
+}
+
+Tensor checkpoint_unpack(const Tensor& codes, const Tensor& ranges, const std::vector<int64_t>& shape, int64_t group) {
+    Tensor x = at::empty(shape, ranges.options());
+    check_checkpoint(codes, ranges, group, x.numel());
+    const c10::cuda::CUDAGuard guard(x.device());
+    check(simnets_checkpoint_unpack(x.scalar_type() == at::kDouble, x.numel(), int32_t(group), ptr(codes), ptr(ranges), ptr(x), stream_of(x)));
+    return x;
+}
+
+std::pair<Tensor, Tensor> mex_checkpoint_grads(const MexPlan& p, const Tensor& codes, const Tensor& ranges, int64_t group, const Tensor& off_in, const Tensor& dy_in,
+                                               uint32_t flags, bool pooled, bool want_dx, bool want_doff, const OptTensor& out) {
+    check_checkpoint(codes, ranges, group, int64_t(p.d.batch) * p.d.channels * p.d.height * p.d.width);
+    require_cuda_all(ranges, off_in, dy_in);
+    if ((ranges.scalar_type() == at::kDouble) != (p.d.dtype == SIMNETS_F64)) throw py::type_error("input does not have the planned dtype");
+    p.check_offsets(off_in);
+    p.check_dy(dy_in, pooled);
+    const Tensor off = off_in.contiguous(), dy = dy_in.contiguous();
+    const c10::cuda::CUDAGuard guard(ranges.device());
+    const cudaStream_t s = stream_of(ranges);
+    const simnets_mex_desc d = p.with(flags | (pooled ? SIMNETS_FLAG_MEX_DY_POOLED2 : 0u));
+    Tensor dx, doff;
+    if (want_dx) dx = at::empty({d.batch, d.channels, d.height, d.width}, ranges.options());
+    if (want_doff) doff = grad_target(off, out);
+    const Tensor ws = scratch(ranges, std::max<size_t>(simnets_mex_checkpoint_workspace_bytes(&d), 256));
+    Timed<MexPlan> timed(p, "mex_checkpoint_backward", "bwd", s);
+    check(simnets_mex_checkpoint_gradients(&d, int32_t(group), ptr(codes), ptr(ranges), ptr(off), ptr(dy), want_dx ? ptr(dx) : nullptr, want_doff ? ptr(doff) : nullptr,
+                                           ptr(ws), ws.numel(), s));
+    timed.done();
+    return {dx, doff};
+}
+
+std::pair<Tensor, Tensor> mex_checkpoint_backward(const MexPlanPtr& p, const Tensor& codes, const Tensor& ranges, int64_t group, const Tensor& off, const Tensor& dy,
+                                                  uint32_t flags, bool pooled, const OptTensor& out) {
+    return mex_checkpoint_grads(*p, codes, ranges, group, off, dy, flags, pooled, true, true, out);
+}
+
+std::tuple<OptTensor, OptTensor, OptTensor> sim_checkpoint_grads(const SimPlan& p, const Tensor& codes, const Tensor& ranges, int64_t group, const Tensor& t_in, const Tensor& w_in,
+                                                                 const Tensor& dy_in, uint32_t flags, bool want_dx, bool want_params, const OptTensor& dt_out, const OptTensor& dw_out) {
+    check_checkpoint(codes, ranges, group, int64_t(p.d.batch) * p.d.channels * p.d.height * p.d.width);
+    require_cuda_all(ranges, t_in, w_in, dy_in);
+    if ((ranges.scalar_type() == at::kDouble) != (p.d.dtype == SIMNETS_F64)) throw py::type_error("input does not have the planned dtype");
+    p.check_params(t_in, w_in);
+    p.check_dy(dy_in);
+    const Tensor t = t_in.contiguous(), w = w_in.contiguous(), dy = dy_in.contiguous();
+    const c10::cuda::CUDAGuard guard(ranges.device());
+    const cudaStream_t s = stream_of(ranges);
+    const simnets_sim_desc d = p.with(flags);
+    OptTensor dx, dt, dw;
+    if (want_dx) dx = at::empty({d.batch, d.channels, d.height, d.width}, ranges.options());
+    if (want_params) { dt = grad_target(t, dt_out); dw = grad_target(w, dw_out); }
+    const Tensor ws = scratch(ranges, std::max<size_t>(simnets_similarity_checkpoint_workspace_bytes(&d), 256));
+    Timed<SimPlan> timed(p, "similarity_checkpoint_backward", "dx", s);
+    check(simnets_similarity_checkpoint_gradients(&d, int32_t(group), ptr(codes), ptr(ranges), ptr(t), ptr(w), ptr(dy), dx ? ptr(*dx) : nullptr, dt ? ptr(*dt) : nullptr,
+                                                  dw ? ptr(*dw) : nullptr, ptr(ws), ws.numel(), s));
+    timed.done();
+    return {dx, dt, dw};
+}
+
+std::tuple<OptTensor, OptTensor, OptTensor> sim_checkpoint_backward(const SimPlanPtr& p, const Tensor& codes, const Tensor& ranges, int64_t group, const Tensor& t, const Tensor& w,
+                                                                    const Tensor& dy, uint32_t flags, const OptTensor& dt_out, const OptTensor& dw_out) {
+    return sim_checkpoint_grads(*p, codes, ranges, group, t, w, dy, flags, true, true, dt_out, dw_out);
+}
+
+// The nodes of layers that keep their input in 8 bits: nothing of the forward pass's output or workspace stays.
+struct MexCheckpointNode : torch::autograd::Node {
+    MexPlanPtr plan;
+    SavedVariable codes, ranges, off;
+    OptTensor sink;
+    int64_t group = 0;
+    uint32_t flags = 0;
+    bool pooled = false;
+    std::string name() const override { return pooled ? "MexSumPool2CheckpointBackward" : "MexCheckpointBackward"; }
+    variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        variable_list out(2);
+        if (!grads[0].defined()) return out;
+        const bool want_dx = task_should_compute_output(0), want_doff = task_should_compute_output(1);
+        if (!want_dx && !want_doff) return out;
+        const auto g = mex_checkpoint_grads(*plan, codes.unpack(), ranges.unpack(), group, off.unpack(), grads[0], flags | (sink ? SIMNETS_FLAG_ACCUMULATE : 0u), pooled,
+                                            want_dx, want_doff, sink);
+        if (want_dx) out[0] = g.first;
+        if (want_doff && !sink) out[1] = g.second;
+        return out;
+    }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        codes.reset_data(); ranges.reset_data(); off.reset_data();
+    }
+};
+
+Tensor mex_checkpoint_apply(const MexPlanPtr& p, const Tensor& x, const Tensor& off, int64_t group, const OptTensor& ws, uint32_t fwd_flags, uint32_t op_flags, bool pooled,
+                            const OptTensor& sink) {
+    refuse_tangents({&x, &off});
+    const bool track = at::GradMode::is_enabled() && (x.requires_grad() || off.requires_grad());
+    Tensor out;
+    Kept kept;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        if (pooled && p->d.dtype == SIMNETS_F32 && p->d.batch > 0) {
+            out = mex_forward_impl(*p, x, off, fwd_flags | op_flags, ws, true, false).second;
+        } else {
+            out = mex_forward_impl(*p, x, off, fwd_flags | op_flags, ws, false).first;
+            if (pooled) out = at::avg_pool2d(out, {2, 2}, {2, 2}, 0, false, true, 1);      // (the sum of each window)
+        }
+        if (track) kept = checkpoint_pack(x, group);
+    }
+    if (!track) return out;
+    auto node = std::shared_ptr<MexCheckpointNode>(new MexCheckpointNode(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x, off));
+    node->plan = p;
+    node->codes = SavedVariable(kept.codes, false);
+    node->ranges = SavedVariable(kept.ranges, false);
+    node->off = SavedVariable(off, false);
+    node->sink = sink;
+    node->group = group;
+    node->flags = op_flags;
+    node->pooled = pooled;
+    torch::autograd::set_history(out, node);
+    return out;
+}
+
+struct SimCheckpointNode : torch::autograd::Node {
+    SimPlanPtr plan;
+    SavedVariable codes, ranges, t, w;
+    OptTensor dt_sink, dw_sink;
+    int64_t group = 0;
+    uint32_t flags = 0;
+    std::string name() const override { return "SimilarityCheckpointBackward"; }
+    variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        variable_list out(3);
+        if (!grads[0].defined()) return out;
+        const bool want_dx = task_should_compute_output(0), want_params = task_should_compute_output(1) || task_should_compute_output(2);
+        if (!want_dx && !want_params) return out;
+        const bool add = dt_sink && dw_sink;        // both parameter gradients are added straight into the caller's tensors
+        const auto g = sim_checkpoint_grads(*plan, codes.unpack(), ranges.unpack(), group, t.unpack(), w.unpack(), grads[0], flags | (add ? SIMNETS_FLAG_ACCUMULATE : 0u),
+                                            want_dx, want_params, add ? dt_sink : std::nullopt, add ? dw_sink : std::nullopt);
+        if (want_dx) out[0] = *std::get<0>(g);
+        if (want_params && !add) { out[1] = *std::get<1>(g); out[2] = *std::get<2>(g); }
+        return out;
+    }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        codes.reset_data(); ranges.reset_data(); t.reset_data(); w.reset_data();
+    }
+};
+
+Tensor sim_checkpoint_apply(const SimPlanPtr& p, const Tensor& x, const Tensor& t, const Tensor& w, int64_t group, uint32_t flags, uint64_t ch_max, uint64_t ch_min,
+                            const OptTensor& dt_sink, const OptTensor& dw_sink) {
+    refuse_tangents({&x, &t, &w});
+    const bool track = at::GradMode::is_enabled() && (x.requires_grad() || t.requires_grad() || w.requires_grad());
+    Tensor y;
+    Kept kept;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        y = sim_forward(p, x, t, w, flags, ch_max, ch_min);
+        if (track) kept = checkpoint_pack(x, group);
+    }
+    if (!track) return y;
+    auto node = std::shared_ptr<SimCheckpointNode>(new SimCheckpointNode(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x, t, w));
+    node->plan = p;
+    node->codes = SavedVariable(kept.codes, false);
+    node->ranges = SavedVariable(kept.ranges, false);
+    node->t = SavedVariable(t, false);
+    node->w = SavedVariable(w, false);
+    node->group = group;
+    node->flags = flags;
+    node->dt_sink = dt_sink;
+    node->dw_sink = dw_sink;
+    torch::autograd::set_history(y, node);
+    return y;
+}
+
+// ----------------------------------------------------------------------------------------------------------------- routing
+simnets_route_desc route_desc(const Tensor& scores, int64_t top_k, int64_t groups, int64_t top_groups, bool sigmoid, double scale) {
+    if (scores.dim() < 2) throw std::invalid_argument("scores must have the components on axis 1");
+    if (scores.scalar_type() != at::kFloat && scores.scalar_type() != at::kDouble) throw py::type_error("simnets ops are registered for float32 and float64 only");
+    const int64_t most = std::numeric_limits<int32_t>::max();
+    if (scores.size(0) > most || scores.size(1) > most || top_k > most || groups > most || top_groups > most) throw std::invalid_argument("scores: too many components or samples");
+    simnets_route_desc d = {};
+    d.dtype = scores.scalar_type() == at::kDouble ? SIMNETS_F64 : SIMNETS_F32;
+    d.batch = int32_t(scores.size(0));
+    d.components = int32_t(scores.size(1));
+    d.positions = 1;
+    for (int64_t i = 2; i < scores.dim(); ++i) d.positions *= scores.size(i);
+    d.top_k = int32_t(top_k);
+    d.groups = int32_t(groups);
+    d.top_groups = int32_t(top_groups);
+    d.sigmoid = sigmoid;
+    d.scale = scale;
+    return d;
+}
+OptTensor per_component(const Tensor& scores, const OptTensor& v, const char* what) {
+    if (!v) return std::nullopt;
+    require_cuda(scores, *v);
+    if (v->dim() != 1 || v->size(0) != scores.size(1)) throw std::invalid_argument(std::string(what) + " must hold one value per component");
+    return v->contiguous();
+}
+
+struct Routed { Tensor index, weights, dense, load, mass; };
+
+Routed route_impl(const Tensor& scores_in, const OptTensor& prior_in, const OptTensor& bias_in, const simnets_route_desc& d, bool dense) {
+    require_cuda_all(scores_in);
+    const OptTensor prior = per_component(scores_in, prior_in, "prior"), bias = per_component(scores_in, bias_in, "bias");
+    const Tensor scores = scores_in.contiguous();
+    const c10::cuda::CUDAGuard guard(scores.device());
+    const size_t need = simnets_route_workspace_bytes(&d);
+    std::vector<int64_t> shape = scores.sizes().vec();
+    Routed r;
+    if (dense) {
+        r.dense = at::empty(shape, scores.options());
+        r.mass = at::empty({shape[1]}, scores.options());
+    } else {
+        shape[1] = d.top_k;
+        r.index = at::empty(shape, scores.options().dtype(at::kInt));
+        r.weights = at::empty(shape, scores.options());
+    }
+    r.load = at::empty({scores.size(1)}, scores.options().dtype(at::kLong));
+    const Tensor ws = scratch(scores, std::max<size_t>(need, 256));
+    check(simnets_route(&d, ptr(scores), prior ? ptr(*prior) : nullptr, bias ? ptr(*bias) : nullptr, dense ? nullptr : r.index.data_ptr<int32_t>(), dense ? nullptr : ptr(r.weights),
+                        dense ? ptr(r.dense) : nullptr, r.load.data_ptr<int64_t>(), dense ? ptr(r.mass) : nullptr, ptr(ws), ws.numel(), stream_of(scores)));
+    return r;
+}
+
+struct RouteNode : torch::autograd::Node {
+    simnets_route_desc d;
+    SavedVariable scores, index, weights;
+    OptTensor prior;
+    std::string name() const override { return "RouteBackward"; }
+    variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        variable_list out(1);
+        if (!grads[0].defined() || !task_should_compute_output(0)) return out;
+        const Tensor iv = index.unpack(), wv = weights.unpack(shared_from_this()), sv = scores.unpack().contiguous(), g = grads[0].contiguous();
+        require_cuda_all(wv, g);
+        if (g.sizes() != wv.sizes()) throw std::invalid_argument("route: gradient must have shape " + shape_text(wv.sizes()) + ", got " + shape_text(g.sizes()));
+        const c10::cuda::CUDAGuard guard(sv.device());
+        Tensor ds = at::empty(sv.sizes(), sv.options());
+        check(simnets_route_gradient(&d, ptr(sv), prior ? ptr(*prior) : nullptr, iv.data_ptr<int32_t>(), ptr(wv), ptr(g), ptr(ds), stream_of(sv)));
+        out[0] = ds;
+        return out;
+    }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        scores.reset_data(); index.reset_data(); weights.reset_data();
+        prior.reset();
+    }
+};
+
+// (index, weights, load); the weights are differentiable with respect to the scores
+std::tuple<Tensor, Tensor, Tensor> route_apply(const Tensor& scores, const OptTensor& prior, const OptTensor& bias, int64_t top_k, int64_t groups, int64_t top_groups, bool sigmoid,
+                                               double scale) {
+    refuse_tangents({&scores});
+    const bool track = at::GradMode::is_enabled() && scores.requires_grad();
+    const simnets_route_desc d = route_desc(scores, top_k, groups, top_groups, sigmoid, scale);
+    Routed r;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        r = route_impl(scores, prior, bias, d, false);
+    }
+    if (track) {
+        auto node = std::shared_ptr<RouteNode>(new RouteNode(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(scores));
+        node->d = d;
+        node->scores = SavedVariable(scores, false);
+        node->index = SavedVariable(r.index, false);
+        if (prior) node->prior = prior->detach().clone();           // (one value per component: not a saved variable, a copy)
+        torch::autograd::set_history(r.weights, node);
+        node->weights = SavedVariable(r.weights, true);
+    }
+    return {r.index, r.weights, r.load};
+}
+
+std::tuple<Tensor, Tensor, Tensor> responsibilities(const Tensor& scores, const OptTensor& prior, const OptTensor& bias, int64_t top_k, int64_t groups, int64_t top_groups, bool sigmoid) {
+    const simnets_route_desc d = route_desc(scores, top_k, groups, top_groups, sigmoid, 1.0);
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Routed r = route_impl(scores, prior, bias, d, true);
+    return {r.dense, r.mass, r.load};
+}
+
 // ---------------------------------------------------------------------------------------------------- softmax cross-entropy
 std::pair<Tensor, Tensor> xent_with_grad(const Tensor& logits_in, const Tensor& labels_in, double scale) {
     require_cuda_all(logits_in);
@@ -563,6 +869,17 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("sim_input_grad", &sim_input_grad);
     m.def("sim_params_grad", &sim_params_grad);
     m.def("sim_apply", &sim_apply);
+    m.def("checkpoint_pack", [](const Tensor& x, int64_t group) {
+        const Kept kept = checkpoint_pack(x, group);
+        return std::make_pair(kept.codes, kept.ranges);
+    });
+    m.def("checkpoint_unpack", &checkpoint_unpack);
+    m.def("mex_checkpoint_backward", &mex_checkpoint_backward);
+    m.def("mex_checkpoint_apply", &mex_checkpoint_apply);
+    m.def("sim_checkpoint_backward", &sim_checkpoint_backward);
+    m.def("sim_checkpoint_apply", &sim_checkpoint_apply);
+    m.def("route_apply", &route_apply);
+    m.def("responsibilities", &responsibilities);
     m.def("mixture_statistics", &mixture_statistics);
     m.def("mixture_parameters", &mixture_parameters);
     m.def("xent_with_grad", &xent_with_grad);

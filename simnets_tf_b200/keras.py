@@ -18,6 +18,8 @@ from . import _torch_glue
 from .ops.mex import _attrs as _mex_attrs, _expand_dim_specification, _mex_dims_helper
 from .ops.mex import mex_plan as _mex_plan, mex_recorded as _mex_recorded, mex_with_plan as _mex_with_plan
 from .ops.similarity import _attrs as _similarity_attrs, similarity_plan as _similarity_plan, similarity_recorded as _similarity_recorded
+from .ops.checkpoint import check_group as _check_group, mex_checkpointed_with_plan as _mex_checkpointed_with_plan
+from .ops.checkpoint import similarity_checkpointed_with_plan as _similarity_checkpointed_with_plan
 
 
 def _sinks(*params):
@@ -52,6 +54,7 @@ class _PlannedLayer(torch.nn.Module):
     attribute may be changed between calls, in place too)."""
 
     _plan_attributes = ()
+    checkpoint = None                       # (layers pickled before there were checkpoints)
 
     def __init__(self):
         super(_PlannedLayer, self).__init__()
@@ -75,8 +78,18 @@ class _PlannedLayer(torch.nn.Module):
         return plan
 
 
+def _checkpoint_of(kwargs):
+    """The `checkpoint` argument of a layer: None, or the group length of the 8-bit checkpoint that it keeps of its input for the
+    backward pass (ops.checkpoint) instead of the input itself; True stands for 128."""
+    group = kwargs.pop("checkpoint", None)
+    if group is None or group is False:
+        return None
+    return _check_group(128 if group is True else group)
+
+
 class Similarity(_PlannedLayer):
-    """Similarity layer; `weights` enter the op as their absolute value, as in the reference's `call`."""
+    """Similarity layer; `weights` enter the op as their absolute value, as in the reference's `call`.  `checkpoint`: see
+    `_checkpoint_of`; not part of the reference's arguments, nor of `get_config` unless set."""
 
     _plan_attributes = ('similarity_function', 'strides', 'blocks', 'padding', 'normalization_term', 'normalization_term_fudge',
                         'ignore_nan_input', 'out_of_bounds_value')
@@ -105,6 +118,7 @@ class Similarity(_PlannedLayer):
         self.weights_initializer = weights_initializer
         self.channels_last = channels_last
         self.generator = kwargs.pop("generator", None)
+        self.checkpoint = _checkpoint_of(kwargs)
         self.sweights = None
         self.templates = None
 
@@ -154,7 +168,9 @@ class Similarity(_PlannedLayer):
             x = x.permute(0, 3, 1, 2)
         # |weights| and its gradient are taken inside the op's kernels
         weights = self.sweights
-        if _torch_glue.is_tracing():
+        if self.checkpoint is not None:
+            y = _similarity_checkpointed_with_plan(self._plan, x, templates, weights, self.checkpoint, abi.FLAG_SIM_ABS_WEIGHTS, extrema, _sinks(templates, weights))
+        elif _torch_glue.is_tracing():
             y = _similarity_recorded(self._plan, x, templates, weights, abi.FLAG_SIM_ABS_WEIGHTS, extrema)
         else:
             up, down = extrema if extrema is not None else (None, None)
@@ -165,7 +181,7 @@ class Similarity(_PlannedLayer):
     def get_config(self):
         names = ['num_instances', 'similarity_function', 'strides', 'blocks', 'padding', 'normalization_term',
                  'normalization_term_fudge', 'ignore_nan_input', 'out_of_bounds_value', 'templates_initializer',
-                 'weights_initializer', 'channels_last']
+                 'weights_initializer', 'channels_last'] + (['checkpoint'] if self.checkpoint is not None else [])
         return {k: getattr(self, k) for k in names}
 
 
@@ -221,7 +237,8 @@ class _NormalizeOffsets(torch.autograd.Function):
 
 
 class Mex(_PlannedLayer):
-    """MEX layer; `normalize_offsets` subtracts a per-(region, instance) logsumexp from the offsets variable."""
+    """MEX layer; `normalize_offsets` subtracts a per-(region, instance) logsumexp from the offsets variable.  `checkpoint`: see
+    `_checkpoint_of`; not part of the reference's arguments, nor of `get_config` unless set."""
 
     _plan_attributes = ('num_instances', 'padding', 'strides', 'blocks', 'epsilon', 'use_unshared_regions', 'shared_offset_region',
                         'unshared_offset_region', 'softmax_mode', 'blocks_out_of_bounds_value', 'blocks_round_down')
@@ -249,6 +266,7 @@ class Mex(_PlannedLayer):
             offsets_initializer = dirichlet_init()
         self.offsets_initializer = offsets_initializer
         self.channels_last = channels_last
+        self.checkpoint = _checkpoint_of(kwargs)
         self.offsets = None
 
     def build(self, input_shape, device=None, dtype=torch.float32):
@@ -347,7 +365,10 @@ class Mex(_PlannedLayer):
         # (the raw offsets are the op's own input, and a gradient bucket its target, only when the op normalises them)
         sink = _sinks(off) if op_flags else None
         fwd_flags = abi.FLAG_MEX_MAXIMA_GIVEN if maxima_given else 0
-        if _torch_glue.is_tracing():
+        if self.checkpoint is not None:
+            y = _mex_checkpointed_with_plan(lambda x: self._plan(x.shape, x.dtype), x, off if op_flags else self.effective_offsets(), self.checkpoint, layer_ws,
+                                            fwd_flags, op_flags, sum_pool2, sink[0] if sink else None)
+        elif _torch_glue.is_tracing():
             y = _mex_recorded(lambda x: self._plan(x.shape, x.dtype), x, off if op_flags else self.effective_offsets(), layer_ws, fwd_flags, op_flags,
                               sum_pool2)
         else:
@@ -358,7 +379,7 @@ class Mex(_PlannedLayer):
     def get_config(self):
         names = ['num_instances', 'padding', 'strides', 'blocks', 'epsilon', 'use_unshared_regions', 'shared_offset_region',
                  'unshared_offset_region', 'softmax_mode', 'blocks_out_of_bounds_value', 'blocks_round_down',
-                 'normalize_offsets', 'offsets_initializer', 'channels_last']
+                 'normalize_offsets', 'offsets_initializer', 'channels_last'] + (['checkpoint'] if self.checkpoint is not None else [])
         return {k: getattr(self, k) for k in names}
 
 

@@ -3,6 +3,8 @@
 `_similarity_grad` (same file, :18-45).  Tensors are torch CUDA tensors; the work is done by the
 CUDA library through the C ABI.
 """
+import torch
+
 from .. import _lib, abi
 from .. import _torch_glue
 from .._torch_glue import dtype_code, sequence_key
@@ -21,18 +23,22 @@ def _attrs(**given):
 
 
 def _desc(input, templates, weights, attrs, flags=0):
-    if input.dim() != 4 or templates.dim() != 4 or weights.dim() != 4:
+    return _desc_of(input.shape, dtype_code(input), templates, weights, attrs, flags)
+
+
+def _desc_of(input_shape, dtype, templates, weights, attrs, flags=0):
+    if len(input_shape) != 4 or templates.dim() != 4 or weights.dim() != 4:
         raise ValueError("input, templates and weights must be 4-D")
     if templates.shape != weights.shape:
         raise ValueError("templates and weights must have the same shape")
-    if templates.shape[1] != input.shape[1]:
+    if templates.shape[1] != input_shape[1]:
         raise ValueError("Number of channels mismatch between input and template")
     blocks = list(attrs["blocks"])
     if list(templates.shape[2:]) != [int(b) for b in blocks]:
         raise ValueError("templates spatial shape %s does not match blocks %s" % (list(templates.shape[2:]), blocks))
-    return abi.make_sim_desc(input.shape, templates.shape[0], attrs["similarity_function"], blocks, attrs["strides"],
+    return abi.make_sim_desc(input_shape, templates.shape[0], attrs["similarity_function"], blocks, attrs["strides"],
                              attrs["padding"], attrs["normalization_term"], attrs["normalization_term_fudge"],
-                             attrs["ignore_nan_input"], attrs["out_of_bounds_value"], dtype=dtype_code(input), flags=flags | _torch_glue.DEFAULT_FLAGS)
+                             attrs["ignore_nan_input"], attrs["out_of_bounds_value"], dtype=dtype, flags=flags | _torch_glue.DEFAULT_FLAGS)
 
 
 _PLANS = _torch_glue.PlanCache()
@@ -42,6 +48,13 @@ def similarity_plan(input, templates, weights, attrs):
     """The native plan of these shapes and attributes (a complete dict, see `_attrs`)."""
     key = (input.shape, input.dtype, templates.shape, weights.shape, _torch_glue.DEFAULT_FLAGS) + tuple(map(sequence_key, attrs.values()))
     return _PLANS.get(key, lambda: _lib.ops().SimPlan(bytes(_desc(input, templates, weights, attrs))))
+
+
+def similarity_plan_of_shape(input_shape, dtype, templates, weights, attrs):
+    """`similarity_plan` of an input that is not there as a tensor."""
+    code = {torch.float32: abi.F32, torch.float64: abi.F64}[dtype]
+    key = (input_shape, dtype, templates.shape, weights.shape, _torch_glue.DEFAULT_FLAGS) + tuple(map(sequence_key, attrs.values()))
+    return _PLANS.get(key, lambda: _lib.ops().SimPlan(bytes(_desc_of(input_shape, code, templates, weights, attrs))))
 
 
 def similarity_forward(input, templates, weights, flags=0, extrema=None, **attrs):

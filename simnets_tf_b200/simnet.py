@@ -80,20 +80,23 @@ def _caller():
 
 
 class SimNet(torch.nn.Module):
-    """A specification instantiated on the CUDA operators."""
+    """A specification instantiated on the CUDA operators.  `checkpoint` (None, True or a group length): the layers behind the first
+    keep their inputs in 8 bits for the backward pass, and neither their outputs nor their workspaces (the first layer's input is
+    the caller's, who has it anyway)."""
 
-    def __init__(self, spec, seed=0, device="cuda", dtype=torch.float32):
+    def __init__(self, spec, seed=0, device="cuda", dtype=torch.float32, checkpoint=None):
         super(SimNet, self).__init__()
         self.spec = spec
         mods, init = [], init_parameters(spec, seed)
         for entry, values in zip(spec["layers"], init):
+            kept = dict(checkpoint=checkpoint) if mods and checkpoint is not None else {}
             if entry[0] == "similarity":
-                m = layers.Similarity(**entry[1])
+                m = layers.Similarity(**entry[1], **kept)
                 m.sweights = torch.nn.Parameter(torch.from_numpy(values["weights"]).to(device=device, dtype=dtype))      # same order as build()
                 m.templates = torch.nn.Parameter(torch.from_numpy(values["templates"]).to(device=device, dtype=dtype))
                 mods.append(m)
             elif entry[0] == "mex":
-                m = layers.Mex(**entry[1])
+                m = layers.Mex(**entry[1], **kept)
                 m.blocks = list(values["offsets"].shape[2:])
                 m.offsets = torch.nn.Parameter(torch.from_numpy(values["offsets"]).to(device=device, dtype=dtype))
                 mods.append(m)

@@ -30,6 +30,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .ops.routing import responsibilities as _responsibilities
 
 _sim = importlib.import_module(__package__ + ".ops.similarity")     # the module: `ops.similarity` itself is the op function
 
@@ -52,6 +53,10 @@ class LibraryPatchOps(object):
         """(sum r (p - c), sum r (p - c)^2), each shaped like `centres`, for resp [batch, k, out_h, out_w]."""
         dt, dw = _sim.similarity_parameters_grad(x, centres, torch.ones_like(centres), resp, flags=self.flags, **self.attrs)
         return dt.mul_(0.5), dw.neg_()
+
+    def responsibilities(self, scores, top_k, prior=None, bias=None):
+        """(responsibilities, mass, load) of scores [batch, k, out_h, out_w], see ops.routing."""
+        return _responsibilities(scores, top_k, prior=prior, bias=bias)
 
     def mixture_statistics(self, x, means, covs):
         """sum r (p - mean), sum r (p - mean)^2 and sum r of a mixture's responsibilities r, in one flat tensor, by the
@@ -94,6 +99,20 @@ class _Estimator(object):
         self.group = group
         self.rng = np.random.RandomState(seed)
 
+    def _balance_of(self, balance):
+        """Every step moves the bias of a component by `balance` (in units of the scores) towards the mean load: up where fewer positions
+        than the mean chose it, down where more did."""
+        self.balance = float(balance)
+        if not (0.0 <= self.balance < float("inf")):
+            raise ValueError("balance must be a finite number that is not negative, got %r" % (balance,))
+        self.bias = None
+
+    def _moved_bias(self, load, like):
+        """The bias for the next step from the loads of this one (summed over the ranks)."""
+        load, = _all_reduce(self.group, load)
+        bias = torch.zeros(self.k, dtype=like.dtype, device=like.device) if self.bias is None else self.bias
+        self.bias = bias - self.balance * torch.sign(load * self.k - load.sum()).to(bias.dtype)
+
     def _check(self, x):
         if x.dim() != 4 or x.shape[2] < self.blocks[0] or x.shape[3] < self.blocks[1]:
             raise ValueError("input must be [batch, channels, height, width] and hold at least one whole patch")
@@ -107,10 +126,13 @@ class KMeans(_Estimator):
     patch drawn with probability proportional to its squared distance to the nearest centre chosen so far.
     update(batch): every patch goes to its nearest centre; with n_c patches of this batch at centre c and N_c seen before,
     `c += (sum of those patches - n_c c) / (N_c + n_c)`, that is, every centre stays the mean of all patches ever assigned
-    to it with their assignment-time weights (per-centre learning rate 1 / count)."""
+    to it with their assignment-time weights (per-centre learning rate 1 / count).
+    balance > 0: a patch goes to the centre with the smallest squared distance minus its bias, and the biases follow the loads
+    (`_balance_of`): a centre that no patch goes to comes closer to all of them until one does."""
 
-    def __init__(self, blocks, strides, num_instances, seed=0, ops=None, group=None):
+    def __init__(self, blocks, strides, num_instances, seed=0, ops=None, group=None, balance=0.0):
         super(KMeans, self).__init__(blocks, strides, num_instances, seed, ops, group)
+        self._balance_of(balance)
         self.centres = None
         self.counts = None
 
@@ -138,9 +160,14 @@ class KMeans(_Estimator):
     def update(self, x):
         x = self._check(x)
         score = self.ops.neg_scaled_sqdist(x, self.centres, torch.ones_like(self.centres))
-        onehot = torch.zeros_like(score).scatter_(1, score.argmax(dim=1, keepdim=True), 1.0)
+        if self.balance > 0:
+            onehot, n, load = self.ops.responsibilities(score, 1, bias=self.bias)
+            self._moved_bias(load, score)
+        else:
+            onehot = torch.zeros_like(score).scatter_(1, score.argmax(dim=1, keepdim=True), 1.0)
+            n = onehot.sum(dim=(0, 2, 3))
         shift, _ = self.ops.moments(x, self.centres, onehot)            # sum over the centre's patches of (p - c)
-        n, shift = _all_reduce(self.group, onehot.sum(dim=(0, 2, 3)), shift)
+        n, shift = _all_reduce(self.group, n, shift)
         self.counts = self.counts + n
         self.centres = self.centres + shift / self.counts.clamp(min=1).view(-1, 1, 1, 1)
         return self.centres
@@ -158,10 +185,20 @@ class DiagonalGMM(_Estimator):
     update(batch): one full EM step on this batch from the current parameters: responsibilities
     `r ∝ exp(-1/2 sum ((p - mu)^2 / var + log var))`, then `mu' = sum r p / sum r` and
     `var' = sum r p^2 / sum r - mu'^2 + floor`.  A component that no patch of the batch claims at all (zero mass, where the
-    textbook step divides zero by zero) keeps its mean and gets the floor as its covariance."""
+    textbook step divides zero by zero) keeps its mean and gets the floor as its covariance.
+    top_k: only the top_k most likely components of a patch share it (None: all of them), and one that gets no patch keeps
+    its covariance as well (at the floor it would never get one again).  balance > 0 (with a top_k): those are
+    chosen by log-likelihood plus a bias that follows the loads (`_balance_of`), so that a component that no patch claims is offered
+    more and more of them; the shares themselves are without the bias."""
 
-    def __init__(self, blocks, strides, num_instances, seed=33, ops=None, group=None, min_var=MIN_VAR):
+    def __init__(self, blocks, strides, num_instances, seed=33, ops=None, group=None, min_var=MIN_VAR, top_k=None, balance=0.0):
         super(DiagonalGMM, self).__init__(blocks, strides, num_instances, seed, ops, group)
+        self._balance_of(balance)
+        if top_k is not None and (isinstance(top_k, bool) or int(top_k) != top_k or not 1 <= top_k <= min(self.k, 16)):
+            raise ValueError("top_k must be a whole number from 1 to %d, got %r" % (min(self.k, 16), top_k))
+        if top_k is None and self.balance > 0:
+            raise ValueError("a mixture whose components all share every patch has no choice to balance: give a top_k")
+        self.top_k = top_k
         self.min_var = float(min_var)
         self.means = None
         self.covs = None
@@ -185,6 +222,12 @@ class DiagonalGMM(_Estimator):
 
     def update(self, x):
         x = self._check(x)
+        if self.top_k is not None:
+            score = self.ops.neg_scaled_sqdist(x, self.means, (0.5 / self.covs).contiguous())
+            resp, mass, load = self.ops.responsibilities(score, self.top_k, prior=-0.5 * self.covs.log().sum(dim=(1, 2, 3)), bias=self.bias)
+            if self.balance > 0:
+                self._moved_bias(load, score)
+            return self._step(x, resp, mass)
         stats = self.ops.mixture_statistics(x, self.means, self.covs) if isinstance(self.ops, LibraryPatchOps) else None
         if stats is not None:
             stats, = _all_reduce(self.group, stats)
@@ -193,11 +236,18 @@ class DiagonalGMM(_Estimator):
         half_mahalanobis = self.ops.neg_scaled_sqdist(x, self.means, (1.0 / self.covs).contiguous())
         logdet = self.covs.log().sum(dim=(1, 2, 3))
         resp = torch.softmax(0.5 * (half_mahalanobis - logdet.view(1, -1, 1, 1)), dim=1)
+        return self._step(x, resp, resp.sum(dim=(0, 2, 3)))
+
+    def _step(self, x, resp, mass):
+        """New means and covariances from the responsibilities of this batch and their sums."""
         shift, sq = self.ops.moments(x, self.means, resp)
-        mass, shift, sq = _all_reduce(self.group, resp.sum(dim=(0, 2, 3)), shift, sq)
+        mass, shift, sq = _all_reduce(self.group, mass, shift, sq)
         mass = mass.clamp(min=torch.finfo(x.dtype).tiny).view(-1, 1, 1, 1)
         step = shift / mass
-        self.covs = (sq / mass - step * step + self.min_var).contiguous()     # second moment about the NEW mean
+        covs = (sq / mass - step * step + self.min_var).contiguous()          # second moment about the NEW mean
+        if self.top_k is not None:
+            covs = torch.where(mass > torch.finfo(x.dtype).tiny, covs, self.covs)
+        self.covs = covs
         self.means = (self.means + step).contiguous()
         return self.means, self.covs
 
@@ -206,14 +256,17 @@ class DiagonalGMM(_Estimator):
         return self.means, self.covs.sqrt()
 
 
-def similarity_unsupervised_init(kind, layer, seed=None, ops=None, group=None):
+def similarity_unsupervised_init(kind, layer, seed=None, ops=None, group=None, top_k=None, balance=0.0):
     """The estimator for a `keras.Similarity` layer (or anything with `blocks`, `strides`, `num_instances`): an object with
     `init(batch)`, to be called once with the first batch, and `update(batch)`, to be called with every batch (the first
-    one too), the counterparts of the reference's `(init_op, update_op)` pair; `assign_to(layer)` stores the result."""
+    one too), the counterparts of the reference's `(init_op, update_op)` pair; `assign_to(layer)` stores the result.
+    `top_k` (mixture) and `balance`: see the estimators."""
     if kind == 'kmeans':
-        est = KMeans(layer.blocks, layer.strides, layer.num_instances, 0 if seed is None else seed, ops, group)
+        if top_k is not None:
+            raise ValueError('top_k belongs to kind "gmm"')
+        est = KMeans(layer.blocks, layer.strides, layer.num_instances, 0 if seed is None else seed, ops, group, balance=balance)
     elif kind == 'gmm':
-        est = DiagonalGMM(layer.blocks, layer.strides, layer.num_instances, 33 if seed is None else seed, ops, group)
+        est = DiagonalGMM(layer.blocks, layer.strides, layer.num_instances, 33 if seed is None else seed, ops, group, top_k=top_k, balance=balance)
     else:
         raise ValueError('kind must be one of "kmeans" or "gmm"')
     return est
@@ -256,10 +309,11 @@ def _input_of(model, layer, x):
     raise ValueError("layer is not part of the model")
 
 
-def perform_unsupervised_init(model, kind='gmm', layers=[], data=None, batch_size=None, seed=None, group=None, device="cuda"):
+def perform_unsupervised_init(model, kind='gmm', layers=[], data=None, batch_size=None, seed=None, group=None, device="cuda", top_k=None,
+                              balance=0.0):
     """Initialise the Similarity layers of `model` one after the other, front to back, each from the activations that reach
     it with the layers in front already initialised (python/simnets/keras.py:191-238).  `data`: an array [n, c, h, w] (then
-    `batch_size` is required) or a callable returning an iterator over batches.  The reference's other branch (PCA filters
+    `batch_size` is required) or a callable returning an iterator over batches.  `top_k`, `balance`: see `DiagonalGMM`, `KMeans`.  The reference's other branch (PCA filters
     for Keras `Conv2D` layers) has no counterpart: there are no convolution layers in this library."""
     from . import keras as _layers
     members = [m for _, m in model._plan if m is not None] if hasattr(model, "_plan") else list(model)
@@ -268,7 +322,7 @@ def perform_unsupervised_init(model, kind='gmm', layers=[], data=None, batch_siz
     for layer in layers:
         if not isinstance(layer, _layers.Similarity):
             raise ValueError("unsupervised initialisation is defined for Similarity layers, got %s" % type(layer).__name__)
-        est = similarity_unsupervised_init(kind, layer, seed=seed, group=group)
+        est = similarity_unsupervised_init(kind, layer, seed=seed, group=group, top_k=top_k, balance=balance)
         with torch.no_grad():
             for idx, batch in enumerate(gen()):
                 x = _input_of(model, layer, torch.as_tensor(batch).to(device))

@@ -1,0 +1,121 @@
+"""Routing without a GPU: what its entry points refuse, the estimators that balance their components on stand-in statistics."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import plain_operators as plain
+from oracle import unsupervised_oracle as uo
+from simnets_tf_b200 import abi
+from simnets_tf_b200 import unsupervised as un
+from simnets_tf_b200.ops.routing import responsibilities, route
+
+
+@pytest.mark.parametrize("call", [route, responsibilities])
+def test_arguments_are_checked(call):
+    s = torch.zeros(2, 12, 3, 3)
+    for kw in (dict(top_k=0), dict(top_k=13), dict(top_k=1.5), dict(top_k=True), dict(groups=5), dict(groups=0), dict(groups=4, top_groups=5), dict(groups=4, top_groups=1, top_k=4),
+               dict(groups=4, top_groups=0)):
+        with pytest.raises(ValueError):
+            call(s, **kw)
+    for kw in (dict(prior=torch.zeros(11)), dict(bias=torch.zeros(12, 1)), dict(bias=torch.zeros(12, requires_grad=True))):
+        with pytest.raises(ValueError, match="prior|bias"):
+            call(s, **kw)
+    for bad in (torch.zeros(4), torch.zeros(2, 0, 3)):
+        with pytest.raises(ValueError, match="axis 1"):
+            call(bad)
+    with pytest.raises(ValueError, match="at most 4096"):
+        call(torch.zeros(1, 4097, 1))
+    with pytest.raises(ValueError, match="top_k = 16"):
+        call(torch.zeros(1, 40, 1), top_k=17)
+    with pytest.raises(ValueError, match="16 of 64"):
+        call(torch.zeros(1, 130, 1), groups=65, top_groups=3)
+    with pytest.raises(TypeError, match="float32 and float64"):
+        call(s.half())
+    with pytest.raises(RuntimeError, match="no CPU kernels"):
+        call(s, top_k=2)
+
+
+def test_the_c_entry_points_check_before_they_launch(cuda_lib):
+    one = C.c_void_p(256)                   # (never dereferenced: every call below is refused)
+
+    def call(ws=one, n=None, load=one, scores=one, mass=None, dense=None, **kw):
+        d = abi.RouteDesc(**dict(dict(dtype=abi.F32, batch=2, components=12, top_k=2, groups=1, top_groups=1, positions=9, scale=1.0), **kw))
+        need = cuda_lib.simnets_route_workspace_bytes(C.byref(d))
+        rc = cuda_lib.simnets_route(C.byref(d), scores, None, None, one, one, dense, load, mass, ws, need if n is None else n, None)
+        assert cuda_lib.simnets_route_gradient(C.byref(d), one, None, None, one, one, one, None) == (rc if need == 0 else abi.E_NULL)
+        return rc
+    assert C.sizeof(abi.RouteDesc) == 48
+    assert call(dtype=3) == abi.E_DTYPE
+    for kw in (dict(batch=-1), dict(positions=-1), dict(components=0), dict(top_k=0), dict(top_k=13), dict(groups=5), dict(top_groups=2), dict(reserved=1), dict(scale=0.0),
+               dict(scale=float("inf")), dict(groups=4, top_groups=1, top_k=4)):
+        assert call(**kw) == abi.E_DESC, kw
+    for kw in (dict(components=4097), dict(components=40, top_k=17), dict(components=130, groups=65, top_groups=3), dict(components=170, groups=34, top_groups=17),
+               dict(batch=1 << 20, positions=1 << 40)):
+        assert call(**kw) == abi.E_UNSUPPORTED, kw
+    assert call(load=None) == abi.E_NULL and call(scores=None) == abi.E_NULL and call(mass=one) == abi.E_NULL
+    assert call(ws=None) == abi.E_WORKSPACE and call(n=8) == abi.E_WORKSPACE
+
+
+def test_the_restatement_routes_by_value_and_index():
+    s = np.zeros((1, 4, 2), np.float32)
+    s[0, :, 1] = [np.nan, 1.0, -np.inf, 1.0]
+    index, weights, load, dense, mass, _ = plain.route(s, 3)
+    assert index[0, :, 0].tolist() == [0, 1, 2] and index[0, :, 1].tolist() == [1, 3, -1]
+    assert np.allclose(weights[0, :, 0], 1 / 3) and weights[0, :, 1].tolist() == [0.5, 0.5, 0.0]
+    assert load.tolist() == [1, 2, 1, 1] and np.allclose(mass, dense.sum((0, 2)))
+
+
+class Ops(uo.OraclePatchOps):
+    def responsibilities(self, scores, top_k, prior=None, bias=None):
+        a = [None if v is None else v.numpy() for v in (prior, bias)]
+        _, _, load, dense, mass, _ = plain.route(scores.numpy(), top_k, *a)
+        return torch.from_numpy(dense).to(scores.dtype), torch.from_numpy(mass).to(scores.dtype), torch.from_numpy(load)
+
+
+def test_a_mixture_cut_to_all_its_components_is_the_mixture():
+    rng = np.random.default_rng(3)
+    batches = [torch.from_numpy(rng.normal(size=(3, 2, 6, 7))) for _ in range(3)]
+    picks = rng.integers(0, 60, 5)
+    full, cut, two = (un.DiagonalGMM([3, 3], [1, 1], 5, ops=Ops((3, 3), (1, 1)), top_k=k) for k in (None, 5, 2))
+    for est in (full, cut, two):
+        est.init(batches[0], picks=picks)
+        for b in batches:
+            est.update(b)
+    assert torch.allclose(full.means, cut.means, rtol=1e-10, atol=1e-12) and torch.allclose(full.covs, cut.covs, rtol=1e-9, atol=1e-12)
+    assert not torch.allclose(full.means, two.means, rtol=1e-3)
+
+
+@pytest.mark.parametrize("kind", ["kmeans", "gmm"])
+def test_balance_brings_idle_components_into_use(kind):
+    """Two components far from all data: without balance they stay where they are.  A patch is at about 4 x 12^2 = 576 from them (half of
+    that in the mixture, whose variances are near one), and the biases of an idle and of a busy component part by at most
+    2 x balance a step: 720 after 60."""
+    rng = np.random.default_rng(5)
+    x = torch.from_numpy(rng.normal(size=(6, 1, 8, 8)))
+    load = {}
+    for balance in (0.0, 6.0):
+        ops = Ops((2, 2), (2, 2))
+        est = un.KMeans([2, 2], [2, 2], 6, ops=ops, balance=balance) if kind == "kmeans" else un.DiagonalGMM([2, 2], [2, 2], 6, ops=ops, top_k=1, balance=balance)
+        est.init(x)
+        centres = est.centres if kind == "kmeans" else est.means
+        centres[4:] = 12.0
+        for _ in range(60):
+            est.update(x)
+        centres = est.centres if kind == "kmeans" else est.means
+        load[balance] = bool((centres[4:] < 11).any())
+    assert load == {0.0: False, 6.0: True}
+
+
+def test_estimators_check_their_new_arguments():
+    class L(object):
+        blocks, strides, num_instances = [3, 3], [1, 1], 4
+    for kw in (dict(top_k=0), dict(top_k=5), dict(top_k=1.5), dict(top_k=True), dict(balance=1.0), dict(top_k=2, balance=-1.0), dict(top_k=2, balance=float("nan"))):
+        with pytest.raises(ValueError):
+            un.similarity_unsupervised_init("gmm", L(), **kw)
+    for kw in (dict(top_k=1), dict(balance=-0.5), dict(balance=float("inf"))):
+        with pytest.raises(ValueError):
+            un.similarity_unsupervised_init("kmeans", L(), **kw)
+    est = un.similarity_unsupervised_init("gmm", L(), top_k=2, balance=0.5)
+    assert est.top_k == 2 and est.balance == 0.5 and est.bias is None
