@@ -446,7 +446,8 @@ int simnets_checkpoint_unpack(int32_t dtype, int64_t count, int32_t group, const
 
 size_t simnets_mex_checkpoint_workspace_bytes(const simnets_mex_desc* d) {
     MexGeo g;
-    return mex_geometry(d, nullptr, &g) ? 0 : mex_checkpoint_carve(g, *d, nullptr).bytes;
+    if (mex_geometry(d, nullptr, &g)) return 0;
+    return mex_checkpoint_shape(g, d->dtype == SIMNETS_F64, d->flags) ? mex_checkpoint_bytes(g) : mex_checkpoint_carve(g, *d, nullptr).bytes;
 }
 
 int simnets_mex_checkpoint_gradients(const simnets_mex_desc* d, int32_t group, const void* codes, const void* ranges, const void* off, const void* dy, void* dx,
@@ -458,6 +459,11 @@ int simnets_mex_checkpoint_gradients(const simnets_mex_desc* d, int32_t group, c
     if (d->flags & (SIMNETS_FLAG_MEX_WORKSPACE_PRIMED | SIMNETS_FLAG_MEX_MAXIMA_GIVEN)) return SIMNETS_E_UNSUPPORTED;
     if (!off || (g.B > 0 && (!codes || !ranges || !dy || (!dx && !doff)))) return SIMNETS_E_NULL;
     if (g.B == 0) return mex_gradients(g, d, nullptr, off, nullptr, nullptr, nullptr, doff, ws, ws_bytes, nullptr, 0, as_stream(stream));
+    if (mex_checkpoint_shape(g, d->dtype == SIMNETS_F64, d->flags)) {
+        if (!ws || ws_bytes < mex_checkpoint_bytes(g)) return SIMNETS_E_WORKSPACE;
+        return from_cuda(launch_mex_checkpoint(g, group, codes, ranges, (const float*)off, (const float*)dy, (float*)dx, (float*)doff, (d->flags & SIMNETS_FLAG_ACCUMULATE) != 0,
+                                               (d->flags & SIMNETS_FLAG_MEX_NORMALIZED_OFFSETS) != 0, ws, as_stream(stream)));
+    }
     const MexCheckpointWs w = mex_checkpoint_carve(g, *d, ws);
     if (!ws || ws_bytes < w.bytes) return SIMNETS_E_WORKSPACE;
     const cudaError_t e = launch_checkpoint_unpack(d->dtype == SIMNETS_F64, 0, (long long)g.B * g.C * g.H * g.W, group, codes, ranges, w.x, as_stream(stream));

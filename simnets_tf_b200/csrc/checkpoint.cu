@@ -8,26 +8,11 @@
 // A program may pack and compare elsewhere, so the bytes are defined to the bit: with x / 2 - base / 2 and 2 / step rounded to the type and
 // their product exact in front of rint (one fused multiply-add onto 1.5 * 2^23 or 2^52, whose last bits are the integer).  The halves keep
 // the range of values of either sign finite.  A range below 252 of the type's smallest normal number has step 0: all bytes 0.
+#include "checkpoint.cuh"
 #include "kernels.cuh"
 
 namespace simnets {
 namespace {
-
-template <typename T> struct Limits;
-template <> struct Limits<float> {
-    static __device__ __forceinline__ float inf() { return CUDART_INF_F; }
-    static __device__ __forceinline__ float tiny() { return 1.17549435e-38f; }
-    static __device__ __forceinline__ float most() { return 3.402823466e38f; }
-    static __device__ __forceinline__ uint32_t nearest(float a, float b) { return __float_as_uint(__fmaf_rn(a, b, 12582912.f)) & 255u; }
-    static __device__ __forceinline__ float at(float code, float step, float base) { return fminf(__fmaf_rn(code, step, base), most()); }
-};
-template <> struct Limits<double> {
-    static __device__ __forceinline__ double inf() { return CUDART_INF; }
-    static __device__ __forceinline__ double tiny() { return 2.2250738585072014e-308; }
-    static __device__ __forceinline__ double most() { return 1.7976931348623157e308; }
-    static __device__ __forceinline__ uint32_t nearest(double a, double b) { return uint32_t(__double_as_longlong(__fma_rn(a, b, 6755399441055744.0))) & 255u; }
-    static __device__ __forceinline__ double at(double code, double step, double base) { return fmin(__fma_rn(code, step, base), most()); }
-};
 
 __device__ __forceinline__ float least(float a, float b) { return fminf(a, b); }
 __device__ __forceinline__ double least(double a, double b) { return fmin(a, b); }
@@ -68,12 +53,6 @@ __global__ void __launch_bounds__(kPackThreads) checkpoint_pack(long long n, con
         }
         if (lane == 0) { ranges[2 * g] = lo; ranges[2 * g + 1] = step; }
     }
-}
-
-template <typename T>
-__device__ __forceinline__ T unpacked(uint32_t c, T base, T step) {
-    const T v = Limits<T>::at(T(int(c)), step, base);
-    return c < 253u ? v : c == 253u ? -Limits<T>::inf() : c == 254u ? Limits<T>::inf() : Limits<T>::inf() - Limits<T>::inf();
 }
 
 // values first .. first + n of a checkpoint of groups of 2^shift
