@@ -25,114 +25,216 @@ template <typename T> __device__ __forceinline__ T below_all() { return -T(CUDAR
 // the TK largest so far, largest first; equal ones keep the order in which they came
 template <typename T, int TK>
 struct Top {
-    T v[TK], l[TK];
+    T v[TK];
     int i[TK];
     __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int t = 0; t < TK; ++t) { v[t] = l[t] = below_all<T>(); i[t] = -1; }
+        for (int t = 0; t < TK; ++t) { v[t] = below_all<T>(); i[t] = -1; }
     }
-    __device__ __forceinline__ void offer(T value, T logit, int index, int want) {
-        bool placed = false;                             // (a NaN and -infinity are above nothing)
+    // (a NaN and -infinity are above nothing; what makes room moves on in front of its equals)
+    __device__ __forceinline__ void offer(T value, int index) {
+        bool above = false;
 #pragma unroll
         for (int t = 0; t < TK; ++t) {
-            if (t < want && (placed || value > v[t])) {
-                const T ov = v[t], ol = l[t];
-                const int oi = i[t];
-                v[t] = value; l[t] = logit; i[t] = index;
-                value = ov; logit = ol; index = oi;
-                placed = true;
+            above = above || value > v[t];
+            const T ov = v[t];
+            const int oi = i[t];
+            v[t] = above ? value : ov; i[t] = above ? index : oi;
+            value = above ? ov : value; index = above ? oi : index;
+        }
+    }
+    // the lists of the G lanes that share a position (RUN lanes apart) as one, the same in all of them; equal values by index
+    template <int G, int RUN>
+    __device__ __forceinline__ void merge() {
+        if constexpr (G > 1) {
+            Top all;
+#pragma unroll
+            for (int t = 0; t < TK; ++t) {
+                T bv = v[0];
+                unsigned bi = unsigned(i[0]);                            // (-1, nothing, is the largest)
+#pragma unroll
+                for (int d = RUN; d < 32; d <<= 1) {
+                    const T ov = __shfl_xor_sync(0xffffffffu, bv, d);
+                    const unsigned oi = __shfl_xor_sync(0xffffffffu, bi, d);
+                    const bool other = ov > bv || (ov == bv && oi < bi);
+                    bv = other ? ov : bv; bi = other ? oi : bi;
+                }
+                all.v[t] = bv; all.i[t] = int(bi);
+                if (bi == unsigned(i[0])) {                              // it was this lane's: the next one comes up
+#pragma unroll
+                    for (int u = 0; u + 1 < TK; ++u) { v[u] = v[u + 1]; i[u] = i[u + 1]; }
+                    v[TK - 1] = below_all<T>(); i[TK - 1] = -1;
+                }
             }
+            *this = all;
         }
     }
 };
 
-// weights of the chosen from their l, in place: they sum to one over the chosen (all 0 if there are none)
-template <typename T, int TK>
-__device__ __forceinline__ void weigh(Top<T, TK>& top, int want, bool sigmoid) {
-    T hi = below_all<T>();
-#pragma unroll
-    for (int t = 0; t < TK; ++t) {
-        if (t >= want || top.i[t] < 0) continue;
-        if (sigmoid) top.l[t] = top.l[t] >= T(0) ? -log1p_of(exp_of(-top.l[t])) : top.l[t] - log1p_of(exp_of(top.l[t]));
-        hi = top.l[t] > hi ? top.l[t] : hi;
-    }
-    T sum = T(0);
-#pragma unroll
-    for (int t = 0; t < TK; ++t) {
-        top.l[t] = t < want && top.i[t] >= 0 ? (top.l[t] == hi ? T(1) : exp_of(top.l[t] - hi)) : T(0);      // (infinities are equal too)
-        sum += top.l[t];
-    }
-    const T inv = sum > T(0) ? T(1) / sum : T(0);
-#pragma unroll
-    for (int t = 0; t < TK; ++t) top.l[t] *= inv;
-}
-
 struct RouteArgs {
     long long positions;         // of the whole batch
     long long N;                 // per sample
+    FastDiv f_N;                 // where `positions` fits 31 bits
     int k, top, groups, size, top_groups;
     int sigmoid;
     double scale;
 };
+// sample and place inside it
+__device__ __forceinline__ long long sample_of(const RouteArgs& a, long long p) { return a.f_N.d ? (long long)fast_div(uint32_t(p), a.f_N) : p / a.N; }
 
-template <typename T, int TK>
+constexpr int kBatch = 8;        // scores of a position in flight
+
+template <typename T> struct alignas(2 * sizeof(T)) Pair { T prior, bias; };
+
+// f(v, c) for components from .. to, every G-th from `sub` on; `add`: prior and bias of every component, or null for none
+template <int G, typename T, class F>
+__device__ __forceinline__ void over_range(const T* __restrict__ s, long long N, const Pair<T>* add, int from, int to, int sub, F f) {
+    int c = from + sub;
+    const T* q = s + c * N;
+    const long long step = G * N;
+    for (; c + G * (kBatch - 1) < to; c += G * kBatch) {
+        T v[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u, q += step) v[u] = __ldg(q);
+        if (add)
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const Pair<T> both = add[c + G * u];
+                f((v[u] + both.prior) + both.bias, c + G * u);
+            }
+        else
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) f(v[u], c + G * u);
+    }
+    for (; c < to; c += G, q += step) {
+        const T v = __ldg(q);
+        f(add ? (v + add[c].prior) + add[c].bias : v, c);
+    }
+}
+// the largest of them, over the lanes of a position
+template <int G, typename T>
+__device__ __forceinline__ T best_of_range(const T* __restrict__ s, long long N, const Pair<T>* add, int from, int to, int sub) {
+    T best = below_all<T>();
+    over_range<G>(s, N, add, from, to, sub, [&](T v, int) { best = v > best ? v : best; });
+#pragma unroll
+    for (int d = 32 / G; d < 32; d <<= 1) {
+        const T other = __shfl_xor_sync(0xffffffffu, best, d);
+        best = other > best ? other : best;
+    }
+    return best;
+}
+
+// Bound: HBM, the scores read once and, for the dense form, as much written (512 x 64 x 30 x 30 float32: 236 MB, 36 us).
+//
+// G lanes share a position, neighbouring lanes are neighbouring positions; a lane has eight scores in flight and keeps a sorted list of TK.
+// With SUMS every thread adds the weights that it gives to sums of its own in shared memory, one per component, which the CTA adds up at its
+// end: the masses cost no second pass over the dense form, and come out the same on every run.
+template <typename T, int TK, int G, bool SUMS>
 __global__ void __launch_bounds__(kRouteThreads) route_choose(RouteArgs a, const T* __restrict__ scores, const T* __restrict__ prior, const T* __restrict__ bias,
-                                                              int* __restrict__ index, T* __restrict__ weights, T* __restrict__ dense,
+                                                              int* __restrict__ index, T* __restrict__ weights, T* __restrict__ dense, T* __restrict__ part_mass,
                                                               unsigned* __restrict__ part_load) {
     stream_order();
-    extern __shared__ unsigned load[];
-    for (int c = threadIdx.x; c < a.k; c += kRouteThreads) load[c] = 0;
+    constexpr int RUN = 32 / G, PLACES = kRouteThreads / G;
+    extern __shared__ __align__(16) unsigned char route_smem[];
+    T* const sums = reinterpret_cast<T*>(route_smem);                                    // [k][PLACES]
+    Pair<T>* const add_s = reinterpret_cast<Pair<T>*>(sums + (SUMS ? (size_t)a.k * PLACES : 0));
+    unsigned* const load = reinterpret_cast<unsigned*>(add_s + a.k);
+    const int lane = threadIdx.x & 31, sub = lane / RUN, place = (threadIdx.x >> 5) * RUN + lane % RUN;
+    for (int c = threadIdx.x; c < a.k; c += kRouteThreads) {
+        load[c] = 0;
+        add_s[c] = Pair<T>{prior ? prior[c] : T(0), bias ? bias[c] : T(0)};
+    }
+    if (SUMS) for (int i = threadIdx.x; i < a.k * PLACES; i += kRouteThreads) sums[i] = T(0);
     __syncthreads();
-    for (long long p = (long long)blockIdx.x * kRouteThreads + threadIdx.x; p < a.positions; p += (long long)gridDim.x * kRouteThreads) {
-        const long long n = p / a.N, j = p - n * a.N;
+    const Pair<T>* const add = prior || bias ? add_s : nullptr;
+    for (long long p0 = (long long)blockIdx.x * PLACES; p0 < a.positions; p0 += (long long)gridDim.x * PLACES) {
+        const long long p = p0 + place;
+        const bool live = p < a.positions;
+        const long long n = sample_of(a, live ? p : p0), j = (live ? p : p0) - n * a.N;
         const T* s = scores + n * a.k * a.N + j;
         unsigned long long open = ~0ull;                 // groups that are in the choice
         Top<T, TK> top;
         if (a.top_groups < a.groups) {
             top.clear();
-            for (int g = 0; g < a.groups; ++g) {
-                T best = below_all<T>();
-                for (int c = g * a.size; c < (g + 1) * a.size; ++c) {
-                    T v = s[c * a.N];
-                    if (prior) v += prior[c];
-                    if (bias) v += bias[c];
-                    best = v > best ? v : best;
-                }
-                top.offer(best, best, g, a.top_groups);
-            }
+            for (int g = 0; g < a.groups; ++g) top.offer(best_of_range<G>(s, a.N, add, g * a.size, (g + 1) * a.size, sub), g);
             open = 0;
 #pragma unroll
             for (int t = 0; t < TK; ++t) if (t < a.top_groups && top.i[t] >= 0) open |= 1ull << top.i[t];
         }
         top.clear();
-        for (int g = 0; g < a.groups; ++g) {
-            if (a.top_groups < a.groups && !(open >> g & 1)) continue;
-            for (int c = g * a.size; c < (g + 1) * a.size; ++c) {
-                T l = s[c * a.N];
-                if (prior) l += prior[c];
-                top.offer(bias ? l + bias[c] : l, l, c, a.top);
-            }
+        if (a.top_groups < a.groups) {
+            for (int g = 0; g < a.groups; ++g)
+                if (open >> g & 1) over_range<G>(s, a.N, add, g * a.size, (g + 1) * a.size, sub, [&](T v, int c) { top.offer(v, c); });
+            __syncwarp();
+        } else {
+            over_range<G>(s, a.N, add, 0, a.k, sub, [&](T v, int c) { top.offer(v, c); });
         }
-        weigh(top, a.top, a.sigmoid);
-        T* d = dense ? dense + n * a.k * a.N + j : nullptr;
-        if (d) for (int c = 0; c < a.k; ++c) d[c * a.N] = T(0);
+        top.template merge<G, RUN>();
+        // weights of the chosen: they sum to one over them
+        T l[TK], hi = below_all<T>(), sum = T(0);
 #pragma unroll
         for (int t = 0; t < TK; ++t) {
-            if (t >= a.top) continue;
-            const long long at = (n * a.top + t) * a.N + j;
-            const T w = T(a.scale) * top.l[t];
-            if (index) index[at] = top.i[t];
-            if (weights) weights[at] = w;
-            if (top.i[t] < 0) continue;
-            if (d) d[top.i[t] * a.N] = w;
-            atomicAdd(load + top.i[t], 1u);
+            l[t] = below_all<T>();
+            if (t >= a.top || top.i[t] < 0) continue;
+            l[t] = __ldg(s + top.i[t] * a.N);
+            if (add) l[t] += add[top.i[t]].prior;
+            if (a.sigmoid) l[t] = l[t] >= T(0) ? -log1p_of(exp_of(-l[t])) : l[t] - log1p_of(exp_of(l[t]));
+            hi = l[t] > hi ? l[t] : hi;
+        }
+#pragma unroll
+        for (int t = 0; t < TK; ++t) {
+            l[t] = t < a.top && top.i[t] >= 0 ? (l[t] == hi ? T(1) : exp_of(l[t] - hi)) : T(0);              // (infinities are equal too)
+            sum += l[t];
+        }
+        const T scale = T(a.scale), inv = sum > T(0) ? T(1) / sum : T(0);
+#pragma unroll
+        for (int t = 0; t < TK; ++t) l[t] = scale * (l[t] * inv);
+        if (live && dense) {
+            T* d = dense + (n * a.k + sub) * a.N + j;
+            const long long step = G * a.N;
+            if constexpr (TK <= 4) {                     // every value once
+#pragma unroll 4
+                for (int c = sub; c < a.k; c += G, d += step) {
+                    T w = T(0);
+#pragma unroll
+                    for (int t = 0; t < TK; ++t) w = t < a.top && c == top.i[t] ? l[t] : w;
+                    __stcs(d, w);
+                }
+            } else {                                     // zeros, then the chosen (each by the lane that wrote its zero)
+#pragma unroll 8
+                for (int c = sub; c < a.k; c += G, d += step) *d = T(0);
+#pragma unroll
+                for (int t = 0; t < TK; ++t)
+                    if (t < a.top && top.i[t] >= 0 && top.i[t] % G == sub) dense[(n * a.k + top.i[t]) * a.N + j] = l[t];
+            }
+        }
+        if (live && sub == 0) {
+#pragma unroll
+            for (int t = 0; t < TK; ++t) {
+                if (t >= a.top) continue;
+                const long long at = (n * a.top + t) * a.N + j;
+                if (index) index[at] = top.i[t];
+                if (weights) weights[at] = l[t];
+                if (top.i[t] < 0) continue;
+                if (SUMS) sums[top.i[t] * PLACES + place] += l[t];
+                atomicAdd(load + top.i[t], 1u);
+            }
         }
     }
     __syncthreads();
     for (int c = threadIdx.x; c < a.k; c += kRouteThreads) part_load[(size_t)blockIdx.x * a.k + c] = load[c];
+    if constexpr (SUMS)
+        for (int c = threadIdx.x >> 5; c < a.k; c += kRouteThreads / 32) {
+            T m = T(0);
+#pragma unroll
+            for (int i = 0; i < PLACES; i += 32) m += sums[c * PLACES + i + lane];
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) m += __shfl_xor_sync(0xffffffffu, m, d);
+            if (lane == 0) part_mass[(size_t)blockIdx.x * a.k + c] = m;
+        }
 }
 
-// part[split][c] = sum of the responsibilities of component c = blockIdx.x in the split's samples
+// part[split][c] = sum of the responsibilities of component c = blockIdx.x in the split's samples (for more components than shared memory has sums for)
 template <typename T>
 __global__ void __launch_bounds__(256) route_mass(RouteArgs a, long long batch, const T* __restrict__ dense, T* __restrict__ part) {
     stream_order();
@@ -180,7 +282,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_gradient(RouteArgs a, con
     stream_order();
     const T inv_scale = T(1.0 / a.scale);
     for (long long p = (long long)blockIdx.x * kRouteThreads + threadIdx.x; p < a.positions; p += (long long)gridDim.x * kRouteThreads) {
-        const long long n = p / a.N, j = p - n * a.N, chosen = n * a.top * a.N + j;
+        const long long n = sample_of(a, p), j = p - n * a.N, chosen = n * a.top * a.N + j;
         const T* s = scores + n * a.k * a.N + j;
         T* d = dscores + n * a.k * a.N + j;
         for (int c = 0; c < a.k; ++c) d[c * a.N] = T(0);
@@ -205,17 +307,41 @@ RouteArgs args_of(const simnets_route_desc& d) {
     RouteArgs a;
     a.N = d.positions;
     a.positions = d.positions * d.batch;
+    a.f_N = FastDiv{0, 0, 0};
+    if (a.positions > 0 && a.positions <= 0x7fffffffLL) a.f_N = make_fastdiv(int(a.N));
     a.k = d.components; a.top = d.top_k; a.groups = d.groups; a.size = d.components / d.groups; a.top_groups = d.top_groups;
     a.sigmoid = d.sigmoid != 0;
     a.scale = d.scale;
     return a;
 }
+// lanes per position: one where the positions fill the GPU
+int route_lanes(const simnets_route_desc& d) { return d.positions * d.batch >= 512LL * device_sm_count() || d.components < 8 ? 1 : 4; }
 int route_ctas(const simnets_route_desc& d) {
-    const long long tiles = (d.positions * d.batch + kRouteThreads - 1) / kRouteThreads;
-    return int(std::max<long long>(1, std::min<long long>(tiles, 8LL * device_sm_count())));
+    const long long places = kRouteThreads / route_lanes(d), tiles = (d.positions * d.batch + places - 1) / places, resident = 12LL * device_sm_count();
+    const long long rounds = std::max<long long>(1, (tiles + resident - 1) / resident);
+    return int(std::max<long long>(1, (tiles + rounds - 1) / rounds));
 }
-int mass_splits(const simnets_route_desc& d) { return int(std::max<long long>(1, std::min<long long>(d.batch, (8LL * device_sm_count() + d.components - 1) / d.components))); }
+// a CTA's sums fit the shared memory of a multiprocessor three times
+size_t sums_bytes(const simnets_route_desc& d) { return (d.dtype == SIMNETS_F64 ? 8 : 4) * (size_t)d.components * (kRouteThreads / route_lanes(d)); }
+bool route_sums(const simnets_route_desc& d) { return sums_bytes(d) <= 64 * 1024; }
+int mass_splits(const simnets_route_desc& d) {
+    if (route_sums(d)) return route_ctas(d);
+    return int(std::max<long long>(1, std::min<long long>(d.batch, (8LL * device_sm_count() + d.components - 1) / d.components)));
+}
 size_t load_bytes(const simnets_route_desc& d) { return (sizeof(unsigned) * (size_t)route_ctas(d) * d.components + 255) & ~size_t(255); }
+
+template <typename T, int TK, int G, bool SUMS>
+cudaError_t choose(const simnets_route_desc& d, const RouteArgs& a, const void* scores, const void* prior, const void* bias, int* index, void* weights, void* dense,
+                   T* part_mass, unsigned* part_load, cudaStream_t s) {
+    const size_t smem = (SUMS ? sums_bytes(d) : 0) + (size_t)a.k * (2 * sizeof(T) + sizeof(unsigned));
+    static SmemLimit limit;
+    if (smem > 32 * 1024) {
+        const cudaError_t e = limit.raise(route_choose<T, TK, G, SUMS>, 160 * 1024);
+        if (e != cudaSuccess) return e;
+    }
+    in_stream_order(route_choose<T, TK, G, SUMS>, route_ctas(d), kRouteThreads, smem, s)(a, (const T*)scores, (const T*)prior, (const T*)bias, index, (T*)weights, (T*)dense, part_mass, part_load);
+    return cudaSuccess;
+}
 
 template <typename T>
 cudaError_t route(const simnets_route_desc& d, const void* scores, const void* prior, const void* bias, int* index, void* weights, void* dense, long long* load,
@@ -224,12 +350,18 @@ cudaError_t route(const simnets_route_desc& d, const void* scores, const void* p
     const int ctas = route_ctas(d), splits = mass_splits(d), want = std::max(a.top, a.top_groups < a.groups ? a.top_groups : 1);
     unsigned* part_load = static_cast<unsigned*>(ws);
     T* part_mass = reinterpret_cast<T*>(static_cast<char*>(ws) + load_bytes(d));
-#define ROUTE(TK) in_stream_order(route_choose<T, TK>, ctas, kRouteThreads, sizeof(unsigned) * a.k, s)(a, (const T*)scores, (const T*)prior, (const T*)bias, index, (T*)weights, (T*)dense, part_load)
+    const bool sums = dense && route_sums(d), one = route_lanes(d) == 1;
+    cudaError_t e = cudaSuccess;
+#define ROUTE(TK) e = sums ? (one ? choose<T, TK, 1, true>(d, a, scores, prior, bias, index, weights, dense, part_mass, part_load, s)                     \
+                                  : choose<T, TK, 4, true>(d, a, scores, prior, bias, index, weights, dense, part_mass, part_load, s))                    \
+                           : (one ? choose<T, TK, 1, false>(d, a, scores, prior, bias, index, weights, dense, part_mass, part_load, s)                    \
+                                  : choose<T, TK, 4, false>(d, a, scores, prior, bias, index, weights, dense, part_mass, part_load, s))
     if (want <= 1) ROUTE(1); else if (want <= 2) ROUTE(2); else if (want <= 4) ROUTE(4); else if (want <= 8) ROUTE(8); else ROUTE(16);
 #undef ROUTE
-    if (mass) in_stream_order(route_mass<T>, dim3(a.k, splits), 256, 0, s)(a, (long long)d.batch, (const T*)dense, part_mass);
+    if (e != cudaSuccess) return e;
+    if (mass && !sums) in_stream_order(route_mass<T>, dim3(a.k, splits), 256, 0, s)(a, (long long)d.batch, (const T*)dense, part_mass);
     in_stream_order(route_totals<T>, a.k, 128, 0, s)(ctas, splits, a.k, part_load, part_mass, load, (T*)mass);
-    count_launch(mass ? 3 : 2);
+    count_launch(mass && !sums ? 3 : 2);
     return cudaGetLastError();
 }
 
