@@ -13,18 +13,23 @@
 // its two axes is summed over, so that Ex serves the first and the third product, Q the second and the third and Eo the first and the second without
 // a second copy; TF32 operands of that kind have no such layout (4-byte elements are transposed under a swizzle only), and their two planes
 // take 16 bytes a value instead of 6.  Six of the nine plane products are taken, small ones first: what an accumulator truncates is
-// 2^-24 of what it holds, which then are the largest products' K / 16 steps only.  Accumulators are emptied into FP32 registers or, the
-// offsets' sums, into the CTA's own partial sums after every 128 positions.
+// 2^-24 of what it holds, which then are the largest products' K / 16 steps only.  An instruction with 64 columns waits for its 128 rows (50
+// cycles instead of 32), so that the second and third product take the planes of their narrow operand side by side, as up to 192 columns
+// (96 cycles for three).  Accumulators are emptied into FP32 after every 128 positions.
+//
+// Sixteen warps work on the values and one issues the products: a tile's bytes are read and exponentiated while the second product of the tile
+// in front runs, its dx leaves during the third.  (All phases in turn, 512 x 64 x 32 x 32 under 128 instances: 519 us, of them 190 for
+// the bytes' way into registers.)
 //
 // Offsets whose spread is beyond what the factors hold raise the status word in the prepass; the kernel then leaves at once and the
 // kernels behind it, gated by that word, evaluate term by term.
 #include "checkpoint.cuh"
-#include "tc.cuh"
+#include "ws.cuh"
 
 namespace simnets {
 namespace {
 
-constexpr int kFuseThreads = 512, kFuseColumns = 256;
+constexpr int kFuseWorkers = 512, kFuseThreads = kFuseWorkers + 32, kFuseColumns = 512;
 
 __device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -38,15 +43,17 @@ __host__ __device__ constexpr uint32_t bf16_idesc(int nt, bool a_across, bool b_
     return (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(a_across) << 15) | (uint32_t(b_across) << 16) | (uint32_t(nt >> 3) << 17) | (uint32_t(128 >> 4) << 24);
 }
 
-// A [rows][cols] operand in three planes of [rows / 8][cols / 8] core matrices (8 rows x 8 columns, 16 bytes a row).
+// A [rows][cols] operand as [rows / 8][3 planes][cols / 8] core matrices (8 rows x 8 columns, 16 bytes a row): the planes are columns side by side.
 template <int ROWS, int COLS>
 struct Planes {
-    static constexpr uint32_t kPlane = ROWS * COLS * 2, kBytes = 3 * kPlane, kRowGroup = COLS / 8 * 128;
-    static __device__ __forceinline__ uint32_t at(int row, int col) { return uint32_t(row >> 3) * kRowGroup + uint32_t(col >> 3) * 128 + uint32_t(row & 7) * 16 + uint32_t(col & 7) * 2; }
-    // operand whose rows are the matrix's, summed over 16 columns from step on
-    static __device__ __forceinline__ uint64_t along(uint32_t base, int plane, int step) { return umma_desc(base + plane * kPlane + step * 256, 128, kRowGroup); }
-    // operand whose rows are the matrix's columns, summed over 16 rows from step on
-    static __device__ __forceinline__ uint64_t across(uint32_t base, int plane, int step) { return umma_desc(base + plane * kPlane + step * 2 * kRowGroup, kRowGroup, 128); }
+    static constexpr uint32_t kPlane = COLS / 8 * 128, kRowGroup = 3 * kPlane, kBytes = ROWS / 8 * kRowGroup;
+    static __host__ __device__ __forceinline__ constexpr uint32_t at(int row, int col) { return uint32_t(row >> 3) * kRowGroup + uint32_t(col >> 3) * 128 + uint32_t(row & 7) * 16 + uint32_t(col & 7) * 2; }
+    // operand whose rows are the matrix's, summed over 16 columns of a plane from step on, from its descriptor at (0, 0)
+    static __device__ __forceinline__ uint64_t along(uint32_t base) { return umma_desc(base, 128, kRowGroup); }
+    static __host__ __device__ constexpr uint32_t along_at(int plane, int step) { return (plane * kPlane + step * 256) >> 4; }
+    // operand whose rows are the matrix's columns from `plane` on, summed over 16 rows from step on
+    static __device__ __forceinline__ uint64_t across(uint32_t base) { return umma_desc(base, kRowGroup, 128); }
+    static __host__ __device__ constexpr uint32_t across_at(int plane, int step) { return (plane * kPlane + step * 2 * kRowGroup) >> 4; }
 };
 
 // the plane products that are taken, small ones first
@@ -88,35 +95,34 @@ __device__ __forceinline__ void store_row(unsigned char* base, int row, int col,
     }
 }
 
-// N consecutive tensor-memory columns of this thread's lane
+// N consecutive tensor-memory columns of this thread's lane; there once tmem_wait() is through
 template <int N>
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[N]) {
-    uint32_t r[N];
-    if constexpr (N == 32) {
-        tmem_ld32(taddr, r);
-    } else if constexpr (N == 16) {
+__device__ __forceinline__ void tmem_request(uint32_t taddr, uint32_t (&r)[N]) {
+    if constexpr (N == 16) {
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
                        "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
     } else if constexpr (N == 8) {
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
     } else {
         static_assert(N == 4);
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr) : "memory");
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
     }
+}
+// (the registers pass through it, so that nothing reads them earlier)
+template <int N>
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
 
 __host__ __device__ constexpr int fuse_taps(int k) { return k <= 16 ? 16 : k <= 32 ? 32 : k <= 64 ? 64 : 128; }
 __host__ __device__ constexpr int fuse_instances(int kp) { return kp <= 64 ? 128 : 64; }        // instances a step: what shared memory holds
 
-// Eo of one row of offsets (blockIdx.x = region * padded instances + instance): plain in eo[R][M][KP], split in the tiles of the main kernel;
-// zeros for what is not there.  128 threads.
+// Eo of one row of offsets (blockIdx.x = region * padded instances + instance): plain in eo[R][M][KP], split in the tiles of the main kernel.
+// Taps that are not there are zeros, instances that are not there ones (S must not be 0).  128 threads.
 __global__ void __launch_bounds__(128) fuse_prepare(MexGeo g, int KP, int MC, int Mp, const float* __restrict__ off, float* __restrict__ eo, unsigned char* __restrict__ tiles,
                                                     int* __restrict__ flag) {
     stream_order();
@@ -133,15 +139,15 @@ __global__ void __launch_bounds__(128) fuse_prepare(MexGeo g, int KP, int MC, in
     lo = fminf(fminf(red[1][0], red[1][1]), fminf(red[1][2], red[1][3]));
     const float eps = float(g.eps);
     if (in && (!(fabsf(v) < CUDART_INF_F) || !(fabsf(eps) * (hi - lo) <= kSafeSpread))) flag[0] = 1;
-    const float e = in ? ex2_ftz(eps * 1.4426950408889634f * (v - (eps > 0.f ? hi : lo))) : 0.f;
+    const float e = in ? ex2_ftz(eps * 1.4426950408889634f * (v - (eps > 0.f ? hi : lo))) : m < g.M ? 0.f : 1.f;
     if (k >= KP) return;
     if (m < g.M) eo[((size_t)r * g.M + m) * KP + k] = e;
     const int row = m % MC;
-    unsigned char* d = tiles + ((size_t)r * (Mp / MC) + m / MC) * (3 * MC * KP * 2) + (row >> 3) * (KP / 8 * 128) + (k >> 3) * 128 + (row & 7) * 16 + (k & 7) * 2;
+    unsigned char* d = tiles + ((size_t)r * (Mp / MC) + m / MC) * (3 * MC * KP * 2) + (row >> 3) * (3 * KP / 8 * 128) + (k >> 3) * 128 + (row & 7) * 16 + (k & 7) * 2;
     const Split2 s = split_bf16(e, 0.f);
     *reinterpret_cast<unsigned short*>(d) = (unsigned short)s.hi;
-    *reinterpret_cast<unsigned short*>(d + MC * KP * 2) = (unsigned short)s.mid;
-    *reinterpret_cast<unsigned short*>(d + 2 * MC * KP * 2) = (unsigned short)s.lo;
+    *reinterpret_cast<unsigned short*>(d + KP / 8 * 128) = (unsigned short)s.mid;
+    *reinterpret_cast<unsigned short*>(d + 2 * (KP / 8 * 128)) = (unsigned short)s.lo;
 }
 
 struct FuseArgs {
@@ -150,165 +156,347 @@ struct FuseArgs {
     const unsigned char* tiles;
     const float* dy;
     float* dx;              // may be null
-    float* part;            // [CTA][Mp][KP], may be null
+    float* part;            // [CTA][step] of what part_at() lays out, may be null
     int* flag;
     int shift;              // log2 of the group
     int tiles_m;            // steps of instances
+    int resident;           // all of them lie in shared memory
     long long tiles_j;      // tiles of positions of a region
+};
+
+// Place of (instance of a step, tap) in the partial sums of the step, neighbouring lanes side by side: a lane has four taps of an instance at
+// once, or, where the taps are the rows, a tap of an instance.
+__host__ __device__ constexpr int part_at(int KP, int MC, int m, int k) { return KP > 64 ? m * KP + k : ((k >> 2) * MC + m) * 4 + (k & 3); }
+
+// barriers of a CTA; every one completes once a step (a tile of positions, 64 or 128 instances)
+struct FuseShared {
+    uint64_t operands;      // workers: Ex (and Eo) of the step are there
+    uint64_t sums;          // products: S is there
+    uint64_t quotients;     // workers: Q is there, S has been read
+    uint64_t taps;          // products: the sums over the instances are there
+    uint64_t instances;     // products: the sums over the positions are there, and Ex and Q may be written anew
+    uint32_t tmem;
+    volatile int failed;
+};
+
+// An operand: its descriptor and where its planes and steps lie from there.  (The products are issued by one thread; what it computes between two of
+// them is what the tensor cores wait for: an addition to the address field here, 100 cycles an instruction with descriptors made anew.)
+template <class P, bool ACROSS>
+struct Operand {
+    uint64_t desc;
+    __device__ __forceinline__ explicit Operand(uint32_t base) : desc(ACROSS ? P::across(base) : P::along(base)) {}
+    __device__ __forceinline__ uint64_t operator()(int plane, int step) const { return desc + (ACROSS ? P::across_at(plane, step) : P::along_at(plane, step)); }
+    static constexpr bool kAcross = ACROSS;
+};
+__device__ __forceinline__ bool elected() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
+}
+
+// D[128 x N] (+)= sum over STEPS x 16 of A B with B's planes side by side: (2,0), (1,0) + (1,1), (0,0) + (0,1) + (0,2), the sums of B's plane j in
+// the j-th N columns.  a(plane, step), b(plane, step): operands.  (A first step that starts some columns and adds to others is two instructions.)
+template <int N, int STEPS, class A, class B>
+__device__ __forceinline__ void issue_side_by_side(uint32_t tmem, A a, B b) {
+    constexpr uint32_t one = bf16_idesc(N, A::kAcross, B::kAcross), two = bf16_idesc(2 * N, A::kAcross, B::kAcross), three = bf16_idesc(3 * N, A::kAcross, B::kAcross);
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) umma_bf16(tmem, a(2, s), b(0, s), one, s != 0);
+    umma_bf16(tmem, a(1, 0), b(0, 0), one, 1);
+    umma_bf16(tmem + N, a(1, 0), b(1, 0), one, 0);
+#pragma unroll
+    for (int s = 1; s < STEPS; ++s) umma_bf16(tmem, a(1, s), b(0, s), two, 1);
+    umma_bf16(tmem, a(0, 0), b(0, 0), two, 1);
+    umma_bf16(tmem + 2 * N, a(0, 0), b(2, 0), one, 0);
+#pragma unroll
+    for (int s = 1; s < STEPS; ++s) umma_bf16(tmem, a(0, s), b(0, s), three, 1);
+}
+// the same one plane product after the other, all into the same N columns
+template <int N, int STEPS, class A, class B>
+__device__ __forceinline__ void issue_in_turn(uint32_t tmem, A a, B b) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i)
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) umma_bf16(tmem, a(plane_a(i), s), b(plane_b(i), s), bf16_idesc(N, A::kAcross, B::kAcross), (i | s) != 0);
+}
+
+// sum of BLOCKS blocks of columns, STEP apart
+template <int N, int BLOCKS, int STEP>
+__device__ __forceinline__ void tmem_sum(uint32_t taddr, float (&v)[N]) {
+    uint32_t r[BLOCKS][N];
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) tmem_request<N>(taddr + b * STEP, r[b]);
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) tmem_wait<N>(r[b]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        v[i] = __uint_as_float(r[0][i]);
+#pragma unroll
+        for (int b = 1; b < BLOCKS; ++b) v[i] += __uint_as_float(r[b][i]);
+    }
+}
+__device__ __forceinline__ float reciprocal(float v) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+
+template <int KP>
+struct Fuse {
+    static constexpr int MC = fuse_instances(KP), KR = KP / 4, MR = MC / 4;     // a worker's taps and instances
+    static constexpr bool kByTaps = KP > 64;             // the offsets' sums with the taps as rows (128 of them), else with the instances
+    using X = Planes<128, KP>;
+    using Q = Planes<128, MC>;
+    using E = Planes<MC, KP>;
+    // tensor memory: S, the sums over the instances (128 taps: one block of columns, three do not fit), the offsets' sums
+    static constexpr int kTapBlocks = KP > 64 ? 1 : 3, kT = MC, kU = kT + kTapBlocks * KP;
+    static constexpr int kUBlock = kByTaps ? MC : KP;
+    static_assert(kU + 3 * kUBlock <= kFuseColumns);
 };
 
 template <int KP>
 __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(MexGeo g, FuseArgs a) {
     stream_order();
-    constexpr int MC = fuse_instances(KP), KR = KP / 4, MR = MC / 4;
-    constexpr bool kByTaps = KP > 64;                    // the offsets' sums with the taps as rows (128 of them), else with the instances
-    using X = Planes<128, KP>;
-    using Q = Planes<128, MC>;
-    using E = Planes<MC, KP>;
+    using F = Fuse<KP>;
+    using X = typename F::X;
+    using Q = typename F::Q;
+    using E = typename F::E;
+    constexpr int MC = F::MC, KR = F::KR, MR = F::MR;
     extern __shared__ __align__(1024) unsigned char sm[];
-    __shared__ TcShared sh;
-    __shared__ float red[4][128];
+    __shared__ FuseShared sh;
+    __shared__ float red[2][4][128];
     __shared__ int tap_off[KP];
     if (a.flag[0]) return;
     unsigned char *const sx = sm, *const sq = sm + X::kBytes, *const se = sq + Q::kBytes;
-    const int p = threadIdx.x & 127, part4 = threadIdx.x >> 7;                          // position (tensor-memory lane) and its quarter of the columns
-    const uint32_t lane_base = uint32_t((threadIdx.x >> 5) & 3) << 21;                   // (32 lanes a warp, lane number in bits 16 and up)
+    const int warp = threadIdx.x >> 5;
     const int r = int(blockIdx.x) % g.R, slot = int(blockIdx.x) / g.R, slots = int(gridDim.x) / g.R;
-    const int Mp = a.tiles_m * MC;
     for (int k = threadIdx.x; k < KP; k += kFuseThreads) {
         const Tap t = tap_of<false>(g, k < g.K ? k : 0);
         tap_off[k] = (t.c * g.H + t.h) * g.W + t.w;
     }
-    const uint32_t tmem = tc_begin(sh, kFuseColumns);                                   // (its barrier also publishes tap_off)
-    const uint32_t tS = tmem, tT = tmem + MC, tU = tT + KP;
-    const float eps = float(g.eps), a2 = eps * 1.4426950408889634f;
-    const long long P = (long long)g.B * g.rs;
+    if (threadIdx.x == 0) {
+        mbar_init(&sh.operands, kFuseWorkers); mbar_init(&sh.quotients, kFuseWorkers);
+        mbar_init(&sh.sums, 1); mbar_init(&sh.taps, 1); mbar_init(&sh.instances, 1);
+        sh.failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kFuseWorkers / 32) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(uint32_t(kFuseColumns)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = sh.tmem;
+    const uint32_t tS = tmem, tT = tmem + F::kT, tU = tmem + F::kU;
     const uint32_t xb = smem_u32(sx), qb = smem_u32(sq), eb = smem_u32(se);
-    bool ok = true;
-    uint32_t phase = 0;                                                                  // of both barriers
-
-    auto load_offsets = [&](int mt) {
-        const unsigned char* src = a.tiles + ((size_t)r * a.tiles_m + mt) * E::kBytes;
-        for (int i = threadIdx.x; i < int(E::kBytes / 16); i += kFuseThreads) cp_async16(reinterpret_cast<float*>(se + i * 16), reinterpret_cast<const float*>(src + i * 16), 16);
+    uint32_t phase = 0;
+    // A wait that runs out sets `failed`; from then on nobody waits and no product is issued, and all leave by the ordinary way.
+    auto wait = [&](uint64_t* bar) {
+        if (!sh.failed && !mbar_wait(bar, phase)) sh.failed = 1;
+        __syncwarp();                                                                    // (what follows is done by whole warps)
     };
-    if (a.tiles_m == 1) load_offsets(0);
 
-    for (long long jt = slot; jt < a.tiles_j && ok; jt += slots) {
-        const Column col = column_of(g, r, jt * 128 + p, P, nullptr);
-        const bool live = col.base >= 0;
-        const long long xi = (((long long)col.n * g.C + col.c0) * g.H + col.h0) * g.W + col.w0;
-        // this thread's taps: part4 * KR .. + KR
-        float ex[KR], tsum[KR];
-        {
-            uint32_t code[KR];
+    if (warp == kFuseWorkers / 32) {
+        const Operand<X, false> x_along(xb);
+        const Operand<X, true> x_across(xb);
+        const Operand<Q, false> q_along(qb);
+        const Operand<Q, true> q_across(qb);
+        for (long long jt = slot; jt < a.tiles_j; jt += slots)
+            for (int mt = 0; mt < a.tiles_m; ++mt, phase ^= 1u) {
+                const uint32_t et = eb + (a.resident ? mt * E::kBytes : 0u);
+                wait(&sh.operands);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const Operand<E, false> e_along(et);
+                const Operand<E, true> e_across(et);
+                if (!sh.failed && elected()) {
+                    issue_in_turn<MC, KP / 16>(tS, x_along, e_along);
+                    umma_commit(&sh.sums);
+                }
+                __syncwarp();
+                wait(&sh.quotients);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (!sh.failed && elected()) {
+                    if (a.dx) {
+                        if constexpr (F::kTapBlocks == 3) issue_side_by_side<KP, MC / 16>(tT, q_along, e_across);
+                        else issue_in_turn<KP, MC / 16>(tT, q_along, e_across);
+                    }
+                    umma_commit(&sh.taps);
+                    if (a.part) {
+                        if constexpr (F::kByTaps) issue_side_by_side<MC, 8>(tU, x_across, q_across);
+                        else issue_side_by_side<KP, 8>(tU, q_across, x_across);
+                    }
+                    umma_commit(&sh.instances);
+                }
+                __syncwarp();
+            }
+    } else {
+        const int p = threadIdx.x & 127, part4 = threadIdx.x >> 7;                      // position (tensor-memory lane) and its quarter of the columns
+        const uint32_t lane_base = uint32_t(warp & 3) << 21;                             // (32 lanes a warp, lane number in bits 16 and up)
+        const int Mp = a.tiles_m * MC, k0 = part4 * KR;
+        const float eps = float(g.eps), a2 = eps * 1.4426950408889634f;
+        const long long P = (long long)g.B * g.rs;
+        auto load_offsets = [&](int mt, unsigned char* to) {
+            const unsigned char* src = a.tiles + ((size_t)r * a.tiles_m + mt) * E::kBytes;
+            for (int i = threadIdx.x; i < int(E::kBytes / 16); i += kFuseWorkers) cp_async16(reinterpret_cast<float*>(to + i * 16), reinterpret_cast<const float*>(src + i * 16), 16);
+        };
+        // where a position lies: first tap in the input, first instance in dy (one that is not there: the first of all, and not live)
+        struct Place { long long x, dy; bool live; };
+        auto place_of = [&](long long jt) {
+            const Column col = column_of(g, r, jt * 128 + p, P, nullptr);
+            Place at = {0, 0, col.base >= 0};
+            if (at.live) { at.x = (((long long)col.n * g.C + col.c0) * g.H + col.h0) * g.W + col.w0; at.dy = col.gbase; }
+            return at;
+        };
+        int turn = 0;
+        // Ex of this worker's taps (k0 .. + KR) of its position.  Taps that are not there read the first one's value and count 0; a position that is
+        // not there has a 1 in its first tap, so that its S is no 0.
+        auto decode = [&](const Place& at, float (&ex)[KR]) {
+            constexpr int H = KR < 16 ? KR : 16;
+            const unsigned char* const codes = a.codes + at.x;
+            const float2* const ranges = a.ranges + (at.x >> a.shift);
+            const int rest = int(at.x) & ((1 << a.shift) - 1);
             float mx = eps > 0.f ? -CUDART_INF_F : CUDART_INF_F;
 #pragma unroll
-            for (int i = 0; i < KR; ++i) code[i] = live && part4 * KR + i < g.K ? a.codes[xi + tap_off[part4 * KR + i]] : 0u;
+            for (int i0 = 0; i0 < KR; i0 += H) {
+                uint32_t code[H], top = 0;
+                float2 range[H];
 #pragma unroll
-            for (int i = 0; i < KR; ++i) {
-                const bool in = live && part4 * KR + i < g.K;
-                const float2 range = in ? __ldg(a.ranges + ((xi + tap_off[part4 * KR + i]) >> a.shift)) : make_float2(0.f, 0.f);
-                ex[i] = unpacked<float>(code[i], range.x, range.y);
-                if (in) mx = eps > 0.f ? fmaxf(mx, ex[i]) : fminf(mx, ex[i]);
-            }
-            red[part4][p] = mx;
-            __syncthreads();
-            mx = eps > 0.f ? fmaxf(fmaxf(red[0][p], red[1][p]), fmaxf(red[2][p], red[3][p])) : fminf(fminf(red[0][p], red[1][p]), fminf(red[2][p], red[3][p]));
+                for (int i = 0; i < H; ++i) {
+                    const int tap = tap_off[k0 + i0 + i];
+                    code[i] = __ldg(codes + tap);
+                    range[i] = __ldg(ranges + ((unsigned(rest) + unsigned(tap)) >> a.shift));
+                }
 #pragma unroll
-            for (int i = 0; i < KR; ++i) {
-                ex[i] = live && part4 * KR + i < g.K ? ex2_ftz(a2 * (ex[i] - mx)) : 0.f;
-                tsum[i] = 0.f;
+                for (int i = 0; i < H; ++i) top = max(top, code[i]);
+                if (__any_sync(0xffffffffu, top > 252u)) {
+#pragma unroll
+                    for (int i = 0; i < H; ++i) ex[i0 + i] = unpacked<float>(code[i], range[i].x, range[i].y);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < H; ++i) ex[i0 + i] = Limits<float>::at(float(code[i]), range[i].y, range[i].x);
+                }
+#pragma unroll
+                for (int i = 0; i < H; ++i) mx = eps > 0.f ? fmaxf(mx, ex[i0 + i]) : fminf(mx, ex[i0 + i]);
             }
-        }
-        store_row<X>(sx, p, part4 * KR, ex);
-        const float* dyp = a.dy + (live ? col.gbase : 0);
-        for (int mt = 0; mt < a.tiles_m; ++mt) {                                          // (`ok` is one value for all threads behind every barrier)
-            if (a.tiles_m > 1) load_offsets(mt);
-            cp_async_wait_all();
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            ok = __syncthreads_and(ok);
-            if (threadIdx.x == 0 && ok) {
+            red[turn][part4][p] = mx;                                                    // (two turns: nobody still reads this one's)
+            asm volatile("bar.sync 1, %0;" ::"n"(kFuseWorkers) : "memory");
+            const float m0 = red[turn][0][p], m1 = red[turn][1][p], m2 = red[turn][2][p], m3 = red[turn][3][p];
+            turn ^= 1;
+            mx = eps > 0.f ? fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) : fminf(fminf(m0, m1), fminf(m2, m3));
+#pragma unroll
+            for (int i = 0; i < KR; ++i) ex[i] = ex2_ftz(a2 * (ex[i] - mx));
+            if (k0 + KR > g.K)
+#pragma unroll
+                for (int i = 0; i < KR; ++i) ex[i] = k0 + i < g.K ? ex[i] : 0.f;
+            if (!at.live)
+#pragma unroll
+                for (int i = 0; i < KR; ++i) ex[i] = k0 + i == 0 ? 1.f : 0.f;
+        };
+        if (a.resident) for (int mt = 0; mt < a.tiles_m; ++mt) load_offsets(mt, se + mt * E::kBytes);
+        Place at = place_of(slot);
+        float ex[KR];
+        decode(at, ex);
+        for (long long jt = slot; jt < a.tiles_j; jt += slots) {
+            store_row<X>(sx, p, k0, ex);
+            float tsum[KR];
+#pragma unroll
+            for (int i = 0; i < KR; ++i) tsum[i] = 0.f;
+            const bool last_tile = jt + slots >= a.tiles_j;
+            Place next = {0, 0, false};
+            for (int mt = 0; mt < a.tiles_m; ++mt, phase ^= 1u) {
+                if (!a.resident) load_offsets(mt, se);
+                cp_async_wait_all();
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                mbar_arrive(&sh.operands);
+                // this worker's instances: m0 .. + MR
+                const int m0 = mt * MC + part4 * MR;
+                const bool live = at.live;
+                const float* dyp = a.dy + at.dy + (long long)m0 * g.Ng;
+                float q[MR];
+                if (m0 + MR <= g.M)
+#pragma unroll
+                    for (int i = 0; i < MR; ++i, dyp += g.Ng) q[i] = live ? __ldcs(dyp) : 0.f;
+                else
+#pragma unroll
+                    for (int i = 0; i < MR; ++i, dyp += g.Ng) q[i] = live && m0 + i < g.M ? __ldcs(dyp) : 0.f;
+                wait(&sh.sums);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-                for (int i = 0; i < 6; ++i)
+                for (int i0 = 0; i0 < MR; i0 += 16) {
+                    float s[16];
+                    tmem_sum<16, 1, 0>(tS + lane_base + part4 * MR + i0, s);
 #pragma unroll
-                    for (int s = 0; s < KP / 16; ++s) umma_bf16(tS, X::along(xb, plane_a(i), s), E::along(eb, plane_b(i), s), bf16_idesc(MC, false, false), (i | s) != 0);
-                umma_commit(&sh.bar_free[0]);
-            }
-            // this thread's instances: m0 .. + MR
-            const int m0 = mt * MC + part4 * MR;
-            float q[MR];
-#pragma unroll
-            for (int i = 0; i < MR; ++i) q[i] = live && m0 + i < g.M ? __ldcs(dyp + (long long)(m0 + i) * g.Ng) : 0.f;
-            if (ok) ok = mbar_wait(&sh.bar_free[0], phase);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            {
-                float s[MR];
-                tmem_ld<MR>(tS + lane_base + part4 * MR, s);
-#pragma unroll
-                for (int i = 0; i < MR; ++i) q[i] = live && m0 + i < g.M ? __fdividef(q[i], s[i]) : 0.f;
-            }
-            store_row<Q>(sq, p, part4 * MR, q);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            ok = __syncthreads_and(ok);
-            if (threadIdx.x == 0 && ok) {
+                    for (int i = 0; i < 16; ++i) s[i] = q[i0 + i] * reciprocal(s[i]);
+                    store_row<Q>(sq, p, part4 * MR + i0, s);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                mbar_arrive(&sh.quotients);
+                const bool last = mt + 1 == a.tiles_m;
+                if (last && !last_tile) {                                                // (while the second product runs)
+                    next = place_of(jt + slots);
+                    decode(next, ex);
+                }
+                wait(&sh.taps);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (a.dx)
+                if (a.dx) {
+                    constexpr int H = KR < 16 ? KR : 16;
 #pragma unroll
-                    for (int i = 0; i < 6; ++i)
+                    for (int i0 = 0; i0 < KR; i0 += H) {
+                        float t[H];
+                        tmem_sum<H, F::kTapBlocks, KP>(tT + lane_base + k0 + i0, t);
 #pragma unroll
-                        for (int s = 0; s < MC / 16; ++s) umma_bf16(tT, Q::along(qb, plane_a(i), s), E::across(eb, plane_b(i), s), bf16_idesc(KP, false, true), (i | s) != 0);
-                if (a.part)
+                        for (int i = 0; i < H; ++i) tsum[i0 + i] += t[i];
+                    }
+                    if (last && live) {                                                  // (while the third runs) Ex from its planes, which add up to it
 #pragma unroll
-                    for (int i = 0; i < 6; ++i)
+                        for (int i = 0; i < KR; i += 2) {
+                            uint32_t w[3];
 #pragma unroll
-                        for (int s = 0; s < 8; ++s) {
-                            if (kByTaps) umma_bf16(tU, X::across(xb, plane_a(i), s), Q::across(qb, plane_b(i), s), bf16_idesc(MC, true, true), (i | s) != 0);
-                            else umma_bf16(tU, Q::across(qb, plane_a(i), s), X::across(xb, plane_b(i), s), bf16_idesc(KP, true, true), (i | s) != 0);
+                            for (int b = 0; b < 3; ++b) w[b] = *reinterpret_cast<const uint32_t*>(sx + X::at(p, k0 + i) + b * X::kPlane);
+                            const float e0 = (__uint_as_float(w[0] << 16) + __uint_as_float(w[1] << 16)) + __uint_as_float(w[2] << 16);
+                            const float e1 = (__uint_as_float(w[0] & 0xffff0000u) + __uint_as_float(w[1] & 0xffff0000u)) + __uint_as_float(w[2] & 0xffff0000u);
+                            if (k0 + i < g.K) a.dx[at.x + tap_off[k0 + i]] = e0 * tsum[i];
+                            if (k0 + i + 1 < g.K) a.dx[at.x + tap_off[k0 + i + 1]] = e1 * tsum[i + 1];
                         }
-                umma_commit(&sh.bar_free[1]);
-            }
-            if (ok) ok = mbar_wait(&sh.bar_free[1], phase);
-            phase ^= 1u;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (a.dx) {
-                float t[KR];
-                tmem_ld<KR>(tT + lane_base + part4 * KR, t);
-#pragma unroll
-                for (int i = 0; i < KR; ++i) tsum[i] += t[i];
-            }
-            if (a.part) {
+                    }
+                }
                 const bool first = jt == slot;
-                if constexpr (kByTaps) {                                                 // row = tap p, columns = instances
-                    float u[MR];
-                    tmem_ld<MR>(tU + lane_base + part4 * MR, u);
-                    float* d = a.part + ((size_t)blockIdx.x * Mp + mt * MC + part4 * MR) * KP + p;
+                if constexpr (F::kByTaps) {                                              // row = tap p, columns = instances
+                    float* d = a.part ? a.part + ((size_t)blockIdx.x * Mp + m0) * KP + p : nullptr;
+                    float old[MR];
 #pragma unroll
-                    for (int i = 0; i < MR; ++i) d[i * KP] = first ? u[i] : d[i * KP] + u[i];
+                    for (int i = 0; i < MR; ++i) old[i] = d && !first ? d[i * KP] : 0.f;
+                    wait(&sh.instances);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (d) {
+                        float u[MR];
+                        tmem_sum<MR, 3, MC>(tU + lane_base + part4 * MR, u);
+#pragma unroll
+                        for (int i = 0; i < MR; ++i) d[i * KP] = old[i] + u[i];
+                    }
                 } else {                                                                 // row = instance p, columns = taps
-                    float u[KR];
-                    tmem_ld<KR>(tU + lane_base + part4 * KR, u);
-                    float4* d = reinterpret_cast<float4*>(a.part + ((size_t)blockIdx.x * Mp + mt * MC + p) * KP + part4 * KR);
+                    float4* d = a.part ? reinterpret_cast<float4*>(a.part + ((size_t)blockIdx.x * Mp + mt * MC) * KP) + (k0 / 4) * MC + p : nullptr;
+                    float4 old[KR / 4];
 #pragma unroll
-                    for (int i = 0; i < KR / 4; ++i) {
-                        const float4 old = first ? make_float4(0.f, 0.f, 0.f, 0.f) : d[i];
-                        d[i] = make_float4(old.x + u[4 * i], old.y + u[4 * i + 1], old.z + u[4 * i + 2], old.w + u[4 * i + 3]);
+                    for (int i = 0; i < KR / 4; ++i) old[i] = d && !first ? d[i * MC] : make_float4(0.f, 0.f, 0.f, 0.f);
+                    wait(&sh.instances);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (d) {
+                        float u[KR];
+                        tmem_sum<KR, 3, KP>(tU + lane_base + k0, u);
+#pragma unroll
+                        for (int i = 0; i < KR / 4; ++i)
+                            d[i * MC] = make_float4(old[i].x + u[4 * i], old[i].y + u[4 * i + 1], old[i].z + u[4 * i + 2], old[i].w + u[4 * i + 3]);
                     }
                 }
             }
+            at = next;
         }
-        if (a.dx && live)
-#pragma unroll
-            for (int i = 0; i < KR; ++i)
-                if (part4 * KR + i < g.K) a.dx[xi + tap_off[part4 * KR + i]] = ex[i] * tsum[i];
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        ok = __syncthreads_and(ok);                                                      // (and Ex may be written anew)
+        cp_async_wait_all();
     }
-    if (!ok && threadIdx.x == 0) atomicExch(&a.flag[0], 1);                              // a wait expired: the kernels behind redo the call
-    cp_async_wait_all();
-    tc_end(tmem, kFuseColumns);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == kFuseWorkers / 32)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(uint32_t(kFuseColumns)) : "memory");
+    if (sh.failed && threadIdx.x == 0) atomicExch(&a.flag[0], 1);                        // a wait ran out: the kernels behind redo the call
 }
 
 // doff of one row (blockIdx.x = region * M + instance) from the CTAs' sums, in their order.  128 threads.
@@ -334,7 +522,7 @@ __device__ __forceinline__ float raw_gradient(const float* __restrict__ row, int
     const float sum = row_sum(e, red), total = row_sum(d, red);
     return d - e / sum * total;
 }
-__global__ void __launch_bounds__(128) fuse_offsets_sum(MexGeo g, int KP, int Mp, int ctas, int normalized, int accumulate, const float* __restrict__ off,
+__global__ void __launch_bounds__(128) fuse_offsets_sum(MexGeo g, int KP, int MC, int Mp, int ctas, int normalized, int accumulate, const float* __restrict__ off,
                                                         const float* __restrict__ eo, const float* __restrict__ part, float* __restrict__ doff, const int* __restrict__ flag) {
     stream_order();
     if (flag[0]) return;
@@ -342,7 +530,7 @@ __global__ void __launch_bounds__(128) fuse_offsets_sum(MexGeo g, int KP, int Mp
     const int r = blockIdx.x / g.M, m = blockIdx.x % g.M, k = threadIdx.x;
     float d = 0.f;
     if (k < g.K) {
-        const float* s = part + ((size_t)r * Mp + m) * KP + k;
+        const float* s = part + ((size_t)r * Mp + m / MC * MC) * KP + part_at(KP, MC, m % MC, k);
         const size_t step = (size_t)g.R * Mp * KP;
         float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
         int c = r;
@@ -497,12 +685,21 @@ FuseWs fuse_carve(const MexGeo& g, void* base) {
     return w;
 }
 
+constexpr int kFuseShared = 220 * 1024;     // (of 227 KB; the barriers, the extremes and the tap offsets are some 5)
+
+// steps of instances whose Eo stays in shared memory beside Ex and Q
+int fuse_resident(int KP) {
+    const int MC = fuse_instances(KP);
+    return (kFuseShared - 128 * (KP + MC) * 6) / (MC * KP * 6);
+}
+
 template <int KP>
 cudaError_t launch_fused(const MexGeo& g, const FuseArgs& a, int ctas, cudaStream_t s) {
-    constexpr int MC = fuse_instances(KP), smem = Planes<128, KP>::kBytes + Planes<128, MC>::kBytes + Planes<MC, KP>::kBytes;
     static SmemLimit limit;
-    const cudaError_t e = limit.raise(mex_gradients_at_checkpoint<KP>, smem);
+    const cudaError_t e = limit.raise(mex_gradients_at_checkpoint<KP>, kFuseShared);
     if (e != cudaSuccess) return e;
+    using F = Fuse<KP>;
+    const size_t smem = F::X::kBytes + F::Q::kBytes + (size_t)F::E::kBytes * (a.resident ? a.tiles_m : 1);
     in_stream_order(mex_gradients_at_checkpoint<KP>, ctas, kFuseThreads, smem, s)(g, a);
     return cudaSuccess;
 }
@@ -530,6 +727,7 @@ cudaError_t launch_mex_checkpoint(const MexGeo& g, int group, const void* codes,
     a.shift = 5;
     while ((1 << a.shift) < group) ++a.shift;
     a.tiles_m = z.Mp / z.MC;
+    a.resident = a.tiles_m <= fuse_resident(z.KP);
     a.tiles_j = ((long long)g.B * g.rs + 127) / 128;
     cudaError_t e = launch_zero_words(w.flag, 2, s);
     if (e != cudaSuccess) return e;
@@ -539,7 +737,7 @@ cudaError_t launch_mex_checkpoint(const MexGeo& g, int group, const void* codes,
     if (e != cudaSuccess) return e;
     count_launch(2);
     if (doff) {
-        in_stream_order(fuse_offsets_sum, g.R * g.M, 128, 0, s)(g, z.KP, z.Mp, ctas, int(normalized), int(accumulate), off, w.eo, w.part, doff, w.flag);
+        in_stream_order(fuse_offsets_sum, g.R * g.M, 128, 0, s)(g, z.KP, z.MC, z.Mp, ctas, int(normalized), int(accumulate), off, w.eo, w.part, doff, w.flag);
         in_stream_order(fuse_redo_doff, std::min(g.R * g.M, 4 * device_sm_count()), 256, 0, s)(g, a, int(normalized), int(accumulate), off, doff);
         count_launch(2);
     }
