@@ -21,8 +21,8 @@
 // in front runs, its dx leaves during the third.  (All phases in turn, 512 x 64 x 32 x 32 under 128 instances: 519 us, of them 190 for
 // the bytes' way into registers.)
 //
-// Offsets whose spread is beyond what the factors hold raise the status word in the prepass; the kernel then leaves at once and the
-// kernels behind it, gated by that word, evaluate term by term.
+// Offsets whose spread is beyond what the factors hold are found in the prepass; the kernel then leaves at once and the one behind it, which
+// else adds up the partial sums, evaluates term by term.
 #include "checkpoint.cuh"
 #include "ws.cuh"
 
@@ -124,7 +124,7 @@ __host__ __device__ constexpr int fuse_instances(int kp) { return kp <= 64 ? 128
 // Eo of one row of offsets (blockIdx.x = region * padded instances + instance): plain in eo[R][M][KP], split in the tiles of the main kernel.
 // Taps that are not there are zeros, instances that are not there ones (S must not be 0).  128 threads.
 __global__ void __launch_bounds__(128) fuse_prepare(MexGeo g, int KP, int MC, int Mp, const float* __restrict__ off, float* __restrict__ eo, unsigned char* __restrict__ tiles,
-                                                    int* __restrict__ flag) {
+                                                    int* __restrict__ status) {
     stream_order();
     __shared__ float red[2][4];
     const int r = blockIdx.x / Mp, m = blockIdx.x % Mp, k = threadIdx.x, lane = k & 31, warp = k >> 5;
@@ -138,7 +138,10 @@ __global__ void __launch_bounds__(128) fuse_prepare(MexGeo g, int KP, int MC, in
     hi = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
     lo = fminf(fminf(red[1][0], red[1][1]), fminf(red[1][2], red[1][3]));
     const float eps = float(g.eps);
-    if (in && (!(fabsf(v) < CUDART_INF_F) || !(fabsf(eps) * (hi - lo) <= kSafeSpread))) flag[0] = 1;
+    // (the extremes leave a NaN out)
+    const int unsafe = __syncthreads_or(in && (!(fabsf(v) < CUDART_INF_F) || !(fabsf(eps) * (hi - lo) <= kSafeSpread)));
+    if (k == 0) status[1 + blockIdx.x] = unsafe;
+    if (k == 0 && blockIdx.x == 0) status[0] = 0;
     const float e = in ? ex2_ftz(eps * 1.4426950408889634f * (v - (eps > 0.f ? hi : lo))) : m < g.M ? 0.f : 1.f;
     if (k >= KP) return;
     if (m < g.M) eo[((size_t)r * g.M + m) * KP + k] = e;
@@ -157,12 +160,20 @@ struct FuseArgs {
     const float* dy;
     float* dx;              // may be null
     float* part;            // [CTA][step] of what part_at() lays out, may be null
-    int* flag;
+    int* status;            // a wait ran out; then, per row of offsets, whether its spread is beyond what the factors hold
+    int rows;               // R Mp of those
     int shift;              // log2 of the group
     int tiles_m;            // steps of instances
     int resident;           // all of them lie in shared memory
     long long tiles_j;      // tiles of positions of a region
 };
+
+// Whether the products have not been, or cannot be, taken (all threads of a CTA ask).
+__device__ __forceinline__ bool term_by_term(const FuseArgs& a) {
+    int any = 0;
+    for (int i = threadIdx.x; i <= a.rows; i += blockDim.x) any |= a.status[i];
+    return __syncthreads_or(any) != 0;
+}
 
 // Place of (instance of a step, tap) in the partial sums of the step, neighbouring lanes side by side: a lane has four taps of an instance at
 // once, or, where the taps are the rows, a tap of an instance.
@@ -261,7 +272,7 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
     __shared__ FuseShared sh;
     __shared__ float red[2][4][128];
     __shared__ int tap_off[KP];
-    if (a.flag[0]) return;
+    if (term_by_term(a)) return;
     unsigned char *const sx = sm, *const sq = sm + X::kBytes, *const se = sq + Q::kBytes;
     const int warp = threadIdx.x >> 5;
     const int r = int(blockIdx.x) % g.R, slot = int(blockIdx.x) / g.R, slots = int(gridDim.x) / g.R;
@@ -496,54 +507,47 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
     __syncthreads();
     if (warp == kFuseWorkers / 32)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(uint32_t(kFuseColumns)) : "memory");
-    if (sh.failed && threadIdx.x == 0) atomicExch(&a.flag[0], 1);                        // a wait ran out: the kernels behind redo the call
+    if (sh.failed && threadIdx.x == 0) atomicExch(&a.status[0], 1);                      // a wait ran out: the kernel behind redoes the call
 }
 
-// doff of one row (blockIdx.x = region * M + instance) from the CTAs' sums, in their order.  128 threads.
-__device__ __forceinline__ float row_sum(float v, float (&red)[4]) {
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    return (red[0] + red[1]) + (red[2] + red[3]);
-}
-// what a raw row's normalisation does to its gradient: d - softmax(row) sum(d)
-__device__ __forceinline__ float raw_gradient(const float* __restrict__ row, int K, float d, float (&red)[4]) {
+// ---- the offsets' gradient from the CTAs' sums, or, for offsets that no factorisation takes, everything term by term ------------------
+struct FinishArgs {
+    const float *off, *eo;
+    float* doff;            // may be null
+    int KP, MC, Mp, ctas;
+    int normalized, accumulate;
+};
+constexpr int kFinishThreads = 256;
+
+// doff of one row from d, its gradient with respect to the row as the op sees it (thread k has tap k): of a raw row d - softmax(row) sum(d).
+// All threads of the CTA call it; `work`: three arrays of 128.
+__device__ __forceinline__ void finish_row(const MexGeo& g, const FinishArgs& f, int row, float d, float (*work)[128]) {
     const int k = threadIdx.x;
-    float hi = k < K ? row[k] : -CUDART_INF_F;
+    const float* o = f.off + (size_t)row * g.K;
+    if (f.normalized) {
+        __syncthreads();
+        if (k < 128) { work[0][k] = k < g.K ? o[k] : -CUDART_INF_F; work[1][k] = k < g.K ? d : 0.f; }
+        __syncthreads();
+        if (k < 32) {
+            float hi = fmaxf(fmaxf(work[0][k], work[0][k + 32]), fmaxf(work[0][k + 64], work[0][k + 96]));
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, s));
-    __syncthreads();
-    if ((k & 31) == 0) red[k >> 5] = hi;
-    __syncthreads();
-    hi = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float e = k < K ? expf(row[k] - hi) : 0.f;
-    const float sum = row_sum(e, red), total = row_sum(d, red);
-    return d - e / sum * total;
-}
-__global__ void __launch_bounds__(128) fuse_offsets_sum(MexGeo g, int KP, int MC, int Mp, int ctas, int normalized, int accumulate, const float* __restrict__ off,
-                                                        const float* __restrict__ eo, const float* __restrict__ part, float* __restrict__ doff, const int* __restrict__ flag) {
-    stream_order();
-    if (flag[0]) return;
-    __shared__ float red[4];
-    const int r = blockIdx.x / g.M, m = blockIdx.x % g.M, k = threadIdx.x;
-    float d = 0.f;
-    if (k < g.K) {
-        const float* s = part + ((size_t)r * Mp + m / MC * MC) * KP + part_at(KP, MC, m % MC, k);
-        const size_t step = (size_t)g.R * Mp * KP;
-        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-        int c = r;
-        for (; c + 3 * g.R < ctas; c += 4 * g.R, s += 4 * step) { s0 += s[0]; s1 += s[step]; s2 += s[2 * step]; s3 += s[3 * step]; }
-        for (; c < ctas; c += g.R, s += step) s0 += s[0];
-        d = eo[((size_t)r * g.M + m) * KP + k] * ((s0 + s1) + (s2 + s3));
+            for (int s = 16; s > 0; s >>= 1) hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, s));
+            float e = 0.f, t = 0.f;
+#pragma unroll
+            for (int i = 0; i < 128; i += 32) { e += expf(work[0][k + i] - hi); t += work[1][k + i]; }
+#pragma unroll
+            for (int s = 16; s > 0; s >>= 1) { e += __shfl_xor_sync(0xffffffffu, e, s); t += __shfl_xor_sync(0xffffffffu, t, s); }
+            if (k == 0) { work[2][0] = hi; work[2][1] = e; work[2][2] = t; }
+        }
+        __syncthreads();
+        if (k < g.K) d -= expf(work[0][k] - work[2][0]) / work[2][1] * work[2][2];
     }
-    const size_t row = ((size_t)r * g.M + m) * g.K;
-    if (normalized) d = raw_gradient(off + row, g.K, d, red);
-    if (k < g.K) doff[row + k] = accumulate ? doff[row + k] + d : d;
+    if (k < g.K) {
+        float* to = f.doff + (size_t)row * g.K + k;
+        *to = f.accumulate ? *to + d : d;
+    }
 }
 
-// ---- term by term, for offsets that no factorisation takes (gated by the status word) -----------------------------------------------
 // a lane has the taps lane + 32 i
 struct Taps4 { float v[4]; };
 __device__ __forceinline__ Taps4 checkpoint_patch(const MexGeo& g, const FuseArgs& a, long long xi) {
@@ -586,12 +590,11 @@ __device__ __forceinline__ Taps4 patch_weights(const MexGeo& g, const Taps4& x, 
     return t;
 }
 
-// a warp per position (of all regions)
-__global__ void __launch_bounds__(256) fuse_redo_dx(MexGeo g, FuseArgs a, const float* __restrict__ off) {
-    stream_order();
-    if (!a.flag[0]) return;
+// dx: a warp per position of any region
+__device__ __forceinline__ void redo_dx(const MexGeo& g, const FuseArgs& a, const float* __restrict__ off) {
+    constexpr int W = kFinishThreads / 32;
     const long long P = (long long)g.B * g.N;
-    for (long long j = blockIdx.x * 8LL + (threadIdx.x >> 5); j < P; j += gridDim.x * 8LL) {
+    for (long long j = (long long)blockIdx.x * W + (threadIdx.x >> 5); j < P; j += (long long)gridDim.x * W) {
         const int n = int(j / g.N), pos = int(j - (long long)n * g.N), w = pos % g.Wo, h = pos / g.Wo % g.Ho, c = pos / (g.Wo * g.Ho), r = mex_region_of(g, c, h, w);
         const long long xi = (((long long)n * g.C + c * g.sc) * g.H + h * g.sh) * g.W + w * g.sw, at = mex_dy_base(g, n, pos);
         const Taps4 x = checkpoint_patch(g, a, xi);
@@ -612,54 +615,68 @@ __global__ void __launch_bounds__(256) fuse_redo_dx(MexGeo g, FuseArgs a, const 
     }
 }
 
-// a CTA per row of offsets, its warps over the positions
-__global__ void __launch_bounds__(256) fuse_redo_doff(MexGeo g, FuseArgs a, int normalized, int accumulate, const float* __restrict__ off, float* __restrict__ doff) {
-    stream_order();
-    if (!a.flag[0]) return;
-    __shared__ double sums[8][128];
+// doff: a CTA per row of offsets, its warps over the positions
+__device__ __forceinline__ void redo_doff(const MexGeo& g, const FuseArgs& a, const FinishArgs& f, double (*sums)[128], float (*work)[128]) {
+    constexpr int W = kFinishThreads / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long P = (long long)g.B * g.rs;
     for (int row = blockIdx.x; row < g.R * g.M; row += gridDim.x) {
         const int r = row / g.M, m = row % g.M;
         double sum[4] = {0, 0, 0, 0};
-        for (long long j = warp; j < P; j += 8) {
+        for (long long j = warp; j < P; j += W) {
             const Column col = column_of(g, r, j, P, nullptr);
             if (col.base < 0) continue;
             const long long xi = (((long long)col.n * g.C + col.c0) * g.H + col.h0) * g.W + col.w0;
-            const Taps4 p = patch_weights(g, checkpoint_patch(g, a, xi), off + (size_t)row * g.K);
+            const Taps4 p = patch_weights(g, checkpoint_patch(g, a, xi), f.off + (size_t)row * g.K);
             const float v = a.dy[col.gbase + (long long)m * g.Ng];
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum[i] += v * p.v[i];
         }
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < 4; ++i) sums[warp][lane + 32 * i] = sum[i];
         __syncthreads();
-        float d = 0.f;
-        if (threadIdx.x < 128) {
-            double t = 0;
-            for (int w = 0; w < 8; ++w) t += sums[w][threadIdx.x];
-            if (int(threadIdx.x) < g.K) d = float(t);
-        }
-        if (normalized) {
-            // (all warps take part in the barriers; the last four hold nothing)
-            const int k = threadIdx.x;
-            __shared__ float e_s[128], d_s[128];
-            if (k < 128) { e_s[k] = k < g.K ? off[(size_t)row * g.K + k] : -CUDART_INF_F; d_s[k] = d; }
-            __syncthreads();
-            float hi = -CUDART_INF_F, se = 0.f, sd = 0.f;
-            for (int i = 0; i < g.K; ++i) hi = fmaxf(hi, e_s[i]);
-            for (int i = 0; i < g.K; ++i) { se += expf(e_s[i] - hi); sd += d_s[i]; }
-            if (k < g.K) d -= expf(e_s[k] - hi) / se * sd;
-        }
-        if (int(threadIdx.x) < g.K) {
-            float* to = doff + (size_t)row * g.K + threadIdx.x;
-            *to = accumulate ? *to + d : d;
-        }
-        __syncthreads();
+        double t = 0;
+        if (threadIdx.x < 128)
+            for (int w = 0; w < W; ++w) t += sums[w][threadIdx.x];
+        finish_row(g, f, row, float(t), work);
     }
 }
 
-struct FuseWs { int* flag; float *eo, *part; unsigned char* tiles; size_t bytes; };
+__global__ void __launch_bounds__(kFinishThreads) fuse_finish(MexGeo g, FuseArgs a, FinishArgs f) {
+    stream_order();
+    __shared__ double sums[kFinishThreads / 32][128];
+    __shared__ float work[3][128];
+    if (term_by_term(a)) {
+        if (a.dx) redo_dx(g, a, f.off);
+        if (f.doff) redo_doff(g, a, f, sums, work);
+        return;
+    }
+    if (!f.doff) return;
+    // the CTAs' sums in their order, in two halves
+    float* const half_sum = reinterpret_cast<float*>(sums);
+    const int k = threadIdx.x & 127, half = threadIdx.x >> 7;
+    for (int row = blockIdx.x; row < g.R * g.M; row += gridDim.x) {
+        const int r = row / g.M, m = row % g.M;
+        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+        if (k < g.K) {
+            const size_t step = (size_t)g.R * f.Mp * f.KP;
+            const int slots = f.ctas / g.R, from = half * ((slots + 1) / 2), to = half ? slots : (slots + 1) / 2;
+            const float* s = a.part + ((size_t)r * f.Mp + m / f.MC * f.MC) * f.KP + part_at(f.KP, f.MC, m % f.MC, k) + from * step;
+            int c = from;
+            for (; c + 3 < to; c += 4, s += 4 * step) { s0 += s[0]; s1 += s[step]; s2 += s[2 * step]; s3 += s[3 * step]; }
+            for (; c < to; ++c, s += step) s0 += s[0];
+        }
+        const float mine = (s0 + s1) + (s2 + s3);
+        __syncthreads();
+        if (half) half_sum[k] = mine;
+        __syncthreads();
+        const float d = threadIdx.x < 128 && k < g.K ? f.eo[((size_t)r * g.M + m) * f.KP + k] * (mine + half_sum[k]) : 0.f;
+        finish_row(g, f, row, d, work);
+    }
+}
+
+struct FuseWs { int* status; float *eo, *part; unsigned char* tiles; size_t bytes; };
 
 struct FuseSizes { int KP, MC, Mp, slots; };
 FuseSizes fuse_sizes(const MexGeo& g) {
@@ -677,7 +694,7 @@ FuseWs fuse_carve(const MexGeo& g, void* base) {
     char* p = static_cast<char*>(base);
     size_t off = 0;
     auto take = [&](size_t bytes) { char* r = p ? p + off : nullptr; off += align256(bytes); return r; };
-    w.flag = reinterpret_cast<int*>(take(256));
+    w.status = reinterpret_cast<int*>(take(sizeof(int) * (1 + (size_t)g.R * z.Mp)));
     w.eo = reinterpret_cast<float*>(take(sizeof(float) * (size_t)g.R * g.M * z.KP));
     w.tiles = reinterpret_cast<unsigned char*>(take((size_t)g.R * z.Mp * z.KP * 6));
     w.part = reinterpret_cast<float*>(take(sizeof(float) * (size_t)z.slots * g.R * z.Mp * z.KP));
@@ -723,28 +740,20 @@ cudaError_t launch_mex_checkpoint(const MexGeo& g, int group, const void* codes,
     a.ranges = static_cast<const float2*>(ranges);
     a.tiles = w.tiles;
     a.dy = dy; a.dx = dx; a.part = doff ? w.part : nullptr;
-    a.flag = w.flag;
+    a.status = w.status;
+    a.rows = g.R * z.Mp;
     a.shift = 5;
     while ((1 << a.shift) < group) ++a.shift;
     a.tiles_m = z.Mp / z.MC;
     a.resident = a.tiles_m <= fuse_resident(z.KP);
     a.tiles_j = ((long long)g.B * g.rs + 127) / 128;
-    cudaError_t e = launch_zero_words(w.flag, 2, s);
-    if (e != cudaSuccess) return e;
-    in_stream_order(fuse_prepare, g.R * z.Mp, 128, 0, s)(g, z.KP, z.MC, z.Mp, off, w.eo, w.tiles, w.flag);
+    in_stream_order(fuse_prepare, g.R * z.Mp, 128, 0, s)(g, z.KP, z.MC, z.Mp, off, w.eo, w.tiles, w.status);
     const int ctas = z.slots * g.R;
-    e = z.KP == 16 ? launch_fused<16>(g, a, ctas, s) : z.KP == 32 ? launch_fused<32>(g, a, ctas, s) : z.KP == 64 ? launch_fused<64>(g, a, ctas, s) : launch_fused<128>(g, a, ctas, s);
+    const cudaError_t e = z.KP == 16 ? launch_fused<16>(g, a, ctas, s) : z.KP == 32 ? launch_fused<32>(g, a, ctas, s) : z.KP == 64 ? launch_fused<64>(g, a, ctas, s) : launch_fused<128>(g, a, ctas, s);
     if (e != cudaSuccess) return e;
-    count_launch(2);
-    if (doff) {
-        in_stream_order(fuse_offsets_sum, g.R * g.M, 128, 0, s)(g, z.KP, z.MC, z.Mp, ctas, int(normalized), int(accumulate), off, w.eo, w.part, doff, w.flag);
-        in_stream_order(fuse_redo_doff, std::min(g.R * g.M, 4 * device_sm_count()), 256, 0, s)(g, a, int(normalized), int(accumulate), off, doff);
-        count_launch(2);
-    }
-    if (dx) {
-        in_stream_order(fuse_redo_dx, 4 * device_sm_count(), 256, 0, s)(g, a, off);
-        count_launch();
-    }
+    const FinishArgs f = {off, w.eo, doff, z.KP, z.MC, z.Mp, ctas, int(normalized), int(accumulate)};
+    in_stream_order(fuse_finish, std::min(std::max(g.R * g.M, device_sm_count()), 4 * device_sm_count()), kFinishThreads, 0, s)(g, a, f);
+    count_launch(3);
     return cudaGetLastError();
 }
 

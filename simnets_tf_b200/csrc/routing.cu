@@ -106,9 +106,13 @@ __device__ __forceinline__ void over_range(const T* __restrict__ s, long long N,
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) f(v[u], c + G * u);
     }
-    for (; c < to; c += G, q += step) {
-        const T v = __ldg(q);
-        f(add ? (v + add[c].prior) + add[c].bias : v, c);
+    if (c < to) {
+        T v[kBatch - 1];
+#pragma unroll
+        for (int u = 0; u < kBatch - 1; ++u, q += step) v[u] = c + G * u < to ? __ldg(q) : T(0);
+#pragma unroll
+        for (int u = 0; u < kBatch - 1; ++u)
+            if (c + G * u < to) f(add ? (v[u] + add[c + G * u].prior) + add[c + G * u].bias : v[u], c + G * u);
     }
 }
 // the largest of them, over the lanes of a position
@@ -275,30 +279,33 @@ __global__ void __launch_bounds__(128) route_totals(int ctas, int splits, int k,
     }
 }
 
-// dscores of the weights' gradient:  dl_i = W_i (g_i - sum_j W_j g_j / scale), times 1 - sigmoid(l_i) where the values are sigmoids
+// dscores of the weights' gradient:  dl_i = W_i (g_i - sum_j W_j g_j / scale), times 1 - sigmoid(l_i) where the values are sigmoids.
+// Bound: HBM, the zeros of the others.  A thread has a position and a run of components (blockIdx.y): its zeros, then the chosen among them.
 template <typename T>
 __global__ void __launch_bounds__(kRouteThreads) route_gradient(RouteArgs a, const T* __restrict__ scores, const T* __restrict__ prior, const int* __restrict__ index,
                                                                 const T* __restrict__ weights, const T* __restrict__ grad, T* __restrict__ dscores) {
     stream_order();
     const T inv_scale = T(1.0 / a.scale);
+    const int from = int((long long)a.k * blockIdx.y / gridDim.y), to = int((long long)a.k * (blockIdx.y + 1) / gridDim.y);
     for (long long p = (long long)blockIdx.x * kRouteThreads + threadIdx.x; p < a.positions; p += (long long)gridDim.x * kRouteThreads) {
         const long long n = sample_of(a, p), j = p - n * a.N, chosen = n * a.top * a.N + j;
         const T* s = scores + n * a.k * a.N + j;
-        T* d = dscores + n * a.k * a.N + j;
-        for (int c = 0; c < a.k; ++c) d[c * a.N] = T(0);
+        T* d = dscores + (n * a.k + from) * a.N + j;
+#pragma unroll 8
+        for (int c = from; c < to; ++c, d += a.N) *d = T(0);
         T sum = T(0);
         for (int t = 0; t < a.top; ++t)
             if (index[chosen + t * a.N] >= 0) sum += weights[chosen + t * a.N] * inv_scale * grad[chosen + t * a.N];
         for (int t = 0; t < a.top; ++t) {
             const int c = index[chosen + t * a.N];
-            if (c < 0) continue;
+            if (c < from || c >= to) continue;
             T v = weights[chosen + t * a.N] * (grad[chosen + t * a.N] - sum);
             if (a.sigmoid) {
                 T l = s[c * a.N];
                 if (prior) l += prior[c];
                 v *= T(1) / (T(1) + exp_of(l));
             }
-            d[c * a.N] = v;
+            dscores[(n * a.k + c) * a.N + j] = v;
         }
     }
 }
@@ -379,7 +386,8 @@ cudaError_t launch_route_gradient(const simnets_route_desc& d, const void* score
                                   void* dscores, cudaStream_t s) {
     const RouteArgs a = args_of(d);
     if (a.positions == 0) return cudaSuccess;
-    const int ctas = route_ctas(d);
+    const long long tiles = (a.positions + kRouteThreads - 1) / kRouteThreads, resident = 12LL * device_sm_count();
+    const dim3 ctas(unsigned(std::min(tiles, resident)), unsigned(std::max<long long>(1, std::min<long long>(a.k / 16, resident / tiles))));
     if (d.dtype == SIMNETS_F64)
         in_stream_order(route_gradient<double>, ctas, kRouteThreads, 0, s)(a, (const double*)scores, (const double*)prior, index, (const double*)weights, (const double*)grad, (double*)dscores);
     else

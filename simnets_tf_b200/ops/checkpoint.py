@@ -46,6 +46,13 @@ class Checkpoint(object):
             raise RuntimeError("codes and ranges must be on the same device")
         self.codes, self.ranges = codes.contiguous(), ranges.contiguous()
 
+    @classmethod
+    def _packed(cls, codes, ranges, shape, group):
+        """What the library has packed itself: nothing to check."""
+        self = cls.__new__(cls)
+        self.codes, self.ranges, self.shape, self.group = codes, ranges, tuple(shape), group
+        return self
+
     @property
     def dtype(self):
         """Type of the values."""
@@ -63,10 +70,8 @@ def checkpoint_pack(input, group=128):
     """A `Checkpoint` of a float32 or float64 CUDA tensor.  Infinities and NaN are kept as such; NaN entries and infinities do not count
     towards a group's range.  Not differentiable: `mex_checkpointed` and `similarity_checkpointed` are."""
     group = check_group(group)
-    _torch_glue.dtype_code(input)
-    _torch_glue.require_cuda(input)
-    codes, ranges = _lib.ops().checkpoint_pack(input.detach(), group)
-    return Checkpoint(codes, ranges, input.shape, group)
+    codes, ranges = _lib.ops().checkpoint_pack(input, group)
+    return Checkpoint._packed(codes, ranges, input.shape, group)
 
 
 def checkpoint_unpack(checkpoint):

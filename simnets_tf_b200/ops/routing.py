@@ -7,28 +7,34 @@ from .. import _torch_glue
 
 
 def _checked(scores, top_k, prior, bias, groups, top_groups):
-    _torch_glue.dtype_code(scores)
-    if scores.dim() < 2 or scores.shape[1] < 1:
+    """top_groups of a call whose arguments fit together (a ValueError, or the TypeError or RuntimeError of an operator, if they do not)."""
+    top_groups = groups if top_groups is None else top_groups
+    k = scores.shape[1] if scores.dim() > 1 else 0
+    whole = type(top_k) is type(groups) is type(top_groups) is int
+    if not (whole and 1 <= k <= 4096 and 1 <= top_k <= 16 and 1 <= top_groups <= groups and k % groups == 0 and top_k <= top_groups * (k // groups) and
+            (top_groups == groups or groups <= 64 and top_groups <= 16)):
+        _explain(scores, k, top_k, groups, top_groups)
+    for name, v in (("prior", prior), ("bias", bias)):
+        if v is None:
+            continue
+        if v.dim() != 1 or v.shape[0] != k:
+            raise ValueError("%s must hold one value per component, got %s" % (name, tuple(v.shape)))
+        if v.requires_grad:
+            raise ValueError("%s is a constant of the choice: it has no gradient" % name)
+    return top_groups
+
+
+def _explain(scores, k, top_k, groups, top_groups):
+    if k < 1:
         raise ValueError("scores must have the components on axis 1, got %s" % (tuple(scores.shape),))
-    k, top_groups = scores.shape[1], groups if top_groups is None else top_groups
     for name, v in (("top_k", top_k), ("groups", groups), ("top_groups", top_groups)):
-        if isinstance(v, bool) or int(v) != v or v < 1:
+        if type(v) is not int or v < 1:
             raise ValueError("%s must be a positive whole number, got %r" % (name, v))
     if k % groups or top_groups > groups:
         raise ValueError("%d components do not fall into %d groups of which %d are taken" % (k, groups, top_groups))
     if top_k > top_groups * (k // groups):
         raise ValueError("top_k = %d of %d components" % (top_k, top_groups * (k // groups)))
-    if k > 4096 or top_k > 16 or (top_groups < groups and (groups > 64 or top_groups > 16)):
-        raise ValueError("at most 4096 components, top_k = 16, and where groups are chosen 16 of 64, got %d, %d, %d of %d" % (k, top_k, top_groups, groups))
-    for name, v in (("prior", prior), ("bias", bias)):
-        if v is None:
-            continue
-        if tuple(v.shape) != (k,):
-            raise ValueError("%s must hold one value per component, got %s" % (name, tuple(v.shape)))
-        if v.requires_grad:
-            raise ValueError("%s is a constant of the choice: it has no gradient" % name)
-    _torch_glue.require_cuda(*[t for t in (scores, prior, bias) if t is not None])
-    return int(top_k), int(groups), int(top_groups)
+    raise ValueError("at most 4096 components, top_k = 16, and where groups are chosen 16 of 64, got %d, %d, %d of %d" % (k, top_k, top_groups, groups))
 
 
 def route(scores, top_k=1, prior=None, bias=None, groups=1, top_groups=None, sigmoid=False, scale=1.0):
@@ -42,15 +48,14 @@ def route(scores, top_k=1, prior=None, bias=None, groups=1, top_groups=None, sig
     is -1 and the weight 0.  Chosen components with an infinite score share alike.
 
     The weights are differentiable with respect to the scores."""
-    top_k, groups, top_groups = _checked(scores, top_k, prior, bias, groups, top_groups)
-    scale = float(scale)
+    top_groups = _checked(scores, top_k, prior, bias, groups, top_groups)
     if _torch_glue.is_tracing():
         raise RuntimeError("route cannot be recorded by torch.jit.trace: its choice depends on the values")
-    return _lib.ops().route_apply(scores, prior, bias, top_k, groups, top_groups, bool(sigmoid), scale)
+    return _lib.ops().route_apply(scores, prior, bias, top_k, groups, top_groups, bool(sigmoid), float(scale))
 
 
 def responsibilities(scores, top_k=1, prior=None, bias=None, groups=1, top_groups=None, sigmoid=False):
     """(responsibilities, mass, load): the weights of `route` as a tensor of the scores' shape, 0 where a component is not chosen, and
     their sum per component over all positions.  What the moments of a mixture take; constants of the scores (not differentiable)."""
-    top_k, groups, top_groups = _checked(scores, top_k, prior, bias, groups, top_groups)
-    return _lib.ops().responsibilities(scores.detach(), prior, bias, top_k, groups, top_groups, bool(sigmoid))
+    top_groups = _checked(scores, top_k, prior, bias, groups, top_groups)
+    return _lib.ops().responsibilities(scores, prior, bias, top_k, groups, top_groups, bool(sigmoid))
