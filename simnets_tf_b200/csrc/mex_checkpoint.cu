@@ -179,10 +179,10 @@ __device__ __forceinline__ bool term_by_term(const FuseArgs& a) {
 // once, or, where the taps are the rows, a tap of an instance.
 __host__ __device__ constexpr int part_at(int KP, int MC, int m, int k) { return KP > 64 ? m * KP + k : ((k >> 2) * MC + m) * 4 + (k & 3); }
 
-// barriers of a CTA; every one completes once a step (a tile of positions, 64 or 128 instances)
+// barriers of a CTA; all but the first two complete once a step (a tile of positions, 64 or 128 instances)
 struct FuseShared {
-    uint64_t operands;      // workers: Ex (and Eo) of the step are there
-    uint64_t sums;          // products: S is there
+    uint64_t operands;      // workers: Ex (and, where it is not kept, Eo) of the step are there; with Eo kept and S twice, once a tile
+    uint64_t sums[2];       // products: S is there (by place in tensor memory)
     uint64_t quotients;     // workers: Q is there, S has been read
     uint64_t taps;          // products: the sums over the instances are there
     uint64_t instances;     // products: the sums over the positions are there, and Ex and Q may be written anew
@@ -254,8 +254,10 @@ struct Fuse {
     using X = Planes<128, KP>;
     using Q = Planes<128, MC>;
     using E = Planes<MC, KP>;
-    // tensor memory: S, the sums over the instances (128 taps: one block of columns, three do not fit), the offsets' sums
-    static constexpr int kTapBlocks = KP > 64 ? 1 : 3, kT = MC, kU = kT + kTapBlocks * KP;
+    // tensor memory: S (where there is room twice, so that the next step's is made while this one's quotients are), the sums over the instances
+    // (128 taps: one block of columns, three do not fit), the offsets' sums
+    static constexpr bool kTwice = KP <= 32;
+    static constexpr int kTapBlocks = KP > 64 ? 1 : 3, kT = kTwice ? 2 * MC : MC, kU = kT + kTapBlocks * KP;
     static constexpr int kUBlock = kByTaps ? MC : KP;
     static_assert(kU + 3 * kUBlock <= kFuseColumns);
 };
@@ -271,7 +273,8 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
     extern __shared__ __align__(1024) unsigned char sm[];
     __shared__ FuseShared sh;
     __shared__ float red[2][4][128];
-    __shared__ int tap_off[KP];
+    __shared__ longlong2 place_s[2][128];
+    __shared__ __align__(16) int tap_off[KP];
     if (term_by_term(a)) return;
     unsigned char *const sx = sm, *const sq = sm + X::kBytes, *const se = sq + Q::kBytes;
     const int warp = threadIdx.x >> 5;
@@ -281,8 +284,8 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
         tap_off[k] = (t.c * g.H + t.h) * g.W + t.w;
     }
     if (threadIdx.x == 0) {
-        mbar_init(&sh.operands, kFuseWorkers); mbar_init(&sh.quotients, kFuseWorkers);
-        mbar_init(&sh.sums, 1); mbar_init(&sh.taps, 1); mbar_init(&sh.instances, 1);
+        mbar_init(&sh.operands, kFuseWorkers / 32); mbar_init(&sh.quotients, kFuseWorkers / 32);
+        mbar_init(&sh.sums[0], 1); mbar_init(&sh.sums[1], 1); mbar_init(&sh.taps, 1); mbar_init(&sh.instances, 1);
         sh.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -296,11 +299,17 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
     const uint32_t tmem = sh.tmem;
     const uint32_t tS = tmem, tT = tmem + F::kT, tU = tmem + F::kU;
     const uint32_t xb = smem_u32(sx), qb = smem_u32(sq), eb = smem_u32(se);
-    uint32_t phase = 0;
+    const bool ahead = F::kTwice && a.resident;
+    uint32_t phase = 0;                                                                  // of the barriers that complete once a step
     // A wait that runs out sets `failed`; from then on nobody waits and no product is issued, and all leave by the ordinary way.
-    auto wait = [&](uint64_t* bar) {
-        if (!sh.failed && !mbar_wait(bar, phase)) sh.failed = 1;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (!sh.failed && !mbar_wait(bar, parity)) sh.failed = 1;
         __syncwarp();                                                                    // (what follows is done by whole warps)
+    };
+    // (one arrival a warp: those of 512 threads follow one another)
+    auto arrive = [&](uint64_t* bar) {
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
     };
 
     if (warp == kFuseWorkers / 32) {
@@ -308,20 +317,28 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
         const Operand<X, true> x_across(xb);
         const Operand<Q, false> q_along(qb);
         const Operand<Q, true> q_across(qb);
+        auto issue_sums = [&](int mt) {
+            const Operand<E, false> e_along(eb + (a.resident ? mt * E::kBytes : 0u));
+            const int to = ahead ? mt & 1 : 0;
+            if (!sh.failed && elected()) {
+                issue_in_turn<MC, KP / 16>(tS + to * MC, x_along, e_along);
+                umma_commit(&sh.sums[to]);
+            }
+            __syncwarp();
+        };
+        uint32_t there = 0;
         for (long long jt = slot; jt < a.tiles_j; jt += slots)
             for (int mt = 0; mt < a.tiles_m; ++mt, phase ^= 1u) {
-                const uint32_t et = eb + (a.resident ? mt * E::kBytes : 0u);
-                wait(&sh.operands);
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const Operand<E, false> e_along(et);
-                const Operand<E, true> e_across(et);
-                if (!sh.failed && elected()) {
-                    issue_in_turn<MC, KP / 16>(tS, x_along, e_along);
-                    umma_commit(&sh.sums);
+                if (!ahead || mt == 0) {
+                    wait(&sh.operands, there);
+                    there ^= 1u;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    issue_sums(mt);
+                    if (ahead && a.tiles_m > 1) issue_sums(1);
                 }
-                __syncwarp();
-                wait(&sh.quotients);
+                wait(&sh.quotients, phase);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const Operand<E, true> e_across(eb + (a.resident ? mt * E::kBytes : 0u));
                 if (!sh.failed && elected()) {
                     if (a.dx) {
                         if constexpr (F::kTapBlocks == 3) issue_side_by_side<KP, MC / 16>(tT, q_along, e_across);
@@ -335,6 +352,7 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
                     umma_commit(&sh.instances);
                 }
                 __syncwarp();
+                if (ahead && mt + 2 < a.tiles_m) issue_sums(mt + 2);                     // (into the place of the S that has been read)
             }
     } else {
         const int p = threadIdx.x & 127, part4 = threadIdx.x >> 7;                      // position (tensor-memory lane) and its quarter of the columns
@@ -346,19 +364,32 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
             const unsigned char* src = a.tiles + ((size_t)r * a.tiles_m + mt) * E::kBytes;
             for (int i = threadIdx.x; i < int(E::kBytes / 16); i += kFuseWorkers) cp_async16(reinterpret_cast<float*>(to + i * 16), reinterpret_cast<const float*>(src + i * 16), 16);
         };
-        // where a position lies: first tap in the input, first instance in dy (one that is not there: the first of all, and not live)
-        struct Place { long long x, dy; bool live; };
-        auto place_of = [&](long long jt) {
-            const Column col = column_of(g, r, jt * 128 + p, P, nullptr);
-            Place at = {0, 0, col.base >= 0};
-            if (at.live) { at.x = (((long long)col.n * g.C + col.c0) * g.H + col.h0) * g.W + col.w0; at.dy = col.gbase; }
-            return at;
-        };
+        // Where the positions of a tile lie, by the first quarter of the workers: first tap in the input (-1: a position that is not there), first
+        // instance in dy.  Their bytes are asked for by the way, a tap a worker: a line has several positions.
         int turn = 0;
-        // Ex of this worker's taps (k0 .. + KR) of its position.  Taps that are not there read the first one's value and count 0; a position that is
-        // not there has a 1 in its first tap, so that its S is no 0.
-        auto decode = [&](const Place& at, float (&ex)[KR]) {
+        auto find_places = [&](long long jt) {
+            if (part4 != 0) return;
+            const Column col = column_of(g, r, jt * 128 + p, P, nullptr);
+            longlong2 at = make_longlong2(-1, 0);
+            if (col.base >= 0) {
+                at = make_longlong2((((long long)col.n * g.C + col.c0) * g.H + col.h0) * g.W + col.w0, col.gbase);
+#pragma unroll
+                for (int k = 0; k < KP; k += 16) {
+                    const long long idx = at.x + tap_off[k + (p & 15)];
+                    asm volatile("prefetch.global.L1 [%0];" ::"l"(a.codes + idx));
+                    asm volatile("prefetch.global.L1 [%0];" ::"l"(a.ranges + (idx >> a.shift)));
+                }
+            }
+            place_s[turn][p] = at;
+        };
+        // Ex of this worker's taps (k0 .. + KR) of its position of the tile that find_places() was called for.  Taps that are not there read the first
+        // one's value and count 0; a position that is not there has a 1 in its first tap, so that its S is no 0.
+        struct Place { long long x, dy; bool live; };
+        auto decode = [&](float (&ex)[KR]) {
             constexpr int H = KR < 16 ? KR : 16;
+            asm volatile("bar.sync 1, %0;" ::"n"(kFuseWorkers) : "memory");
+            const longlong2 found = place_s[turn][p];
+            const Place at = {found.x < 0 ? 0 : found.x, found.y, found.x >= 0};
             const unsigned char* const codes = a.codes + at.x;
             const float2* const ranges = a.ranges + (at.x >> a.shift);
             const int rest = int(at.x) & ((1 << a.shift) - 1);
@@ -368,10 +399,14 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
                 uint32_t code[H], top = 0;
                 float2 range[H];
 #pragma unroll
-                for (int i = 0; i < H; ++i) {
-                    const int tap = tap_off[k0 + i0 + i];
-                    code[i] = __ldg(codes + tap);
-                    range[i] = __ldg(ranges + ((unsigned(rest) + unsigned(tap)) >> a.shift));
+                for (int i = 0; i < H; i += 4) {
+                    const int4 t4 = *reinterpret_cast<const int4*>(tap_off + k0 + i0 + i);
+                    const int tap[4] = {t4.x, t4.y, t4.z, t4.w};
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        code[i + u] = __ldg(codes + tap[u]);
+                        range[i + u] = __ldg(ranges + ((unsigned(rest) + unsigned(tap[u])) >> a.shift));
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < H; ++i) top = max(top, code[i]);
@@ -398,54 +433,99 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
             if (!at.live)
 #pragma unroll
                 for (int i = 0; i < KR; ++i) ex[i] = k0 + i == 0 ? 1.f : 0.f;
+            return at;
         };
+        // dy of this worker's instances (a quarter of a step's) of its position
+        float q[MR];
+        auto load_dy = [&](const Place& at, int mt) {
+            const int m0 = mt * MC + part4 * MR;
+            const float* from = a.dy + at.dy + (long long)m0 * g.Ng;
+            if (m0 + MR <= g.M)
+#pragma unroll
+                for (int i = 0; i < MR; ++i, from += g.Ng) q[i] = at.live ? __ldcs(from) : 0.f;
+            else
+#pragma unroll
+                for (int i = 0; i < MR; ++i, from += g.Ng) q[i] = at.live && m0 + i < g.M ? __ldcs(from) : 0.f;
+        };
+        // the offsets' sums of a step onto the CTA's
+        auto add_offsets = [&](int mt, bool first) {
+            if (!a.part) return;
+            float* const to = a.part + ((size_t)blockIdx.x * Mp + mt * MC) * KP;
+            if constexpr (F::kByTaps) {                                                  // row = tap p, columns = instances
+                float* const d = to + part4 * MR * KP + p;
+#pragma unroll
+                for (int i0 = 0; i0 < MR; i0 += 8) {
+                    float old[8], u[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) old[i] = first ? 0.f : d[(i0 + i) * KP];
+                    tmem_sum<8, 3, MC>(tU + lane_base + part4 * MR + i0, u);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) d[(i0 + i) * KP] = old[i] + u[i];
+                }
+            } else {                                                                     // row = instance p, columns = taps
+                constexpr int H = KR < 8 ? KR : 8;
+                float4* const d = reinterpret_cast<float4*>(to) + (k0 / 4) * MC + p;
+#pragma unroll
+                for (int i0 = 0; i0 < KR; i0 += H) {
+                    float4 old[H / 4];
+                    float u[H];
+#pragma unroll
+                    for (int i = 0; i < H / 4; ++i) old[i] = first ? make_float4(0.f, 0.f, 0.f, 0.f) : d[(i0 / 4 + i) * MC];
+                    tmem_sum<H, 3, KP>(tU + lane_base + k0 + i0, u);
+#pragma unroll
+                    for (int i = 0; i < H / 4; ++i)
+                        d[(i0 / 4 + i) * MC] = make_float4(old[i].x + u[4 * i], old[i].y + u[4 * i + 1], old[i].z + u[4 * i + 2], old[i].w + u[4 * i + 3]);
+                }
+            }
+        };
+
         if (a.resident) for (int mt = 0; mt < a.tiles_m; ++mt) load_offsets(mt, se + mt * E::kBytes);
-        Place at = place_of(slot);
         float ex[KR];
-        decode(at, ex);
+        find_places(slot);
+        Place at = decode(ex);
+        if (ahead) load_dy(at, 0);
+        uint32_t sum_phase[2] = {0, 0};
+        bool due = false;                                                                // the offsets' sums of the step before are to be added
         for (long long jt = slot; jt < a.tiles_j; jt += slots) {
             store_row<X>(sx, p, k0, ex);
             float tsum[KR];
 #pragma unroll
             for (int i = 0; i < KR; ++i) tsum[i] = 0.f;
-            const bool last_tile = jt + slots >= a.tiles_j;
-            Place next = {0, 0, false};
+            const bool last_tile = jt + slots >= a.tiles_j, first = jt == slot;
+            Place next = at;
             for (int mt = 0; mt < a.tiles_m; ++mt, phase ^= 1u) {
                 if (!a.resident) load_offsets(mt, se);
-                cp_async_wait_all();
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                mbar_arrive(&sh.operands);
-                // this worker's instances: m0 .. + MR
-                const int m0 = mt * MC + part4 * MR;
-                const bool live = at.live;
-                const float* dyp = a.dy + at.dy + (long long)m0 * g.Ng;
-                float q[MR];
-                if (m0 + MR <= g.M)
-#pragma unroll
-                    for (int i = 0; i < MR; ++i, dyp += g.Ng) q[i] = live ? __ldcs(dyp) : 0.f;
-                else
-#pragma unroll
-                    for (int i = 0; i < MR; ++i, dyp += g.Ng) q[i] = live && m0 + i < g.M ? __ldcs(dyp) : 0.f;
-                wait(&sh.sums);
+                if (!ahead || mt == 0) {
+                    cp_async_wait_all();
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    arrive(&sh.operands);
+                }
+                // (while the first product runs)
+                if (!ahead) load_dy(at, mt);
+                if (due) add_offsets(mt == 0 ? a.tiles_m - 1 : mt - 1, mt == 0 ? jt - slots == slot : first);
+                due = true;
+                const bool last = mt + 1 == a.tiles_m;
+                if (last && !last_tile) find_places(jt + slots);
+                const int from = ahead ? mt & 1 : 0;
+                wait(&sh.sums[from], from ? sum_phase[1] : sum_phase[0]);
+                if (from) sum_phase[1] ^= 1u; else sum_phase[0] ^= 1u;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
                 for (int i0 = 0; i0 < MR; i0 += 16) {
                     float s[16];
-                    tmem_sum<16, 1, 0>(tS + lane_base + part4 * MR + i0, s);
+                    tmem_sum<16, 1, 0>(tS + from * MC + lane_base + part4 * MR + i0, s);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[i] = q[i0 + i] * reciprocal(s[i]);
                     store_row<Q>(sq, p, part4 * MR + i0, s);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                mbar_arrive(&sh.quotients);
-                const bool last = mt + 1 == a.tiles_m;
-                if (last && !last_tile) {                                                // (while the second product runs)
-                    next = place_of(jt + slots);
-                    decode(next, ex);
-                }
-                wait(&sh.taps);
+                arrive(&sh.quotients);
+                // (while the second product runs)
+                if (last && !last_tile) next = decode(ex);
+                if (ahead && !(last && last_tile)) load_dy(last ? next : at, last ? 0 : mt + 1);
+                wait(&sh.taps, phase);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (a.dx) {
                     constexpr int H = KR < 16 ? KR : 16;
@@ -456,51 +536,31 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
 #pragma unroll
                         for (int i = 0; i < H; ++i) tsum[i0 + i] += t[i];
                     }
-                    if (last && live) {                                                  // (while the third runs) Ex from its planes, which add up to it
+                    if (last && at.live) {                                               // (while the third runs) Ex from its planes, which add up to it
+                        float* const dx = a.dx + at.x;
 #pragma unroll
-                        for (int i = 0; i < KR; i += 2) {
-                            uint32_t w[3];
+                        for (int i = 0; i < KR; i += 4) {
+                            const int4 tap = *reinterpret_cast<const int4*>(tap_off + k0 + i);
+                            uint2 w[3];
 #pragma unroll
-                            for (int b = 0; b < 3; ++b) w[b] = *reinterpret_cast<const uint32_t*>(sx + X::at(p, k0 + i) + b * X::kPlane);
-                            const float e0 = (__uint_as_float(w[0] << 16) + __uint_as_float(w[1] << 16)) + __uint_as_float(w[2] << 16);
-                            const float e1 = (__uint_as_float(w[0] & 0xffff0000u) + __uint_as_float(w[1] & 0xffff0000u)) + __uint_as_float(w[2] & 0xffff0000u);
-                            if (k0 + i < g.K) a.dx[at.x + tap_off[k0 + i]] = e0 * tsum[i];
-                            if (k0 + i + 1 < g.K) a.dx[at.x + tap_off[k0 + i + 1]] = e1 * tsum[i + 1];
+                            for (int b = 0; b < 3; ++b) w[b] = *reinterpret_cast<const uint2*>(sx + X::at(p, k0 + i) + b * X::kPlane);
+                            auto low = [](uint32_t v) { return __uint_as_float(v << 16); };
+                            auto high = [](uint32_t v) { return __uint_as_float(v & 0xffff0000u); };
+                            const float e0 = (low(w[0].x) + low(w[1].x)) + low(w[2].x), e1 = (high(w[0].x) + high(w[1].x)) + high(w[2].x);
+                            const float e2 = (low(w[0].y) + low(w[1].y)) + low(w[2].y), e3 = (high(w[0].y) + high(w[1].y)) + high(w[2].y);
+                            if (k0 + i < g.K) dx[tap.x] = e0 * tsum[i];
+                            if (k0 + i + 1 < g.K) dx[tap.y] = e1 * tsum[i + 1];
+                            if (k0 + i + 2 < g.K) dx[tap.z] = e2 * tsum[i + 2];
+                            if (k0 + i + 3 < g.K) dx[tap.w] = e3 * tsum[i + 3];
                         }
                     }
                 }
-                const bool first = jt == slot;
-                if constexpr (F::kByTaps) {                                              // row = tap p, columns = instances
-                    float* d = a.part ? a.part + ((size_t)blockIdx.x * Mp + m0) * KP + p : nullptr;
-                    float old[MR];
-#pragma unroll
-                    for (int i = 0; i < MR; ++i) old[i] = d && !first ? d[i * KP] : 0.f;
-                    wait(&sh.instances);
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (d) {
-                        float u[MR];
-                        tmem_sum<MR, 3, MC>(tU + lane_base + part4 * MR, u);
-#pragma unroll
-                        for (int i = 0; i < MR; ++i) d[i * KP] = old[i] + u[i];
-                    }
-                } else {                                                                 // row = instance p, columns = taps
-                    float4* d = a.part ? reinterpret_cast<float4*>(a.part + ((size_t)blockIdx.x * Mp + mt * MC) * KP) + (k0 / 4) * MC + p : nullptr;
-                    float4 old[KR / 4];
-#pragma unroll
-                    for (int i = 0; i < KR / 4; ++i) old[i] = d && !first ? d[i * MC] : make_float4(0.f, 0.f, 0.f, 0.f);
-                    wait(&sh.instances);
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (d) {
-                        float u[KR];
-                        tmem_sum<KR, 3, KP>(tU + lane_base + k0, u);
-#pragma unroll
-                        for (int i = 0; i < KR / 4; ++i)
-                            d[i * MC] = make_float4(old[i].x + u[4 * i], old[i].y + u[4 * i + 1], old[i].z + u[4 * i + 2], old[i].w + u[4 * i + 3]);
-                    }
-                }
+                wait(&sh.instances, phase);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             }
             at = next;
         }
+        if (due) add_offsets(a.tiles_m - 1, a.tiles_j - slot <= slots);
         cp_async_wait_all();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -702,7 +762,7 @@ FuseWs fuse_carve(const MexGeo& g, void* base) {
     return w;
 }
 
-constexpr int kFuseShared = 220 * 1024;     // (of 227 KB; the barriers, the extremes and the tap offsets are some 5)
+constexpr int kFuseShared = 217 * 1024;     // (of 227 KB; the barriers, the extremes, the places and the tap offsets are some 9)
 
 // steps of instances whose Eo stays in shared memory beside Ex and Q
 int fuse_resident(int KP) {
