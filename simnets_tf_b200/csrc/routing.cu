@@ -196,14 +196,9 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose(RouteArgs a, const
         if (live && dense) {
             T* d = dense + (n * a.k + sub) * a.N + j;
             const long long step = G * a.N;
-            if constexpr (TK <= 4) {                     // every value once
+            if constexpr (TK == 1) {                     // every value once
 #pragma unroll 4
-                for (int c = sub; c < a.k; c += G, d += step) {
-                    T w = T(0);
-#pragma unroll
-                    for (int t = 0; t < TK; ++t) w = t < a.top && c == top.i[t] ? l[t] : w;
-                    __stcs(d, w);
-                }
+                for (int c = sub; c < a.k; c += G, d += step) __stcs(d, c == top.i[0] ? l[0] : T(0));
             } else {                                     // zeros, then the chosen (each by the lane that wrote its zero)
 #pragma unroll 8
                 for (int c = sub; c < a.k; c += G, d += step) *d = T(0);
@@ -275,7 +270,7 @@ __global__ void __launch_bounds__(128) route_totals(int ctas, int splits, int k,
     }
     if (threadIdx.x == 0) {
         load[blockIdx.x] = red[0];
-        if (mass) mass[blockIdx.x] = redm[0];
+        if (mass) mass[blockIdx.x] = splits > 0 ? redm[0] : T(red[0]);
     }
 }
 
@@ -323,30 +318,34 @@ RouteArgs args_of(const simnets_route_desc& d) {
 }
 // lanes per position: one where the positions fill the GPU
 int route_lanes(const simnets_route_desc& d) { return d.positions * d.batch >= 512LL * device_sm_count() || d.components < 8 ? 1 : 4; }
-int route_ctas(const simnets_route_desc& d) {
-    const long long places = kRouteThreads / route_lanes(d), tiles = (d.positions * d.batch + places - 1) / places, resident = 12LL * device_sm_count();
+// a CTA's sums fit the shared memory of a multiprocessor three times
+size_t sums_bytes(const simnets_route_desc& d) { return (d.dtype == SIMNETS_F64 ? 8 : 4) * (size_t)d.components * (kRouteThreads / route_lanes(d)); }
+bool route_sums(const simnets_route_desc& d) { return d.top_k > 1 && sums_bytes(d) <= 64 * 1024; }
+size_t choose_bytes(const simnets_route_desc& d, bool sums) { return (sums ? sums_bytes(d) : 0) + (size_t)d.components * (2 * (d.dtype == SIMNETS_F64 ? 8 : 4) + sizeof(unsigned)); }
+// as many CTAs as are resident together, each with as many tiles as the others
+int route_ctas(const simnets_route_desc& d, bool sums) {
+    const long long places = kRouteThreads / route_lanes(d), tiles = (d.positions * d.batch + places - 1) / places;
+    const long long resident = std::max<long long>(1, std::min<long long>(12, 220 * 1024 / (choose_bytes(d, sums) + 2048))) * device_sm_count();
     const long long rounds = std::max<long long>(1, (tiles + resident - 1) / resident);
     return int(std::max<long long>(1, (tiles + rounds - 1) / rounds));
 }
-// a CTA's sums fit the shared memory of a multiprocessor three times
-size_t sums_bytes(const simnets_route_desc& d) { return (d.dtype == SIMNETS_F64 ? 8 : 4) * (size_t)d.components * (kRouteThreads / route_lanes(d)); }
-bool route_sums(const simnets_route_desc& d) { return sums_bytes(d) <= 64 * 1024; }
+int most_ctas(const simnets_route_desc& d) { return std::max(route_ctas(d, false), route_ctas(d, route_sums(d))); }
 int mass_splits(const simnets_route_desc& d) {
-    if (route_sums(d)) return route_ctas(d);
+    if (route_sums(d)) return most_ctas(d);
     return int(std::max<long long>(1, std::min<long long>(d.batch, (8LL * device_sm_count() + d.components - 1) / d.components)));
 }
-size_t load_bytes(const simnets_route_desc& d) { return (sizeof(unsigned) * (size_t)route_ctas(d) * d.components + 255) & ~size_t(255); }
+size_t load_bytes(const simnets_route_desc& d) { return (sizeof(unsigned) * (size_t)most_ctas(d) * d.components + 255) & ~size_t(255); }
 
 template <typename T, int TK, int G, bool SUMS>
 cudaError_t choose(const simnets_route_desc& d, const RouteArgs& a, const void* scores, const void* prior, const void* bias, int* index, void* weights, void* dense,
                    T* part_mass, unsigned* part_load, cudaStream_t s) {
-    const size_t smem = (SUMS ? sums_bytes(d) : 0) + (size_t)a.k * (2 * sizeof(T) + sizeof(unsigned));
+    const size_t smem = choose_bytes(d, SUMS);
     static SmemLimit limit;
     if (smem > 32 * 1024) {
         const cudaError_t e = limit.raise(route_choose<T, TK, G, SUMS>, 160 * 1024);
         if (e != cudaSuccess) return e;
     }
-    in_stream_order(route_choose<T, TK, G, SUMS>, route_ctas(d), kRouteThreads, smem, s)(a, (const T*)scores, (const T*)prior, (const T*)bias, index, (T*)weights, (T*)dense, part_mass, part_load);
+    in_stream_order(route_choose<T, TK, G, SUMS>, route_ctas(d, SUMS), kRouteThreads, smem, s)(a, (const T*)scores, (const T*)prior, (const T*)bias, index, (T*)weights, (T*)dense, part_mass, part_load);
     return cudaSuccess;
 }
 
@@ -354,10 +353,10 @@ template <typename T>
 cudaError_t route(const simnets_route_desc& d, const void* scores, const void* prior, const void* bias, int* index, void* weights, void* dense, long long* load,
                   void* mass, void* ws, cudaStream_t s) {
     const RouteArgs a = args_of(d);
-    const int ctas = route_ctas(d), splits = mass_splits(d), want = std::max(a.top, a.top_groups < a.groups ? a.top_groups : 1);
+    const bool sums = dense && route_sums(d), one = route_lanes(d) == 1, counted = a.top == 1;      // (of one chosen the weight is one: the mass is the load)
+    const int ctas = route_ctas(d, sums), splits = sums ? ctas : mass_splits(d), want = std::max(a.top, a.top_groups < a.groups ? a.top_groups : 1);
     unsigned* part_load = static_cast<unsigned*>(ws);
     T* part_mass = reinterpret_cast<T*>(static_cast<char*>(ws) + load_bytes(d));
-    const bool sums = dense && route_sums(d), one = route_lanes(d) == 1;
     cudaError_t e = cudaSuccess;
 #define ROUTE(TK) e = sums ? (one ? choose<T, TK, 1, true>(d, a, scores, prior, bias, index, weights, dense, part_mass, part_load, s)                     \
                                   : choose<T, TK, 4, true>(d, a, scores, prior, bias, index, weights, dense, part_mass, part_load, s))                    \
@@ -366,9 +365,9 @@ cudaError_t route(const simnets_route_desc& d, const void* scores, const void* p
     if (want <= 1) ROUTE(1); else if (want <= 2) ROUTE(2); else if (want <= 4) ROUTE(4); else if (want <= 8) ROUTE(8); else ROUTE(16);
 #undef ROUTE
     if (e != cudaSuccess) return e;
-    if (mass && !sums) in_stream_order(route_mass<T>, dim3(a.k, splits), 256, 0, s)(a, (long long)d.batch, (const T*)dense, part_mass);
-    in_stream_order(route_totals<T>, a.k, 128, 0, s)(ctas, splits, a.k, part_load, part_mass, load, (T*)mass);
-    count_launch(mass && !sums ? 3 : 2);
+    if (mass && !sums && !counted) in_stream_order(route_mass<T>, dim3(a.k, splits), 256, 0, s)(a, (long long)d.batch, (const T*)dense, part_mass);
+    in_stream_order(route_totals<T>, a.k, 128, 0, s)(ctas, counted ? 0 : splits, a.k, part_load, part_mass, load, (T*)mass);
+    count_launch(mass && !sums && !counted ? 3 : 2);
     return cudaGetLastError();
 }
 
