@@ -83,7 +83,8 @@ enum { SIMNETS_SIM_L1 = 0, SIMNETS_SIM_L2 = 1 };
 /* Test hook, simnets_mex_forward on a pair-tile shape only: the kernel's MMA role withholds the completion signal of
  * its first accumulator and every bounded wait is shortened to a fraction of a millisecond, so that one wait runs out.
  * Nothing hangs or faults: the roles leave their loops, tensor memory is freed, word 1 of the workspace status is set
- * (simnets_mex_workspace_status) and the exact kernels launched behind the tensor-core kernel redo the work. */
+ * (simnets_mex_workspace_status) and the exact kernels launched behind the tensor-core kernel redo the work.  Likewise for
+ * simnets_mex_checkpoint_gradients where simnets_mex_checkpoint_one_pass says so. */
 #define SIMNETS_FLAG_MEX_TEST_EXPIRE_WAIT (1u << 10)
 
 /* simnets_similarity_forward only, float32, L2 without ignore_nan_input (other calls ignore the flag): evaluate the
@@ -400,6 +401,11 @@ SIMNETS_API int simnets_checkpoint_unpack(int32_t dtype, int64_t count, int32_t 
  * simnets_mex_gradients, without SIMNETS_FLAG_MEX_WORKSPACE_PRIMED and SIMNETS_FLAG_MEX_MAXIMA_GIVEN
  * (SIMNETS_E_UNSUPPORTED).  Similarity: a NULL dx is not computed, nor are dtemplates and dweights where both are NULL. */
 SIMNETS_API size_t simnets_mex_checkpoint_workspace_bytes(const simnets_mex_desc* d);
+/* 1 where one kernel makes both gradients from the bytes (float32, finite epsilon, blocks of up to 128 taps that cover the
+ * input once, up to 16 regions); neither x nor y is written there, and simnets_mex_workspace_status reads the workspace.
+ * Elsewhere the bytes become x in the workspace, and y is computed from it by the kernels of the other entry points with sums
+ * in FP32. */
+SIMNETS_API int simnets_mex_checkpoint_one_pass(const simnets_mex_desc* d);
 SIMNETS_API int simnets_mex_checkpoint_gradients(const simnets_mex_desc* d, int32_t group, const void* codes, const void* ranges,
                                                  const void* offsets, const void* dy, void* dx, void* doffsets,
                                                  void* workspace, size_t workspace_bytes, void* stream);

@@ -69,6 +69,7 @@ def lib():
             f.argtypes = [C.c_int32, C.c_int64, C.c_int32, _P, _P, _P, _P]
         for f, d in ((l.simnets_mex_checkpoint_workspace_bytes, md), (l.simnets_similarity_checkpoint_workspace_bytes, sd)):
             f.restype, f.argtypes = C.c_size_t, [d]
+        l.simnets_mex_checkpoint_one_pass.argtypes = [md]
         l.simnets_mex_checkpoint_gradients.argtypes = [md, C.c_int32, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]
         l.simnets_similarity_checkpoint_gradients.argtypes = [sd, C.c_int32, _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]
         rd = C.POINTER(abi.RouteDesc)

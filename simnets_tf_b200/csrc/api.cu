@@ -450,6 +450,11 @@ size_t simnets_mex_checkpoint_workspace_bytes(const simnets_mex_desc* d) {
     return mex_checkpoint_shape(g, d->dtype == SIMNETS_F64, d->flags) ? mex_checkpoint_bytes(g) : mex_checkpoint_carve(g, *d, nullptr).bytes;
 }
 
+int simnets_mex_checkpoint_one_pass(const simnets_mex_desc* d) {
+    MexGeo g;
+    return d && !mex_geometry(d, nullptr, &g) && mex_checkpoint_shape(g, d->dtype == SIMNETS_F64, d->flags);
+}
+
 int simnets_mex_checkpoint_gradients(const simnets_mex_desc* d, int32_t group, const void* codes, const void* ranges, const void* off, const void* dy, void* dx,
                                      void* doff, void* ws, size_t ws_bytes, void* stream) {
     MexGeo g;
@@ -462,7 +467,7 @@ int simnets_mex_checkpoint_gradients(const simnets_mex_desc* d, int32_t group, c
     if (mex_checkpoint_shape(g, d->dtype == SIMNETS_F64, d->flags)) {
         if (!ws || ws_bytes < mex_checkpoint_bytes(g)) return SIMNETS_E_WORKSPACE;
         return from_cuda(launch_mex_checkpoint(g, group, codes, ranges, (const float*)off, (const float*)dy, (float*)dx, (float*)doff, (d->flags & SIMNETS_FLAG_ACCUMULATE) != 0,
-                                               (d->flags & SIMNETS_FLAG_MEX_NORMALIZED_OFFSETS) != 0, ws, as_stream(stream)));
+                                               (d->flags & SIMNETS_FLAG_MEX_NORMALIZED_OFFSETS) != 0, (d->flags & SIMNETS_FLAG_MEX_TEST_EXPIRE_WAIT) != 0, ws, as_stream(stream)));
     }
     const MexCheckpointWs w = mex_checkpoint_carve(g, *d, ws);
     if (!ws || ws_bytes < w.bytes) return SIMNETS_E_WORKSPACE;

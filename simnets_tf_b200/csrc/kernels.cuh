@@ -167,7 +167,7 @@ cudaError_t launch_checkpoint_unpack(bool f64, long long first, long long n, int
 bool mex_checkpoint_shape(const MexGeo&, bool f64, uint32_t flags);
 size_t mex_checkpoint_bytes(const MexGeo&);
 cudaError_t launch_mex_checkpoint(const MexGeo&, int group, const void* codes, const void* ranges, const float* off, const float* dy, float* dx, float* doff,
-                                  bool accumulate, bool normalized, void* ws, cudaStream_t);
+                                  bool accumulate, bool normalized, bool expire, void* ws, cudaStream_t);
 // routing.cu -- positions to components; index and weights, or dense and mass, may be null
 size_t route_workspace_bytes(const simnets_route_desc&);
 cudaError_t launch_route(const simnets_route_desc&, const void* scores, const void* prior, const void* bias, int* index, void* weights, void* dense,

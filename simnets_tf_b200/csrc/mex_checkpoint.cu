@@ -25,6 +25,7 @@
 // else adds up the partial sums, evaluates term by term.
 #include "checkpoint.cuh"
 #include "ws.cuh"
+#include <cmath>
 
 namespace simnets {
 namespace {
@@ -140,8 +141,8 @@ __global__ void __launch_bounds__(128) fuse_prepare(MexGeo g, int KP, int MC, in
     const float eps = float(g.eps);
     // (the extremes leave a NaN out)
     const int unsafe = __syncthreads_or(in && (!(fabsf(v) < CUDART_INF_F) || !(fabsf(eps) * (hi - lo) <= kSafeSpread)));
-    if (k == 0) status[1 + blockIdx.x] = unsafe;
-    if (k == 0 && blockIdx.x == 0) status[0] = 0;
+    if (k == 0) status[2 + blockIdx.x] = unsafe;
+    if (k < 2 && blockIdx.x == 0) status[k] = 0;
     const float e = in ? ex2_ftz(eps * 1.4426950408889634f * (v - (eps > 0.f ? hi : lo))) : m < g.M ? 0.f : 1.f;
     if (k >= KP) return;
     if (m < g.M) eo[((size_t)r * g.M + m) * KP + k] = e;
@@ -160,19 +161,30 @@ struct FuseArgs {
     const float* dy;
     float* dx;              // may be null
     float* part;            // [CTA][step] of what part_at() lays out, may be null
-    int* status;            // a wait ran out; then, per row of offsets, whether its spread is beyond what the factors hold
+    int* status;            // the two words of a MEX workspace; then, per row of offsets, whether its spread is beyond what the factors hold
     int rows;               // R Mp of those
     int shift;              // log2 of the group
     int tiles_m;            // steps of instances
     int resident;           // all of them lie in shared memory
+    int expire;             // test hook: the first product is not taken, and waits are short
     long long tiles_j;      // tiles of positions of a region
 };
 
 // Whether the products have not been, or cannot be, taken (all threads of a CTA ask).
 __device__ __forceinline__ bool term_by_term(const FuseArgs& a) {
     int any = 0;
-    for (int i = threadIdx.x; i <= a.rows; i += blockDim.x) any |= a.status[i];
+    for (int i = threadIdx.x; i <= a.rows; i += blockDim.x) any |= a.status[1 + i];
     return __syncthreads_or(any) != 0;
+}
+
+// some tens of microseconds instead of two seconds
+__device__ __forceinline__ bool mbar_wait_briefly(uint64_t* bar, uint32_t parity) {
+    const uint32_t addr = smem_u32(bar);
+    for (int i = 0; i < 64; ++i) {
+        if (mbar_try(addr, parity)) return true;
+        __nanosleep(256);
+    }
+    return false;
 }
 
 // Place of (instance of a step, tap) in the partial sums of the step, neighbouring lanes side by side: a lane has four taps of an instance at
@@ -186,6 +198,7 @@ struct FuseShared {
     uint64_t quotients;     // workers: Q is there, S has been read
     uint64_t taps;          // products: the sums over the instances are there
     uint64_t instances;     // products: the sums over the positions are there, and Ex and Q may be written anew
+    uint64_t drained;       // products, after a wait that ran out: none is under way any more
     uint32_t tmem;
     volatile int failed;
 };
@@ -285,7 +298,7 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
     }
     if (threadIdx.x == 0) {
         mbar_init(&sh.operands, kFuseWorkers / 32); mbar_init(&sh.quotients, kFuseWorkers / 32);
-        mbar_init(&sh.sums[0], 1); mbar_init(&sh.sums[1], 1); mbar_init(&sh.taps, 1); mbar_init(&sh.instances, 1);
+        mbar_init(&sh.sums[0], 1); mbar_init(&sh.sums[1], 1); mbar_init(&sh.taps, 1); mbar_init(&sh.instances, 1); mbar_init(&sh.drained, 1);
         sh.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -303,7 +316,7 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
     uint32_t phase = 0;                                                                  // of the barriers that complete once a step
     // A wait that runs out sets `failed`; from then on nobody waits and no product is issued, and all leave by the ordinary way.
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (!sh.failed && !mbar_wait(bar, parity)) sh.failed = 1;
+        if (!sh.failed && !(a.expire ? mbar_wait_briefly(bar, parity) : mbar_wait(bar, parity))) sh.failed = 1;
         __syncwarp();                                                                    // (what follows is done by whole warps)
     };
     // (one arrival a warp: those of 512 threads follow one another)
@@ -320,7 +333,7 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
         auto issue_sums = [&](int mt) {
             const Operand<E, false> e_along(eb + (a.resident ? mt * E::kBytes : 0u));
             const int to = ahead ? mt & 1 : 0;
-            if (!sh.failed && elected()) {
+            if (!sh.failed && !a.expire && elected()) {
                 issue_in_turn<MC, KP / 16>(tS + to * MC, x_along, e_along);
                 umma_commit(&sh.sums[to]);
             }
@@ -354,6 +367,11 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
                 __syncwarp();
                 if (ahead && mt + 2 < a.tiles_m) issue_sums(mt + 2);                     // (into the place of the S that has been read)
             }
+        if (sh.failed) {                                                                 // tensor memory must not be freed under a product
+            if (elected()) umma_commit(&sh.drained);
+            __syncwarp();
+            mbar_wait(&sh.drained, 0);
+        }
     } else {
         const int p = threadIdx.x & 127, part4 = threadIdx.x >> 7;                      // position (tensor-memory lane) and its quarter of the columns
         const uint32_t lane_base = uint32_t(warp & 3) << 21;                             // (32 lanes a warp, lane number in bits 16 and up)
@@ -567,7 +585,7 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
     __syncthreads();
     if (warp == kFuseWorkers / 32)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(uint32_t(kFuseColumns)) : "memory");
-    if (sh.failed && threadIdx.x == 0) atomicExch(&a.status[0], 1);                      // a wait ran out: the kernel behind redoes the call
+    if (sh.failed && threadIdx.x == 0) atomicExch(&a.status[1], 1);                      // a wait ran out: the kernel behind redoes the call
 }
 
 // ---- the offsets' gradient from the CTAs' sums, or, for offsets that no factorisation takes, everything term by term ------------------
@@ -707,7 +725,14 @@ __global__ void __launch_bounds__(kFinishThreads) fuse_finish(MexGeo g, FuseArgs
     stream_order();
     __shared__ double sums[kFinishThreads / 32][128];
     __shared__ float work[3][128];
-    if (term_by_term(a)) {
+    const bool redo = term_by_term(a);
+    if (blockIdx.x == 0) {
+        int unsafe = 0;
+        for (int i = threadIdx.x; i < a.rows; i += kFinishThreads) unsafe |= a.status[2 + i];
+        unsafe = __syncthreads_or(unsafe);
+        if (threadIdx.x == 0) a.status[0] = unsafe != 0;
+    }
+    if (redo) {
         if (a.dx) redo_dx(g, a, f.off);
         if (f.doff) redo_doff(g, a, f, sums, work);
         return;
@@ -754,7 +779,7 @@ FuseWs fuse_carve(const MexGeo& g, void* base) {
     char* p = static_cast<char*>(base);
     size_t off = 0;
     auto take = [&](size_t bytes) { char* r = p ? p + off : nullptr; off += align256(bytes); return r; };
-    w.status = reinterpret_cast<int*>(take(sizeof(int) * (1 + (size_t)g.R * z.Mp)));
+    w.status = reinterpret_cast<int*>(take(sizeof(int) * (2 + (size_t)g.R * z.Mp)));
     w.eo = reinterpret_cast<float*>(take(sizeof(float) * (size_t)g.R * g.M * z.KP));
     w.tiles = reinterpret_cast<unsigned char*>(take((size_t)g.R * z.Mp * z.KP * 6));
     w.part = reinterpret_cast<float*>(take(sizeof(float) * (size_t)z.slots * g.R * z.Mp * z.KP));
@@ -785,14 +810,15 @@ cudaError_t launch_fused(const MexGeo& g, const FuseArgs& a, int ctas, cudaStrea
 
 // Blocks that cover the input once, in few regions (a CTA works for one).
 bool mex_checkpoint_shape(const MexGeo& g, bool f64, uint32_t flags) {
-    if (f64 || !g.finite || g.B == 0 || g.K > 128 || (flags & (SIMNETS_FLAG_FORCE_DIRECT | SIMNETS_FLAG_MEX_EXACT | SIMNETS_FLAG_MEX_NO_TENSORCORE))) return false;
+    // (a larger epsilon times log2 e is no float any more)
+    if (f64 || !g.finite || std::fabs(g.eps) > 1e30 || g.B == 0 || g.K > 128 || (flags & (SIMNETS_FLAG_FORCE_DIRECT | SIMNETS_FLAG_MEX_EXACT | SIMNETS_FLAG_MEX_NO_TENSORCORE))) return false;
     const bool cover = g.sc == g.bc && g.sh == g.bh && g.sw == g.bw && g.pc == 0 && g.ph == 0 && g.pw == 0 && g.Co * g.bc == g.C && g.Ho * g.bh == g.H && g.Wo * g.bw == g.W;
     return cover && g.R <= 16 && g.M <= 8192 && (long long)g.C * g.H * g.W < (1LL << 31) && (long long)g.B * g.rs < (1LL << 38);
 }
 size_t mex_checkpoint_bytes(const MexGeo& g) { return fuse_carve(g, nullptr).bytes; }
 
 cudaError_t launch_mex_checkpoint(const MexGeo& g, int group, const void* codes, const void* ranges, const float* off, const float* dy, float* dx, float* doff,
-                                  bool accumulate, bool normalized, void* ws, cudaStream_t s) {
+                                  bool accumulate, bool normalized, bool expire, void* ws, cudaStream_t s) {
     const FuseSizes z = fuse_sizes(g);
     const FuseWs w = fuse_carve(g, ws);
     FuseArgs a;
@@ -802,6 +828,7 @@ cudaError_t launch_mex_checkpoint(const MexGeo& g, int group, const void* codes,
     a.dy = dy; a.dx = dx; a.part = doff ? w.part : nullptr;
     a.status = w.status;
     a.rows = g.R * z.Mp;
+    a.expire = expire;
     a.shift = 5;
     while ((1 << a.shift) < group) ++a.shift;
     a.tiles_m = z.Mp / z.MC;

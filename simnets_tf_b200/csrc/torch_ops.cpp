@@ -488,6 +488,7 @@ struct Kept { Tensor codes, ranges; };
 Kept checkpoint_pack(const Tensor& x_in, int64_t group) {
     if (x_in.scalar_type() != at::kFloat && x_in.scalar_type() != at::kDouble) throw py::type_error("simnets ops are registered for float32 and float64 only");
     require_cuda_all(x_in);
+    refuse_tangents({&x_in});
     const at::AutoDispatchBelowADInplaceOrView below;
     const Tensor x = x_in.contiguous();
     const c10::cuda::CUDAGuard guard(x.device());
@@ -779,6 +780,7 @@ std::tuple<Tensor, Tensor, Tensor> route_apply(const Tensor& scores, const OptTe
 }
 
 std::tuple<Tensor, Tensor, Tensor> responsibilities(const Tensor& scores, const OptTensor& prior, const OptTensor& bias, int64_t top_k, int64_t groups, int64_t top_groups, bool sigmoid) {
+    refuse_tangents({&scores});
     const simnets_route_desc d = route_desc(scores, top_k, groups, top_groups, sigmoid, 1.0);
     const at::AutoDispatchBelowADInplaceOrView below;
     const Routed r = route_impl(scores, prior, bias, d, true);

@@ -252,6 +252,44 @@ def test_an_empty_batch():
     assert dx.shape == c["shape"] and float(dt.abs().max()) == 0.0 and float(dw.abs().max()) == 0.0
 
 
+def test_a_wait_that_runs_out_is_reported_and_recomputed(port, cuda_lib):
+    """abi.FLAG_MEX_TEST_EXPIRE_WAIT: the one-pass kernel's first product is withheld and its waits are short.  It must return (no hang, no
+    fault), say so in word 1 of the workspace, and the gradients must be right because the kernel behind redoes them."""
+    import ctypes as C
+    for name in ("k17", "k64", "k100", "tiles_4x2x2"):
+        c = next(c for c in DISJOINT if c["name"] == name)
+        x, off, dy = _mex_inputs(port, c, torch.float32)
+        kept = ck.checkpoint_pack(_dev(x), 64)
+        (rdx, rdoff), (adx, adoff) = _mex_oracle(port, c, ck.checkpoint_unpack(kept).cpu().numpy(), off, dy)
+        tol = _mex_tolerance(torch.float32, c, x, off, dy.size // c["M"])
+        od, dyd = _dev(off), _dev(dy)
+        unsafe = off.copy()
+        unsafe.reshape(off.shape[0] * off.shape[1], -1)[0, 0] = 200.0
+        for flags, given, want in ((0, od, (0, 0)), (abi.FLAG_MEX_TEST_EXPIRE_WAIT, od, (0, 1)), (0, _dev(unsafe), (1, 0)), (0, od, (0, 0))):
+            d = cases.mex_desc(c, flags=flags)
+            assert cuda_lib.simnets_mex_checkpoint_one_pass(C.byref(d)) == 1
+            ws = torch.full((cuda_lib.simnets_mex_checkpoint_workspace_bytes(C.byref(d)),), 255, dtype=torch.uint8, device="cuda")
+            dx, doff = torch.full(x.shape, float("nan"), device="cuda"), torch.full(off.shape, float("nan"), device="cuda")
+            stream = torch.cuda.current_stream().cuda_stream
+            assert cuda_lib.simnets_mex_checkpoint_gradients(C.byref(d), 64, kept.codes.data_ptr(), kept.ranges.data_ptr(), given.data_ptr(), dyd.data_ptr(), dx.data_ptr(),
+                                                             doff.data_ptr(), ws.data_ptr(), ws.numel(), stream) == 0
+            status = (C.c_int32 * 2)(7, 7)
+            assert cuda_lib.simnets_mex_workspace_status(ws.data_ptr(), stream, status) == 0
+            torch.cuda.synchronize()
+            assert (status[0], status[1]) == want, (name, flags)
+            if given is od:
+                assert (np.abs(dx.cpu().numpy() - rdx) <= tol * adx + 1e-30).all() and (np.abs(doff.cpu().numpy() - rdoff) <= tol * adoff + 1e-30).all()
+
+
+def test_which_shapes_take_one_pass(cuda_lib):
+    import ctypes as C
+    ask = lambda c, dtype=abi.F32, flags=0: cuda_lib.simnets_mex_checkpoint_one_pass(C.byref(cases.mex_desc(c, dtype=dtype, flags=flags)))
+    by_name = {c["name"]: c for c in DISJOINT + cases.MEX_SMALL}
+    assert [ask(by_name[n]) for n in ("one_tap", "k64", "k128", "tiles_2x3x3", "k129", "tiled_padded", "eps_pinf", "head_overlap")] == [1, 1, 1, 1, 0, 0, 0, 0]
+    assert ask(by_name["k64"], abi.F64) == 0 and ask(by_name["k64"], flags=abi.FLAG_MEX_EXACT) == 0
+    assert ask(dict(by_name["k64"], eps=1e31)) == 0 and ask(dict(by_name["k64"], shape=(0, 64, 16, 16))) == 0
+
+
 # ---- Similarity -----------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("c", cases.SIM_SMALL, ids=lambda c: c["name"])
@@ -396,6 +434,8 @@ def test_tangents_are_refused_and_recorded_calls_run_again():
     with forward_ad.dual_level():
         with pytest.raises(NotImplementedError):
             ck.mex_checkpointed(forward_ad.make_dual(x, torch.ones_like(x)), off, 20, **ATTRS)
+        with pytest.raises(NotImplementedError):
+            ck.checkpoint_pack(forward_ad.make_dual(x, torch.ones_like(x)))
     net = SimNet(SPECS["cfg3"], seed=1, checkpoint=128)
     image = torch.rand(3, 1, 28, 28, device="cuda") - 0.5
     traced = torch.jit.trace(net, (image,), check_trace=False)
