@@ -82,12 +82,10 @@ struct RouteArgs {
 // sample and place inside it
 __device__ __forceinline__ long long sample_of(const RouteArgs& a, long long p) { return a.f_N.d ? (long long)fast_div(uint32_t(p), a.f_N) : p / a.N; }
 
-constexpr int kBatch = 8;        // scores of a position in flight
-
 template <typename T> struct alignas(2 * sizeof(T)) Pair { T prior, bias; };
 
 // f(v, c) for components from .. to, every G-th from `sub` on; `add`: prior and bias of every component, or null for none
-template <int G, typename T, class F>
+template <int G, int kBatch, typename T, class F>
 __device__ __forceinline__ void over_range(const T* __restrict__ s, long long N, const Pair<T>* add, int from, int to, int sub, F f) {
     int c = from + sub;
     const T* q = s + c * N;
@@ -116,10 +114,10 @@ __device__ __forceinline__ void over_range(const T* __restrict__ s, long long N,
     }
 }
 // the largest of them, over the lanes of a position
-template <int G, typename T>
+template <int G, int kBatch, typename T>
 __device__ __forceinline__ T best_of_range(const T* __restrict__ s, long long N, const Pair<T>* add, int from, int to, int sub) {
     T best = below_all<T>();
-    over_range<G>(s, N, add, from, to, sub, [&](T v, int) { best = v > best ? v : best; });
+    over_range<G, kBatch>(s, N, add, from, to, sub, [&](T v, int) { best = v > best ? v : best; });
 #pragma unroll
     for (int d = 32 / G; d < 32; d <<= 1) {
         const T other = __shfl_xor_sync(0xffffffffu, best, d);
@@ -139,6 +137,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose(RouteArgs a, const
                                                               unsigned* __restrict__ part_load) {
     stream_order();
     constexpr int RUN = 32 / G, PLACES = kRouteThreads / G;
+    constexpr int kBatch = SUMS ? 16 : 8;                                                // scores of a position in flight (there are fewer warps beside the sums)
     extern __shared__ __align__(16) unsigned char route_smem[];
     T* const sums = reinterpret_cast<T*>(route_smem);                                    // [k][PLACES]
     Pair<T>* const add_s = reinterpret_cast<Pair<T>*>(sums + (SUMS ? (size_t)a.k * PLACES : 0));
@@ -160,7 +159,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose(RouteArgs a, const
         Top<T, TK> top;
         if (a.top_groups < a.groups) {
             top.clear();
-            for (int g = 0; g < a.groups; ++g) top.offer(best_of_range<G>(s, a.N, add, g * a.size, (g + 1) * a.size, sub), g);
+            for (int g = 0; g < a.groups; ++g) top.offer(best_of_range<G, kBatch>(s, a.N, add, g * a.size, (g + 1) * a.size, sub), g);
             open = 0;
 #pragma unroll
             for (int t = 0; t < TK; ++t) if (t < a.top_groups && top.i[t] >= 0) open |= 1ull << top.i[t];
@@ -168,10 +167,10 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose(RouteArgs a, const
         top.clear();
         if (a.top_groups < a.groups) {
             for (int g = 0; g < a.groups; ++g)
-                if (open >> g & 1) over_range<G>(s, a.N, add, g * a.size, (g + 1) * a.size, sub, [&](T v, int c) { top.offer(v, c); });
+                if (open >> g & 1) over_range<G, kBatch>(s, a.N, add, g * a.size, (g + 1) * a.size, sub, [&](T v, int c) { top.offer(v, c); });
             __syncwarp();
         } else {
-            over_range<G>(s, a.N, add, 0, a.k, sub, [&](T v, int c) { top.offer(v, c); });
+            over_range<G, kBatch>(s, a.N, add, 0, a.k, sub, [&](T v, int c) { top.offer(v, c); });
         }
         top.template merge<G, RUN>();
         // weights of the chosen: they sum to one over them
@@ -322,12 +321,11 @@ int route_lanes(const simnets_route_desc& d) { return d.positions * d.batch >= 5
 size_t sums_bytes(const simnets_route_desc& d) { return (d.dtype == SIMNETS_F64 ? 8 : 4) * (size_t)d.components * (kRouteThreads / route_lanes(d)); }
 bool route_sums(const simnets_route_desc& d) { return d.top_k > 1 && sums_bytes(d) <= 64 * 1024; }
 size_t choose_bytes(const simnets_route_desc& d, bool sums) { return (sums ? sums_bytes(d) : 0) + (size_t)d.components * (2 * (d.dtype == SIMNETS_F64 ? 8 : 4) + sizeof(unsigned)); }
-// as many CTAs as are resident together, each with as many tiles as the others
+// as many CTAs as are resident together
 int route_ctas(const simnets_route_desc& d, bool sums) {
     const long long places = kRouteThreads / route_lanes(d), tiles = (d.positions * d.batch + places - 1) / places;
     const long long resident = std::max<long long>(1, std::min<long long>(12, 220 * 1024 / (choose_bytes(d, sums) + 2048))) * device_sm_count();
-    const long long rounds = std::max<long long>(1, (tiles + resident - 1) / resident);
-    return int(std::max<long long>(1, (tiles + rounds - 1) / rounds));
+    return int(std::max<long long>(1, std::min(tiles, resident)));
 }
 int most_ctas(const simnets_route_desc& d) { return std::max(route_ctas(d, false), route_ctas(d, route_sums(d))); }
 int mass_splits(const simnets_route_desc& d) {
