@@ -399,7 +399,8 @@ SIMNETS_API int simnets_checkpoint_unpack(int32_t dtype, int64_t count, int32_t 
 /* Gradients of a layer at a checkpoint of its input: those of the op at the values that the codes stand for.
  * MEX: y is computed again from them instead of being kept; a NULL dx or doffsets is not computed; d->flags as for
  * simnets_mex_gradients, without SIMNETS_FLAG_MEX_WORKSPACE_PRIMED and SIMNETS_FLAG_MEX_MAXIMA_GIVEN
- * (SIMNETS_E_UNSUPPORTED).  Similarity: a NULL dx is not computed, nor are dtemplates and dweights where both are NULL. */
+ * (SIMNETS_E_UNSUPPORTED); where it takes one pass (below) ranges must lie on a multiple of 8 bytes (SIMNETS_E_UNSUPPORTED).
+ * Similarity: a NULL dx is not computed, nor are dtemplates and dweights where both are NULL. */
 SIMNETS_API size_t simnets_mex_checkpoint_workspace_bytes(const simnets_mex_desc* d);
 /* 1 where one kernel makes both gradients from the bytes (float32, finite epsilon, blocks of up to 128 taps that cover the
  * input once, up to 16 regions); neither x nor y is written there, and simnets_mex_workspace_status reads the workspace.

@@ -465,6 +465,7 @@ int simnets_mex_checkpoint_gradients(const simnets_mex_desc* d, int32_t group, c
     if (!off || (g.B > 0 && (!codes || !ranges || !dy || (!dx && !doff)))) return SIMNETS_E_NULL;
     if (g.B == 0) return mex_gradients(g, d, nullptr, off, nullptr, nullptr, nullptr, doff, ws, ws_bytes, nullptr, 0, as_stream(stream));
     if (mex_checkpoint_shape(g, d->dtype == SIMNETS_F64, d->flags)) {
+        if (reinterpret_cast<uintptr_t>(ranges) % 8) return SIMNETS_E_UNSUPPORTED;          // (read as pairs)
         if (!ws || ws_bytes < mex_checkpoint_bytes(g)) return SIMNETS_E_WORKSPACE;
         return from_cuda(launch_mex_checkpoint(g, group, codes, ranges, (const float*)off, (const float*)dy, (float*)dx, (float*)doff, (d->flags & SIMNETS_FLAG_ACCUMULATE) != 0,
                                                (d->flags & SIMNETS_FLAG_MEX_NORMALIZED_OFFSETS) != 0, (d->flags & SIMNETS_FLAG_MEX_TEST_EXPIRE_WAIT) != 0, ws, as_stream(stream)));

@@ -514,11 +514,12 @@ Tensor checkpoint_unpack(const Tensor& codes, const Tensor& ranges, const std::v
     return x;
 }
 
-std::pair<Tensor, Tensor> mex_checkpoint_grads(const MexPlan& p, const Tensor& codes, const Tensor& ranges, int64_t group, const Tensor& off_in, const Tensor& dy_in,
+std::pair<Tensor, Tensor> mex_checkpoint_grads(const MexPlan& p, const Tensor& codes, const Tensor& ranges_in, int64_t group, const Tensor& off_in, const Tensor& dy_in,
                                                uint32_t flags, bool pooled, bool want_dx, bool want_doff, const OptTensor& out) {
-    check_checkpoint(codes, ranges, group, int64_t(p.d.batch) * p.d.channels * p.d.height * p.d.width);
-    require_cuda_all(ranges, off_in, dy_in);
-    if ((ranges.scalar_type() == at::kDouble) != (p.d.dtype == SIMNETS_F64)) throw py::type_error("input does not have the planned dtype");
+    check_checkpoint(codes, ranges_in, group, int64_t(p.d.batch) * p.d.channels * p.d.height * p.d.width);
+    require_cuda_all(ranges_in, off_in, dy_in);
+    if ((ranges_in.scalar_type() == at::kDouble) != (p.d.dtype == SIMNETS_F64)) throw py::type_error("input does not have the planned dtype");
+    const Tensor ranges = reinterpret_cast<uintptr_t>(ranges_in.data_ptr()) % 8 ? ranges_in.clone() : ranges_in;        // (read as pairs)
     p.check_offsets(off_in);
     p.check_dy(dy_in, pooled);
     const Tensor off = off_in.contiguous(), dy = dy_in.contiguous();

@@ -216,13 +216,13 @@ def test_offsets_that_no_factorisation_takes(port, name):
 
 @pytest.mark.parametrize("name", ["k17", "k64", "k100", "tiles_4x2x2"])
 def test_missing_and_infinite_activations(port, name):
-    """-infinity is a tap of no weight; a patch with a NaN has NaN gradients, and so have the offsets that it adds to."""
+    """-infinity is a tap of no weight; a patch with a NaN or infinity has NaN gradients, and so have the offsets that it adds to."""
     c = next(c for c in DISJOINT if c["name"] == name)
     x, off, dy = _mex_inputs(port, c, torch.float32)
     x = x.copy()
     x[:, 1::3] = -np.inf
     _check_mex(port, c, torch.float32, x, off, dy, 32)
-    x[0, 0, 0, 0] = np.nan
+    x[0, 0, 0, 0], x[-1, 0, -1, -1] = np.nan, np.inf
     kept = ck.checkpoint_pack(_dev(x), 32)
     dx, doff = ck.mex_checkpoint_backward(kept, _dev(off), _dev(dy), c["M"], **cases.mex_attrs(c))
     (rdx, rdoff), (adx, _) = _mex_oracle(port, c, ck.checkpoint_unpack(kept).cpu().numpy(), off, dy)
@@ -279,6 +279,24 @@ def test_a_wait_that_runs_out_is_reported_and_recomputed(port, cuda_lib):
             assert (status[0], status[1]) == want, (name, flags)
             if given is od:
                 assert (np.abs(dx.cpu().numpy() - rdx) <= tol * adx + 1e-30).all() and (np.abs(doff.cpu().numpy() - rdoff) <= tol * adoff + 1e-30).all()
+
+
+def test_codes_and_ranges_anywhere_in_memory(cuda_lib):
+    import ctypes as C
+    c = next(c for c in DISJOINT if c["name"] == "k64")
+    x, off, dy = (torch.randn(s, device="cuda") for s in (c["shape"], (4, 128, 64, 1, 1), (4, 128, 16, 16)))
+    kept = ck.checkpoint_pack(x, 32)
+    codes, ranges = torch.zeros(kept.codes.numel() + 3, dtype=torch.uint8, device="cuda"), torch.zeros(kept.ranges.numel() + 1, device="cuda")
+    codes[3:], ranges[1:] = kept.codes, kept.ranges.reshape(-1)
+    moved = ck.Checkpoint(codes[3:], ranges[1:].view(-1, 2), kept.shape, 32)
+    assert moved.ranges.data_ptr() % 8 == 4 and moved.codes.data_ptr() % 4 == 3
+    want = ck.mex_checkpoint_backward(kept, off, dy, 128, **cases.mex_attrs(c))
+    for got, ref in zip(ck.mex_checkpoint_backward(moved, off, dy, 128, **cases.mex_attrs(c)), want):
+        assert torch.equal(got, ref)
+    d = cases.mex_desc(c)
+    ws = torch.empty(cuda_lib.simnets_mex_checkpoint_workspace_bytes(C.byref(d)), dtype=torch.uint8, device="cuda")
+    assert cuda_lib.simnets_mex_checkpoint_gradients(C.byref(d), 32, moved.codes.data_ptr(), moved.ranges.data_ptr(), off.data_ptr(), dy.data_ptr(), x.data_ptr(), off.data_ptr(),
+                                                     ws.data_ptr(), ws.numel(), None) == abi.E_UNSUPPORTED
 
 
 def test_which_shapes_take_one_pass(cuda_lib):

@@ -1,9 +1,13 @@
 """Routing without a GPU: what its entry points refuse, the estimators that balance their components on stand-in statistics."""
 import ctypes as C
+import os
+import socket
 
 import numpy as np
 import pytest
 import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
 
 import plain_operators as plain
 from oracle import unsupervised_oracle as uo
@@ -106,6 +110,39 @@ def test_balance_brings_idle_components_into_use(kind):
         centres = est.centres if kind == "kmeans" else est.means
         load[balance] = bool((centres[4:] < 11).any())
     assert load == {0.0: False, 6.0: True}
+
+
+def _worker(rank, world, port, out):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        rng = np.random.default_rng(4)
+        first, batches = rng.normal(size=(4, 2, 5, 5)), [rng.normal(size=(4, 2, 5, 5)) for _ in range(3)]
+        u, picks, res = rng.random(3), rng.integers(0, 36, 3), []
+        for group, lo, hi in ((dist.group.WORLD, 2 * rank, 2 * rank + 2), (None, 0, 4)):
+            km = un.KMeans((3, 3), (1, 1), 3, ops=Ops((3, 3), (1, 1)), group=group, balance=0.75)
+            gm = un.DiagonalGMM((3, 3), (1, 1), 3, ops=Ops((3, 3), (1, 1)), group=group, top_k=2, balance=0.25)
+            km.init(torch.from_numpy(first), uniforms=u)
+            gm.init(torch.from_numpy(first), picks=picks)
+            for b in batches:
+                km.update(torch.from_numpy(b[lo:hi]))
+                gm.update(torch.from_numpy(b[lo:hi]))
+            res.append(torch.cat([km.centres.flatten(), km.counts, km.bias, gm.means.flatten(), gm.covs.flatten(), gm.bias]))
+        if rank == 0:
+            np.save(out, np.array([float((res[0] - res[1]).abs().max()), float(res[1].abs().max())]))
+    finally:
+        dist.destroy_process_group()
+
+
+def test_balance_over_two_ranks_equals_the_unsharded_step(tmp_path):
+    """Biases follow the loads of all ranks."""
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    out = str(tmp_path / "r.npy")
+    mp.spawn(_worker, args=(2, port, out), nprocs=2, join=True)
+    err, scale = np.load(out)
+    assert scale > 0 and err < 1e-12 * max(scale, 1.0)
 
 
 def test_estimators_check_their_new_arguments():
