@@ -130,6 +130,12 @@ enum { SIMNETS_SIM_L1 = 0, SIMNETS_SIM_L2 = 1 };
  * workspace that was reused in between gives wrong gradients, not an error. */
 #define SIMNETS_FLAG_MEX_WORKSPACE_PRIMED (1u << 8)
 
+/* simnets_mex_checkpoint_gradients where it does not take one pass: run the kernels that simnets_mex_forward and the gradient
+ * entry points run for the layer, tensor cores included, whose truncated sums put y of a 256-tap layer 8e-6 of its norm from
+ * float64 and its gradients 1e-5.  Without the flag sums are in FP32 (256 taps under 512 instances, 2048 x 8 x 8 positions:
+ * 4.7 ms against 0.9).  The layers set it: their gradients are then as exact as without a checkpoint. */
+#define SIMNETS_FLAG_MEX_CHECKPOINT_TENSORCORE (1u << 16)
+
 /* ---- Similarity ---------------------------------------------------------- */
 /* Mirrors the attrs of the Similarity op family (src/ops/similarity_op.cpp:61-75)
  * and the dimensions SimilarityKernelCommon::CalculateDimensions derives
@@ -404,8 +410,8 @@ SIMNETS_API int simnets_checkpoint_unpack(int32_t dtype, int64_t count, int32_t 
 SIMNETS_API size_t simnets_mex_checkpoint_workspace_bytes(const simnets_mex_desc* d);
 /* 1 where one kernel makes both gradients from the bytes (float32, finite epsilon, blocks of up to 128 taps that cover the
  * input once, up to 16 regions); neither x nor y is written there, and simnets_mex_workspace_status reads the workspace.
- * Elsewhere the bytes become x in the workspace, and y is computed from it by the kernels of the other entry points with sums
- * in FP32. */
+ * Elsewhere the bytes become x in the workspace, and y is computed from it by the kernels of the other entry points, with sums
+ * in FP32 unless SIMNETS_FLAG_MEX_CHECKPOINT_TENSORCORE is set. */
 SIMNETS_API int simnets_mex_checkpoint_one_pass(const simnets_mex_desc* d);
 SIMNETS_API int simnets_mex_checkpoint_gradients(const simnets_mex_desc* d, int32_t group, const void* codes, const void* ranges,
                                                  const void* offsets, const void* dy, void* dx, void* doffsets,

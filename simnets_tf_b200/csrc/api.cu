@@ -73,6 +73,7 @@ int checkpoint_check(int32_t dtype, int64_t count, int32_t group) {
 // 524288 positions: gradients 1.2e-5 of their norm off, with FP32 sums 1.3e-6).
 uint32_t checkpoint_route(const MexGeo& g, const simnets_mex_desc& d) {
     const bool f64 = d.dtype == SIMNETS_F64;
+    if (d.flags & SIMNETS_FLAG_MEX_CHECKPOINT_TENSORCORE) return 0u;
     return mex_use_gemm(g, f64, d.flags) || mex_gradients_by_gemm(g, f64, d.flags) ? 0u : uint32_t(SIMNETS_FLAG_MEX_NO_TENSORCORE);
 }
 

@@ -621,7 +621,7 @@ Tensor mex_checkpoint_apply(const MexPlanPtr& p, const Tensor& x, const Tensor& 
     node->off = SavedVariable(off, false);
     node->sink = sink;
     node->group = group;
-    node->flags = op_flags;
+    node->flags = op_flags | SIMNETS_FLAG_MEX_CHECKPOINT_TENSORCORE;           // (as exact as the layer's gradients without a checkpoint)
     node->pooled = pooled;
     torch::autograd::set_history(out, node);
     return out;

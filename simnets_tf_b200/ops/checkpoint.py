@@ -87,7 +87,8 @@ def _four(checkpoint):
 
 def mex_checkpoint_backward(checkpoint, offsets, output_grad, num_instances, flags=0, pooled=False, doff_out=None, **attrs):
     """(input_grad, offsets_grad) of the `Mex` op at a checkpoint of its input; the output is computed again.  `pooled`, FLAG_ACCUMULATE
-    with `doff_out`, and `attrs` as in `mex_backward`."""
+    with `doff_out`, and `attrs` as in `mex_backward`.  Sums are in FP32; abi.FLAG_MEX_CHECKPOINT_TENSORCORE (which `mex_checkpointed` and the
+    layers set) lets blocks of more than 128 taps take the tensor-core kernels of the ordinary gradients, with their accuracy."""
     plan = mex_plan(_four(checkpoint), checkpoint.dtype, num_instances, _mex_attrs(**attrs))
     return _lib.ops().mex_checkpoint_backward(plan, checkpoint.codes, checkpoint.ranges, checkpoint.group, offsets, output_grad, flags, pooled, doff_out)
 

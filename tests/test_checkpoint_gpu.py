@@ -281,6 +281,22 @@ def test_a_wait_that_runs_out_is_reported_and_recomputed(port, cuda_lib):
                 assert (np.abs(dx.cpu().numpy() - rdx) <= tol * adx + 1e-30).all() and (np.abs(doff.cpu().numpy() - rdoff) <= tol * adoff + 1e-30).all()
 
 
+def test_long_patches_with_the_sums_of_the_ordinary_gradients(port):
+    """abi.FLAG_MEX_CHECKPOINT_TENSORCORE: what the ordinary gradients give at the checkpoint's values, to the library's bound."""
+    c = _pixel("k200", 3, 200, 16, 16, 96, seed=30, flags=abi.FLAG_MEX_NO_SMALL_TILES)
+    x, off, dy = _mex_inputs(port, c, torch.float32)
+    kept = ck.checkpoint_pack(_dev(x), 64)
+    at = ck.checkpoint_unpack(kept)
+    got = ck.mex_checkpoint_backward(kept, _dev(off), _dev(dy), 96, flags=c["flags"] | abi.FLAG_MEX_CHECKPOINT_TENSORCORE, **cases.mex_attrs(c))
+    y = mex_ops.mex_forward(at, _dev(off), 96, flags=c["flags"], **cases.mex_attrs(c))
+    for a, b in zip(got, mex_ops.mex_backward(at, _dev(off), y, _dev(dy), 96, flags=c["flags"], **cases.mex_attrs(c))):
+        assert torch.equal(a, b)
+    (rdx, rdoff), _ = _mex_oracle(port, c, at.cpu().numpy(), off, dy)
+    # y and the sums over instances are each 3 x 2^-23 off for every eight terms (library bound on its tensor-core sums)
+    for a, ref in zip(got, (rdx, rdoff)):
+        assert np.abs(a.cpu().numpy() - ref).max() <= 3 * 2.0 ** -23 * ((200 + 96) / 8 + 768 / 8) * np.abs(ref).max()
+
+
 def test_codes_and_ranges_anywhere_in_memory(cuda_lib):
     import ctypes as C
     c = next(c for c in DISJOINT if c["name"] == "k64")
