@@ -18,8 +18,11 @@
 // (96 cycles for three).  Accumulators are emptied into FP32 after every 128 positions.
 //
 // Sixteen warps work on the values and one issues the products: a tile's bytes are read and exponentiated while the second product of the tile
-// in front runs, its dx leaves during the third.  (All phases in turn, 512 x 64 x 32 x 32 under 128 instances: 519 us, of them 190 for
-// the bytes' way into registers.)
+// in front runs, the offsets' sums are added to the CTA's while the first one runs.  512 x 64 x 32 x 32 under 128 instances, pooled: 252 us
+// (all phases in turn, descriptors made anew for every instruction: 519; the FP32 kernels of the other entry points 1267; the floor of the
+// products 95); 32 x 256 x 32 x 32 under 256 instances over 4x2x2 blocks 224 us (499; 1463; bytes 88).  Where the rest goes: a tile is a chain of
+// Ex, S, Q, sums, next Ex, the operands of one tile fill shared memory, and 96 registers a thread are what 17 warps have; warps wait for loads 3.6 of
+// 9 cycles, the tensor pipe is busy 27 %.  Half of the warps for the taps and half for the instances were slower (266, 280).
 //
 // Offsets whose spread is beyond what the factors hold are found in the prepass; the kernel then leaves at once and the one behind it, which
 // else adds up the partial sums, evaluates term by term.

@@ -126,9 +126,11 @@ __device__ __forceinline__ T best_of_range(const T* __restrict__ s, long long N,
     return best;
 }
 
-// Bound: HBM, the scores read once and, for the dense form, as much written (512 x 64 x 30 x 30 float32: 236 MB, 36 us).
+// Bound: HBM, the scores read once and, for the dense form, as much written (512 x 64 x 30 x 30 float32: 236 MB, 36 us).  The nearest one of
+// 64 components takes 52 us (4.5 TB/s); cut to four 80: a place of the list is five instructions of the half-rate pipe per component (66 % busy).
 //
-// G lanes share a position, neighbouring lanes are neighbouring positions; a lane has eight scores in flight and keeps a sorted list of TK.
+// G lanes share a position (four where positions are few), neighbouring lanes are neighbouring positions; a lane has eight or sixteen scores in
+// flight and keeps a sorted list of TK.  (A position's scores in the registers of four lanes, with lists of values only: 105 us.)
 // With SUMS every thread adds the weights that it gives to sums of its own in shared memory, one per component, which the CTA adds up at its
 // end: the masses cost no second pass over the dense form, and come out the same on every run.
 template <typename T, int TK, int G, bool SUMS>
