@@ -133,7 +133,7 @@ __device__ __forceinline__ T best_of_range(const T* __restrict__ s, long long N,
 // flight and keeps a sorted list of TK.  (A position's scores in the registers of four lanes, with lists of values only: 105 us.)
 // With SUMS every thread adds the weights that it gives to sums of its own in shared memory, one per component, which the CTA adds up at its
 // end: the masses cost no second pass over the dense form, and come out the same on every run.
-template <typename T, int TK, int G, bool SUMS>
+template <typename T, int TK, int G, bool SUMS, bool GROUPS>
 __global__ void __launch_bounds__(kRouteThreads) route_choose(RouteArgs a, const T* __restrict__ scores, const T* __restrict__ prior, const T* __restrict__ bias,
                                                               int* __restrict__ index, T* __restrict__ weights, T* __restrict__ dense, T* __restrict__ part_mass,
                                                               unsigned* __restrict__ part_load) {
@@ -157,19 +157,51 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose(RouteArgs a, const
         const bool live = p < a.positions;
         const long long n = sample_of(a, live ? p : p0), j = (live ? p : p0) - n * a.N;
         const T* s = scores + n * a.k * a.N + j;
-        unsigned long long open = ~0ull;                 // groups that are in the choice
+        unsigned long long open = 0;                     // groups that are in the choice
         Top<T, TK> top;
-        if (a.top_groups < a.groups) {
+        if constexpr (GROUPS) {
             top.clear();
-            for (int g = 0; g < a.groups; ++g) top.offer(best_of_range<G, kBatch>(s, a.N, add, g * a.size, (g + 1) * a.size, sub), g);
-            open = 0;
+            if (a.size <= G * kBatch) {                  // several groups in flight
+                constexpr int S = 4;
+                for (int g0 = 0; g0 < a.groups; g0 += S) {
+                    T v[S][kBatch], best[S];
+#pragma unroll
+                    for (int j = 0; j < S; ++j)
+#pragma unroll
+                        for (int u = 0; u < kBatch; ++u) {
+                            const int c = sub + G * u;
+                            v[j][u] = c < a.size && g0 + j < a.groups ? __ldg(s + ((g0 + j) * a.size + c) * a.N) : below_all<T>();
+                        }
+#pragma unroll
+                    for (int j = 0; j < S; ++j) {
+                        best[j] = below_all<T>();
+#pragma unroll
+                        for (int u = 0; u < kBatch; ++u) {
+                            const int c = (g0 + j) * a.size + sub + G * u;
+                            if (add && sub + G * u < a.size && g0 + j < a.groups) v[j][u] = (v[j][u] + add[c].prior) + add[c].bias;
+                            best[j] = v[j][u] > best[j] ? v[j][u] : best[j];
+                        }
+#pragma unroll
+                        for (int d = RUN; d < 32; d <<= 1) {
+                            const T other = __shfl_xor_sync(0xffffffffu, best[j], d);
+                            best[j] = other > best[j] ? other : best[j];
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < S; ++j) top.offer(best[j], g0 + j);
+                }
+            } else {
+                for (int g = 0; g < a.groups; ++g) top.offer(best_of_range<G, kBatch>(s, a.N, add, g * a.size, (g + 1) * a.size, sub), g);
+            }
 #pragma unroll
             for (int t = 0; t < TK; ++t) if (t < a.top_groups && top.i[t] >= 0) open |= 1ull << top.i[t];
         }
         top.clear();
-        if (a.top_groups < a.groups) {
-            for (int g = 0; g < a.groups; ++g)
-                if (open >> g & 1) over_range<G, kBatch>(s, a.N, add, g * a.size, (g + 1) * a.size, sub, [&](T v, int c) { top.offer(v, c); });
+        if constexpr (GROUPS) {
+            for (; open; open &= open - 1) {             // (by rising index; every position has about as many)
+                const int g = __ffsll((long long)open) - 1;
+                over_range<G, kBatch>(s, a.N, add, g * a.size, (g + 1) * a.size, sub, [&](T v, int c) { top.offer(v, c); });
+            }
             __syncwarp();
         } else {
             over_range<G, kBatch>(s, a.N, add, 0, a.k, sub, [&](T v, int c) { top.offer(v, c); });
@@ -321,7 +353,7 @@ RouteArgs args_of(const simnets_route_desc& d) {
 int route_lanes(const simnets_route_desc& d) { return d.positions * d.batch >= 512LL * device_sm_count() || d.components < 8 ? 1 : 4; }
 // a CTA's sums fit the shared memory of a multiprocessor three times
 size_t sums_bytes(const simnets_route_desc& d) { return (d.dtype == SIMNETS_F64 ? 8 : 4) * (size_t)d.components * (kRouteThreads / route_lanes(d)); }
-bool route_sums(const simnets_route_desc& d) { return d.top_k > 1 && sums_bytes(d) <= 64 * 1024; }
+bool route_sums(const simnets_route_desc& d) { return d.top_k > 1 && d.top_groups == d.groups && sums_bytes(d) <= 64 * 1024; }
 size_t choose_bytes(const simnets_route_desc& d, bool sums) { return (sums ? sums_bytes(d) : 0) + (size_t)d.components * (2 * (d.dtype == SIMNETS_F64 ? 8 : 4) + sizeof(unsigned)); }
 // as many CTAs as are resident together
 int route_ctas(const simnets_route_desc& d, bool sums) {
@@ -336,16 +368,16 @@ int mass_splits(const simnets_route_desc& d) {
 }
 size_t load_bytes(const simnets_route_desc& d) { return (sizeof(unsigned) * (size_t)most_ctas(d) * d.components + 255) & ~size_t(255); }
 
-template <typename T, int TK, int G, bool SUMS>
+template <typename T, int TK, int G, bool SUMS, bool GROUPS>
 cudaError_t choose(const simnets_route_desc& d, const RouteArgs& a, const void* scores, const void* prior, const void* bias, int* index, void* weights, void* dense,
                    T* part_mass, unsigned* part_load, cudaStream_t s) {
     const size_t smem = choose_bytes(d, SUMS);
     static SmemLimit limit;
     if (smem > 32 * 1024) {
-        const cudaError_t e = limit.raise(route_choose<T, TK, G, SUMS>, 160 * 1024);
+        const cudaError_t e = limit.raise(route_choose<T, TK, G, SUMS, GROUPS>, 160 * 1024);
         if (e != cudaSuccess) return e;
     }
-    in_stream_order(route_choose<T, TK, G, SUMS>, route_ctas(d, SUMS), kRouteThreads, smem, s)(a, (const T*)scores, (const T*)prior, (const T*)bias, index, (T*)weights, (T*)dense, part_mass, part_load);
+    in_stream_order(route_choose<T, TK, G, SUMS, GROUPS>, route_ctas(d, SUMS), kRouteThreads, smem, s)(a, (const T*)scores, (const T*)prior, (const T*)bias, index, (T*)weights, (T*)dense, part_mass, part_load);
     return cudaSuccess;
 }
 
@@ -358,11 +390,15 @@ cudaError_t route(const simnets_route_desc& d, const void* scores, const void* p
     unsigned* part_load = static_cast<unsigned*>(ws);
     T* part_mass = reinterpret_cast<T*>(static_cast<char*>(ws) + load_bytes(d));
     cudaError_t e = cudaSuccess;
-#define ROUTE(TK) e = sums ? (one ? choose<T, TK, 1, true>(d, a, scores, prior, bias, index, weights, dense, part_mass, part_load, s)                     \
-                                  : choose<T, TK, 4, true>(d, a, scores, prior, bias, index, weights, dense, part_mass, part_load, s))                    \
-                           : (one ? choose<T, TK, 1, false>(d, a, scores, prior, bias, index, weights, dense, part_mass, part_load, s)                    \
-                                  : choose<T, TK, 4, false>(d, a, scores, prior, bias, index, weights, dense, part_mass, part_load, s))
-    if (want <= 1) ROUTE(1); else if (want <= 2) ROUTE(2); else if (want <= 4) ROUTE(4); else if (want <= 8) ROUTE(8); else ROUTE(16);
+#define CHOOSE(TK, G, SUMS, GROUPS) choose<T, TK, G, SUMS, GROUPS>(d, a, scores, prior, bias, index, weights, dense, part_mass, part_load, s)
+#define ROUTE(TK) e = sums ? (one ? CHOOSE(TK, 1, true, false) : CHOOSE(TK, 4, true, false))                                                            \
+                           : a.top_groups < a.groups ? (one ? CHOOSE(TK, 1, false, true) : CHOOSE(TK, 4, false, true))                                   \
+                                                     : (one ? CHOOSE(TK, 1, false, false) : CHOOSE(TK, 4, false, false))
+    if (want <= 1) ROUTE(1);
+    else if (sizeof(T) == 8 ? want <= 4 : false) ROUTE(4);               // (float64: fewer lengths of the list)
+    else if constexpr (sizeof(T) == 4) { if (want <= 2) ROUTE(2); else if (want <= 4) ROUTE(4); else if (want <= 8) ROUTE(8); else ROUTE(16); }
+    else ROUTE(16);
+#undef CHOOSE
 #undef ROUTE
     if (e != cudaSuccess) return e;
     if (mass && !sums && !counted) in_stream_order(route_mass<T>, dim3(a.k, splits), 256, 0, s)(a, (long long)d.batch, (const T*)dense, part_mass);

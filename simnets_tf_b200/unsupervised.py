@@ -153,7 +153,7 @@ class KMeans(_Estimator):
             cum = np.cumsum(nearest.double().cpu().numpy())
             pick = n - 1 if cum[-1] <= 0 else min(int(np.searchsorted(cum, u[c] * cum[-1], side="right")), n - 1)
             centres.append(_patch_at(x, self.blocks, self.strides, pick))
-        self.centres = torch.stack(centres).contiguous()
+        self.centres, self.bias = torch.stack(centres).contiguous(), None
         self.counts = torch.zeros(self.k, dtype=x.dtype, device=x.device)
         return self.centres
 
@@ -210,7 +210,7 @@ class DiagonalGMM(_Estimator):
         oh, ow = _patch_grid(x, self.blocks, self.strides)
         n = x.shape[0] * oh * ow
         picks = self.rng.randint(0, n, size=self.k) if picks is None else picks
-        self.means = torch.stack([_patch_at(x, self.blocks, self.strides, p) for p in picks]).contiguous()
+        self.means, self.bias = torch.stack([_patch_at(x, self.blocks, self.strides, p) for p in picks]).contiguous(), None
         # variance of the data in two passes (mean first, then squares about it: no cancellation in float32)
         ones = torch.ones((x.shape[0], 1, oh, ow), dtype=x.dtype, device=x.device)
         zero = torch.zeros_like(self.means[:1])

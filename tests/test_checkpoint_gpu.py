@@ -151,6 +151,7 @@ DISJOINT = [
     _pixel("k17", 3, 17, 8, 8, 33, seed=5), _pixel("k32", 2, 32, 16, 16, 64, seed=6), _pixel("k33", 5, 33, 6, 10, 65, 0, seed=7), _pixel("k64", 4, 64, 16, 16, 128, seed=8),
     _pixel("k64_m129", 3, 64, 8, 8, 129, seed=9), _pixel("k65", 2, 65, 10, 10, 70, seed=10), _pixel("k100", 3, 100, 6, 8, 200, seed=11), _pixel("k128", 2, 128, 16, 16, 256, seed=12),
     _pixel("k129", 2, 129, 6, 6, 60, seed=13), _pixel("uneven", 2, 40, 7, 9, 50, 4, seed=14), _pixel("one_position", 1, 24, 1, 1, 5, 0, seed=15),
+    _pixel("many_instances", 2, 16, 6, 6, 1200, seed=22), _pixel("many_of_k64", 2, 50, 4, 4, 300, 0, seed=23), _pixel("many_of_k128", 1, 90, 4, 4, 400, seed=24),
     _pixel("eps_small", 2, 48, 8, 8, 48, seed=16, eps=0.25), _pixel("eps_negative", 2, 48, 8, 8, 48, 0, seed=17, eps=-1.5), _pixel("wide", 7, 20, 30, 30, 300, 0, seed=18),
     cases.mex_case("tiles_4x2x2", (3, 32, 8, 8), 60, (4, 2, 2), (4, 2, 2), eps=0.5, unshared=False, seed=19),
     cases.mex_case("tiles_2x3x3", (2, 8, 9, 12), 130, (2, 3, 3), (2, 3, 3), softmax=True, unshared_region=(2,), seed=20),
