@@ -127,10 +127,12 @@ __device__ __forceinline__ T best_of_range(const T* __restrict__ s, long long N,
 }
 
 // Bound: HBM, the scores read once and, for the dense form, as much written (512 x 64 x 30 x 30 float32: 236 MB, 36 us).  The nearest one of
-// 64 components takes 52 us (4.5 TB/s); cut to four 80: a place of the list is five instructions of the half-rate pipe per component (66 % busy).
+// 64 components takes 54 us (4.4 TB/s); cut to four 81: a place of the list is five instructions of the half-rate pipe per component (66 % busy).
 //
 // G lanes share a position (four where positions are few), neighbouring lanes are neighbouring positions; a lane has eight or sixteen scores in
-// flight and keeps a sorted list of TK.  (A position's scores in the registers of four lanes, with lists of values only: 105 us.)
+// flight and keeps a sorted list of TK.  (A position's scores in the registers of four lanes, with lists of values only: 105 us; two passes, values
+// alone in sorting networks and then who reaches the last of them: 100.)  192 components in groups, 64 x 15 x 15, six of three of eight groups: 17 us with the
+// maxima of four groups in flight (23 with one).
 // With SUMS every thread adds the weights that it gives to sums of its own in shared memory, one per component, which the CTA adds up at its
 // end: the masses cost no second pass over the dense form, and come out the same on every run.
 template <typename T, int TK, int G, bool SUMS, bool GROUPS>
@@ -286,7 +288,7 @@ __global__ void __launch_bounds__(256) route_mass(RouteArgs a, long long batch, 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(128) route_totals(int ctas, int splits, int k, const unsigned* __restrict__ part_load, const T* __restrict__ part_mass,
+__global__ void __launch_bounds__(128) route_totals(int ctas, int splits, int k, T weight, const unsigned* __restrict__ part_load, const T* __restrict__ part_mass,
                                                     long long* __restrict__ load, T* __restrict__ mass) {
     stream_order();
     __shared__ long long red[128];
@@ -303,7 +305,7 @@ __global__ void __launch_bounds__(128) route_totals(int ctas, int splits, int k,
     }
     if (threadIdx.x == 0) {
         load[blockIdx.x] = red[0];
-        if (mass) mass[blockIdx.x] = splits > 0 ? redm[0] : T(red[0]);
+        if (mass) mass[blockIdx.x] = splits > 0 ? redm[0] : weight * T(red[0]);
     }
 }
 
@@ -385,7 +387,7 @@ template <typename T>
 cudaError_t route(const simnets_route_desc& d, const void* scores, const void* prior, const void* bias, int* index, void* weights, void* dense, long long* load,
                   void* mass, void* ws, cudaStream_t s) {
     const RouteArgs a = args_of(d);
-    const bool sums = dense && route_sums(d), one = route_lanes(d) == 1, counted = a.top == 1;      // (of one chosen the weight is one: the mass is the load)
+    const bool sums = dense && route_sums(d), one = route_lanes(d) == 1, counted = a.top == 1;      // (of one chosen the weight is the scale: the mass is that many of the load)
     const int ctas = route_ctas(d, sums), splits = sums ? ctas : mass_splits(d), want = std::max(a.top, a.top_groups < a.groups ? a.top_groups : 1);
     unsigned* part_load = static_cast<unsigned*>(ws);
     T* part_mass = reinterpret_cast<T*>(static_cast<char*>(ws) + load_bytes(d));
@@ -402,7 +404,7 @@ cudaError_t route(const simnets_route_desc& d, const void* scores, const void* p
 #undef ROUTE
     if (e != cudaSuccess) return e;
     if (mass && !sums && !counted) in_stream_order(route_mass<T>, dim3(a.k, splits), 256, 0, s)(a, (long long)d.batch, (const T*)dense, part_mass);
-    in_stream_order(route_totals<T>, a.k, 128, 0, s)(ctas, counted ? 0 : splits, a.k, part_load, part_mass, load, (T*)mass);
+    in_stream_order(route_totals<T>, a.k, 128, 0, s)(ctas, counted ? 0 : splits, a.k, T(a.scale), part_load, part_mass, load, (T*)mass);
     count_launch(mass && !sums && !counted ? 3 : 2);
     return cudaGetLastError();
 }

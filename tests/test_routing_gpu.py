@@ -1,11 +1,13 @@
 """Routing on the GPU against the restatement in plain_operators.py: choices and loads exactly, weights, masses and gradients in 64 bits."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
 
 import plain_operators as plain
 from oracle import unsupervised_oracle as uo
-from simnets_tf_b200 import keras
+from simnets_tf_b200 import abi, keras
 from simnets_tf_b200 import unsupervised as un
 from simnets_tf_b200.ops.routing import responsibilities, route
 
@@ -129,6 +131,23 @@ def test_the_choice_is_no_input_of_the_gradient():
         route(x, top_k=2, bias=torch.zeros(6))
     with pytest.raises(TypeError):
         route(x, top_k=2, bias=torch.zeros(6, device="cuda", dtype=torch.float64))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_masses_are_sums_of_scaled_weights(cuda_lib, kind):
+    """simnets_route with the dense form and a scale, which `responsibilities` does not take."""
+    s = torch.randn(3, 20, 70, device="cuda", dtype=kind)
+    for top, groups, top_groups in ((1, 1, 1), (1, 5, 2), (4, 1, 1), (4, 5, 2)):
+        d = abi.RouteDesc(dtype=abi.F32 if kind == torch.float32 else abi.F64, batch=3, components=20, top_k=top, groups=groups, top_groups=top_groups, positions=70, scale=2.5)
+        dense, mass, load = torch.empty_like(s), torch.empty(20, device="cuda", dtype=kind), torch.empty(20, device="cuda", dtype=torch.int64)
+        ws = torch.empty(cuda_lib.simnets_route_workspace_bytes(C.byref(d)), dtype=torch.uint8, device="cuda")
+        assert cuda_lib.simnets_route(C.byref(d), s.data_ptr(), None, None, None, None, dense.data_ptr(), load.data_ptr(), mass.data_ptr(), ws.data_ptr(), ws.numel(),
+                                      torch.cuda.current_stream().cuda_stream) == 0
+        _, _, want_load, _, want, _ = plain.route(s.cpu().numpy(), top, groups=groups, top_groups=top_groups, scale=2.5)
+        assert np.array_equal(load.cpu().numpy(), want_load)
+        # (weights as in the test above, scores of up to 12 nats apart; a sum of 210 at most)
+        assert (np.abs(mass.cpu().numpy() - want) <= _units(kind, 8 + top + 24 + 210) * want + 1e-30).all()
+        assert torch.allclose(dense.sum(dim=(0, 2)), mass, rtol=_units(kind, 420), atol=0)
 
 
 class Ops(uo.OraclePatchOps):
