@@ -520,7 +520,7 @@ int simnets_route_gradient(const simnets_route_desc* d, const void* scores, cons
                            void* dscores, void* stream) {
     const int rc = route_check(d);
     if (rc) return rc;
-    if (d->batch > 0 && d->positions > 0 && (!scores || !index || !weights || !grad || !dscores)) return SIMNETS_E_NULL;
+    if (d->batch > 0 && d->positions > 0 && ((d->sigmoid && !scores) || !index || !weights || !grad || !dscores)) return SIMNETS_E_NULL;
     return from_cuda(launch_route_gradient(*d, scores, prior, index, weights, grad, dscores, as_stream(stream)));
 }
 

@@ -731,8 +731,10 @@ Routed route_impl(const Tensor& scores_in, const OptTensor& prior_in, const OptT
     return r;
 }
 
+// (only the gradient of sigmoids reads the scores again)
 struct RouteNode : torch::autograd::Node {
     simnets_route_desc d;
+    std::vector<int64_t> shape;
     SavedVariable scores, index, weights;
     OptTensor prior;
     std::string name() const override { return "RouteBackward"; }
@@ -740,12 +742,12 @@ struct RouteNode : torch::autograd::Node {
         std::lock_guard<std::mutex> lock(mutex_);
         variable_list out(1);
         if (!grads[0].defined() || !task_should_compute_output(0)) return out;
-        const Tensor iv = index.unpack(), wv = weights.unpack(shared_from_this()), sv = scores.unpack().contiguous(), g = grads[0].contiguous();
+        const Tensor iv = index.unpack(), wv = weights.unpack(shared_from_this()), sv = d.sigmoid ? scores.unpack().contiguous() : Tensor(), g = grads[0].contiguous();
         require_cuda_all(wv, g);
         if (g.sizes() != wv.sizes()) throw std::invalid_argument("route: gradient must have shape " + shape_text(wv.sizes()) + ", got " + shape_text(g.sizes()));
-        const c10::cuda::CUDAGuard guard(sv.device());
-        Tensor ds = at::empty(sv.sizes(), sv.options());
-        check(simnets_route_gradient(&d, ptr(sv), prior ? ptr(*prior) : nullptr, iv.data_ptr<int32_t>(), ptr(wv), ptr(g), ptr(ds), stream_of(sv)));
+        const c10::cuda::CUDAGuard guard(wv.device());
+        Tensor ds = at::empty(shape, wv.options());
+        check(simnets_route_gradient(&d, d.sigmoid ? ptr(sv) : nullptr, prior ? ptr(*prior) : nullptr, iv.data_ptr<int32_t>(), ptr(wv), ptr(g), ptr(ds), stream_of(wv)));
         out[0] = ds;
         return out;
     }
@@ -771,9 +773,10 @@ std::tuple<Tensor, Tensor, Tensor> route_apply(const Tensor& scores, const OptTe
         auto node = std::shared_ptr<RouteNode>(new RouteNode(), torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(scores));
         node->d = d;
-        node->scores = SavedVariable(scores, false);
+        node->shape = scores.sizes().vec();
         node->index = SavedVariable(r.index, false);
-        if (prior) node->prior = prior->detach().clone();           // (one value per component: not a saved variable, a copy)
+        if (d.sigmoid) node->scores = SavedVariable(scores, false);
+        if (d.sigmoid && prior) node->prior = prior->detach().clone();           // (one value per component: not a saved variable, a copy)
         torch::autograd::set_history(r.weights, node);
         node->weights = SavedVariable(r.weights, true);
     }

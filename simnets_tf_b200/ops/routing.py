@@ -47,7 +47,8 @@ def route(scores, top_k=1, prior=None, bias=None, groups=1, top_groups=None, sig
     are in the choice.  A component whose v is NaN or -infinity is not chosen; where fewer than `top_k` are left the index
     is -1 and the weight 0.  Chosen components with an infinite score share alike.
 
-    The weights are differentiable with respect to the scores."""
+    The weights are differentiable with respect to the scores, once; what stays for the gradient are index and weights, and the scores with
+    sigmoid=True."""
     top_groups = _checked(scores, top_k, prior, bias, groups, top_groups)
     if _torch_glue.is_tracing():
         raise RuntimeError("route cannot be recorded by torch.jit.trace: its choice depends on the values")

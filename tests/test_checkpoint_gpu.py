@@ -230,6 +230,41 @@ def test_missing_and_infinite_activations(port, name):
     assert np.array_equal(np.isnan(dx.cpu().numpy()), np.isnan(rdx)) and np.array_equal(np.isnan(doff.cpu().numpy()), np.isnan(rdoff))
 
 
+@pytest.mark.parametrize("name", ["k17", "k64", "k100", "tiles_4x2x2"])
+def test_patches_that_hold_nothing(port, name):
+    """Whole samples of -infinity have no weights: NaN there and in the offsets that they add to, as of the formula, and nowhere else."""
+    c = next(c for c in DISJOINT if c["name"] == name)
+    x, off, dy = _mex_inputs(port, c, torch.float32)
+    x, dy = x.copy(), dy.copy()
+    x[0] = -np.inf
+    kept = ck.checkpoint_pack(_dev(x), 32)
+    dx, doff = (t.cpu().numpy() for t in ck.mex_checkpoint_backward(kept, _dev(off), _dev(dy), c["M"], **cases.mex_attrs(c)))
+    (rdx, rdoff), _ = _mex_oracle(port, c, ck.checkpoint_unpack(kept).cpu().numpy(), off, dy)
+    assert np.array_equal(np.isnan(dx), np.isnan(rdx)) and np.array_equal(np.isnan(doff), np.isnan(rdoff))
+    assert np.isfinite(dx[1:]).all()
+
+
+@pytest.mark.parametrize("name", ["k17", "k64", "k100", "tiles_4x2x2"])
+def test_gradients_that_are_no_numbers_stay_where_they_are(port, name):
+    """An infinity or NaN in dy: neither dx of its patch nor its instance's offsets are finite, and all others are what they were."""
+    c = next(c for c in DISJOINT if c["name"] == name)
+    x, off, dy = _mex_inputs(port, c, torch.float32)
+    kept = ck.checkpoint_pack(_dev(x), 32)
+    at = ck.checkpoint_unpack(kept).cpu().numpy()
+    dx, doff = ck.mex_checkpoint_backward(kept, _dev(off), _dev(dy), c["M"], **cases.mex_attrs(c))
+    for bad in (np.inf, np.nan):
+        b = dy.copy()
+        b[0, 1, 0, 0] = bad
+        dxb, doffb = ck.mex_checkpoint_backward(kept, _dev(off), _dev(b), c["M"], **cases.mex_attrs(c))
+        for got, want in ((dxb, dx), (doffb, doff)):
+            fine = torch.isfinite(got)
+            assert bool((~fine).any()) and torch.equal(got[fine], want[fine])
+        # (which those are depends on how the instances of several blocks lie in dy: the oracle's)
+        (rdx, rdoff), _ = _mex_oracle(port, c, at, off, b)
+        assert np.array_equal(torch.isfinite(dxb).cpu().numpy(), np.isfinite(rdx)) and np.array_equal(torch.isfinite(doffb).cpu().numpy(), np.isfinite(rdoff))
+        assert (~np.isfinite(rdx)).sum() == (~np.isfinite(rdoff)).sum() == np.prod(c["blocks"])
+
+
 @pytest.mark.parametrize("name", ["eps_pinf", "eps_ninf"])
 def test_maxima_at_a_checkpoint(port, name):
     c = next(c for c in cases.MEX_SMALL if c["name"] == name)
@@ -309,6 +344,10 @@ def test_codes_and_ranges_anywhere_in_memory(cuda_lib):
     assert moved.ranges.data_ptr() % 8 == 4 and moved.codes.data_ptr() % 4 == 3
     want = ck.mex_checkpoint_backward(kept, off, dy, 128, **cases.mex_attrs(c))
     for got, ref in zip(ck.mex_checkpoint_backward(moved, off, dy, 128, **cases.mex_attrs(c)), want):
+        assert torch.equal(got, ref)
+    odd_off, odd_dy = (torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape) for t in (off, dy))
+    assert odd_off.data_ptr() % 8 == 4 and odd_dy.data_ptr() % 8 == 4
+    for got, ref in zip(ck.mex_checkpoint_backward(kept, odd_off, odd_dy, 128, **cases.mex_attrs(c)), want):
         assert torch.equal(got, ref)
     d = cases.mex_desc(c)
     ws = torch.empty(cuda_lib.simnets_mex_checkpoint_workspace_bytes(C.byref(d)), dtype=torch.uint8, device="cuda")

@@ -133,6 +133,24 @@ def test_the_choice_is_no_input_of_the_gradient():
         route(x, top_k=2, bias=torch.zeros(6, device="cuda", dtype=torch.float64))
 
 
+def test_what_stays_for_the_gradient():
+    """Index and weights; the scores only where the values are sigmoids of them."""
+    s = torch.randn(4, 12, 50, device="cuda", dtype=torch.float64)
+    g = torch.randn(4, 3, 50, device="cuda", dtype=torch.float64)
+    for sigmoid in (False, True):
+        x = s.clone().requires_grad_()
+        y = x * 1.0
+        i, w, _ = route(y, top_k=3, prior=torch.arange(12.0, device="cuda", dtype=torch.float64) / 8, sigmoid=sigmoid)
+        want = torch.autograd.grad(w, x, g, retain_graph=True)[0]
+        with torch.no_grad():
+            y.zero_()
+        if sigmoid:
+            with pytest.raises(RuntimeError, match="inplace"):
+                torch.autograd.grad(w, x, g)
+        else:
+            assert torch.equal(torch.autograd.grad(w, x, g)[0], want)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_masses_are_sums_of_scaled_weights(cuda_lib, kind):
     """simnets_route with the dense form and a scale, which `responsibilities` does not take."""
