@@ -13,7 +13,7 @@
 namespace simnets {
 namespace {
 
-constexpr int kRouteThreads = 128;
+constexpr int kRouteThreads = 128, kKeyed = 256, kSums = 16 * 1024;
 
 __device__ __forceinline__ float exp_of(float v) { return expf(v); }
 __device__ __forceinline__ double exp_of(double v) { return exp(v); }
@@ -43,6 +43,19 @@ struct Top {
             value = above ? ov : value; index = above ? oi : index;
         }
     }
+    // by falling value, equal ones by index, empty places last
+    __device__ __forceinline__ void sort() {
+#pragma unroll
+        for (int n = TK - 1; n > 0; --n)
+#pragma unroll
+            for (int t = 0; t < n; ++t) {
+                const bool swap = v[t + 1] > v[t] || (v[t + 1] == v[t] && unsigned(i[t + 1]) < unsigned(i[t]));
+                const T ov = v[t];
+                const int oi = i[t];
+                v[t] = swap ? v[t + 1] : ov; i[t] = swap ? i[t + 1] : oi;
+                v[t + 1] = swap ? ov : v[t + 1]; i[t + 1] = swap ? oi : i[t + 1];
+            }
+    }
     // the lists of the G lanes that share a position (RUN lanes apart) as one, the same in all of them; equal values by index
     template <int G, int RUN>
     __device__ __forceinline__ void merge() {
@@ -71,11 +84,52 @@ struct Top {
     }
 };
 
+// The TK + 1 largest of float32 values whose last bits are replaced by the component: one key instead of a value and an index, so that a place of the
+// list is a minimum and a maximum instead of five instructions.  What the bits decide, keys of one bucket, is looked at afterwards.
+__device__ __forceinline__ float min_or_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+template <int TK>
+struct Keys {
+    float t[TK + 1], total;
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i <= TK; ++i) t[i] = below_all<float>();
+        total = 0.f;
+    }
+    // (-infinity becomes a NaN, which moves nothing; infinity and NaN show in the total, which is scaled so that numbers do not make an infinity)
+    __device__ __forceinline__ void offer(float v, int c, uint32_t mask) {
+        v += 0.f;                                                        // (-0 = 0)
+        total = fmaf(v, 0x1p-13f, total);
+        const float key = __uint_as_float((__float_as_uint(v) & ~mask) | uint32_t(c));
+#pragma unroll
+        for (int i = TK; i > 0; --i) t[i] = fmaxf(t[i], min_or_nan(t[i - 1], key));
+        t[0] = fmaxf(t[0], key);
+    }
+    __device__ __forceinline__ bool empty(int i) const { return t[i] == below_all<float>(); }
+    __device__ __forceinline__ int at(int i, uint32_t mask) const { return empty(i) ? -1 : int(__float_as_uint(t[i]) & mask); }
+    __device__ __forceinline__ bool alike(int i, uint32_t mask) const { return !empty(i) && ((__float_as_uint(t[i - 1]) ^ __float_as_uint(t[i])) & ~mask) == 0; }
+    // whether the first `top` are not known by the keys
+    __device__ __forceinline__ bool unknown(int top, uint32_t mask) const {
+        bool yes = !(total < CUDART_INF_F);
+#pragma unroll
+        for (int i = 1; i <= TK; ++i) yes = yes || (i == top && alike(i, mask));
+        return yes;
+    }
+    // whether their order is not
+    __device__ __forceinline__ bool unordered(int top, uint32_t mask) const {
+        bool yes = false;
+#pragma unroll
+        for (int i = 1; i < TK; ++i) yes = yes || (i < top && alike(i, mask));
+        return yes;
+    }
+};
+
 struct RouteArgs {
     long long positions;         // of the whole batch
     long long N;                 // per sample
     FastDiv f_N;                 // where `positions` fits 31 bits
     int k, top, groups, size, top_groups;
+    int turns;                   // in which the warps of a CTA add to their common sums
+    uint32_t key_mask;           // last bits of a key that hold the component, 0 for no keys
     int sigmoid;
     double scale;
 };
@@ -85,27 +139,42 @@ __device__ __forceinline__ long long sample_of(const RouteArgs& a, long long p) 
 template <typename T> struct alignas(2 * sizeof(T)) Pair { T prior, bias; };
 
 // f(v, c) for components from .. to, every G-th from `sub` on; `add`: prior and bias of every component, or null for none
-template <int G, int kBatch, typename T, class F>
+template <int G, int kBatch, bool AHEAD = true, typename T, class F>
 __device__ __forceinline__ void over_range(const T* __restrict__ s, long long N, const Pair<T>* add, int from, int to, int sub, F f) {
     int c = from + sub;
     const T* q = s + c * N;
     const long long step = G * N;
-    for (; c + G * (kBatch - 1) < to; c += G * kBatch) {
-        T v[kBatch];
+    T v[kBatch], w[kBatch];
+    auto load = [&](T (&b)[kBatch]) {
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u, q += step) v[u] = __ldg(q);
+        for (int u = 0; u < kBatch; ++u, q += step) b[u] = __ldg(q);
+    };
+    auto give = [&](const T (&b)[kBatch]) {
         if (add)
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
                 const Pair<T> both = add[c + G * u];
-                f((v[u] + both.prior) + both.bias, c + G * u);
+                f((b[u] + both.prior) + both.bias, c + G * u);
             }
         else
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) f(v[u], c + G * u);
+            for (int u = 0; u < kBatch; ++u) f(b[u], c + G * u);
+        c += G * kBatch;
+    };
+    if (!AHEAD)
+        for (; c + G * (kBatch - 1) < to;) { load(v); give(v); }
+    int left = AHEAD && c < to ? ((to - c - 1) / G + 1) / kBatch : 0;             // whole batches, the next one under way while one is worked on
+    if (left > 0) load(v);
+    while (left > 0) {
+        if (left > 1) load(w);
+        give(v);
+        if (left > 1) {
+            if (left > 2) load(v);
+            give(w);
+        }
+        left -= 2;
     }
     if (c < to) {
-        T v[kBatch - 1];
 #pragma unroll
         for (int u = 0; u < kBatch - 1; ++u, q += step) v[u] = c + G * u < to ? __ldg(q) : T(0);
 #pragma unroll
@@ -127,31 +196,35 @@ __device__ __forceinline__ T best_of_range(const T* __restrict__ s, long long N,
 }
 
 // Bound: HBM, the scores read once and, for the dense form, as much written (512 x 64 x 30 x 30 float32: 236 MB, 36 us).  The nearest one of
-// 64 components takes 54 us (4.4 TB/s); cut to four 81: a place of the list is five instructions of the half-rate pipe per component (66 % busy).
+// 64 components takes 51 us (4.6 TB/s); cut to four 72: loads of a warp wait for the list of the ones in front (sparse 43, three of 24 components 22).
 //
-// G lanes share a position (four where positions are few), neighbouring lanes are neighbouring positions; a lane has eight or sixteen scores in
-// flight and keeps a sorted list of TK.  (A position's scores in the registers of four lanes, with lists of values only: 105 us; two passes, values
-// alone in sorting networks and then who reaches the last of them: 100.)  192 components in groups, 64 x 15 x 15, six of three of eight groups: 17 us with the
-// maxima of four groups in flight (23 with one).
-// With SUMS every thread adds the weights that it gives to sums of its own in shared memory, one per component, which the CTA adds up at its
-// end: the masses cost no second pass over the dense form, and come out the same on every run.
+// G lanes share a position where positions are few, neighbouring lanes are neighbouring positions; a lane has eight scores in flight beside the eight
+// that it puts into a sorted list of TK.  Up to 256 components lists are of keys (`Keys`; with values and indices 81 and 52 us); what keys do not
+// tell, a tie at the end of the list or infinities, is done again with values and indices (scores rounded to integers, where every warp does both: 94 and
+// 70), and ties inside the list are sorted.  (Also tried: a position's scores in the registers of four lanes, with lists of values only, 105 us; two
+// passes, values alone in sorting networks and then who reaches the last of them, 100; registers held down to nine CTAs a multiprocessor, 87.)  192
+// components in groups, 64 x 15 x 15, six of three of eight groups: 17 us with the maxima of four groups in flight (23 with one).
+//
+// With SUMS a CTA adds the weights up in shared memory: a column of sums per thread, or, where those would keep CTAs out, per two or four threads of
+// different warps, which then take turns (78 -> 72 us).  The masses cost no second pass over the dense form, and come out the same on every run.
 template <typename T, int TK, int G, bool SUMS, bool GROUPS>
 __global__ void __launch_bounds__(kRouteThreads) route_choose(RouteArgs a, const T* __restrict__ scores, const T* __restrict__ prior, const T* __restrict__ bias,
                                                               int* __restrict__ index, T* __restrict__ weights, T* __restrict__ dense, T* __restrict__ part_mass,
                                                               unsigned* __restrict__ part_load) {
     stream_order();
     constexpr int RUN = 32 / G, PLACES = kRouteThreads / G;
-    constexpr int kBatch = SUMS ? 16 : 8;                                                // scores of a position in flight (there are fewer warps beside the sums)
+    constexpr int kBatch = 8;                                                // scores of a position in flight (there are fewer warps beside the sums)
     extern __shared__ __align__(16) unsigned char route_smem[];
-    T* const sums = reinterpret_cast<T*>(route_smem);                                    // [k][PLACES]
-    Pair<T>* const add_s = reinterpret_cast<Pair<T>*>(sums + (SUMS ? (size_t)a.k * PLACES : 0));
+    const int columns = SUMS ? PLACES / a.turns : 0;
+    T* const sums = reinterpret_cast<T*>(route_smem);                                    // [k][columns]
+    Pair<T>* const add_s = reinterpret_cast<Pair<T>*>(sums + (size_t)a.k * columns);
     unsigned* const load = reinterpret_cast<unsigned*>(add_s + a.k);
     const int lane = threadIdx.x & 31, sub = lane / RUN, place = (threadIdx.x >> 5) * RUN + lane % RUN;
     for (int c = threadIdx.x; c < a.k; c += kRouteThreads) {
         load[c] = 0;
         add_s[c] = Pair<T>{prior ? prior[c] : T(0), bias ? bias[c] : T(0)};
     }
-    if (SUMS) for (int i = threadIdx.x; i < a.k * PLACES; i += kRouteThreads) sums[i] = T(0);
+    if (SUMS) for (int i = threadIdx.x; i < a.k * columns; i += kRouteThreads) sums[i] = T(0);
     __syncthreads();
     const Pair<T>* const add = prior || bias ? add_s : nullptr;
     for (long long p0 = (long long)blockIdx.x * PLACES; p0 < a.positions; p0 += (long long)gridDim.x * PLACES) {
@@ -206,7 +279,32 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose(RouteArgs a, const
             }
             __syncwarp();
         } else {
-            over_range<G, kBatch>(s, a.N, add, 0, a.k, sub, [&](T v, int c) { top.offer(v, c); });
+            constexpr bool KEYS = sizeof(T) == 4 && TK > 1;
+            bool whole = true;                           // values and indices are compared one by one
+            if constexpr (KEYS) {
+                const uint32_t mask = a.key_mask;
+                if (mask) {
+                    Keys<TK> keys;
+                    keys.clear();
+                    over_range<G, kBatch, (TK < 16 || G > 1)>(s, a.N, add, 0, a.k, sub, [&](T v, int c) { keys.offer(v, c, mask); });
+                    whole = __any_sync(0xffffffffu, keys.unknown(a.top, mask));
+                    if (!whole) {
+#pragma unroll
+                        for (int t = 0; t < TK; ++t) top.i[t] = t < a.top ? keys.at(t, mask) : -1;
+                        const bool sort = __any_sync(0xffffffffu, keys.unordered(a.top, mask));
+                        if (G > 1 || sort) {             // (sorted by value, then index)
+#pragma unroll
+                            for (int t = 0; t < TK; ++t) {
+                                if (top.i[t] < 0) continue;
+                                const T v = __ldg(s + top.i[t] * a.N);
+                                top.v[t] = add ? (v + add[top.i[t]].prior) + add[top.i[t]].bias : v;
+                            }
+                            if (sort) top.sort();
+                        }
+                    }
+                }
+            }
+            if (whole) over_range<G, kBatch, !KEYS || (G > 1)>(s, a.N, add, 0, a.k, sub, [&](T v, int c) { top.offer(v, c); });
         }
         top.template merge<G, RUN>();
         // weights of the chosen: they sum to one over them
@@ -250,18 +348,25 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose(RouteArgs a, const
                 if (index) index[at] = top.i[t];
                 if (weights) weights[at] = l[t];
                 if (top.i[t] < 0) continue;
-                if (SUMS) sums[top.i[t] * PLACES + place] += l[t];
                 atomicAdd(load + top.i[t], 1u);
             }
         }
+        if constexpr (SUMS)
+            for (int turn = 0; turn < a.turns; ++turn) {
+                if (turn == (threadIdx.x >> 5) * a.turns / (kRouteThreads / 32) && live && sub == 0) {
+#pragma unroll
+                    for (int t = 0; t < TK; ++t)
+                        if (t < a.top && top.i[t] >= 0) sums[top.i[t] * columns + (place & (columns - 1))] += l[t];
+                }
+                if (a.turns > 1) __syncthreads();
+            }
     }
     __syncthreads();
     for (int c = threadIdx.x; c < a.k; c += kRouteThreads) part_load[(size_t)blockIdx.x * a.k + c] = load[c];
     if constexpr (SUMS)
         for (int c = threadIdx.x >> 5; c < a.k; c += kRouteThreads / 32) {
             T m = T(0);
-#pragma unroll
-            for (int i = 0; i < PLACES; i += 32) m += sums[c * PLACES + i + lane];
+            for (int i = lane; i < columns; i += 32) m += sums[c * columns + i];
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) m += __shfl_xor_sync(0xffffffffu, m, d);
             if (lane == 0) part_mass[(size_t)blockIdx.x * a.k + c] = m;
@@ -347,15 +452,25 @@ RouteArgs args_of(const simnets_route_desc& d) {
     a.f_N = FastDiv{0, 0, 0};
     if (a.positions > 0 && a.positions <= 0x7fffffffLL) a.f_N = make_fastdiv(int(a.N));
     a.k = d.components; a.top = d.top_k; a.groups = d.groups; a.size = d.components / d.groups; a.top_groups = d.top_groups;
+    a.turns = 1;
+    a.key_mask = 0;
+    if (a.k > 1 && a.k <= kKeyed)
+        while (int(a.key_mask) < a.k - 1) a.key_mask = 2 * a.key_mask + 1;
     a.sigmoid = d.sigmoid != 0;
     a.scale = d.scale;
     return a;
 }
-// lanes per position: one where the positions fill the GPU
-int route_lanes(const simnets_route_desc& d) { return d.positions * d.batch >= 512LL * device_sm_count() || d.components < 8 ? 1 : 4; }
-// a CTA's sums fit the shared memory of a multiprocessor three times
-size_t sums_bytes(const simnets_route_desc& d) { return (d.dtype == SIMNETS_F64 ? 8 : 4) * (size_t)d.components * (kRouteThreads / route_lanes(d)); }
-bool route_sums(const simnets_route_desc& d) { return d.top_k > 1 && d.top_groups == d.groups && sums_bytes(d) <= 64 * 1024; }
+// lanes per position: one where the positions fill the GPU, else eight (4 x 16 x 16 positions, eight of 4096: 47 us; with four lanes 80), where groups
+// are chosen four (64 x 15 x 15, six of 192: 17 us; with eight, whose maxima go over one lane more each, 26)
+int route_lanes(const simnets_route_desc& d) {
+    if (d.positions * d.batch >= 512LL * device_sm_count() || d.components < 8) return 1;
+    return d.top_groups < d.groups ? 4 : 8;
+}
+// a CTA's sums: a column per position, or for two or four of them one after the other where that leaves room for more CTAs
+size_t sums_bytes(const simnets_route_desc& d, int turns) { return (d.dtype == SIMNETS_F64 ? 8 : 4) * (size_t)d.components * (kRouteThreads / route_lanes(d) / turns); }
+int sums_turns(const simnets_route_desc& d) { return sums_bytes(d, 1) <= kSums ? 1 : sums_bytes(d, 2) <= kSums ? 2 : 4; }
+size_t sums_bytes(const simnets_route_desc& d) { return sums_bytes(d, sums_turns(d)); }
+bool route_sums(const simnets_route_desc& d) { return d.top_k > 1 && d.top_groups == d.groups && sums_bytes(d) <= 2 * kSums; }
 size_t choose_bytes(const simnets_route_desc& d, bool sums) { return (sums ? sums_bytes(d) : 0) + (size_t)d.components * (2 * (d.dtype == SIMNETS_F64 ? 8 : 4) + sizeof(unsigned)); }
 // as many CTAs as are resident together
 int route_ctas(const simnets_route_desc& d, bool sums) {
@@ -386,16 +501,17 @@ cudaError_t choose(const simnets_route_desc& d, const RouteArgs& a, const void* 
 template <typename T>
 cudaError_t route(const simnets_route_desc& d, const void* scores, const void* prior, const void* bias, int* index, void* weights, void* dense, long long* load,
                   void* mass, void* ws, cudaStream_t s) {
-    const RouteArgs a = args_of(d);
+    RouteArgs a = args_of(d);
+    a.turns = sums_turns(d);
     const bool sums = dense && route_sums(d), one = route_lanes(d) == 1, counted = a.top == 1;      // (of one chosen the weight is the scale: the mass is that many of the load)
     const int ctas = route_ctas(d, sums), splits = sums ? ctas : mass_splits(d), want = std::max(a.top, a.top_groups < a.groups ? a.top_groups : 1);
     unsigned* part_load = static_cast<unsigned*>(ws);
     T* part_mass = reinterpret_cast<T*>(static_cast<char*>(ws) + load_bytes(d));
     cudaError_t e = cudaSuccess;
 #define CHOOSE(TK, G, SUMS, GROUPS) choose<T, TK, G, SUMS, GROUPS>(d, a, scores, prior, bias, index, weights, dense, part_mass, part_load, s)
-#define ROUTE(TK) e = sums ? (one ? CHOOSE(TK, 1, true, false) : CHOOSE(TK, 4, true, false))                                                            \
+#define ROUTE(TK) e = sums ? (one ? CHOOSE(TK, 1, true, false) : CHOOSE(TK, 8, true, false))                                                            \
                            : a.top_groups < a.groups ? (one ? CHOOSE(TK, 1, false, true) : CHOOSE(TK, 4, false, true))                                   \
-                                                     : (one ? CHOOSE(TK, 1, false, false) : CHOOSE(TK, 4, false, false))
+                                                     : (one ? CHOOSE(TK, 1, false, false) : CHOOSE(TK, 8, false, false))
     if (want <= 1) ROUTE(1);
     else if (sizeof(T) == 8 ? want <= 4 : false) ROUTE(4);               // (float64: fewer lengths of the list)
     else if constexpr (sizeof(T) == 4) { if (want <= 2) ROUTE(2); else if (want <= 4) ROUTE(4); else if (want <= 8) ROUTE(8); else ROUTE(16); }

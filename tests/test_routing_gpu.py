@@ -83,6 +83,41 @@ def test_choice_weights_loads_and_gradient(shape, top, groups, top_groups, sigmo
         assert (np.abs(want - mass / scale) <= _units(kind, 8 + top + 2 * min(a, 100.0)) * mass / scale + 1e-30).all()
 
 
+@pytest.mark.parametrize("shape,top", [((2, 64, 37), 4), ((1, 13, 300), 2), ((1, 256, 129), 7), ((1, 257, 40), 5), ((3, 40, 41), 16), ((700, 24, 110), 3)])
+@pytest.mark.parametrize("style", ["neighbours", "below_zero", "zeros", "subnormal", "infinite", "few"])
+def test_choices_between_values_that_are_nearly_equal(shape, top, style):
+    """Values a few units in the last place apart, zeros of both signs, numbers below the normal ones, positions of which little is left."""
+    rng = np.random.default_rng(9)
+    near = np.array(1.75, np.float32).view(np.int32) + rng.integers(0, 90, shape)
+    s = near.astype(np.int32).view(np.float32)
+    if style == "below_zero":
+        s = -s
+    elif style == "zeros":
+        s = np.where(rng.random(shape) < 0.5, np.float32(0.0), np.float32(-0.0)) * rng.choice(np.array([1.0, 0.0], np.float32), shape)
+        s[rng.random(shape) < 0.02] = 1e-30
+    elif style == "subnormal":
+        s = (rng.integers(0, 300, shape) * rng.choice([-1, 1], shape)).astype(np.float32) * np.float32(1e-45)
+    elif style == "infinite":
+        s = np.where(rng.random(shape) < 0.1, np.float32(np.inf), s)
+        s[:, :, ::2] = np.finfo(np.float32).max * rng.choice(np.array([-1.0, 1.0], np.float32), s[:, :, ::2].shape)
+    elif style == "few":
+        s = np.where(rng.random(shape) < 2.0 / shape[1], s, -np.float32(np.inf))
+        s[:, 0, 1::5] = -np.finfo(np.float32).max
+    s = s.astype(np.float32)
+    for bias in (None, np.where(rng.random(shape[1]) < 0.5, np.float32(0), np.float32(2.0 ** -22))):
+        if shape[0] > 100 and bias is not None:
+            continue
+        n = 3 if shape[0] > 100 else shape[0]               # (many samples: a lane has a whole position; the first ones tell)
+        index, weights, load, dense, _, _ = plain.route(s[:n], top, bias=bias)
+        i, w, _ = route(_dev(s), top_k=top, bias=_dev(bias))
+        assert np.array_equal(i[:n].cpu().numpy(), index)
+        r, _, count = responsibilities(_dev(s), top_k=top, bias=_dev(bias))
+        assert np.array_equal((r[:n] > 0).cpu().numpy(), dense > 0)
+        assert np.abs(w[:n].cpu().numpy() - weights).max() <= _units(torch.float32, 8 + top)      # (exponentials of differences near 0, or of infinities)
+        if n == shape[0]:
+            assert np.array_equal(count.cpu().numpy(), load)
+
+
 @pytest.mark.parametrize("sigmoid", [False, True])
 def test_the_gradient_is_that_of_differences(sigmoid):
     torch.manual_seed(0)
