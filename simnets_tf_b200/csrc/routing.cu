@@ -9,6 +9,7 @@
 //
 // Loads are added up as integers and masses (sums of weights) from the written weights in a fixed order: the same on every run.
 #include "kernels.cuh"
+#include <atomic>
 
 namespace simnets {
 namespace {
@@ -196,17 +197,18 @@ __device__ __forceinline__ T best_of_range(const T* __restrict__ s, long long N,
 }
 
 // Bound: HBM, the scores read once and, for the dense form, as much written (512 x 64 x 30 x 30 float32: 236 MB, 36 us).  The nearest one of
-// 64 components takes 51 us (4.6 TB/s); cut to four 72: loads of a warp wait for the list of the ones in front (sparse 43, three of 24 components 22).
+// 64 components takes 47 us (5.0 TB/s); cut to four 66: loads of a warp wait for the list of the ones in front (sparse 42, three of 24 components 22).
 //
 // G lanes share a position where positions are few, neighbouring lanes are neighbouring positions; a lane has eight scores in flight beside the eight
 // that it puts into a sorted list of TK.  Up to 256 components lists are of keys (`Keys`; with values and indices 81 and 52 us); what keys do not
-// tell, a tie at the end of the list or infinities, is done again with values and indices (scores rounded to integers, where every warp does both: 94 and
-// 70), and ties inside the list are sorted.  (Also tried: a position's scores in the registers of four lanes, with lists of values only, 105 us; two
+// tell, a tie at the end of the list or infinities, is done again with values and indices (scores rounded to integers, where every warp does both: 91 and
+// 72), and ties inside the list are sorted.  (Also tried: a position's scores in the registers of four lanes, with lists of values only, 105 us; two
 // passes, values alone in sorting networks and then who reaches the last of them, 100; registers held down to nine CTAs a multiprocessor, 87.)  192
 // components in groups, 64 x 15 x 15, six of three of eight groups: 17 us with the maxima of four groups in flight (23 with one).
 //
 // With SUMS a CTA adds the weights up in shared memory: a column of sums per thread, or, where those would keep CTAs out, per two or four threads of
-// different warps, which then take turns (78 -> 72 us).  The masses cost no second pass over the dense form, and come out the same on every run.
+// different warps, which then take turns (78 -> 72 us).  As many CTAs as are resident by their registers too: more of them begin when the SMs run empty
+// (72 -> 66).  The masses cost no second pass over the dense form, and come out the same on every run.
 template <typename T, int TK, int G, bool SUMS, bool GROUPS>
 __global__ void __launch_bounds__(kRouteThreads) route_choose(RouteArgs a, const T* __restrict__ scores, const T* __restrict__ prior, const T* __restrict__ bias,
                                                               int* __restrict__ index, T* __restrict__ weights, T* __restrict__ dense, T* __restrict__ part_mass,
@@ -485,8 +487,21 @@ int mass_splits(const simnets_route_desc& d) {
 }
 size_t load_bytes(const simnets_route_desc& d) { return (sizeof(unsigned) * (size_t)most_ctas(d) * d.components + 255) & ~size_t(255); }
 
+// CTAs of a kernel that the registers of a multiprocessor hold (its own answer, asked for once)
+template <typename K>
+int held_by_registers(K kernel, std::atomic<int>& known) {
+    int n = known.load(std::memory_order_relaxed);
+    if (n == 0) {
+        cudaFuncAttributes at;
+        n = cudaFuncGetAttributes(&at, kernel) == cudaSuccess && at.numRegs > 0 ? std::max(1, 65536 / (kRouteThreads * ((at.numRegs + 7) / 8 * 8))) : 4;
+        known.store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+// `ctas`: how many it launched
 template <typename T, int TK, int G, bool SUMS, bool GROUPS>
-cudaError_t choose(const simnets_route_desc& d, const RouteArgs& a, const void* scores, const void* prior, const void* bias, int* index, void* weights, void* dense,
+cudaError_t choose(int& ctas, const simnets_route_desc& d, const RouteArgs& a, const void* scores, const void* prior, const void* bias, int* index, void* weights, void* dense,
                    T* part_mass, unsigned* part_load, cudaStream_t s) {
     const size_t smem = choose_bytes(d, SUMS);
     static SmemLimit limit;
@@ -494,7 +509,9 @@ cudaError_t choose(const simnets_route_desc& d, const RouteArgs& a, const void* 
         const cudaError_t e = limit.raise(route_choose<T, TK, G, SUMS, GROUPS>, 160 * 1024);
         if (e != cudaSuccess) return e;
     }
-    in_stream_order(route_choose<T, TK, G, SUMS, GROUPS>, route_ctas(d, SUMS), kRouteThreads, smem, s)(a, (const T*)scores, (const T*)prior, (const T*)bias, index, (T*)weights, (T*)dense, part_mass, part_load);
+    static std::atomic<int> held{0};
+    ctas = std::min(route_ctas(d, SUMS), held_by_registers(route_choose<T, TK, G, SUMS, GROUPS>, held) * device_sm_count());
+    in_stream_order(route_choose<T, TK, G, SUMS, GROUPS>, ctas, kRouteThreads, smem, s)(a, (const T*)scores, (const T*)prior, (const T*)bias, index, (T*)weights, (T*)dense, part_mass, part_load);
     return cudaSuccess;
 }
 
@@ -504,11 +521,12 @@ cudaError_t route(const simnets_route_desc& d, const void* scores, const void* p
     RouteArgs a = args_of(d);
     a.turns = sums_turns(d);
     const bool sums = dense && route_sums(d), one = route_lanes(d) == 1, counted = a.top == 1;      // (of one chosen the weight is the scale: the mass is that many of the load)
-    const int ctas = route_ctas(d, sums), splits = sums ? ctas : mass_splits(d), want = std::max(a.top, a.top_groups < a.groups ? a.top_groups : 1);
+    int ctas = 0;
+    const int want = std::max(a.top, a.top_groups < a.groups ? a.top_groups : 1);
     unsigned* part_load = static_cast<unsigned*>(ws);
     T* part_mass = reinterpret_cast<T*>(static_cast<char*>(ws) + load_bytes(d));
     cudaError_t e = cudaSuccess;
-#define CHOOSE(TK, G, SUMS, GROUPS) choose<T, TK, G, SUMS, GROUPS>(d, a, scores, prior, bias, index, weights, dense, part_mass, part_load, s)
+#define CHOOSE(TK, G, SUMS, GROUPS) choose<T, TK, G, SUMS, GROUPS>(ctas, d, a, scores, prior, bias, index, weights, dense, part_mass, part_load, s)
 #define ROUTE(TK) e = sums ? (one ? CHOOSE(TK, 1, true, false) : CHOOSE(TK, 8, true, false))                                                            \
                            : a.top_groups < a.groups ? (one ? CHOOSE(TK, 1, false, true) : CHOOSE(TK, 4, false, true))                                   \
                                                      : (one ? CHOOSE(TK, 1, false, false) : CHOOSE(TK, 8, false, false))
@@ -519,6 +537,7 @@ cudaError_t route(const simnets_route_desc& d, const void* scores, const void* p
 #undef CHOOSE
 #undef ROUTE
     if (e != cudaSuccess) return e;
+    const int splits = sums ? ctas : mass_splits(d);
     if (mass && !sums && !counted) in_stream_order(route_mass<T>, dim3(a.k, splits), 256, 0, s)(a, (long long)d.batch, (const T*)dense, part_mass);
     in_stream_order(route_totals<T>, a.k, 128, 0, s)(ctas, counted ? 0 : splits, a.k, T(a.scale), part_load, part_mass, load, (T*)mass);
     count_launch(mass && !sums && !counted ? 3 : 2);
