@@ -15,7 +15,8 @@
 // take 16 bytes a value instead of 6.  Six of the nine plane products are taken, small ones first: what an accumulator truncates is
 // 2^-24 of what it holds, which then are the largest products' K / 16 steps only.  An instruction with 64 columns waits for its 128 rows (50
 // cycles instead of 32), so that the second and third product take the planes of their narrow operand side by side, as up to 192 columns
-// (96 cycles for three).  Accumulators are emptied into FP32 after every 128 positions.
+// (96 cycles for three).  Accumulators are emptied into FP32 after every 128 positions (after 512:
+// 4 us less of the 252 below, and the offsets' gradient 1.5e-6 of its norm off instead of 3.7e-7).
 //
 // Sixteen warps work on the values and one issues the products: a tile's bytes are read and exponentiated while the second product of the tile
 // in front runs, the offsets' sums are added to the CTA's while the first one runs.  512 x 64 x 32 x 32 under 128 instances, pooled: 252 us
