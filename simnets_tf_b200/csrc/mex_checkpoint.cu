@@ -26,7 +26,9 @@
 // 9 cycles, the tensor pipe is busy 27 %.  Half of the warps for the taps and half for the instances were slower (266, 280).
 //
 // Offsets whose spread is beyond what the factors hold are found in the prepass; the kernel then leaves at once and the one behind it, which
-// else adds up the partial sums, evaluates term by term.
+// else adds up the partial sums, evaluates term by term.  Gradients that are infinite, or so large that a quotient or a sum of quotients is no float
+// any more (S is as small as e^-60): infinity has no bfloat16 planes that add up to it, so that the results they enter come out as no numbers, and
+// the kernel behind evaluates those term by term, and only those.
 #include "checkpoint.cuh"
 #include "ws.cuh"
 #include <cmath>
@@ -79,9 +81,12 @@ __device__ __forceinline__ Split2 split_bf16(float a, float b) {
     return s;
 }
 
-// C values of one row from column `col` on (4: half a core row) into the planes
+// a sum of squares of the values' top parts, two at once: infinity or NaN where one of them is no number or above 2^64
+__device__ __forceinline__ void add_squares(uint32_t& sum, uint32_t tops) { asm("fma.rn.bf16x2 %0, %1, %1, %0;" : "+r"(sum) : "r"(tops)); }
+
+// C values of one row from column `col` on (4: half a core row) into the planes; `squares`: see add_squares
 template <class P, int C>
-__device__ __forceinline__ void store_row(unsigned char* base, int row, int col, const float (&v)[C]) {
+__device__ __forceinline__ void store_row(unsigned char* base, int row, int col, const float (&v)[C], uint32_t& squares) {
     if constexpr (C == 4) {
         const Split2 s0 = split_bf16(v[0], v[1]), s1 = split_bf16(v[2], v[3]);
         unsigned char* d = base + P::at(row, col);
@@ -93,11 +98,18 @@ __device__ __forceinline__ void store_row(unsigned char* base, int row, int col,
         for (int c = 0; c < C; c += 8) {
             const Split2 s0 = split_bf16(v[c], v[c + 1]), s1 = split_bf16(v[c + 2], v[c + 3]), s2 = split_bf16(v[c + 4], v[c + 5]), s3 = split_bf16(v[c + 6], v[c + 7]);
             unsigned char* d = base + P::at(row, col + c);
+            add_squares(squares, s0.hi); add_squares(squares, s1.hi); add_squares(squares, s2.hi); add_squares(squares, s3.hi);
             *reinterpret_cast<uint4*>(d) = make_uint4(s0.hi, s1.hi, s2.hi, s3.hi);
             *reinterpret_cast<uint4*>(d + P::kPlane) = make_uint4(s0.mid, s1.mid, s2.mid, s3.mid);
             *reinterpret_cast<uint4*>(d + 2 * P::kPlane) = make_uint4(s0.lo, s1.lo, s2.lo, s3.lo);
         }
     }
+}
+
+template <class P, int C>
+__device__ __forceinline__ void store_row(unsigned char* base, int row, int col, const float (&v)[C]) {
+    uint32_t squares = 0;
+    store_row<P, C>(base, row, col, v, squares);
 }
 
 // N consecutive tensor-memory columns of this thread's lane; there once tmem_wait() is through
@@ -146,7 +158,7 @@ __global__ void __launch_bounds__(128) fuse_prepare(MexGeo g, int KP, int MC, in
     // (the extremes leave a NaN out)
     const int unsafe = __syncthreads_or(in && (!(fabsf(v) < CUDART_INF_F) || !(fabsf(eps) * (hi - lo) <= kSafeSpread)));
     if (k == 0) status[2 + blockIdx.x] = unsafe;
-    if (k < 2 && blockIdx.x == 0) status[k] = 0;
+    if (k < 3 && blockIdx.x == 0) status[k < 2 ? k : 2 + gridDim.x] = 0;
     const float e = in ? ex2_ftz(eps * 1.4426950408889634f * (v - (eps > 0.f ? hi : lo))) : m < g.M ? 0.f : 1.f;
     if (k >= KP) return;
     if (m < g.M) eo[((size_t)r * g.M + m) * KP + k] = e;
@@ -165,7 +177,8 @@ struct FuseArgs {
     const float* dy;
     float* dx;              // may be null
     float* part;            // [CTA][step] of what part_at() lays out, may be null
-    int* status;            // the two words of a MEX workspace; then, per row of offsets, whether its spread is beyond what the factors hold
+    int* status;            // the two words of a MEX workspace; then, per row of offsets, whether its spread is beyond what the factors hold; then
+                            // whether a quotient was beyond kMostQuotient
     int rows;               // R Mp of those
     int shift;              // log2 of the group
     int tiles_m;            // steps of instances
@@ -205,7 +218,11 @@ struct FuseShared {
     uint64_t drained;       // products, after a wait that ran out: none is under way any more
     uint32_t tmem;
     volatile int failed;
+    volatile int beyond;    // a quotient was beyond kMostQuotient
 };
+
+// Quotients up to here give finite sums: over 8192 instances 2^105, over the positions of any tensor that fits the memory (2^35 values) 2^127.
+constexpr float kMostQuotient = 0x1p92f;
 
 // An operand: its descriptor and where its planes and steps lie from there.  (The products are issued by one thread; what it computes between two of
 // them is what the tensor cores wait for: an addition to the address field here, 100 cycles an instruction with descriptors made anew.)
@@ -303,7 +320,7 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
     if (threadIdx.x == 0) {
         mbar_init(&sh.operands, kFuseWorkers / 32); mbar_init(&sh.quotients, kFuseWorkers / 32);
         mbar_init(&sh.sums[0], 1); mbar_init(&sh.sums[1], 1); mbar_init(&sh.taps, 1); mbar_init(&sh.instances, 1); mbar_init(&sh.drained, 1);
-        sh.failed = 0;
+        sh.failed = sh.beyond = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kFuseWorkers / 32) {
@@ -533,17 +550,21 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
                 wait(&sh.sums[from], from ? sum_phase[1] : sum_phase[0]);
                 if (from) sum_phase[1] ^= 1u; else sum_phase[0] ^= 1u;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t squares = 0;
 #pragma unroll
                 for (int i0 = 0; i0 < MR; i0 += 16) {
                     float s[16];
                     tmem_sum<16, 1, 0>(tS + from * MC + lane_base + part4 * MR + i0, s);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[i] = q[i0 + i] * reciprocal(s[i]);
-                    store_row<Q>(sq, p, part4 * MR + i0, s);
+                    store_row<Q>(sq, p, part4 * MR + i0, s, squares);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 arrive(&sh.quotients);
+                if ((squares & 0x7f80u) == 0x7f80u || (squares & 0x7f800000u) == 0x7f800000u)            // a NaN or a quotient above 2^64
+                    for (int m = part4 * MR; m < (part4 + 1) * MR; ++m)
+                        if (fabsf(__uint_as_float(uint32_t(*reinterpret_cast<const unsigned short*>(sq + Q::at(p, m))) << 16)) >= kMostQuotient) sh.beyond = 1;
                 // (while the second product runs)
                 if (last && !last_tile) next = decode(ex);
                 if (ahead && !(last && last_tile)) load_dy(last ? next : at, last ? 0 : mt + 1);
@@ -590,6 +611,7 @@ __global__ void __launch_bounds__(kFuseThreads, 1) mex_gradients_at_checkpoint(M
     if (warp == kFuseWorkers / 32)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(uint32_t(kFuseColumns)) : "memory");
     if (sh.failed && threadIdx.x == 0) atomicExch(&a.status[1], 1);                      // a wait ran out: the kernel behind redoes the call
+    if (sh.beyond && threadIdx.x == 0) atomicExch(&a.status[2 + a.rows], 1);             // the kernel behind redoes what is no number
 }
 
 // ---- the offsets' gradient from the CTAs' sums, or, for offsets that no factorisation takes, everything term by term ------------------
@@ -672,13 +694,21 @@ __device__ __forceinline__ Taps4 patch_weights(const MexGeo& g, const Taps4& x, 
     return t;
 }
 
-// dx: a warp per position of any region
-__device__ __forceinline__ void redo_dx(const MexGeo& g, const FuseArgs& a, const float* __restrict__ off) {
+// dx: a warp per position of any region; `some`: only of the patches whose dx is no number
+__device__ __forceinline__ void redo_dx(const MexGeo& g, const FuseArgs& a, const float* __restrict__ off, bool some) {
     constexpr int W = kFinishThreads / 32;
     const long long P = (long long)g.B * g.N;
     for (long long j = (long long)blockIdx.x * W + (threadIdx.x >> 5); j < P; j += (long long)gridDim.x * W) {
         const int n = int(j / g.N), pos = int(j - (long long)n * g.N), w = pos % g.Wo, h = pos / g.Wo % g.Ho, c = pos / (g.Wo * g.Ho), r = mex_region_of(g, c, h, w);
         const long long xi = (((long long)n * g.C + c * g.sc) * g.H + h * g.sh) * g.W + w * g.sw, at = mex_dy_base(g, n, pos);
+        if (some) {
+            bool bad = false;
+            for (int k = threadIdx.x & 31; k < g.K; k += 32) {
+                const Tap tap = tap_of<false>(g, k);
+                bad = bad || !(fabsf(a.dx[xi + ((long long)tap.c * g.H + tap.h) * g.W + tap.w]) < CUDART_INF_F);
+            }
+            if (!__any_sync(0xffffffffu, bad)) continue;
+        }
         const Taps4 x = checkpoint_patch(g, a, xi);
         double sum[4] = {0, 0, 0, 0};
         for (int m = 0; m < g.M; ++m) {
@@ -697,35 +727,32 @@ __device__ __forceinline__ void redo_dx(const MexGeo& g, const FuseArgs& a, cons
     }
 }
 
-// doff: a CTA per row of offsets, its warps over the positions
-__device__ __forceinline__ void redo_doff(const MexGeo& g, const FuseArgs& a, const FinishArgs& f, double (*sums)[128], float (*work)[128]) {
+// doff of one row by a whole CTA, its warps over the positions; thread k has tap k's
+__device__ __forceinline__ double redo_row(const MexGeo& g, const FuseArgs& a, const float* __restrict__ off, int row, double (*sums)[128]) {
     constexpr int W = kFinishThreads / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = row / g.M, m = row % g.M;
     const long long P = (long long)g.B * g.rs;
-    for (int row = blockIdx.x; row < g.R * g.M; row += gridDim.x) {
-        const int r = row / g.M, m = row % g.M;
-        double sum[4] = {0, 0, 0, 0};
-        for (long long j = warp; j < P; j += W) {
-            const Column col = column_of(g, r, j, P, nullptr);
-            if (col.base < 0) continue;
-            const long long xi = (((long long)col.n * g.C + col.c0) * g.H + col.h0) * g.W + col.w0;
-            const Taps4 p = patch_weights(g, checkpoint_patch(g, a, xi), f.off + (size_t)row * g.K);
-            const float v = a.dy[col.gbase + (long long)m * g.Ng];
+    double sum[4] = {0, 0, 0, 0};
+    for (long long j = warp; j < P; j += W) {
+        const Column col = column_of(g, r, j, P, nullptr);
+        if (col.base < 0) continue;
+        const long long xi = (((long long)col.n * g.C + col.c0) * g.H + col.h0) * g.W + col.w0;
+        const Taps4 p = patch_weights(g, checkpoint_patch(g, a, xi), off + (size_t)row * g.K);
+        const float v = a.dy[col.gbase + (long long)m * g.Ng];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum[i] += v * p.v[i];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sums[warp][lane + 32 * i] = sum[i];
-        __syncthreads();
-        double t = 0;
-        if (threadIdx.x < 128)
-            for (int w = 0; w < W; ++w) t += sums[w][threadIdx.x];
-        finish_row(g, f, row, float(t), work);
+        for (int i = 0; i < 4; ++i) sum[i] += v * p.v[i];
     }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sums[warp][lane + 32 * i] = sum[i];
+    __syncthreads();
+    double t = 0;
+    if (threadIdx.x < 128)
+        for (int w = 0; w < W; ++w) t += sums[w][threadIdx.x];
+    return t;
 }
 
-__global__ void __launch_bounds__(kFinishThreads) fuse_finish(MexGeo g, FuseArgs a, FinishArgs f) {
+__global__ void __launch_bounds__(kFinishThreads, 4) fuse_finish(MexGeo g, FuseArgs a, FinishArgs f) {
     stream_order();
     __shared__ double sums[kFinishThreads / 32][128];
     __shared__ float work[3][128];
@@ -736,31 +763,32 @@ __global__ void __launch_bounds__(kFinishThreads) fuse_finish(MexGeo g, FuseArgs
         unsafe = __syncthreads_or(unsafe);
         if (threadIdx.x == 0) a.status[0] = unsafe != 0;
     }
-    if (redo) {
-        if (a.dx) redo_dx(g, a, f.off);
-        if (f.doff) redo_doff(g, a, f, sums, work);
-        return;
-    }
+    const bool some = !redo && a.status[2 + a.rows] != 0;
+    if (a.dx && (redo || some)) redo_dx(g, a, f.off, some);
     if (!f.doff) return;
     // the CTAs' sums in their order, in two halves
     float* const half_sum = reinterpret_cast<float*>(sums);
     const int k = threadIdx.x & 127, half = threadIdx.x >> 7;
     for (int row = blockIdx.x; row < g.R * g.M; row += gridDim.x) {
-        const int r = row / g.M, m = row % g.M;
-        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-        if (k < g.K) {
-            const size_t step = (size_t)g.R * f.Mp * f.KP;
-            const int slots = f.ctas / g.R, from = half * ((slots + 1) / 2), to = half ? slots : (slots + 1) / 2;
-            const float* s = a.part + ((size_t)r * f.Mp + m / f.MC * f.MC) * f.KP + part_at(f.KP, f.MC, m % f.MC, k) + from * step;
-            int c = from;
-            for (; c + 3 < to; c += 4, s += 4 * step) { s0 += s[0]; s1 += s[step]; s2 += s[2 * step]; s3 += s[3 * step]; }
-            for (; c < to; ++c, s += step) s0 += s[0];
+        float d = 0.f;
+        if (!redo) {
+            const int r = row / g.M, m = row % g.M;
+            float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+            if (k < g.K) {
+                const size_t step = (size_t)g.R * f.Mp * f.KP;
+                const int slots = f.ctas / g.R, from = half * ((slots + 1) / 2), to = half ? slots : (slots + 1) / 2;
+                const float* s = a.part + ((size_t)r * f.Mp + m / f.MC * f.MC) * f.KP + part_at(f.KP, f.MC, m % f.MC, k) + from * step;
+                int c = from;
+                for (; c + 3 < to; c += 4, s += 4 * step) { s0 += s[0]; s1 += s[step]; s2 += s[2 * step]; s3 += s[3 * step]; }
+                for (; c < to; ++c, s += step) s0 += s[0];
+            }
+            const float mine = (s0 + s1) + (s2 + s3);
+            __syncthreads();
+            if (half) half_sum[k] = mine;
+            __syncthreads();
+            if (threadIdx.x < 128 && k < g.K) d = f.eo[((size_t)r * g.M + m) * f.KP + k] * (mine + half_sum[k]);
         }
-        const float mine = (s0 + s1) + (s2 + s3);
-        __syncthreads();
-        if (half) half_sum[k] = mine;
-        __syncthreads();
-        const float d = threadIdx.x < 128 && k < g.K ? f.eo[((size_t)r * g.M + m) * f.KP + k] * (mine + half_sum[k]) : 0.f;
+        if (redo || (some && __syncthreads_or(!(fabsf(d) < CUDART_INF_F)))) d = float(redo_row(g, a, f.off, row, sums));
         finish_row(g, f, row, d, work);
     }
 }
@@ -783,7 +811,7 @@ FuseWs fuse_carve(const MexGeo& g, void* base) {
     char* p = static_cast<char*>(base);
     size_t off = 0;
     auto take = [&](size_t bytes) { char* r = p ? p + off : nullptr; off += align256(bytes); return r; };
-    w.status = reinterpret_cast<int*>(take(sizeof(int) * (2 + (size_t)g.R * z.Mp)));
+    w.status = reinterpret_cast<int*>(take(sizeof(int) * (3 + (size_t)g.R * z.Mp)));
     w.eo = reinterpret_cast<float*>(take(sizeof(float) * (size_t)g.R * g.M * z.KP));
     w.tiles = reinterpret_cast<unsigned char*>(take((size_t)g.R * z.Mp * z.KP * 6));
     w.part = reinterpret_cast<float*>(take(sizeof(float) * (size_t)z.slots * g.R * z.Mp * z.KP));
