@@ -198,7 +198,7 @@ class DiagonalGMM(_Estimator):
             raise ValueError("top_k must be a whole number from 1 to %d, got %r" % (min(self.k, 16), top_k))
         if top_k is None and self.balance > 0:
             raise ValueError("a mixture whose components all share every patch has no choice to balance: give a top_k")
-        self.top_k = top_k
+        self.top_k = None if top_k is None else int(top_k)
         self.min_var = float(min_var)
         self.means = None
         self.covs = None

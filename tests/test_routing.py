@@ -156,3 +156,17 @@ def test_estimators_check_their_new_arguments():
             un.similarity_unsupervised_init("kmeans", L(), **kw)
     est = un.similarity_unsupervised_init("gmm", L(), top_k=2, balance=0.5)
     assert est.top_k == 2 and est.balance == 0.5 and est.bias is None
+
+
+@pytest.mark.parametrize("top_k", [2, 2.0, np.int64(2), np.float32(2)])
+def test_whole_numbers_of_any_type_are_taken_for_top_k(top_k):
+    """What the constructor takes every update takes: `responsibilities` wants an int."""
+    class Strict(Ops):
+        def responsibilities(self, scores, top_k, prior=None, bias=None):
+            assert type(top_k) is int
+            return super(Strict, self).responsibilities(scores, top_k, prior, bias)
+    x = torch.from_numpy(np.random.default_rng(6).normal(size=(3, 2, 5, 5)))
+    est = un.DiagonalGMM([3, 3], [1, 1], 4, ops=Strict((3, 3), (1, 1)), top_k=top_k)
+    est.init(x)
+    est.update(x)
+    assert est.top_k == 2
