@@ -9,6 +9,7 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <algorithm>
@@ -569,6 +570,19 @@ std::tuple<OptTensor, OptTensor, OptTensor> sim_checkpoint_backward(const SimPla
     return sim_checkpoint_grads(*p, codes, ranges, group, t, w, dy, flags, true, true, dt_out, dw_out);
 }
 
+// The gradients of an operator that is differentiable once: where a graph of them is asked for, they lead to the operator's inputs and to the
+// incoming gradient by a node that refuses (without it a term with a second derivative would be dropped).
+variable_list once(const torch::autograd::Node& op, const Tensor& grad, variable_list out) {
+    if (!at::GradMode::is_enabled()) return out;
+    torch::autograd::edge_list edges = op.next_edges();
+    edges.push_back(torch::autograd::impl::gradient_edge(grad));
+    const std::shared_ptr<torch::autograd::Node> refusal(new torch::autograd::Error("simnets_b200: " + op.name() + " is differentiable once", std::move(edges)),
+                                                         torch::autograd::deleteNode);
+    for (const Tensor& t : out)
+        if (t.defined()) torch::autograd::set_history(t, refusal);
+    return out;
+}
+
 // The nodes of layers that keep their input in 8 bits: nothing of the forward pass's output or workspace stays.
 struct MexCheckpointNode : torch::autograd::Node {
     MexPlanPtr plan;
@@ -588,7 +602,7 @@ struct MexCheckpointNode : torch::autograd::Node {
                                             want_dx, want_doff, sink);
         if (want_dx) out[0] = g.first;
         if (want_doff && !sink) out[1] = g.second;
-        return out;
+        return once(*this, grads[0], std::move(out));
     }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
@@ -645,7 +659,7 @@ struct SimCheckpointNode : torch::autograd::Node {
                                             want_dx, want_params, add ? dt_sink : std::nullopt, add ? dw_sink : std::nullopt);
         if (want_dx) out[0] = *std::get<0>(g);
         if (want_params && !add) { out[1] = *std::get<1>(g); out[2] = *std::get<2>(g); }
-        return out;
+        return once(*this, grads[0], std::move(out));
     }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
@@ -749,7 +763,7 @@ struct RouteNode : torch::autograd::Node {
         Tensor ds = at::empty(shape, wv.options());
         check(simnets_route_gradient(&d, d.sigmoid ? ptr(sv) : nullptr, prior ? ptr(*prior) : nullptr, iv.data_ptr<int32_t>(), ptr(wv), ptr(g), ptr(ds), stream_of(wv)));
         out[0] = ds;
-        return out;
+        return once(*this, grads[0], std::move(out));
     }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);

@@ -128,13 +128,13 @@ def similarity_checkpointed_with_plan(plan_of, input, templates, weights, group,
 
 
 def mex_checkpointed(input, offsets, num_instances, group=128, sum_pool2=False, **attrs):
-    """`mex(...)` (with sum_pool2=True `mex_sum_pool2(...)`), differentiable, keeping its input in 8 bits and nothing else."""
+    """`mex(...)` (with sum_pool2=True `mex_sum_pool2(...)`), differentiable (once), keeping its input in 8 bits and nothing else."""
     group, attrs = check_group(group), _mex_attrs(**{k: v for k, v in attrs.items() if k != "name"})
     _torch_glue.dtype_code(input)
     return mex_checkpointed_with_plan(lambda x: mex_plan(x.shape, x.dtype, num_instances, attrs), input, offsets, group, sum_pool2=sum_pool2)
 
 
 def similarity_checkpointed(input, templates, weights, group=128, **attrs):
-    """`similarity(...)`, differentiable, keeping its input in 8 bits and its parameters."""
+    """`similarity(...)`, differentiable (once), keeping its input in 8 bits and its parameters."""
     group, attrs = check_group(group), _sim_attrs(**{k: v for k, v in attrs.items() if k != "name"})
     return similarity_checkpointed_with_plan(lambda x, t, w: similarity_plan_of_shape(tuple(x.shape), x.dtype, t, w, attrs), input, templates, weights, group)

@@ -7,6 +7,7 @@ import torch
 import cases
 from simnets_tf_b200 import abi
 from simnets_tf_b200.ops import checkpoint as ck
+from simnets_tf_b200.ops.routing import route
 from test_checkpoint_gpu import DISJOINT, _dev, _mex_inputs, _mex_oracle, _mex_tolerance
 
 pytestmark = pytest.mark.gpu
@@ -57,3 +58,25 @@ def test_gradients_whose_quotients_are_no_floats(port, name, exponent):
     tol = _mex_tolerance(torch.float32, c, at, off, dy.size // c["M"])
     for got, ref, size in ((dx.cpu().numpy(), rdx, adx), (doff.cpu().numpy(), rdoff, adoff)):
         assert (np.abs(got - ref) <= tol * size + 1e-30 * 2.0 ** exponent).all()
+
+
+def test_second_derivatives_are_refused():
+    """A term with a second derivative must not be dropped: the gradients of a graph that is kept lead to a refusal."""
+    torch.manual_seed(6)
+    x, off = torch.randn(2, 8, 4, 4, device="cuda"), torch.randn(1, 5, 8, 1, 1, device="cuda")
+    t, w = torch.randn(5, 8, 2, 2, device="cuda"), torch.rand(5, 8, 2, 2, device="cuda")
+    mex = dict(blocks=[8, 1, 1], strides=[8, 1, 1], softmax_mode=True, use_unshared_regions=False, shared_offset_region=[-1])
+    calls = {"Route": (lambda v: route(v, top_k=3)[1], x), "MexCheckpoint": (lambda v: ck.mex_checkpointed(v, off, 5, **mex), x),
+             "MexCheckpoint of offsets": (lambda v: ck.mex_checkpointed(x, v, 5, **mex), off),
+             "SimilarityCheckpoint": (lambda v: ck.similarity_checkpointed(v, t, w, blocks=[2, 2], strides=[1, 1]), x),
+             "SimilarityCheckpoint of weights": (lambda v: ck.similarity_checkpointed(x, t, v, blocks=[2, 2], strides=[1, 1]), w)}
+    for name, (call, at) in calls.items():
+        v = at.clone().requires_grad_()
+        y = call(v)
+        weigh = torch.randn_like(y).requires_grad_()
+        first = torch.autograd.grad((y * weigh).sum(), v, retain_graph=True)[0]
+        kept = torch.autograd.grad((y * weigh).sum(), v, create_graph=True)[0]
+        assert torch.equal(first, kept) and not first.requires_grad
+        for inputs in (v, weigh):
+            with pytest.raises(RuntimeError, match=name.split()[0] + "Backward is differentiable once"):
+                torch.autograd.grad(kept.square().sum() + v.sum() + weigh.sum(), inputs, retain_graph=True)
