@@ -431,8 +431,9 @@ SIMNETS_API int simnets_similarity_checkpoint_gradients(const simnets_sim_desc* 
  *   index[batch, top_k, positions] (-1 where nothing is left), weights likewise, by falling v; either may be NULL
  *   dense[batch, components, positions]: weights of the chosen, 0 elsewhere; may be NULL
  *   load[components]: number of positions that chose it; mass[components]: sum of dense (NULL if dense is)
- * components <= 4096, top_k <= 16, groups <= 64, top_groups <= 16.  simnets_route_gradient: dscores[batch, components,
- * positions] of `grad`, the gradient of weights; scores and prior are read where sigmoid != 0 and may else be NULL.  The unsupervised initialisation assigns patches with it. */
+ * components <= 4096, top_k <= 16, groups <= 64, top_groups <= 16; scale: a normal number of the type (SIMNETS_E_DESC).
+ * simnets_route_gradient: dscores[batch, components, positions] of `grad`, the gradient of weights; scores and prior are read
+ * where sigmoid != 0 and may else be NULL.  The unsupervised initialisation assigns patches with it. */
 typedef struct simnets_route_desc {
     int32_t dtype;
     int32_t batch, components;

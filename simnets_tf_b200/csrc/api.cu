@@ -4,6 +4,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstdio>
+#include <limits>
 #include "simnets_b200.h"
 #include "host_dims.hpp"
 #include "kernels.cuh"
@@ -106,7 +107,10 @@ int route_check(const simnets_route_desc* d) {
     if (d->dtype != SIMNETS_F32 && d->dtype != SIMNETS_F64) return SIMNETS_E_DTYPE;
     if (d->batch < 0 || d->positions < 0 || d->components < 1 || d->top_k < 1 || d->groups < 1 || d->top_groups < 1 || d->reserved != 0) return SIMNETS_E_DESC;
     if (d->components % d->groups || d->top_groups > d->groups || d->top_k > (long long)d->top_groups * (d->components / d->groups)) return SIMNETS_E_DESC;
-    if (!std::isfinite(d->scale) || d->scale == 0.0) return SIMNETS_E_DESC;
+    // (a normal number of the weights' type, so that it and its reciprocal are numbers there)
+    const bool f64 = d->dtype == SIMNETS_F64;
+    const double most = f64 ? std::numeric_limits<double>::max() : std::numeric_limits<float>::max(), least = f64 ? std::numeric_limits<double>::min() : std::numeric_limits<float>::min();
+    if (!(std::fabs(d->scale) >= least && std::fabs(d->scale) <= most)) return SIMNETS_E_DESC;
     const bool all = d->top_groups == d->groups;        // (then there is no choice of groups)
     if (d->components > 4096 || d->top_k > 16 || (!all && (d->groups > 64 || d->top_groups > 16))) return SIMNETS_E_UNSUPPORTED;
     // (a load is counted in 32 bits by every CTA)

@@ -170,3 +170,16 @@ def test_whole_numbers_of_any_type_are_taken_for_top_k(top_k):
     est.init(x)
     est.update(x)
     assert est.top_k == 2
+
+
+@pytest.mark.parametrize("dtype,scale,ok", [(abi.F32, 1e-50, False), (abi.F32, 1e-40, False), (abi.F32, -1e39, False), (abi.F32, 1.2e-38, True), (abi.F32, -3e38, True),
+                                            (abi.F64, 1e-50, True), (abi.F64, 1e-310, False), (abi.F64, 1e300, True)])
+def test_scales_must_be_numbers_of_the_weights_type(cuda_lib, dtype, scale, ok):
+    """A scale that rounds to 0 or infinity in float32, or whose reciprocal (which the gradient takes) does, would give weights of 0 and
+    gradients of 0 x infinity."""
+    one = C.c_void_p(256)                   # (never dereferenced: every call below is refused)
+    d = abi.RouteDesc(dtype=dtype, batch=2, components=12, top_k=2, groups=1, top_groups=1, positions=9, scale=scale)
+    assert (cuda_lib.simnets_route_workspace_bytes(C.byref(d)) > 0) == ok
+    rc = abi.E_NULL if ok else abi.E_DESC
+    assert cuda_lib.simnets_route(C.byref(d), None, None, None, one, one, None, one, None, one, 1 << 30, None) == rc
+    assert cuda_lib.simnets_route_gradient(C.byref(d), one, None, None, one, one, one, None) == rc
