@@ -93,6 +93,8 @@ def _all_reduce(group, *tensors):
 
 
 class _Estimator(object):
+    balance, bias, top_k = 0.0, None, None          # (estimators pickled before there were these)
+
     def __init__(self, blocks, strides, num_instances, seed, ops=None, group=None):
         self.blocks, self.strides, self.k = list(blocks), list(strides), int(num_instances)
         self.ops = ops if ops is not None else LibraryPatchOps(blocks, strides)

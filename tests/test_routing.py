@@ -183,3 +183,16 @@ def test_scales_must_be_numbers_of_the_weights_type(cuda_lib, dtype, scale, ok):
     rc = abi.E_NULL if ok else abi.E_DESC
     assert cuda_lib.simnets_route(C.byref(d), None, None, None, one, one, None, one, None, one, 1 << 30, None) == rc
     assert cuda_lib.simnets_route_gradient(C.byref(d), one, None, None, one, one, one, None) == rc
+
+
+def test_estimators_stored_before_there_was_a_balance_go_on():
+    """An estimator pickled by an earlier version has neither `balance` nor `bias` nor `top_k`."""
+    x = torch.from_numpy(np.random.default_rng(6).normal(size=(3, 2, 5, 5)))
+    for make in (lambda: un.KMeans([3, 3], [1, 1], 4, ops=Ops((3, 3), (1, 1))), lambda: un.DiagonalGMM([3, 3], [1, 1], 4, ops=Ops((3, 3), (1, 1)))):
+        new, old = make(), make()
+        new.init(x)
+        old.init(x)
+        for name in ("balance", "bias", "top_k"):
+            old.__dict__.pop(name, None)
+        for a, b in zip(new.update(x), old.update(x)):
+            assert torch.equal(a, b)
