@@ -8,6 +8,8 @@ from .. import _torch_glue
 
 def _checked(scores, top_k, prior, bias, groups, top_groups):
     """top_groups of a call whose arguments fit together (a ValueError, or the TypeError or RuntimeError of an operator, if they do not)."""
+    if _torch_glue.is_tracing():
+        raise RuntimeError("routing cannot be recorded by torch.jit.trace: its choice depends on the values")
     top_groups = groups if top_groups is None else top_groups
     k = scores.shape[1] if scores.dim() > 1 else 0
     whole = type(top_k) is type(groups) is type(top_groups) is int
@@ -50,8 +52,6 @@ def route(scores, top_k=1, prior=None, bias=None, groups=1, top_groups=None, sig
     The weights are differentiable with respect to the scores, once; what stays for the gradient are index and weights, and the scores with
     sigmoid=True."""
     top_groups = _checked(scores, top_k, prior, bias, groups, top_groups)
-    if _torch_glue.is_tracing():
-        raise RuntimeError("route cannot be recorded by torch.jit.trace: its choice depends on the values")
     return _lib.ops().route_apply(scores, prior, bias, top_k, groups, top_groups, bool(sigmoid), float(scale))
 
 

@@ -196,3 +196,12 @@ def test_estimators_stored_before_there_was_a_balance_go_on():
             old.__dict__.pop(name, None)
         for a, b in zip(new.update(x), old.update(x)):
             assert torch.equal(a, b)
+
+
+def test_responsibilities_refuse_to_be_recorded():
+    """torch.jit.trace would keep their result as a constant."""
+    class Cut(torch.nn.Module):
+        def forward(self, s):
+            return responsibilities(s, top_k=2)[0]
+    with pytest.raises(RuntimeError, match="cannot be recorded"):
+        torch.jit.trace(Cut(), (torch.zeros(2, 4, 3),), check_trace=False)
