@@ -446,7 +446,7 @@ int simnets_checkpoint_unpack(int32_t dtype, int64_t count, int32_t group, const
     const int rc = checkpoint_check(dtype, count, group);
     if (rc) return rc;
     if (count > 0 && (!x || !codes || !ranges)) return SIMNETS_E_NULL;
-    return from_cuda(launch_checkpoint_unpack(dtype == SIMNETS_F64, 0, count, group, codes, ranges, x, as_stream(stream)));
+    return from_cuda(launch_checkpoint_unpack(dtype == SIMNETS_F64, count, group, codes, ranges, x, as_stream(stream)));
 }
 
 size_t simnets_mex_checkpoint_workspace_bytes(const simnets_mex_desc* d) {
@@ -477,7 +477,7 @@ int simnets_mex_checkpoint_gradients(const simnets_mex_desc* d, int32_t group, c
     }
     const MexCheckpointWs w = mex_checkpoint_carve(g, *d, ws);
     if (!ws || ws_bytes < w.bytes) return SIMNETS_E_WORKSPACE;
-    const cudaError_t e = launch_checkpoint_unpack(d->dtype == SIMNETS_F64, 0, (long long)g.B * g.C * g.H * g.W, group, codes, ranges, w.x, as_stream(stream));
+    const cudaError_t e = launch_checkpoint_unpack(d->dtype == SIMNETS_F64, (long long)g.B * g.C * g.H * g.W, group, codes, ranges, w.x, as_stream(stream));
     if (e != cudaSuccess) return from_cuda(e);
     simnets_mex_desc f = *d;
     const uint32_t route = checkpoint_route(g, *d);
@@ -501,7 +501,7 @@ int simnets_similarity_checkpoint_gradients(const simnets_sim_desc* d, int32_t g
     if ((rc = checkpoint_check(d->dtype, 1, group))) return rc;
     if (!t || !w || (dt == nullptr) != (dw == nullptr) || (!dx && !dt && g.B > 0) || (g.B > 0 && (!codes || !ranges || !dy))) return SIMNETS_E_NULL;
     if (!ws || ws_bytes < simnets_similarity_checkpoint_workspace_bytes(d)) return SIMNETS_E_WORKSPACE;
-    const cudaError_t e = launch_checkpoint_unpack(d->dtype == SIMNETS_F64, 0, (long long)g.B * g.C * g.H * g.W, group, codes, ranges, ws, as_stream(stream));
+    const cudaError_t e = launch_checkpoint_unpack(d->dtype == SIMNETS_F64, (long long)g.B * g.C * g.H * g.W, group, codes, ranges, ws, as_stream(stream));
     if (e != cudaSuccess) return from_cuda(e);
     const size_t values = sim_checkpoint_values(g, *d);
     void* rest = static_cast<char*>(ws) + values;

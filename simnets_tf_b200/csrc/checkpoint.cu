@@ -174,10 +174,10 @@ __global__ void __launch_bounds__(kPackThreads) checkpoint_pack(long long n, boo
     pack_groups<T, G>(n, steps * (R::kUnit * U / G) + warp, (n + G - 1) / G, warps, x, codes, ranges);
 }
 
-// Values first .. first + n of a checkpoint of groups of 2^shift.  Bound: HBM; eight loads of four bytes in flight a thread: 118 us for 134 million
+// The n values of a checkpoint of groups of 2^shift.  Bound: HBM; eight loads of four bytes in flight a thread: 118 us for 134 million
 // float32 (5.75 TB/s; with four 125, with one value a thread 165).
 template <typename T>
-__global__ void __launch_bounds__(kPackThreads) checkpoint_unpack(long long first, long long n, int shift, bool aligned, const unsigned char* __restrict__ codes,
+__global__ void __launch_bounds__(kPackThreads) checkpoint_unpack(long long n, int shift, bool aligned, const unsigned char* __restrict__ codes,
                                                                   const T* __restrict__ ranges, T* __restrict__ x) {
     stream_order();
     constexpr int V = 16 / int(sizeof(T)), U = 8;
@@ -191,9 +191,9 @@ __global__ void __launch_bounds__(kPackThreads) checkpoint_unpack(long long firs
             const long long q = q0 + j * kPackThreads;
             c[j] = 0; base[j] = step[j] = T(0);
             if (q >= quads) continue;
-            if constexpr (V == 4) c[j] = __ldcs(reinterpret_cast<const uint32_t*>(codes + first) + q);
-            else c[j] = __ldcs(reinterpret_cast<const unsigned short*>(codes + first) + q);
-            const T* r = ranges + 2 * ((first + q * V) >> shift);
+            if constexpr (V == 4) c[j] = __ldcs(reinterpret_cast<const uint32_t*>(codes) + q);
+            else c[j] = __ldcs(reinterpret_cast<const unsigned short*>(codes) + q);
+            const T* r = ranges + 2 * ((q * V) >> shift);
             base[j] = __ldg(r); step[j] = __ldg(r + 1);
         }
 #pragma unroll
@@ -207,8 +207,8 @@ __global__ void __launch_bounds__(kPackThreads) checkpoint_unpack(long long firs
         }
     }
     for (long long i = quads * V + thread; i < n; i += threads) {
-        const long long g = (first + i) >> shift;
-        x[i] = unpacked<T>(codes[first + i], ranges[2 * g], ranges[2 * g + 1]);
+        const long long g = i >> shift;
+        x[i] = unpacked<T>(codes[i], ranges[2 * g], ranges[2 * g + 1]);
     }
 }
 
@@ -227,11 +227,11 @@ cudaError_t pack(long long n, int group, const void* x, void* codes, void* range
 }
 
 template <typename T>
-cudaError_t unpack(long long first, long long n, int group, const void* codes, const void* ranges, void* x, cudaStream_t s) {
+cudaError_t unpack(long long n, int group, const void* codes, const void* ranges, void* x, cudaStream_t s) {
     int shift = 5;
     while ((1 << shift) < group) ++shift;
-    const bool aligned = lies_on(x, 16) && lies_on(static_cast<const char*>(codes) + first, 16 / sizeof(T)) && first % (16 / sizeof(T)) == 0;
-    in_stream_order(checkpoint_unpack<T>, pack_grid((n + 2048) / 2048), kPackThreads, 0, s)(first, n, shift, aligned, (const unsigned char*)codes, (const T*)ranges, (T*)x);
+    const bool aligned = lies_on(x, 16) && lies_on(codes, 16 / sizeof(T));
+    in_stream_order(checkpoint_unpack<T>, pack_grid((n + 2048) / 2048), kPackThreads, 0, s)(n, shift, aligned, (const unsigned char*)codes, (const T*)ranges, (T*)x);
     count_launch();
     return cudaGetLastError();
 }
@@ -242,9 +242,9 @@ cudaError_t launch_checkpoint_pack(bool f64, long long n, int group, const void*
     if (n == 0) return cudaSuccess;
     return f64 ? pack<double>(n, group, x, codes, ranges, s) : pack<float>(n, group, x, codes, ranges, s);
 }
-cudaError_t launch_checkpoint_unpack(bool f64, long long first, long long n, int group, const void* codes, const void* ranges, void* x, cudaStream_t s) {
+cudaError_t launch_checkpoint_unpack(bool f64, long long n, int group, const void* codes, const void* ranges, void* x, cudaStream_t s) {
     if (n == 0) return cudaSuccess;
-    return f64 ? unpack<double>(first, n, group, codes, ranges, x, s) : unpack<float>(first, n, group, codes, ranges, x, s);
+    return f64 ? unpack<double>(n, group, codes, ranges, x, s) : unpack<float>(n, group, codes, ranges, x, s);
 }
 
 }  // namespace simnets

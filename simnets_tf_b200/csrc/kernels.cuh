@@ -160,9 +160,9 @@ cudaError_t launch_mex_bwd_gemm(const MexGeo&, bool f64, const void* x, const vo
 // number of multiprocessors of the current device (148 when no device answers)
 int device_sm_count();
 
-// checkpoint.cu -- activations in 8 bits; unpack: values first .. first + n of a checkpoint
+// checkpoint.cu -- activations in 8 bits
 cudaError_t launch_checkpoint_pack(bool f64, long long n, int group, const void* x, void* codes, void* ranges, cudaStream_t);
-cudaError_t launch_checkpoint_unpack(bool f64, long long first, long long n, int group, const void* codes, const void* ranges, void* x, cudaStream_t);
+cudaError_t launch_checkpoint_unpack(bool f64, long long n, int group, const void* codes, const void* ranges, void* x, cudaStream_t);
 // mex_checkpoint.cu -- both MEX gradients from the bytes, for disjoint blocks; dx or doff may be null
 bool mex_checkpoint_shape(const MexGeo&, bool f64, uint32_t flags);
 size_t mex_checkpoint_bytes(const MexGeo&);
