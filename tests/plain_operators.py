@@ -88,3 +88,25 @@ def route_gradient(index, weights, grad, logit, sigmoid=False, scale=1.0):
                     d = d / (1.0 + np.exp(l[i, c, j]))
             out[i, c, j] = d
     return out.reshape(logit.shape)
+
+
+def route_sorted(scores, top_k, prior=None, bias=None, groups=1, top_groups=None, sigmoid=False, scale=1.0):
+    """`route` for torch tensors with many positions, by a stable sort: (index, weights, load, chosen logits), weights and logits in 64 bits."""
+    import torch
+    along = lambda v: v.view((1, -1) + (1,) * (scores.dim() - 2))
+    logit = scores if prior is None else scores + along(prior)
+    value = logit if bias is None else logit + along(bias)
+    value = torch.where(value.isnan(), -INF, value)
+    if top_groups is not None and top_groups < groups:
+        best, order = value.unflatten(1, (groups, -1)).amax(2).sort(dim=1, descending=True, stable=True)
+        keep = torch.zeros_like(best, dtype=torch.bool).scatter_(1, order[:, :top_groups], best[:, :top_groups] > -INF)
+        value = torch.where(keep.repeat_interleave(value.shape[1] // groups, 1), value, -INF)
+    best, order = value.sort(dim=1, descending=True, stable=True)
+    some = best[:, :top_k] > -INF
+    index = torch.where(some, order[:, :top_k], -1)
+    chosen = logit.gather(1, index.clamp(min=0)).double()
+    l = torch.where(some, torch.nn.functional.logsigmoid(chosen) if sigmoid else chosen, -INF)
+    hi = l.amax(1, keepdim=True)
+    e = torch.where(some, torch.where(l == hi, 1.0, (l - hi).exp()), 0.0)
+    weights = scale * e / e.sum(1, keepdim=True).clamp(min=1.0)
+    return index, weights, torch.bincount(index[some], minlength=scores.shape[1]), chosen

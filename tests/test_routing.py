@@ -205,3 +205,17 @@ def test_responsibilities_refuse_to_be_recorded():
             return responsibilities(s, top_k=2)[0]
     with pytest.raises(RuntimeError, match="cannot be recorded"):
         torch.jit.trace(Cut(), (torch.zeros(2, 4, 3),), check_trace=False)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(groups=4, top_groups=2), dict(sigmoid=True, scale=2.5)])
+def test_the_two_restatements_agree(kw):
+    rng = np.random.default_rng(2)
+    s = np.round(2 * rng.normal(size=(3, 12, 40)))
+    u = rng.random(s.shape)
+    s = np.where(u < 0.4, -np.inf, np.where(u < 0.5, np.nan, np.where(u > 0.97, np.inf, s)))
+    s[:, :, ::7] = -np.inf
+    prior, bias = np.round(rng.normal(size=12)), np.round(rng.normal(size=12))
+    for p, b in ((None, None), (prior, bias)):
+        index, weights, load, _, _, _ = plain.route(s, 3, p, b, **kw)
+        i, w, n, _ = plain.route_sorted(torch.from_numpy(s), 3, None if p is None else torch.from_numpy(p), None if b is None else torch.from_numpy(b), **kw)
+        assert np.array_equal(i.numpy(), index) and np.array_equal(n.numpy(), load) and np.allclose(w.numpy(), weights, rtol=1e-12, atol=0)
