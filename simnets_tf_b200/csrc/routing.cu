@@ -14,6 +14,9 @@
 namespace simnets {
 namespace {
 
+// Keys hold up to 256 components: beyond, what their last bits tell apart is too little, and more positions do both passes (normal scores, 131072
+// positions, index and weights, keys / values and indices: four of 256 53 / 58 us, four of 300 64 / 67, four of 512 109 / 108, four of 1024 222 / 206,
+// 2048 493 / 401; eight of 300 92 / 115).
 constexpr int kRouteThreads = 128, kKeyed = 256, kSums = 16 * 1024;
 
 __device__ __forceinline__ float exp_of(float v) { return expf(v); }
@@ -462,11 +465,17 @@ RouteArgs args_of(const simnets_route_desc& d) {
     a.scale = d.scale;
     return a;
 }
-// lanes per position: one where the positions fill the GPU, else eight (4 x 16 x 16 positions, eight of 4096: 47 us; with four lanes 80), where groups
-// are chosen four (64 x 15 x 15, six of 192: 17 us; with eight, whose maxima go over one lane more each, 26)
+// Lanes per position: eight where positions are few for their components (a lane each leaves the loads of a position in turn), where groups are
+// chosen four (64 x 15 x 15, six of 192: 17 us; with eight, whose maxima go over one lane more each, 26), else one (no lists to merge).  Index and
+// weights of scores that are not in L2, us with eight lanes / with one, over 4096, 14400 and 57600 positions:
+//     two of 16      4.9 / 4.1     6.8 / 4.5    13.4 / 7.0        eight of 192   11.4 / 24.8    19.3 / 28.8    54.8 / 43.0
+//     four of 64     6.3 / 7.2    11.3 / 9.5    22.2 / 13.1       four of 1024   18.2 / 105     33.2 / 107      100 / 133
+//     four of 128    8.1 / 13.0   12.8 / 14.8   26.9 / 20.8       six of 192 in three of eight groups, four lanes / one   15.9 / 20.7  22.0 / 23.0  59.2 / 35.5
+// They meet near 128 positions a component, with groups near 64; many components with the dense form earlier (1024: 14).
 int route_lanes(const simnets_route_desc& d) {
-    if (d.positions * d.batch >= 512LL * device_sm_count() || d.components < 8) return 1;
-    return d.top_groups < d.groups ? 4 : 8;
+    const bool groups = d.top_groups < d.groups;
+    if (d.positions * d.batch >= std::min<long long>(512LL * device_sm_count(), (groups ? 64LL : 128LL) * d.components) || d.components < 8) return 1;
+    return groups ? 4 : 8;
 }
 // a CTA's sums: a column per position, or for two or four of them one after the other where that leaves room for more CTAs
 size_t sums_bytes(const simnets_route_desc& d, int turns) { return (d.dtype == SIMNETS_F64 ? 8 : 4) * (size_t)d.components * (kRouteThreads / route_lanes(d) / turns); }

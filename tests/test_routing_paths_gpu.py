@@ -10,11 +10,12 @@ from test_routing_gpu import KINDS, _dev, _inputs, _units
 
 pytestmark = pytest.mark.gpu
 
-# (shape, top, groups, top_groups).  A lane a position from 512 positions a multiprocessor on; 12 CTAs of 128 a multiprocessor at most, fewer by registers.
+# (shape, top, groups, top_groups).  A lane a position from 512 positions a multiprocessor or 128 a component on (64 with groups); 12 CTAs of 128 threads
+# a multiprocessor at most, fewer by registers.
 MANY = [((2000, 24, 130), 3, 4, 2), ((2000, 48, 130), 8, 1, 1), ((2000, 40, 130), 16, 1, 1), ((2000, 33, 130), 6, 11, 5), ((2000, 48, 130), 7, 4, 2), ((1000, 300, 130), 5, 1, 1),
         ((1000, 200, 130), 2, 1, 1), ((2000, 64, 130), 1, 1, 1), ((1000, 96, 130), 12, 32, 16), ((1000, 100, 130), 4, 1, 1), ((1000, 5, 1031), 5, 1, 1), ((2000, 20, 130), 1, 5, 3)]
 # the same with the lanes of a warp shared, in several tiles a CTA
-SHARED = [((300, 60, 130), 4, 1, 1), ((300, 60, 130), 1, 1, 1), ((300, 60, 130), 5, 6, 2), ((300, 300, 130), 9, 1, 1)]
+SHARED = [((250, 300, 130), 1, 1, 1), ((200, 300, 130), 9, 1, 1), ((150, 1024, 130), 4, 1, 1), ((250, 512, 130), 5, 8, 3), ((140, 256, 130), 4, 1, 1)]
 
 
 @pytest.mark.parametrize("kind", KINDS)
