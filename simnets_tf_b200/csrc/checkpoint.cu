@@ -3,7 +3,7 @@
 // Per group of G consecutive values the lowest finite one (base) and a step of 1 / 252 of the range; per value the byte
 // rint((x - base) / step), or 253, 254, 255 for -infinity, infinity, NaN.  Activations of these networks are log-likelihoods that enter
 // exponentials: what counts is their absolute error, which is at most step / 2 here, wherever the range lies (an 8-bit float
-// is off by 2 % of a value, which is 1 nat at -50).
+// is off by 2 % of a value, which is 1 nat at -50); with step 0 it is below 252 of the type's smallest normal number.
 //
 // A program may pack and compare elsewhere, so the bytes are defined to the bit: with x / 2 - base / 2 and 2 / step rounded to the type and
 // their product exact in front of rint (one fused multiply-add onto 1.5 * 2^23 or 2^52, whose last bits are the integer).  The halves keep
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kPackThreads) checkpoint_pack(long long n, boo
         for (int j = 0; j < U; ++j) extremes<R::kLanes>(lo[j], hi[j]);
         if constexpr (sizeof(T) == 8 && U == 2) {
             // (divisions of float64 are some thirty instructions each: a lane makes those of one unit, and its group's lanes share them.  Groups of
-            // 128: 231 -> 215 us; with four units of one row the shuffles are already the bound: 375 -> 504)
+            // 128, 134 million values: 231 -> 215 us; with four units of one row the shuffles are already the bound: groups of 32 375 -> 504)
             T my_lo = lo[0], my_hi = hi[0], my_step, my_per;
 #pragma unroll
             for (int j = 1; j < U; ++j)

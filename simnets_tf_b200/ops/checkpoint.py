@@ -1,7 +1,8 @@
 """Activations in 8 bits for the backward pass: `checkpoint_pack` / `checkpoint_unpack`, and the gradients of the two operators at such a
 checkpoint of their input.  A layer differentiated the ordinary way keeps its input, its output and a workspace; with a checkpoint
 it keeps one byte per input value and 8 (float64: 16) per group, and computes the rest again.  The gradients are those of the operator at
-the values that the checkpoint stands for, which lie within half a step, 1 / 504 of the range of a group, of the input.
+the values that the checkpoint stands for, which lie within half a step, 1 / 504 of the range of a group, of the input (in a group whose
+range is below 252 of the type's smallest normal number all values become its lowest one).
 
 The reference has no counterpart: its graphs keep every activation (HUJI-Deep/simnets-tf python/simnets/ops/mex.py:47-81 takes the op's
 input and output into the gradient ops)."""
