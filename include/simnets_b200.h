@@ -476,6 +476,48 @@ SIMNETS_API int simnets_softmax_cross_entropy(int32_t batch, int32_t classes, fl
                                               const float* logits, const int64_t* labels, float* loss, float* dlogits,
                                               void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- log probabilities -------------------------------------------------------- */
+/* What a classifier answers at every position of logits [batch, classes, positions], whose element (b, c, p) is at
+ * b * stride_batch + c * stride_class + p * stride_position.  With m the largest logit of a position, d_c = x_c - m, S = sum exp(d_c):
+ *   label[b, p]          = log p_c of c = labels[b, p], log p_c = d_c - log S; 0 where labels[b, p] is outside [0, classes)
+ *   entropy[b, p]        = log S - sum exp(d_c) d_c / S
+ *   top_index, top       = the top_k classes with the largest logits by falling logit, equal ones by index (int32), and their log p_c;
+ *                          [batch, top_k, positions], with top_last != 0 [batch, positions, top_k]
+ * label, entropy and the pair of top_index and top may each be NULL; labels may be NULL where label is; top_k = 0 .. 16 is 0 where top is NULL.
+ * A logit of -infinity is a class that cannot be: it is not among the alternatives, and where fewer than top_k can be the index is -1
+ * and the log probability -infinity.  Where no class can be every log p_c is -infinity and the entropy 0.  A NaN or infinity makes label,
+ * entropy and top of its position NaN; alternatives are chosen among the others, infinity first.
+ * stats [3, batch, positions] (m, log S and entropy of every position; may be NULL) is what the gradient needs besides the logits.
+ * simnets_log_probabilities_gradient: the gradient of all logits for the gradients g_label, g_entropy and g_top (each may be NULL) of the outputs,
+ *   dlogits_c = -p_c (g_label + sum g_top + g_entropy (log p_c + entropy)) + g_label [c = labels] + sum over g_top [c = top_index],
+ * 0 where no class can be; a label or an alternative that is none adds nothing.  dlogits is dense, [batch, positions, classes] if
+ * stride_class is 1, else [batch, classes, positions].  The reference has softmax and cross-entropy of its framework only (README.md:108-111). */
+typedef struct simnets_likelihood_desc {
+    int32_t dtype;
+    int32_t classes;
+    int32_t top_k, top_last;
+    int64_t batch, positions;
+    int64_t stride_batch, stride_class, stride_position;    /* in elements, not negative */
+} simnets_likelihood_desc;
+SIMNETS_API int simnets_log_probabilities(const simnets_likelihood_desc* d, const void* logits, const int64_t* labels, void* label, void* entropy,
+                                          int32_t* top_index, void* top, void* stats, void* stream);
+SIMNETS_API int simnets_log_probabilities_gradient(const simnets_likelihood_desc* d, const void* logits, const int64_t* labels, const void* stats,
+                                                   const int32_t* top_index, const void* g_label, const void* g_entropy, const void* g_top,
+                                                   void* dlogits, void* stream);
+
+/* ---- norm and clipping of gradients -------------------------------------------- */
+/* norm[0] of a list of dense tensors on the device: order 2: sqrt(sum of all squares), order 0: the largest magnitude.  dtypes[i] (SIMNETS_F32, SIMNETS_F64;
+ * NULL: all float32), counts[i] values, tensors[i] its address; the three lists are read on the host before the call returns.  norm is float64
+ * if a tensor is, else float32.  Sums are in 64 bits and of a fixed order; float64 squares neither overflow nor vanish.
+ * simnets_clip_gradients also writes out[i] = tensors[i] * (max_norm / norm where norm > max_norm, else 1), the product rounded once; a norm that is
+ * NaN or, as returned, infinite leaves the values as they are.  out[i] may be tensors[i]; otherwise no two of the tensors written and read may
+ * overlap (not checked here).  max_norm: at least 0, infinity for no limit.  The reference leaves its gradients to its framework's optimisers. */
+SIMNETS_API size_t simnets_gradient_norm_workspace_bytes(int32_t num_tensors);
+SIMNETS_API int simnets_gradient_norm(int32_t order, int32_t num_tensors, const int32_t* dtypes, const int64_t* counts, const void* const* tensors,
+                                      void* norm, void* workspace, size_t workspace_bytes, void* stream);
+SIMNETS_API int simnets_clip_gradients(int32_t order, double max_norm, int32_t num_tensors, const int32_t* dtypes, const int64_t* counts,
+                                       const void* const* tensors, void* const* out, void* norm, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- normalize_offsets ------------------------------------------------------ */
 /* The `normalize_offsets` option of the reference's Keras Mex layer (python/simnets/keras.py:155-160): each of the
  * `rows` = num_regions * num_instances rows of `k` = block_c * block_h * block_w float32 offsets minus its log-sum-exp;

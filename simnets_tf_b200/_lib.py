@@ -77,6 +77,13 @@ def lib():
         l.simnets_route_workspace_bytes.argtypes = [rd]
         l.simnets_route.argtypes = [rd, _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]
         l.simnets_route_gradient.argtypes = [rd, _P, _P, _P, _P, _P, _P, _P]
+        kd = C.POINTER(abi.LikelihoodDesc)
+        l.simnets_log_probabilities.argtypes = [kd, _P, _P, _P, _P, _P, _P, _P, _P]
+        l.simnets_log_probabilities_gradient.argtypes = [kd, _P, _P, _P, _P, _P, _P, _P, _P, _P]
+        l.simnets_gradient_norm_workspace_bytes.restype = C.c_size_t
+        l.simnets_gradient_norm_workspace_bytes.argtypes = [C.c_int32]
+        l.simnets_gradient_norm.argtypes = [C.c_int32, C.c_int32, _P, _P, _P, _P, _P, C.c_size_t, _P]
+        l.simnets_clip_gradients.argtypes = [C.c_int32, C.c_double, C.c_int32, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]
         l.simnets_fp32_fma_probe.restype = C.c_int64
         l.simnets_fp32_fma_probe.argtypes = [C.c_int32, C.c_int32, _P, _P]
         l.get_mex_offsets_nregions.restype = C.c_int

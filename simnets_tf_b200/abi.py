@@ -77,6 +77,16 @@ class RouteDesc(C.Structure):
     ]
 
 
+class LikelihoodDesc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("classes", C.c_int32),
+        ("top_k", C.c_int32), ("top_last", C.c_int32),
+        ("batch", C.c_int64), ("positions", C.c_int64),
+        ("stride_batch", C.c_int64), ("stride_class", C.c_int64), ("stride_position", C.c_int64),
+    ]
+
+
 class MexGeometry(C.Structure):
     _fields_ = [(n, C.c_int32) for n in (
         "block_c", "block_h", "block_w", "stride_c", "stride_h", "stride_w", "pad_c", "pad_h", "pad_w",

@@ -116,6 +116,38 @@ int route_check(const simnets_route_desc* d) {
     // (a load is counted in 32 bits by every CTA)
     return d->batch > 0 && d->positions > ((1LL << 40) / d->batch) ? SIMNETS_E_UNSUPPORTED : SIMNETS_OK;
 }
+
+// ---- log probabilities, norms of gradients
+int likelihood_check(const simnets_likelihood_desc* d) {
+    if (!d) return SIMNETS_E_NULL;
+    if (d->dtype != SIMNETS_F32 && d->dtype != SIMNETS_F64) return SIMNETS_E_DTYPE;
+    if (d->classes < 1 || d->batch < 0 || d->positions < 0 || d->top_k < 0 || d->top_k > d->classes || d->stride_batch < 0 || d->stride_class < 0 || d->stride_position < 0)
+        return SIMNETS_E_DESC;
+    // (places of classes are counted in 32 bits, CTAs of positions as well)
+    if (d->top_k > 16 || d->classes > (1 << 30) || (d->batch > 0 && d->positions > (1LL << 36) / d->batch)) return SIMNETS_E_UNSUPPORTED;
+    return SIMNETS_OK;
+}
+
+int gradients_check(int32_t order, int32_t tensors, const int32_t* dtypes, const int64_t* counts, const void* const* in, const void* norm, const void* ws, size_t ws_bytes) {
+    if ((order != 0 && order != 2) || tensors < 0) return SIMNETS_E_DESC;
+    if (!norm || (tensors > 0 && (!counts || !in))) return SIMNETS_E_NULL;
+    long long total = 0;
+    for (int i = 0; i < tensors; ++i) {
+        if (dtypes && dtypes[i] != SIMNETS_F32 && dtypes[i] != SIMNETS_F64) return SIMNETS_E_DTYPE;
+        if (counts[i] < 0) return SIMNETS_E_DESC;
+        if (counts[i] > 0 && !in[i]) return SIMNETS_E_NULL;
+        if (counts[i] > (1LL << 40) - total) return SIMNETS_E_UNSUPPORTED;          // (pieces of 16 KB are counted in 32 bits)
+        total += counts[i];
+    }
+    return !ws || ws_bytes < gradient_norm_workspace_bytes(tensors) ? SIMNETS_E_WORKSPACE : SIMNETS_OK;
+}
+
+int gradients(int32_t order, double limit, int32_t tensors, const int32_t* dtypes, const int64_t* counts, const void* const* in, void* const* out, void* norm, void* ws,
+              void* stream) {
+    bool f64 = false;
+    for (int i = 0; dtypes && i < tensors; ++i) f64 = f64 || dtypes[i] == SIMNETS_F64;
+    return from_cuda(launch_gradient_norm(order, tensors, dtypes, reinterpret_cast<const long long*>(counts), in, out, limit, norm, f64, ws, as_stream(stream)));
+}
 }  // namespace
 
 extern "C" {
@@ -526,6 +558,46 @@ int simnets_route_gradient(const simnets_route_desc* d, const void* scores, cons
     if (rc) return rc;
     if (d->batch > 0 && d->positions > 0 && ((d->sigmoid && !scores) || !index || !weights || !grad || !dscores)) return SIMNETS_E_NULL;
     return from_cuda(launch_route_gradient(*d, scores, prior, index, weights, grad, dscores, as_stream(stream)));
+}
+
+int simnets_log_probabilities(const simnets_likelihood_desc* d, const void* logits, const int64_t* labels, void* label, void* entropy, int32_t* top_index, void* top,
+                              void* stats, void* stream) {
+    const int rc = likelihood_check(d);
+    if (rc) return rc;
+    if (d->batch == 0 || d->positions == 0) return SIMNETS_OK;
+    if (!logits || (label && !labels) || (top == nullptr) != (top_index == nullptr)) return SIMNETS_E_NULL;
+    if ((d->top_k > 0) != (top != nullptr)) return SIMNETS_E_DESC;
+    return from_cuda(launch_log_probabilities(*d, logits, reinterpret_cast<const long long*>(labels), label, entropy, top_index, top, stats, as_stream(stream)));
+}
+
+int simnets_log_probabilities_gradient(const simnets_likelihood_desc* d, const void* logits, const int64_t* labels, const void* stats, const int32_t* top_index,
+                                       const void* g_label, const void* g_entropy, const void* g_top, void* dlogits, void* stream) {
+    const int rc = likelihood_check(d);
+    if (rc) return rc;
+    if (d->batch == 0 || d->positions == 0) return SIMNETS_OK;
+    if (!logits || !stats || !dlogits || (g_label && !labels) || (g_top && !top_index)) return SIMNETS_E_NULL;
+    if ((d->top_k > 0) != (g_top != nullptr)) return SIMNETS_E_DESC;
+    return from_cuda(launch_log_probabilities_gradient(*d, logits, reinterpret_cast<const long long*>(labels), stats, top_index, g_label, g_entropy, g_top, dlogits,
+                                                       as_stream(stream)));
+}
+
+size_t simnets_gradient_norm_workspace_bytes(int32_t tensors) { return tensors < 0 ? 0 : gradient_norm_workspace_bytes(tensors); }
+
+int simnets_gradient_norm(int32_t order, int32_t tensors, const int32_t* dtypes, const int64_t* counts, const void* const* in, void* norm, void* ws, size_t ws_bytes,
+                          void* stream) {
+    const int rc = gradients_check(order, tensors, dtypes, counts, in, norm, ws, ws_bytes);
+    return rc ? rc : gradients(order, 0.0, tensors, dtypes, counts, in, nullptr, norm, ws, stream);
+}
+
+int simnets_clip_gradients(int32_t order, double max_norm, int32_t tensors, const int32_t* dtypes, const int64_t* counts, const void* const* in, void* const* out, void* norm,
+                           void* ws, size_t ws_bytes, void* stream) {
+    if (!(max_norm >= 0)) return SIMNETS_E_DESC;
+    if (tensors > 0 && !out) return SIMNETS_E_NULL;
+    const int rc = gradients_check(order, tensors, dtypes, counts, in, norm, ws, ws_bytes);
+    if (rc) return rc;
+    for (int i = 0; i < tensors; ++i)
+        if (counts[i] > 0 && !out[i]) return SIMNETS_E_NULL;
+    return gradients(order, max_norm, tensors, dtypes, counts, in, out, norm, ws, stream);
 }
 
 int64_t simnets_fp32_fma_probe(int32_t packed, int32_t iters, void* scratch, void* stream) {

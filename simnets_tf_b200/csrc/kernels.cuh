@@ -175,6 +175,16 @@ cudaError_t launch_route(const simnets_route_desc&, const void* scores, const vo
 cudaError_t launch_route_gradient(const simnets_route_desc&, const void* scores, const void* prior, const int* index, const void* weights, const void* grad,
                                   void* dscores, cudaStream_t);
 
+// likelihood.cu -- log probabilities of given classes, entropies, likeliest classes; any output may be null
+cudaError_t launch_log_probabilities(const simnets_likelihood_desc&, const void* logits, const long long* labels, void* label, void* entropy, int* top_index,
+                                     void* top, void* stats, cudaStream_t);
+cudaError_t launch_log_probabilities_gradient(const simnets_likelihood_desc&, const void* logits, const long long* labels, const void* stats, const int* top_index,
+                                              const void* g_label, const void* g_entropy, const void* g_top, void* dlogits, cudaStream_t);
+// gradients.cu -- the norm of a list of tensors (order 0: the largest magnitude), and, where out is given, the tensors scaled to a limit
+size_t gradient_norm_workspace_bytes(int tensors);
+cudaError_t launch_gradient_norm(int order, int tensors, const int* dtypes, const long long* values, const void* const* in, void* const* out, double limit, void* norm,
+                                 bool norm_f64, void* ws, cudaStream_t);
+
 size_t softmax_xent_workspace_bytes(int batch);
 cudaError_t launch_softmax_xent(int batch, int classes, float scale, const float* logits, const long long* labels, float* loss,
                                 float* dlogits, void* ws, cudaStream_t);

@@ -571,11 +571,12 @@ std::tuple<OptTensor, OptTensor, OptTensor> sim_checkpoint_backward(const SimPla
 }
 
 // The gradients of an operator that is differentiable once: where a graph of them is asked for, they lead to the operator's inputs and to the
-// incoming gradient by a node that refuses (without it a term with a second derivative would be dropped).
-variable_list once(const torch::autograd::Node& op, const Tensor& grad, variable_list out) {
+// incoming gradients, by a node that refuses (without it a term with a second derivative would be dropped).
+variable_list once(const torch::autograd::Node& op, const variable_list& grads, variable_list out) {
     if (!at::GradMode::is_enabled()) return out;
     torch::autograd::edge_list edges = op.next_edges();
-    edges.push_back(torch::autograd::impl::gradient_edge(grad));
+    for (const Tensor& g : grads)
+        if (g.defined()) edges.push_back(torch::autograd::impl::gradient_edge(g));
     const std::shared_ptr<torch::autograd::Node> refusal(new torch::autograd::Error("simnets_b200: " + op.name() + " is differentiable once", std::move(edges)),
                                                          torch::autograd::deleteNode);
     for (const Tensor& t : out)
@@ -602,7 +603,7 @@ struct MexCheckpointNode : torch::autograd::Node {
                                             want_dx, want_doff, sink);
         if (want_dx) out[0] = g.first;
         if (want_doff && !sink) out[1] = g.second;
-        return once(*this, grads[0], std::move(out));
+        return once(*this, grads, std::move(out));
     }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
@@ -659,7 +660,7 @@ struct SimCheckpointNode : torch::autograd::Node {
                                             want_dx, want_params, add ? dt_sink : std::nullopt, add ? dw_sink : std::nullopt);
         if (want_dx) out[0] = *std::get<0>(g);
         if (want_params && !add) { out[1] = *std::get<1>(g); out[2] = *std::get<2>(g); }
-        return once(*this, grads[0], std::move(out));
+        return once(*this, grads, std::move(out));
     }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
@@ -763,7 +764,7 @@ struct RouteNode : torch::autograd::Node {
         Tensor ds = at::empty(shape, wv.options());
         check(simnets_route_gradient(&d, d.sigmoid ? ptr(sv) : nullptr, prior ? ptr(*prior) : nullptr, iv.data_ptr<int32_t>(), ptr(wv), ptr(g), ptr(ds), stream_of(wv)));
         out[0] = ds;
-        return once(*this, grads[0], std::move(out));
+        return once(*this, grads, std::move(out));
     }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
@@ -850,6 +851,246 @@ Tensor xent_apply(const Tensor& logits, const Tensor& labels, double scale) {
     return loss;
 }
 
+// ------------------------------------------------------------------------------------------------------- log probabilities
+// Sizes [batch, classes, positions] of logits with the classes on `axis` (1, or the last), and their strides; false where the positions
+// have no common stride.
+bool likelihood_desc(const Tensor& x, int64_t axis, int64_t top_k, simnets_likelihood_desc* d) {
+    *d = {};
+    d->dtype = x.scalar_type() == at::kDouble ? SIMNETS_F64 : SIMNETS_F32;
+    d->top_k = int32_t(top_k);
+    d->top_last = axis != 1;
+    d->classes = int32_t(x.size(axis));
+    d->stride_class = x.size(axis) == 1 ? 1 : x.stride(axis);
+    d->batch = x.size(0);
+    d->stride_batch = x.stride(0);
+    d->positions = 1;
+    for (int64_t i = x.dim() - 1; i > 0; --i) {                       // from the innermost out
+        if (i == axis || x.size(i) == 1) continue;
+        if (d->positions == 1) d->stride_position = x.stride(i);
+        else if (x.stride(i) != d->stride_position * d->positions) return false;
+        d->positions *= x.size(i);
+    }
+    if (d->positions == 1 || d->batch == 1) {                         // one axis of positions
+        if (d->positions == 1) { d->positions = d->batch; d->stride_position = d->stride_batch; }
+        if (d->batch != 1 && d->top_k > 0) d->top_last = 1;           // ([batch, top_k])
+        d->batch = 1;
+        d->stride_batch = 0;
+    }
+    return d->stride_class == 1 || d->stride_position == 1;
+}
+
+struct Likelihood { Tensor label, entropy, top_index, top, stats; };
+
+// logits as the library reads them
+Tensor likelihood_logits(const Tensor& x, int64_t axis, int64_t top_k, simnets_likelihood_desc* d) {
+    if (likelihood_desc(x, axis, top_k, d)) return x;
+    const Tensor dense = x.contiguous();
+    likelihood_desc(dense, axis, top_k, d);
+    return dense;
+}
+
+void check_likelihood(const Tensor& logits, const OptTensor& labels, int64_t top_k, int64_t axis) {
+    if (logits.dim() < 2 || (axis != 1 && axis != logits.dim() - 1)) throw std::invalid_argument("logits must have the classes on axis 1 or the last one");
+    if (logits.scalar_type() != at::kFloat && logits.scalar_type() != at::kDouble) throw py::type_error("simnets ops are registered for float32 and float64 only");
+    const int64_t k = logits.size(axis);
+    if (k < 1 || k > (1 << 30)) throw std::invalid_argument("logits must have 1 to 2^30 classes, got " + std::to_string(k));
+    if (top_k < 0 || top_k > 16 || top_k > k) throw std::invalid_argument("top_k must be 0 to 16 and at most the number of classes, got " + std::to_string(top_k));
+    require_cuda_all(logits);
+    if (!labels) return;
+    if (!labels->is_cuda() || labels->device() != logits.device()) throw std::runtime_error("labels must live on the device of the logits");
+    if (labels->scalar_type() != at::kLong) throw py::type_error("labels must be int64");
+    std::vector<int64_t> want = logits.sizes().vec();
+    want.erase(want.begin() + axis);
+    if (labels->sizes() != at::IntArrayRef(want)) throw std::invalid_argument("labels must have shape " + shape_text(want) + ", got " + shape_text(labels->sizes()));
+}
+
+Likelihood likelihood_impl(const Tensor& logits_in, const OptTensor& labels_in, int64_t top_k, bool entropy, int64_t axis, bool stats) {
+    simnets_likelihood_desc d;
+    const c10::cuda::CUDAGuard guard(logits_in.device());
+    const Tensor logits = likelihood_logits(logits_in, axis, top_k, &d);
+    OptTensor labels;
+    if (labels_in) labels = labels_in->contiguous();
+    std::vector<int64_t> shape = logits.sizes().vec(), top_shape = shape;
+    shape.erase(shape.begin() + axis);
+    top_shape[axis] = top_k;
+    const auto like = at::TensorOptions().dtype(logits.scalar_type()).device(logits.device());
+    Likelihood r;
+    if (labels) r.label = at::empty(shape, like);
+    if (entropy) r.entropy = at::empty(shape, like);
+    if (top_k > 0) {
+        r.top = at::empty(top_shape, like);
+        r.top_index = at::empty(top_shape, like.dtype(at::kInt));
+    }
+    if (stats) r.stats = at::empty({3, d.batch * d.positions}, like);
+    auto at_or_null = [](const Tensor& t) { return t.defined() ? ptr(t) : nullptr; };
+    if (d.batch * d.positions > 0)
+        check(simnets_log_probabilities(&d, ptr(logits), labels ? labels->data_ptr<int64_t>() : nullptr, at_or_null(r.label), at_or_null(r.entropy),
+                                        r.top_index.defined() ? r.top_index.data_ptr<int32_t>() : nullptr, at_or_null(r.top), at_or_null(r.stats), stream_of(logits)));
+    return r;
+}
+
+struct LikelihoodNode : torch::autograd::Node {
+    SavedVariable logits, labels, stats, top_index;
+    int64_t axis = 1, top_k = 0;
+    int label_at = -1, entropy_at = -1, top_at = -1;          // places of the outputs among those of the node
+    std::string name() const override { return "LogProbabilitiesBackward"; }
+    variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        variable_list out(1);
+        auto given = [&](int i) { return i >= 0 && grads[i].defined() ? OptTensor(grads[i].contiguous()) : OptTensor(); };
+        const OptTensor gl = given(label_at), ge = given(entropy_at), gt = given(top_at);
+        if ((!gl && !ge && !gt) || !task_should_compute_output(0)) return out;
+        const Tensor xv = logits.unpack(), lv = labels.unpack(), sv = stats.unpack(), iv = top_index.unpack();
+        simnets_likelihood_desc d;
+        const c10::cuda::CUDAGuard guard(xv.device());
+        const Tensor x = likelihood_logits(xv, axis, gt ? top_k : 0, &d);
+        std::vector<int64_t> shape = x.sizes().vec();
+        shape.erase(shape.begin() + axis);
+        for (const OptTensor* g : {&gl, &ge, &gt}) {
+            if (!*g) continue;
+            require_cuda(x, **g);
+            if (g == &gt ? (*g)->sizes() != iv.sizes() : (*g)->sizes() != at::IntArrayRef(shape))
+                throw std::invalid_argument("log_probabilities: gradient has shape " + shape_text((*g)->sizes()));
+        }
+        Tensor dx = empty_in_order(x, d);
+        if (x.numel() > 0)
+            check(simnets_log_probabilities_gradient(&d, ptr(x), lv.defined() ? lv.data_ptr<int64_t>() : nullptr, ptr(sv), gt ? iv.data_ptr<int32_t>() : nullptr,
+                                                     gl ? ptr(*gl) : nullptr, ge ? ptr(*ge) : nullptr, gt ? ptr(*gt) : nullptr, ptr(dx), stream_of(x)));
+        out[0] = dx;
+        return once(*this, grads, std::move(out));
+    }
+    // dense in the order in which dlogits is written: the classes of a position together, or the positions of a class
+    Tensor empty_in_order(const Tensor& x, const simnets_likelihood_desc& d) const {
+        std::vector<int64_t> shape = x.sizes().vec();
+        shape.erase(shape.begin() + axis);
+        const int64_t place = d.stride_class == 1 ? x.dim() - 1 : d.batch == 1 ? 0 : 1;
+        shape.insert(shape.begin() + place, x.size(axis));
+        return at::empty(shape, at::TensorOptions().dtype(x.scalar_type()).device(x.device())).movedim(place, axis);
+    }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        logits.reset_data(); labels.reset_data(); stats.reset_data(); top_index.reset_data();
+    }
+};
+
+using LikelihoodOut = std::tuple<OptTensor, OptTensor, OptTensor, OptTensor>;
+
+// (label, entropy, top_index, top), each only if asked for; all but the index differentiable with respect to the logits
+LikelihoodOut log_probabilities_apply(const Tensor& logits, const OptTensor& labels, int64_t top_k, bool entropy, int64_t axis) {
+    refuse_tangents({&logits});
+    check_likelihood(logits, labels, top_k, axis);
+    const bool track = at::GradMode::is_enabled() && logits.requires_grad();
+    Likelihood r;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        r = likelihood_impl(logits, labels, top_k, entropy, axis, track);
+    }
+    if (track && (labels || entropy || top_k > 0)) {
+        auto node = std::shared_ptr<LikelihoodNode>(new LikelihoodNode(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(logits));
+        node->axis = axis;
+        node->top_k = top_k;
+        node->logits = SavedVariable(logits, false);
+        if (labels) node->labels = SavedVariable(labels->contiguous(), false);
+        node->stats = SavedVariable(r.stats, false);
+        if (r.top_index.defined()) node->top_index = SavedVariable(r.top_index, false);
+        int n = 0;
+        for (auto& [t, at] : {std::pair<Tensor*, int*>{&r.label, &node->label_at}, {&r.entropy, &node->entropy_at}, {&r.top, &node->top_at}})
+            if (t->defined()) {
+                torch::autograd::set_history(*t, node);
+                *at = n++;
+            }
+    }
+    auto given = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+    return {given(r.label), given(r.entropy), given(r.top_index), given(r.top)};
+}
+
+// -------------------------------------------------------------------------------------------------- norm of many gradients
+// Whether no two elements share their memory.
+bool elements_apart(const Tensor& t) {
+    if (t.is_non_overlapping_and_dense()) return true;
+    std::vector<std::pair<int64_t, int64_t>> dims;            // (stride, size)
+    for (int64_t i = 0; i < t.dim(); ++i)
+        if (t.size(i) > 1) dims.emplace_back(t.stride(i), t.size(i));
+    std::sort(dims.begin(), dims.end());
+    int64_t span = 1;
+    for (const auto& [stride, size] : dims) {
+        if (stride < span) return false;
+        span += stride * (size - 1);
+    }
+    return true;
+}
+
+// Refuses a list where a tensor that is written shares memory with another of the list (a tensor may be its own destination).
+void refuse_overlaps(const std::vector<Tensor>& in, const std::vector<Tensor>& out) {
+    struct Range { uintptr_t begin, end; bool written; };
+    std::vector<Range> ranges;
+    for (size_t i = 0; i < out.size(); ++i) {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(ptr(out[i])), b = reinterpret_cast<uintptr_t>(ptr(in[i]));
+        const size_t bytes = out[i].nbytes();
+        if (bytes == 0) continue;
+        ranges.push_back({a, a + bytes, true});
+        if (a != b) ranges.push_back({b, b + bytes, false});
+    }
+    std::sort(ranges.begin(), ranges.end(), [](const Range& x, const Range& y) { return x.begin < y.begin; });
+    uintptr_t read = 0, written = 0;
+    for (const Range& r : ranges) {
+        if (r.begin < written || (r.written && r.begin < read)) throw std::invalid_argument("two of the tensors share memory: each must be given once");
+        (r.written ? written : read) = std::max(r.written ? written : read, r.end);
+    }
+}
+
+// The norm (order 2, or 0: the largest magnitude) of all tensors; with `scaled` they are clipped, into `out` where it is given, else in place.
+Tensor gradients_impl(const std::vector<Tensor>& given, int64_t order, bool scaled, double max_norm, const std::optional<std::vector<Tensor>>& out) {
+    if (given.empty()) throw std::invalid_argument("gradients: no tensors");
+    if (out && out->size() != given.size()) throw std::invalid_argument("out must have one tensor for each gradient");
+    const std::vector<Tensor>& to = out ? *out : given;
+    bool f64 = false;
+    for (size_t i = 0; i < given.size(); ++i) {
+        const Tensor& t = given[i];
+        if (t.layout() != at::kStrided) throw py::type_error("gradients must be dense tensors");
+        if (t.scalar_type() != at::kFloat && t.scalar_type() != at::kDouble) throw py::type_error("simnets ops are registered for float32 and float64 only");
+        if (!t.is_cuda()) throw std::runtime_error("simnets_b200 has no CPU kernels: every tensor must live on a CUDA device");
+        if (t.device() != given[0].device()) throw std::runtime_error("all tensors of one op call must be on the same device");
+        if (at::GradMode::is_enabled() && (t.requires_grad() || (scaled && to[i].requires_grad()))) throw std::invalid_argument("the norm of gradients has no gradient itself: detach them");
+        f64 = f64 || t.scalar_type() == at::kDouble;
+        if (!scaled) continue;
+        if (to[i].layout() != at::kStrided || to[i].sizes() != t.sizes() || to[i].scalar_type() != t.scalar_type() || to[i].device() != t.device())
+            throw std::invalid_argument("out must have the shapes, types and device of the gradients");
+        if (!elements_apart(to[i])) throw std::invalid_argument("a tensor that is written has elements that share memory");
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::cuda::CUDAGuard guard(given[0].device());
+    // dense ones as they lie; a copy of the others, which is scaled and copied back
+    std::vector<Tensor> in, dst;
+    std::vector<int32_t> dtypes;
+    std::vector<int64_t> counts;
+    std::vector<const void*> from;
+    std::vector<void*> into;
+    for (size_t i = 0; i < given.size(); ++i) {
+        in.push_back(given[i].is_non_overlapping_and_dense() ? given[i] : given[i].contiguous());
+        dtypes.push_back(in[i].scalar_type() == at::kDouble ? SIMNETS_F64 : SIMNETS_F32);
+        counts.push_back(in[i].numel());
+        from.push_back(ptr(in[i]));
+        if (!scaled) continue;
+        const bool direct = to[i].is_non_overlapping_and_dense() && (to[i].strides() == in[i].strides() || to[i].numel() < 2);
+        dst.push_back(direct ? to[i] : in[i].data_ptr() != given[i].data_ptr() ? in[i] : at::empty_strided(in[i].sizes(), in[i].strides(), in[i].options()));
+        into.push_back(ptr(dst[i]));
+    }
+    if (scaled) {
+        refuse_overlaps(in, dst);
+        for (const Tensor& t : to) torch::autograd::impl::bump_version(t);
+    }
+    const Tensor norm = at::empty({}, given[0].options().dtype(f64 ? at::kDouble : at::kFloat));
+    const int32_t n = int32_t(in.size());
+    const Tensor ws = scratch(norm, std::max<size_t>(simnets_gradient_norm_workspace_bytes(n), 256));
+    check(scaled ? simnets_clip_gradients(int32_t(order), max_norm, n, dtypes.data(), counts.data(), from.data(), into.data(), ptr(norm), ptr(ws), ws.numel(), stream_of(norm))
+                 : simnets_gradient_norm(int32_t(order), n, dtypes.data(), counts.data(), from.data(), ptr(norm), ptr(ws), ws.numel(), stream_of(norm)));
+    for (size_t i = 0; i < dst.size(); ++i)
+        if (!dst[i].is_same(to[i])) to[i].copy_(dst[i]);
+    return norm;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -905,6 +1146,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("mixture_parameters", &mixture_parameters);
     m.def("xent_with_grad", &xent_with_grad);
     m.def("xent_apply", &xent_apply);
+    m.def("log_probabilities", &log_probabilities_apply);
+    m.def("gradient_norm", [](const std::vector<Tensor>& given, int64_t order) { return gradients_impl(given, order, false, 0.0, std::nullopt); });
+    m.def("clip_gradients", [](const std::vector<Tensor>& given, double max_norm, int64_t order, const std::optional<std::vector<Tensor>>& out) {
+        return gradients_impl(given, order, true, max_norm, out);
+    });
     m.def("profile_start", [] { py::list dropped = profile_take(); g_profiling = true; });
     m.def("profile_stop", [] { g_profiling = false; return profile_take(); });
 }

@@ -9,6 +9,8 @@ src/kernels/mex_grad_kernel_cpu.cpp:298-368).  Summing shard results over ranks 
 import torch
 import torch.distributed as dist
 
+from .ops.gradients import clip_gradients, gradient_norm
+
 
 class GradBucket(object):
     """Flat gradient storage: each parameter's `.grad` is a view into `flat`, so autograd accumulates
@@ -44,6 +46,15 @@ class GradBucket(object):
             return None
         return dist.all_reduce(self.flat, op=dist.ReduceOp.SUM, group=group, async_op=async_op)
 
+    def norm(self, order=2):
+        """The norm of all gradients in the bucket (order 2, or math.inf for the largest magnitude), as a 0-d tensor on its device."""
+        return gradient_norm(self.flat, order=order)
+
+    def clip(self, max_norm, order=2):
+        """Scales the gradients so that their norm is at most `max_norm` (see `ops.gradients.clip_gradients`) and returns the norm before.
+        Behind `all_reduce` every rank has the same gradients, takes the same norm and needs no collective for it."""
+        return clip_gradients(self.flat, max_norm, order=order)
+
     def nbytes(self):
         return self.flat.numel() * self.flat.element_size()
 
@@ -71,12 +82,13 @@ class OverlappedStep(object):
     Per step: A on the main stream; the tail's all-reduce on a second stream as soon as A is done; B on the main
     stream meanwhile; the head's all-reduce behind B; join.  With `graphs=True` A and B are two CUDA graphs captured
     once and replayed; the collectives are always enqueued eagerly, outside any capture (capture needs that no autograd
-    graph built on another stream is still alive, e.g. through a loss tensor kept from an earlier step).  The reference has no
-    distributed code; the sums continued here are its batch loops (src/kernels/mex_grad_kernel_cpu.cpp:298-368,
-    similarity_grad_kernel_cpu.cpp:84-144)."""
+    graph built on another stream is still alive, e.g. through a loss tensor kept from an earlier step).  With `max_norm` the
+    summed gradients are clipped behind the collectives, and `norm` is their norm before.  The reference has no distributed code;
+    the sums continued here are its batch loops (src/kernels/mex_grad_kernel_cpu.cpp:298-368, similarity_grad_kernel_cpu.cpp:84-144)."""
 
-    def __init__(self, net, bucket, x, labels, global_batch, graphs=True):
+    def __init__(self, net, bucket, x, labels, global_batch, graphs=True, max_norm=None, order=2):
         import torch
+        self.max_norm, self.order, self.norm = max_norm, order, None
         self.torch, self.net, self.bucket, self.x, self.labels, self.gb = torch, net, bucket, x, labels, global_batch
         self.cut = net.split_point()
         tail = net.parameters_from(self.cut) if self.cut > 0 else []
@@ -151,6 +163,8 @@ class OverlappedStep(object):
             self._piece_b()
         self.bucket.all_reduce_range(0, self.tail_begin)
         main.wait_stream(self.side)
+        if self.max_norm is not None:
+            self.norm = self.bucket.clip(self.max_norm, self.order)
         return self.loss
 
 

@@ -20,6 +20,7 @@ from torch.nn.modules import module as _module
 
 from . import keras as layers
 from ._torch_glue import is_tracing
+from .ops.likelihood import log_probabilities
 from .ops.loss import softmax_cross_entropy
 
 
@@ -164,6 +165,11 @@ class SimNet(torch.nn.Module):
         if logits.is_cuda and logits.dtype == torch.float32 and labels.dtype == torch.int64:
             return softmax_cross_entropy(logits, labels, 1.0 / n)       # loss and gradient in one library launch
         return F.cross_entropy(logits, labels, reduction="sum") / n
+
+    def log_probabilities(self, x, labels=None, top_k=0, entropy=False):
+        """What the network answers for `x`: log probabilities of `labels`, entropy, the `top_k` likeliest classes (see
+        `ops.likelihood.log_probabilities`).  A network without a flattening last layer answers at every position of its map."""
+        return log_probabilities(self.forward(x), labels, top_k, entropy)
 
     def loss(self, x, labels, global_batch=None):
         """Softmax cross-entropy summed over this shard and divided by the global batch."""
