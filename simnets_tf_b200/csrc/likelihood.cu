@@ -8,6 +8,7 @@
 //
 // Logits of -infinity are classes that cannot be: exp(-infinity) = 0, and d is held at kFar in T, where exp(d) is 0 already.  Where all are, the
 // answer is log p = -infinity, H = 0, dx = 0.  A NaN, and an infinity by d = infinity - infinity, makes S a NaN and with it every answer of the position.
+#include <cooperative_groups.h>
 #include "kernels.cuh"
 
 namespace simnets {
@@ -36,10 +37,10 @@ struct Sums {
         s *= r;
         m = to;
     }
-    // (where nothing can be, m stays -infinity and is no base for differences; what comes together is added up by itself first, which
+    // the largest of U more classes, which are added.  (Where nothing can be, m stays -infinity and is no base for differences; what comes together is added up by itself first, which
     // makes the chains of roundings U times shorter)
     template <int U>
-    __device__ __forceinline__ void add(const T (&x)[U]) {
+    __device__ __forceinline__ T add(const T (&x)[U]) {
         T hi = x[0];
 #pragma unroll
         for (int u = 1; u < U; ++u) hi = larger(hi, x[u]);
@@ -54,6 +55,7 @@ struct Sums {
         }
         s += more_s;
         t += more_t;
+        return hi;
     }
     __device__ __forceinline__ void join(Sums o) {
         if (o.m > m) raise(o.m);
@@ -127,12 +129,10 @@ struct Answers {
     int* top_index;
 };
 
+// `x` the logits of position q, `of_label` that of its label
 template <typename T>
-__device__ __forceinline__ void write_position(const Logits& g, const Answers<T>& a, long long q, const T* x, const Answer<T>& w) {
-    if (a.label) {
-        const long long c = a.labels[q];
-        a.label[q] = c >= 0 && c < g.classes ? w.of(x[c * g.stride_class]) : T(0);
-    }
+__device__ __forceinline__ void write_position(const Logits& g, const Answers<T>& a, long long q, T of_label, bool labelled, const Answer<T>& w) {
+    if (a.label) a.label[q] = labelled ? w.of(of_label) : T(0);
     if (a.entropy) a.entropy[q] = w.entropy;
     if (a.stats) {
         const long long n = g.count();
@@ -142,39 +142,222 @@ __device__ __forceinline__ void write_position(const Logits& g, const Answers<T>
     }
 }
 
-// ---------------------------------------------------------------------------------------------------- a lane a position
 constexpr int kAhead = 8;        // loads that a lane has under way
 
+// ---------------------------------------------------------------------------------------------------- a lane a position
+// For maps, whose positions lie side by side, and for rows of so few classes that a warp's rows are a few lines of memory.  Where there
+// are few positions several warps share 32 of them, each a run of the classes; what they found is joined pair by pair, lower classes first.
 template <typename T, int TOP>
-__global__ void __launch_bounds__(128) answer_lanes(Logits g, Answers<T> a) {
-    stream_order();
-    const long long q = (long long)blockIdx.x * 128 + threadIdx.x;
-    if (q >= g.count()) return;
-    const T* x = a.logits + g.at(q);
+struct Found {
     Sums<T> sums;
     Largest<T, TOP> top;
-    sums.clear();
-    top.clear();
-    for (int c = 0; c < g.classes; c += kAhead) {
-        T v[kAhead];
+    static constexpr size_t kBytes = 32 * (3 * sizeof(T) + TOP * (sizeof(T) + sizeof(int)));
+    __device__ __forceinline__ void put(char* to, int lane) const {
+        T* v = reinterpret_cast<T*>(to) + lane;
+        v[0] = sums.m; v[32] = sums.s; v[64] = sums.t;
+        int* i = reinterpret_cast<int*>(reinterpret_cast<T*>(to) + 32 * (3 + TOP)) + lane;
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) v[u] = c + u < g.classes ? x[(c + u) * g.stride_class] : -infinity<T>();
-        sums.add(v);
-        if (TOP > 0) {
+        for (int j = 0; j < TOP; ++j) { v[32 * (3 + j)] = top.v[j]; i[32 * j] = top.i[j]; }
+    }
+    __device__ __forceinline__ void join(const char* from, int lane) {
+        const T* v = reinterpret_cast<const T*>(from) + lane;
+        sums.join({v[0], v[32], v[64]});
+        const int* i = reinterpret_cast<const int*>(reinterpret_cast<const T*>(from) + 32 * (3 + TOP)) + lane;
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) top.offer(v[u], c + u);
+        for (int j = 0; j < TOP; ++j) {
+            const T x = v[32 * (3 + j)];
+            if (!__any_sync(0xffffffffu, x > top.v[TOP - 1])) break;
+            top.offer(x, i[32 * j]);
         }
     }
-    const Answer<T> w(sums);
-    write_position(g, a, q, x, w);
+};
+
+// position of a lane, the same for all threads of a column; beyond the last one it is that one again, and nothing is written
+__device__ __forceinline__ long long lane_position(const Logits& g, bool* mine) {
+    const long long q = ((long long)blockIdx.x * blockDim.z + threadIdx.z) * 32 + threadIdx.x, n = g.count();
+    *mine = q < n;
+    return q < n ? q : n - 1;
+}
+// the classes [begin, end) of a warp
+__device__ __forceinline__ void warp_classes(const Logits& g, int* begin, int* end) {
+    const int share = (g.classes + int(blockDim.y) - 1) / int(blockDim.y);
+    *begin = min(g.classes, int(threadIdx.y) * share);
+    *end = min(g.classes, *begin + share);
+}
+
+template <typename T, int TOP>
+__global__ void __launch_bounds__(512) answer_lanes(Logits g, Answers<T> a) {
+    stream_order();
+    extern __shared__ __align__(16) char room[];
+    bool mine;
+    const long long q = lane_position(g, &mine);
+    const T* x = a.logits + g.at(q);
+    const long long label = a.label && threadIdx.y == 0 ? a.labels[q] : -1;
+    const bool labelled = label >= 0 && label < g.classes;
+    const T of_label = labelled ? x[label * g.stride_class] : T(0);
+    Found<T, TOP> f;
+    f.sums.clear();
+    f.top.clear();
+    int begin, end;
+    warp_classes(g, &begin, &end);
+    for (int c = begin; c < end; c += kAhead) {
+        T v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) v[u] = c + u < end ? x[(c + u) * g.stride_class] : -infinity<T>();
+        const T hi = f.sums.add(v);
+        if (TOP > 0 && __any_sync(0xffffffffu, hi > f.top.v[TOP > 0 ? TOP - 1 : 0])) {
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) f.top.offer(v[u], c + u);
+        }
+    }
+    char* at = room + (threadIdx.z * blockDim.y + threadIdx.y) * Found<T, TOP>::kBytes;
+    for (int d = 1; d < int(blockDim.y); d *= 2) {
+        if (threadIdx.y % (2 * d) == d) f.put(at, threadIdx.x);
+        __syncthreads();
+        if (threadIdx.y % (2 * d) == 0 && threadIdx.y + d < blockDim.y) f.join(at + d * Found<T, TOP>::kBytes, threadIdx.x);
+    }
+    if (threadIdx.y != 0 || !mine) return;
+    const Answer<T> w(f.sums);
+    write_position(g, a, q, of_label, labelled, w);
 #pragma unroll
     for (int j = 0; j < TOP; ++j) {
         if (j >= g.top_k) break;
-        a.top_index[g.top_at(q, j)] = top.i[j];
-        a.top[g.top_at(q, j)] = top.i[j] < 0 ? -infinity<T>() : w.of(top.v[j]);
+        a.top_index[g.top_at(q, j)] = f.top.i[j];
+        a.top[g.top_at(q, j)] = f.top.i[j] < 0 ? -infinity<T>() : w.of(f.top.v[j]);
     }
 }
 
+// ----------------------------------------------------------------------------------------------- several lanes a position
+// For rows, whose classes lie side by side: a warp, a CTA or a cluster of CTAs a row.  The largest so far are a list of the warp, the j-th of them in
+// lane j; a class is compared with the last one that counts, and only one above it moves the list.
+template <typename T>
+struct WarpList {
+    T v, last;               // this lane's value; the value of place top_k - 1
+    int i;
+    __device__ __forceinline__ void clear() { v = last = -infinity<T>(); i = -1; }
+    __device__ __forceinline__ void insert(T x, int c, int top_k) {
+        // (a free place is -infinity and -1, the largest of unsigned indices)
+        const unsigned behind = __ballot_sync(0xffffffffu, x > v || (x == v && unsigned(c) < unsigned(i)));
+        const T up = __shfl_up_sync(0xffffffffu, v, 1);
+        const int up_i = __shfl_up_sync(0xffffffffu, i, 1);
+        const int lane = threadIdx.x % 32, place = __ffs(behind) - 1;
+        if (behind && lane >= place) { v = lane == place ? x : up; i = lane == place ? c : up_i; }
+        last = __shfl_sync(0xffffffffu, v, top_k - 1);
+    }
+    // one value of each lane, of class `first` + lane; those in the list are of lower classes, or of these
+    __device__ __forceinline__ void offer(T x, int first, int top_k) {
+        unsigned who = __ballot_sync(0xffffffffu, x > last);
+        while (who) {
+            const int from = __ffs(who) - 1;
+            insert(__shfl_sync(0xffffffffu, x, from), first + from, top_k);
+            who &= ~(1u << from) & __ballot_sync(0xffffffffu, x > last);
+        }
+    }
+    // another list, place j of it in lane j
+    __device__ __forceinline__ void join(T x, int c, int top_k) {
+        for (int j = 0; j < top_k; ++j) {
+            const T xj = __shfl_sync(0xffffffffu, x, j);
+            if (!(xj >= last) || xj == -infinity<T>()) break;
+            insert(xj, __shfl_sync(0xffffffffu, c, j), top_k);
+        }
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ Sums<T> over_warp(Sums<T> a) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        const Sums<T> o = {__shfl_xor_sync(0xffffffffu, a.m, d), __shfl_xor_sync(0xffffffffu, a.s, d), __shfl_xor_sync(0xffffffffu, a.t, d)};
+        a.join(o);
+    }
+    return a;
+}
+
+// what a warp, and then a CTA, found
+template <typename T>
+struct RowFound {
+    Sums<T> sums;
+    T top[16];
+    int top_index[16];
+};
+
+// WARPS = 1: a warp a row, kRowWarps rows a CTA; else a cluster of gridDim.y CTAs of WARPS warps a row
+constexpr int kRowWarps = 8;
+template <typename T, bool TOP, int WARPS>
+__global__ void __launch_bounds__(32 * (WARPS == 1 ? kRowWarps : WARPS)) answer_rows(Logits g, Answers<T> a) {
+    stream_order();
+    __shared__ RowFound<T> found[WARPS == 1 ? 1 : WARPS];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const long long q = WARPS == 1 ? (long long)blockIdx.x * kRowWarps + warp : blockIdx.x;
+    if (WARPS == 1 && q >= g.count()) return;
+    const T* x = a.logits + g.at(q);
+    const long long label = a.label ? a.labels[q] : -1;
+    const bool labelled = label >= 0 && label < g.classes;
+    const T of_label = labelled ? x[label] : T(0);
+    Sums<T> sums;
+    WarpList<T> list;
+    sums.clear();
+    list.clear();
+    constexpr int kStep = 32 * WARPS;
+    const int span = kStep * kAhead;
+    for (long long c0 = (WARPS == 1 ? 0LL : (long long)blockIdx.y * span) + 32 * (WARPS == 1 ? 0 : warp); c0 < g.classes; c0 += (long long)span * gridDim.y) {
+        T v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) v[u] = c0 + u * kStep + lane < g.classes ? x[c0 + u * kStep + lane] : -infinity<T>();
+        const T hi = sums.add(v);
+        if (TOP && __any_sync(0xffffffffu, hi > list.last)) {
+#pragma unroll 1
+            for (int u = 0; u < kAhead; ++u) {
+                T x_u = v[0];
+#pragma unroll
+                for (int w = 1; w < kAhead; ++w) x_u = u == w ? v[w] : x_u;
+                list.offer(x_u, int(c0) + u * kStep, g.top_k);
+            }
+        }
+    }
+    sums = over_warp(sums);
+    if (WARPS > 1) {
+        // the warps of the CTA, then the CTAs of the cluster, into the first of them
+        const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+        RowFound<T>& own = found[warp];
+        if (lane == 0) own.sums = sums;
+        if (TOP && lane < 16) { own.top[lane] = list.v; own.top_index[lane] = list.i; }
+        __syncthreads();
+        if (warp == 0) {
+            if (TOP)
+                for (int w = 1; w < WARPS; ++w) list.join(lane < 16 ? found[w].top[lane] : -infinity<T>(), lane < 16 ? found[w].top_index[lane] : -1, g.top_k);
+            sums.clear();
+            if (lane < WARPS) sums = found[lane].sums;
+            sums = over_warp(sums);
+        }
+        if (gridDim.y > 1) {
+            __syncwarp();
+            if (warp == 0 && lane == 0) own.sums = sums;
+            if (TOP && warp == 0 && lane < 16) { own.top[lane] = list.v; own.top_index[lane] = list.i; }
+            cluster.sync();
+            if (warp == 0 && blockIdx.y == 0) {
+                sums.clear();
+                if (lane < int(gridDim.y)) sums = cluster.map_shared_rank(found, lane)->sums;
+                sums = over_warp(sums);
+                if (TOP)
+                    for (int r = 1; r < int(gridDim.y); ++r) {
+                        const RowFound<T>* other = cluster.map_shared_rank(found, r);
+                        list.join(lane < 16 ? other->top[lane] : -infinity<T>(), lane < 16 ? other->top_index[lane] : -1, g.top_k);
+                    }
+            }
+            cluster.sync();
+        }
+        if (warp != 0 || blockIdx.y != 0) return;
+    }
+    const Answer<T> w(sums);
+    if (lane == 0) write_position(g, a, q, of_label, labelled, w);
+    if (TOP && lane < g.top_k) {
+        a.top_index[g.top_at(q, lane)] = list.i;
+        a.top[g.top_at(q, lane)] = list.i < 0 ? -infinity<T>() : w.of(list.v);
+    }
+}
+
+// ----------------------------------------------------------------------------------------------------------- the gradient
 // What comes in for a position; any of the gradients may be null
 template <typename T>
 struct Gradients {
@@ -208,48 +391,118 @@ struct Share {
             for (int j = 0; j < g.top_k; ++j)
                 if (a.top_index[g.top_at(q, j)] >= 0) taken += a.top[g.top_at(q, j)];
     }
-    __device__ __forceinline__ T of(T x) const {
+    __device__ __forceinline__ T of(T x, long long c) const {
         const T l = (x - m) - log_s, p = exp_of(l);
-        return -p * (taken + g_entropy * (larger(l, far_below<T>()) + entropy));
+        const T dx = -p * (taken + g_entropy * (larger(l, far_below<T>()) + entropy));
+        return nothing ? T(0) : c == label ? dx + g_label : dx;
     }
 };
 
 template <typename T>
-__global__ void __launch_bounds__(128) gradient_lanes(Logits g, Gradients<T> a) {
+__global__ void __launch_bounds__(512) gradient_lanes(Logits g, Gradients<T> a) {
     stream_order();
-    const long long q = (long long)blockIdx.x * 128 + threadIdx.x;
-    if (q >= g.count()) return;
+    bool mine;
+    const long long q = lane_position(g, &mine);
+    if (!mine) return;
     const T* x = a.logits + g.at(q);
     T* dx = a.dlogits + (q / g.positions) * a.out_batch + (q % g.positions) * a.out_position;
     const Share<T> share(g, a, q);
-    for (int c = 0; c < g.classes; c += kAhead) {
+    int begin, end;
+    warp_classes(g, &begin, &end);
+    for (int c = begin; c < end; c += kAhead) {
         T v[kAhead];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) v[u] = c + u < g.classes ? x[(c + u) * g.stride_class] : -infinity<T>();
+        for (int u = 0; u < kAhead; ++u) v[u] = c + u < end ? x[(c + u) * g.stride_class] : -infinity<T>();
 #pragma unroll
         for (int u = 0; u < kAhead; ++u)
-            if (c + u < g.classes) dx[(c + u) * a.out_class] = share.nothing ? T(0) : share.of(v[u]) + (c + u == share.label ? share.g_label : T(0));
+            if (c + u < end) dx[(c + u) * a.out_class] = share.of(v[u], c + u);
     }
     if (a.top && !share.nothing)
         for (int j = 0; j < g.top_k; ++j) {
             const int c = a.top_index[g.top_at(q, j)];
-            if (c >= 0 && c < g.classes) dx[c * a.out_class] += a.top[g.top_at(q, j)];
+            if (c >= begin && c < end) dx[c * a.out_class] += a.top[g.top_at(q, j)];
         }
 }
 
+// WARPS = 1: a warp a row; else CTAs of WARPS warps share a row, blockIdx.y of them each kSegment classes
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(32 * (WARPS == 1 ? kRowWarps : WARPS)) gradient_rows(Logits g, Gradients<T> a) {
+    stream_order();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const long long q = WARPS == 1 ? (long long)blockIdx.x * kRowWarps + warp : blockIdx.x;
+    if (WARPS == 1 && q >= g.count()) return;
+    const T* x = a.logits + g.at(q);
+    T* dx = a.dlogits + (q / g.positions) * a.out_batch + (q % g.positions) * a.out_position;
+    const Share<T> share(g, a, q);
+    constexpr int kStep = 32 * WARPS;
+    const long long segment = ((g.classes + gridDim.y - 1) / gridDim.y + 31) / 32 * 32;
+    const long long begin = blockIdx.y * segment, end = begin + segment < g.classes ? begin + segment : g.classes;
+    for (long long c0 = begin + (WARPS == 1 ? lane : threadIdx.x); c0 < end; c0 += kStep * kAhead) {
+        T v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) v[u] = c0 + u * kStep < end ? x[c0 + u * kStep] : -infinity<T>();
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (c0 + u * kStep < end) dx[c0 + u * kStep] = share.of(v[u], c0 + u * kStep);
+    }
+    if (a.top) {
+        if (WARPS == 1) __syncwarp();
+        else __syncthreads();
+        if (!share.nothing && (WARPS == 1 || warp == 0) && lane < g.top_k) {
+            const int c = a.top_index[g.top_at(q, lane)];
+            if (c >= begin && c < end) dx[c] += a.top[g.top_at(q, lane)];
+        }
+    }
+}
+
+// --------------------------------------------------------------------------------------------------------------- launches
 Logits logits_of(const simnets_likelihood_desc& d) {
     return {d.batch, d.positions, d.stride_batch, d.stride_class, d.stride_position, d.classes, d.top_k, d.top_last};
 }
 
+// rows of more classes than this are read by several lanes
+bool by_rows(const Logits& g) { return g.stride_class == 1 && g.classes > 32; }
+
+// warps that share 32 positions
+int warps_of_lanes(const Logits& g, size_t bytes_a_warp) {
+    const long long tiles = (g.count() + 31) / 32;
+    int w = 1;
+    while (w < 16 && tiles * w < 32LL * device_sm_count() && g.classes >= 2 * w * kAhead && 2 * w * bytes_a_warp <= 48 * 1024) w *= 2;
+    return w;
+}
+
+template <class Kernel, class A>
+cudaError_t launch_lanes(Kernel* kernel, const Logits& g, const A& a, int warps, size_t bytes_a_warp, cudaStream_t s) {
+    const int tiles = warps < 4 ? 4 / warps : 1;
+    const unsigned grid = unsigned((g.count() + 32 * tiles - 1) / (32 * tiles));
+    in_stream_order(kernel, grid, dim3(32, warps, tiles), warps > 1 ? bytes_a_warp * warps * tiles : 0, s)(g, a);
+    count_launch();
+    return cudaGetLastError();
+}
+
 template <typename T, int TOP>
 cudaError_t answer_lanes_of(const Logits& g, const Answers<T>& a, cudaStream_t s) {
-    in_stream_order(answer_lanes<T, TOP>, unsigned((g.count() + 127) / 128), 128, 0, s)(g, a);
+    return launch_lanes(answer_lanes<T, TOP>, g, a, warps_of_lanes(g, Found<T, TOP>::kBytes), Found<T, TOP>::kBytes, s);
+}
+
+template <typename T, bool TOP>
+cudaError_t answer_rows_of(const Logits& g, const Answers<T>& a, cudaStream_t s) {
+    if (g.classes <= 1024) {
+        in_stream_order(answer_rows<T, TOP, 1>, unsigned((g.count() + kRowWarps - 1) / kRowWarps), 32 * kRowWarps, 0, s)(g, a);
+    } else {
+        int cluster = 1;
+        while (cluster < 8 && g.count() * cluster < 2LL * device_sm_count() && g.classes > 2048 * cluster) cluster *= 2;
+        const dim3 grid(unsigned(g.count()), cluster);
+        if (cluster > 1) in_stream_order(answer_rows<T, TOP, 32>, grid, 1024, 0, s, cluster)(g, a);
+        else in_stream_order(answer_rows<T, TOP, 8>, grid, 256, 0, s)(g, a);
+    }
     count_launch();
     return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t answer_as(const Logits& g, const Answers<T>& a, cudaStream_t s) {
+    if (by_rows(g)) return g.top_k > 0 ? answer_rows_of<T, true>(g, a, s) : answer_rows_of<T, false>(g, a, s);
     if (g.top_k == 0) return answer_lanes_of<T, 0>(g, a, s);
     if (g.top_k == 1) return answer_lanes_of<T, 1>(g, a, s);
     if (g.top_k <= 4) return answer_lanes_of<T, 4>(g, a, s);
@@ -259,7 +512,13 @@ cudaError_t answer_as(const Logits& g, const Answers<T>& a, cudaStream_t s) {
 
 template <typename T>
 cudaError_t gradient_as(const Logits& g, const Gradients<T>& a, cudaStream_t s) {
-    in_stream_order(gradient_lanes<T>, unsigned((g.count() + 127) / 128), 128, 0, s)(g, a);
+    if (!by_rows(g)) return launch_lanes(gradient_lanes<T>, g, a, warps_of_lanes(g, 0), 0, s);
+    if (g.classes <= 1024) {
+        in_stream_order(gradient_rows<T, 1>, unsigned((g.count() + kRowWarps - 1) / kRowWarps), 32 * kRowWarps, 0, s)(g, a);
+    } else {
+        const dim3 grid(unsigned(g.count()), (g.classes + 8191) / 8192 < 65535 ? (g.classes + 8191) / 8192 : 65535);
+        in_stream_order(gradient_rows<T, 8>, grid, 256, 0, s)(g, a);
+    }
     count_launch();
     return cudaGetLastError();
 }

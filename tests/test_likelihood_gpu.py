@@ -122,6 +122,15 @@ def test_each_number_of_alternatives_and_output(shape, axis, top_k, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=["f32", "f64"])
+@pytest.mark.parametrize("style", ["plain", "ties", "masked", "broken", "rising"])
+@pytest.mark.parametrize("rows,classes", [(1, 131072), (1, 1 << 20), (3, 40001), (40, 8193), (300, 2049), (5, 1025), (9, 1024)])
+def test_long_rows(rows, classes, style, kind):
+    """Up to a million classes; 256 lanes at least share a row from 1025 on, which makes chains of classes / 2048."""
+    x, labels = make((rows, classes), 1, style, kind)
+    verify(x, labels, 1, 8, True, torch.from_numpy(x).cuda(), chain=classes // 2048 + 64)
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=["f32", "f64"])
 def test_any_layout(kind):
     """The same values wherever they lie: slices, transposed, channels last, every other value, broadcast, at an odd address."""
     def laid(x, how):
