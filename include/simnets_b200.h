@@ -491,7 +491,7 @@ SIMNETS_API int simnets_softmax_cross_entropy(int32_t batch, int32_t classes, fl
  * simnets_log_probabilities_gradient: the gradient of all logits for the gradients g_label, g_entropy and g_top (each may be NULL) of the outputs,
  *   dlogits_c = -p_c (g_label + sum g_top + g_entropy (log p_c + entropy)) + g_label [c = labels] + sum over g_top [c = top_index],
  * 0 where no class can be; a label or an alternative that is none adds nothing.  dlogits is dense, [batch, positions, classes] if
- * stride_class is 1, else [batch, classes, positions].  The reference has softmax and cross-entropy of its framework only (README.md:108-111). */
+ * stride_class is 1, else [batch, classes, positions], and must not overlap the logits.  The reference has softmax and cross-entropy of its framework only (README.md:108-111). */
 typedef struct simnets_likelihood_desc {
     int32_t dtype;
     int32_t classes;

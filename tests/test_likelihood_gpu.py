@@ -163,6 +163,20 @@ def test_any_layout(kind):
     verify(np.ascontiguousarray(np.broadcast_to(x, (3, 40, 5))), np.broadcast_to(labels, (3, 5)).copy(), 1, 3, True, torch.from_numpy(x).cuda().expand(3, 40, 5))
 
 
+@pytest.mark.parametrize("kind", KINDS, ids=["f32", "f64"])
+def test_runs_of_nan_and_alternatives_behind_them(kind):
+    """Whole loads and whole chunks of NaN or of classes that cannot be, in front of the likeliest."""
+    for shape in ((2, 300), (2, 5000), (1, 70000), (2, 300, 3)):
+        for fill in (NAN, -INF, INF):
+            x, labels = make(shape, 1, "plain", kind)
+            x[:, :shape[1] * 3 // 4] = fill
+            verify(x, labels, 1, 9, True, torch.from_numpy(x).cuda())
+        x, labels = make(shape, 1, "plain", kind)
+        x[:] = NAN
+        x[:, -2] = 1.0
+        verify(x, labels, 1, 9, True, torch.from_numpy(x).cuda())
+
+
 def test_nothing_to_answer():
     for shape, axis in (((0, 5), 1), ((2, 5, 0), 1), ((0, 3, 5), 2), ((2, 0, 5), 2)):
         x = torch.zeros(shape, device="cuda", requires_grad=True)
