@@ -2,8 +2,10 @@
 //
 //     norm = sqrt(sum of g^2) over all tensors, or max |g|;   out = g * (limit / norm where norm > limit, else 1)
 //
-// Two launches: the partial results of a grid of CTAs, then every CTA of the second combines them again, in the same order and so to the same norm, and
-// scales its share.  The host never learns the norm.  Bound by memory: g is read twice and written once, the second time from L2 as far as it fits.
+// The partial results of a grid of CTAs are combined in a fixed order, and the host never learns the norm.  Bound by memory: g is read twice and
+// written once, the second time from the end, so that what was read last comes from L2.  A list that one wave of CTAs takes (up to 19 MB) is two launches,
+// and every CTA of the second combines the partial results again; beyond, one CTA does so in a launch between, which lets the last one
+// have as many CTAs as there is work (2.6e8 values: 295 us with a CTA for 16 KB, 310 with 64 a multiprocessor, 324 with 8, a plain copy 318).
 //
 // Sums are in 64 bits: squares of float32 are exact there and neither overflow nor vanish.  Squares of float64 can do both, so there are three sums of
 // them, of g, of g * 2^-600 and of g * 2^600, of which the one that holds numbers is taken.  The product g * scale is rounded once, from 64 bits.
@@ -177,19 +179,25 @@ __global__ void __launch_bounds__(kThreads) norm_finish(const Partial* partials,
     if (threadIdx.x == 0) write_norm(norm, f64, v);
 }
 
-// in_place: every tensor is its own destination, and nothing is to be done where the norm is within the limit
-template <bool MAX, typename T, int N>
-__global__ void __launch_bounds__(kThreads) scale_tensors(const __grid_constant__ Table<N> t, const Partial* partials, int count, bool f64, double limit, bool in_place, void* norm) {
+// ALONE: combines the partial results itself; else `norm` is there already.  in_place: every tensor is its own destination, and nothing is to be done
+// where the norm is within the limit.
+template <bool ALONE, bool MAX, typename T, int N>
+__global__ void __launch_bounds__(kThreads) scale_tensors(const __grid_constant__ Table<N> t, const Partial* partials, int count, bool f64, double limit, bool in_place, void* norm,
+                                                          bool writes_norm) {
     stream_order();
-    __shared__ Partial room[kThreads / 32];
     constexpr int kWidth = Vector<T>::kWidth, kSteps = kItemBytes / 16 / kThreads;
-    const double v = norm_of<MAX>(partials, count, f64, room);
-    if (norm && blockIdx.x == 0 && threadIdx.x == 0) write_norm(norm, f64, v);
+    double v;
+    if (ALONE) {
+        __shared__ Partial room[kThreads / 32];
+        v = norm_of<MAX>(partials, count, f64, room);
+        if (writes_norm && blockIdx.x == 0 && threadIdx.x == 0) write_norm(norm, f64, v);
+    } else {
+        v = f64 ? *static_cast<const double*>(norm) : double(*static_cast<const float*>(norm));
+    }
     // (a norm that is no number, or infinite, changes nothing)
     const bool scaled = v > limit && v < double(CUDART_INF);
     if (!scaled && in_place) return;
     const double scale = scaled ? limit / v : 1.0;
-    // from the end: what was read last is still in L2
     for (int item = t.first[t.tensors] - 1 - int(blockIdx.x); item >= 0; item -= gridDim.x) {
         const Item<T> it(t, item);
         Vector<T> x[kSteps];
@@ -219,7 +227,7 @@ long long items_of(const void* in, long long values, int size) {
     const long long skip = (long long)(reinterpret_cast<uintptr_t>(in) % 16) / size;
     return values > 0 ? (skip + values + kItemBytes / size - 1) / (kItemBytes / size) : 0;
 }
-int grid_of(long long items) { return int(std::min<long long>(items, 8LL * device_sm_count())); }
+int grid_of(long long items, int a_multiprocessor) { return int(std::min<long long>(items, (long long)a_multiprocessor * device_sm_count())); }
 // body(dtype, table, items, last) for every launch
 template <int N, class Body>
 cudaError_t each_table(const Call& c, Body body) {
@@ -251,7 +259,7 @@ template <bool MAX, int N>
 cudaError_t run(const Call& c, bool f64, bool in_place, double limit, void* norm, Partial* partials, cudaStream_t s) {
     int count = 0;
     cudaError_t e = each_table<N>(c, [&](int dtype, const Table<N>& t) {
-        const int grid = grid_of(t.first[t.tensors]);
+        const int grid = grid_of(t.first[t.tensors], 8);
         if (dtype == SIMNETS_F64) in_stream_order(norm_partials<MAX, double, N>, grid, kThreads, 0, s)(t, partials + count);
         else in_stream_order(norm_partials<MAX, float, N>, grid, kThreads, 0, s)(t, partials + count);
         count_launch();
@@ -259,18 +267,22 @@ cudaError_t run(const Call& c, bool f64, bool in_place, double limit, void* norm
         return cudaGetLastError();
     });
     if (e != cudaSuccess) return e;
-    if (!c.out || count == 0) {
+    const bool alone = c.out && count > 0 && count < 8 * device_sm_count();
+    if (!alone) {
         in_stream_order(norm_finish<MAX>, 1, kThreads, 0, s)(partials, count, f64, norm);
         count_launch();
-        return cudaGetLastError();
+        e = cudaGetLastError();
+        if (e != cudaSuccess || !c.out || count == 0) return e;
     }
-    void* to = norm;                                        // (the first launch writes it)
+    bool first = true;
     return each_table<N>(c, [&](int dtype, const Table<N>& t) {
-        const int grid = grid_of(t.first[t.tensors]);
-        if (dtype == SIMNETS_F64) in_stream_order(scale_tensors<MAX, double, N>, grid, kThreads, 0, s)(t, partials, count, f64, limit, in_place, to);
-        else in_stream_order(scale_tensors<MAX, float, N>, grid, kThreads, 0, s)(t, partials, count, f64, limit, in_place, to);
+        // (in place most calls have nothing to scale: fewer CTAs that come and go)
+        const int grid = grid_of(t.first[t.tensors], in_place ? 64 : 1 << 20);
+        auto launch = [&](auto kernel) { in_stream_order(kernel, grid, kThreads, 0, s)(t, partials, count, f64, limit, in_place, norm, first); };
+        if (alone) launch(dtype == SIMNETS_F64 ? scale_tensors<true, MAX, double, N> : scale_tensors<true, MAX, float, N>);
+        else launch(dtype == SIMNETS_F64 ? scale_tensors<false, MAX, double, N> : scale_tensors<false, MAX, float, N>);
         count_launch();
-        to = nullptr;
+        first = false;
         return cudaGetLastError();
     });
 }

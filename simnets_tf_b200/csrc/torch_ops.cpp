@@ -1021,18 +1021,11 @@ bool elements_apart(const Tensor& t) {
     return true;
 }
 
-// Refuses a list where a tensor that is written shares memory with another of the list (a tensor may be its own destination).
-void refuse_overlaps(const std::vector<Tensor>& in, const std::vector<Tensor>& out) {
-    struct Range { uintptr_t begin, end; bool written; };
-    std::vector<Range> ranges;
-    for (size_t i = 0; i < out.size(); ++i) {
-        const uintptr_t a = reinterpret_cast<uintptr_t>(ptr(out[i])), b = reinterpret_cast<uintptr_t>(ptr(in[i]));
-        const size_t bytes = out[i].nbytes();
-        if (bytes == 0) continue;
-        ranges.push_back({a, a + bytes, true});
-        if (a != b) ranges.push_back({b, b + bytes, false});
-    }
-    std::sort(ranges.begin(), ranges.end(), [](const Range& x, const Range& y) { return x.begin < y.begin; });
+struct Range { uintptr_t begin, end; bool written; };
+// Refuses ranges of memory of which one that is written overlaps another.
+void refuse_overlaps(std::vector<Range>& ranges) {
+    auto in_front = [](const Range& x, const Range& y) { return x.begin < y.begin; };
+    if (!std::is_sorted(ranges.begin(), ranges.end(), in_front)) std::sort(ranges.begin(), ranges.end(), in_front);
     uintptr_t read = 0, written = 0;
     for (const Range& r : ranges) {
         if (r.begin < written || (r.written && r.begin < read)) throw std::invalid_argument("two of the tensors share memory: each must be given once");
@@ -1040,54 +1033,102 @@ void refuse_overlaps(const std::vector<Tensor>& in, const std::vector<Tensor>& o
     }
 }
 
-// The norm (order 2, or 0: the largest magnitude) of all tensors; with `scaled` they are clipped, into `out` where it is given, else in place.
-Tensor gradients_impl(const std::vector<Tensor>& given, int64_t order, bool scaled, double max_norm, const std::optional<std::vector<Tensor>>& out) {
-    if (given.empty()) throw std::invalid_argument("gradients: no tensors");
-    if (out && out->size() != given.size()) throw std::invalid_argument("out must have one tensor for each gradient");
-    const std::vector<Tensor>& to = out ? *out : given;
+// The tensors of a Python sequence, or one tensor, as they are held there; None stays a null pointer.
+struct TensorList {
+    py::object held;
+    std::vector<const Tensor*> tensors;
+    explicit TensorList(const py::object& given) {
+        if (THPVariable_Check(given.ptr())) {
+            held = given;
+            tensors.push_back(&THPVariable_Unpack(given.ptr()));
+            return;
+        }
+        held = py::reinterpret_steal<py::object>(PySequence_Fast(given.ptr(), "a tensor or an iterable of tensors is wanted"));
+        if (!held) throw py::error_already_set();
+        const Py_ssize_t n = PySequence_Fast_GET_SIZE(held.ptr());
+        tensors.reserve(n);
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            PyObject* o = PySequence_Fast_GET_ITEM(held.ptr(), i);
+            if (o != Py_None && !THPVariable_CheckExact(o) && !THPVariable_Check(o)) throw py::type_error("a tensor or an iterable of tensors is wanted");
+            tensors.push_back(o == Py_None ? nullptr : &THPVariable_Unpack(o));
+        }
+    }
+};
+
+// The norm (order 2, or 0: the largest magnitude) of all tensors (None is left out); with `scaled` they are clipped, into `out` unless it is None, else in place.
+Tensor gradients_impl(const py::object& given_in, int64_t order, bool scaled, double max_norm, const py::object& out_in) {
+    const TensorList given(given_in);
+    std::optional<TensorList> out;
+    if (!out_in.is_none()) out.emplace(out_in);
+    const size_t n = given.tensors.size();
+    if (out && out->tensors.size() != n) throw std::invalid_argument("out must have one tensor for each gradient, got " + std::to_string(out->tensors.size()) + " for " + std::to_string(n));
+    const Tensor* first = nullptr;
     bool f64 = false;
-    for (size_t i = 0; i < given.size(); ++i) {
-        const Tensor& t = given[i];
+    for (size_t i = 0; i < n; ++i) {
+        const Tensor* const p = given.tensors[i];
+        if (!p) continue;
+        const Tensor& t = *p;
         if (t.layout() != at::kStrided) throw py::type_error("gradients must be dense tensors");
         if (t.scalar_type() != at::kFloat && t.scalar_type() != at::kDouble) throw py::type_error("simnets ops are registered for float32 and float64 only");
         if (!t.is_cuda()) throw std::runtime_error("simnets_b200 has no CPU kernels: every tensor must live on a CUDA device");
-        if (t.device() != given[0].device()) throw std::runtime_error("all tensors of one op call must be on the same device");
-        if (at::GradMode::is_enabled() && (t.requires_grad() || (scaled && to[i].requires_grad()))) throw std::invalid_argument("the norm of gradients has no gradient itself: detach them");
+        if (!first) first = p;
+        if (t.device() != first->device()) throw std::runtime_error("all tensors of one op call must be on the same device");
+        const Tensor* const q = out ? out->tensors[i] : p;
+        if (at::GradMode::is_enabled() && (t.requires_grad() || (q && q->requires_grad()))) throw std::invalid_argument("the norm of gradients has no gradient itself: detach them");
         f64 = f64 || t.scalar_type() == at::kDouble;
         if (!scaled) continue;
-        if (to[i].layout() != at::kStrided || to[i].sizes() != t.sizes() || to[i].scalar_type() != t.scalar_type() || to[i].device() != t.device())
+        if (!q || q->layout() != at::kStrided || q->sizes() != t.sizes() || q->scalar_type() != t.scalar_type() || q->device() != t.device())
             throw std::invalid_argument("out must have the shapes, types and device of the gradients");
-        if (!elements_apart(to[i])) throw std::invalid_argument("a tensor that is written has elements that share memory");
+        if (!elements_apart(*q)) throw std::invalid_argument("a tensor that is written has elements that share memory");
     }
+    if (!first) throw std::invalid_argument("gradients: no tensors");
     at::AutoDispatchBelowADInplaceOrView below;
-    const c10::cuda::CUDAGuard guard(given[0].device());
+    const c10::cuda::CUDAGuard guard(first->device());
     // dense ones as they lie; a copy of the others, which is scaled and copied back
-    std::vector<Tensor> in, dst;
+    std::vector<Tensor> copies;
+    std::vector<std::pair<const Tensor*, size_t>> back;                     // a destination, and the copy that goes there
+    std::vector<Range> ranges;
     std::vector<int32_t> dtypes;
     std::vector<int64_t> counts;
     std::vector<const void*> from;
     std::vector<void*> into;
-    for (size_t i = 0; i < given.size(); ++i) {
-        in.push_back(given[i].is_non_overlapping_and_dense() ? given[i] : given[i].contiguous());
-        dtypes.push_back(in[i].scalar_type() == at::kDouble ? SIMNETS_F64 : SIMNETS_F32);
-        counts.push_back(in[i].numel());
-        from.push_back(ptr(in[i]));
+    dtypes.reserve(n), counts.reserve(n), from.reserve(n);
+    if (scaled) into.reserve(n), ranges.reserve(2 * n);
+    for (size_t i = 0; i < n; ++i) {
+        const Tensor* const p = given.tensors[i];
+        if (!p) continue;
+        Tensor copy;
+        if (!p->is_non_overlapping_and_dense()) copies.push_back(copy = p->contiguous());
+        const Tensor& in = copy.defined() ? copy : *p;
+        dtypes.push_back(in.scalar_type() == at::kDouble ? SIMNETS_F64 : SIMNETS_F32);
+        counts.push_back(in.numel());
+        from.push_back(ptr(in));
         if (!scaled) continue;
-        const bool direct = to[i].is_non_overlapping_and_dense() && (to[i].strides() == in[i].strides() || to[i].numel() < 2);
-        dst.push_back(direct ? to[i] : in[i].data_ptr() != given[i].data_ptr() ? in[i] : at::empty_strided(in[i].sizes(), in[i].strides(), in[i].options()));
-        into.push_back(ptr(dst[i]));
+        const Tensor& to = out ? *out->tensors[i] : *p;
+        const size_t bytes = in.nbytes();
+        void* dst = to.is_non_overlapping_and_dense() && (to.strides() == in.strides() || in.numel() < 2) ? ptr(to) : nullptr;
+        if (!dst) {
+            if (!copy.defined()) copies.push_back(copy = at::empty_strided(in.sizes(), in.strides(), in.options()));
+            back.emplace_back(&to, copies.size() - 1);
+            dst = ptr(copy);
+        }
+        into.push_back(dst);
+        if (bytes == 0) continue;
+        const uintptr_t a = reinterpret_cast<uintptr_t>(dst), b = reinterpret_cast<uintptr_t>(from.back());
+        ranges.push_back({a, a + bytes, true});
+        if (a != b) ranges.push_back({b, b + bytes, false});
     }
     if (scaled) {
-        refuse_overlaps(in, dst);
-        for (const Tensor& t : to) torch::autograd::impl::bump_version(t);
+        refuse_overlaps(ranges);
+        for (size_t i = 0; i < n; ++i)
+            if (given.tensors[i]) torch::autograd::impl::bump_version(out ? *out->tensors[i] : *given.tensors[i]);
     }
-    const Tensor norm = at::empty({}, given[0].options().dtype(f64 ? at::kDouble : at::kFloat));
-    const int32_t n = int32_t(in.size());
-    const Tensor ws = scratch(norm, std::max<size_t>(simnets_gradient_norm_workspace_bytes(n), 256));
-    check(scaled ? simnets_clip_gradients(int32_t(order), max_norm, n, dtypes.data(), counts.data(), from.data(), into.data(), ptr(norm), ptr(ws), ws.numel(), stream_of(norm))
-                 : simnets_gradient_norm(int32_t(order), n, dtypes.data(), counts.data(), from.data(), ptr(norm), ptr(ws), ws.numel(), stream_of(norm)));
-    for (size_t i = 0; i < dst.size(); ++i)
-        if (!dst[i].is_same(to[i])) to[i].copy_(dst[i]);
+    const Tensor norm = at::empty({}, first->options().dtype(f64 ? at::kDouble : at::kFloat));
+    const int32_t k = int32_t(counts.size());
+    const Tensor ws = scratch(norm, std::max<size_t>(simnets_gradient_norm_workspace_bytes(k), 256));
+    check(scaled ? simnets_clip_gradients(int32_t(order), max_norm, k, dtypes.data(), counts.data(), from.data(), into.data(), ptr(norm), ptr(ws), ws.numel(), stream_of(norm))
+                 : simnets_gradient_norm(int32_t(order), k, dtypes.data(), counts.data(), from.data(), ptr(norm), ptr(ws), ws.numel(), stream_of(norm)));
+    for (const auto& [to, copy] : back) to->copy_(copies[copy]);
     return norm;
 }
 
@@ -1147,10 +1188,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("xent_with_grad", &xent_with_grad);
     m.def("xent_apply", &xent_apply);
     m.def("log_probabilities", &log_probabilities_apply);
-    m.def("gradient_norm", [](const std::vector<Tensor>& given, int64_t order) { return gradients_impl(given, order, false, 0.0, std::nullopt); });
-    m.def("clip_gradients", [](const std::vector<Tensor>& given, double max_norm, int64_t order, const std::optional<std::vector<Tensor>>& out) {
-        return gradients_impl(given, order, true, max_norm, out);
-    });
+    m.def("gradient_norm", [](const py::object& tensors, int64_t order) { return gradients_impl(tensors, order, false, 0.0, py::none()); });
+    m.def("clip_gradients", [](const py::object& tensors, double max_norm, int64_t order, const py::object& out) { return gradients_impl(tensors, order, true, max_norm, out); });
     m.def("profile_start", [] { py::list dropped = profile_take(); g_profiling = true; });
     m.def("profile_stop", [] { g_profiling = false; return profile_take(); });
 }

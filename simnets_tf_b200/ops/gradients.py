@@ -2,21 +2,8 @@
 The reference leaves its gradients to the optimisers of its framework (HUJI-Deep/simnets-tf README.md:108-111)."""
 import math
 
-import torch
-
 from .. import _lib
 from .. import _torch_glue
-
-
-def _listed(tensors, out=None):
-    """The tensors without those that are None (parameters that have no gradient), and what `out` has for them."""
-    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    if out is not None:
-        out = [out] if isinstance(out, torch.Tensor) else list(out)
-        if len(out) != len(tensors):
-            raise ValueError("out must have one tensor for each gradient, got %d for %d" % (len(out), len(tensors)))
-        out = [o for t, o in zip(tensors, out) if t is not None]
-    return [t for t in tensors if t is not None], out
 
 
 def _order(order):
@@ -31,7 +18,7 @@ def _order(order):
 def gradient_norm(tensors, order=2):
     """The norm of all values of all `tensors` together (None is left out), as a 0-d tensor on their device: order 2, or math.inf for the largest
     magnitude.  float32 and float64 tensors may be mixed; the norm is float64 if one of them is.  Summed in 64 bits and in a fixed order."""
-    return _lib.ops().gradient_norm(_listed(tensors)[0], _order(order))
+    return _lib.ops().gradient_norm(tensors, _order(order))
 
 
 def clip_gradients(tensors, max_norm, order=2, out=None):
@@ -42,5 +29,4 @@ def clip_gradients(tensors, max_norm, order=2, out=None):
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError("max_norm must not be negative, got %r" % max_norm)
-    tensors, out = _listed(tensors, out)
     return _lib.ops().clip_gradients(tensors, max_norm, _order(order), out)
