@@ -499,8 +499,9 @@ typedef struct simnets_likelihood_desc {
     int64_t batch, positions;
     int64_t stride_batch, stride_class, stride_position;    /* in elements, not negative */
 } simnets_likelihood_desc;
+SIMNETS_API size_t simnets_log_probabilities_workspace_bytes(const simnets_likelihood_desc* d);          /* 0: none, and it may be NULL */
 SIMNETS_API int simnets_log_probabilities(const simnets_likelihood_desc* d, const void* logits, const int64_t* labels, void* label, void* entropy,
-                                          int32_t* top_index, void* top, void* stats, void* stream);
+                                          int32_t* top_index, void* top, void* stats, void* workspace, size_t workspace_bytes, void* stream);
 SIMNETS_API int simnets_log_probabilities_gradient(const simnets_likelihood_desc* d, const void* logits, const int64_t* labels, const void* stats,
                                                    const int32_t* top_index, const void* g_label, const void* g_entropy, const void* g_top,
                                                    void* dlogits, void* stream);

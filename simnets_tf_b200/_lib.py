@@ -78,7 +78,9 @@ def lib():
         l.simnets_route.argtypes = [rd, _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]
         l.simnets_route_gradient.argtypes = [rd, _P, _P, _P, _P, _P, _P, _P]
         kd = C.POINTER(abi.LikelihoodDesc)
-        l.simnets_log_probabilities.argtypes = [kd, _P, _P, _P, _P, _P, _P, _P, _P]
+        l.simnets_log_probabilities_workspace_bytes.restype = C.c_size_t
+        l.simnets_log_probabilities_workspace_bytes.argtypes = [kd]
+        l.simnets_log_probabilities.argtypes = [kd, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]
         l.simnets_log_probabilities_gradient.argtypes = [kd, _P, _P, _P, _P, _P, _P, _P, _P, _P]
         l.simnets_gradient_norm_workspace_bytes.restype = C.c_size_t
         l.simnets_gradient_norm_workspace_bytes.argtypes = [C.c_int32]

@@ -560,14 +560,17 @@ int simnets_route_gradient(const simnets_route_desc* d, const void* scores, cons
     return from_cuda(launch_route_gradient(*d, scores, prior, index, weights, grad, dscores, as_stream(stream)));
 }
 
+size_t simnets_log_probabilities_workspace_bytes(const simnets_likelihood_desc* d) { return likelihood_check(d) ? 0 : log_probabilities_workspace_bytes(*d); }
+
 int simnets_log_probabilities(const simnets_likelihood_desc* d, const void* logits, const int64_t* labels, void* label, void* entropy, int32_t* top_index, void* top,
-                              void* stats, void* stream) {
+                              void* stats, void* ws, size_t ws_bytes, void* stream) {
     const int rc = likelihood_check(d);
     if (rc) return rc;
     if (d->batch == 0 || d->positions == 0) return SIMNETS_OK;
     if (!logits || (label && !labels) || (top == nullptr) != (top_index == nullptr)) return SIMNETS_E_NULL;
     if ((d->top_k > 0) != (top != nullptr)) return SIMNETS_E_DESC;
-    return from_cuda(launch_log_probabilities(*d, logits, reinterpret_cast<const long long*>(labels), label, entropy, top_index, top, stats, as_stream(stream)));
+    if (const size_t need = log_probabilities_workspace_bytes(*d); need > 0 && (!ws || ws_bytes < need)) return SIMNETS_E_WORKSPACE;
+    return from_cuda(launch_log_probabilities(*d, logits, reinterpret_cast<const long long*>(labels), label, entropy, top_index, top, stats, ws, as_stream(stream)));
 }
 
 int simnets_log_probabilities_gradient(const simnets_likelihood_desc* d, const void* logits, const int64_t* labels, const void* stats, const int32_t* top_index,

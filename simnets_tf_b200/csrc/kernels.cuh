@@ -177,7 +177,8 @@ cudaError_t launch_route_gradient(const simnets_route_desc&, const void* scores,
 
 // likelihood.cu -- log probabilities of given classes, entropies, likeliest classes; any output may be null
 cudaError_t launch_log_probabilities(const simnets_likelihood_desc&, const void* logits, const long long* labels, void* label, void* entropy, int* top_index,
-                                     void* top, void* stats, cudaStream_t);
+                                     void* top, void* stats, void* ws, cudaStream_t);
+size_t log_probabilities_workspace_bytes(const simnets_likelihood_desc&);
 cudaError_t launch_log_probabilities_gradient(const simnets_likelihood_desc&, const void* logits, const long long* labels, const void* stats, const int* top_index,
                                               const void* g_label, const void* g_entropy, const void* g_top, void* dlogits, cudaStream_t);
 // gradients.cu -- the norm of a list of tensors (order 0: the largest magnitude), and, where out is given, the tensors scaled to a limit

@@ -8,7 +8,6 @@
 //
 // Logits of -infinity are classes that cannot be: exp(-infinity) = 0, and in T d is held where exp(d) is 0 already.  Where all are, the
 // answer is log p = -infinity, H = 0, dx = 0.  A NaN, and an infinity by d = infinity - infinity, makes S a NaN and with it every answer of the position.
-#include <cooperative_groups.h>
 #include "kernels.cuh"
 
 namespace simnets {
@@ -138,6 +137,13 @@ struct Largest {
             x = above ? ov : x; c = above ? oi : c;
         }
     }
+    // U more classes from c on, `hi` the largest of them
+    template <int U>
+    __device__ __forceinline__ void offer(const T (&x)[U], T hi, int c) {
+        if (!__any_sync(0xffffffffu, hi > v[N - 1])) return;
+#pragma unroll
+        for (int u = 0; u < U; ++u) offer(x[u], c + u);
+    }
 };
 template <typename T>
 struct Largest<T, 0> {
@@ -145,17 +151,24 @@ struct Largest<T, 0> {
     int i[1];
     __device__ __forceinline__ void clear() {}
     __device__ __forceinline__ void offer(T, int) {}
+    template <int U> __device__ __forceinline__ void offer(const T (&)[U], T, int) {}
 };
 
 struct Logits {
     long long batch, positions, stride_batch, stride_class, stride_position;
     int classes, top_k, top_last;
     __host__ __device__ long long count() const { return batch * positions; }
-    __device__ __forceinline__ long long at(long long q) const { return (q / positions) * stride_batch + (q % positions) * stride_position; }
-    // of the place j of the likeliest of position q
-    __device__ __forceinline__ long long top_at(long long q, int j) const {
-        return top_last ? q * top_k + j : ((q / positions) * top_k + j) * positions + q % positions;
+    // where position q = b * positions + p is in an array with these steps; the places of the likeliest of a position are top_step apart from
+    // top_first on.  (A division of 64-bit numbers is a hundred instructions, as many as a dozen classes take.)
+    __device__ __forceinline__ long long at(long long q, long long of_batch, long long of_position) const {
+        if (batch == 1) return q * of_position;
+        if ((unsigned long long)q >> 32 || (unsigned long long)positions >> 32) return (q / positions) * of_batch + (q % positions) * of_position;
+        const unsigned b = unsigned(q) / unsigned(positions);
+        return b * of_batch + (unsigned(q) - b * unsigned(positions)) * of_position;
     }
+    __device__ __forceinline__ long long at(long long q) const { return at(q, stride_batch, stride_position); }
+    __device__ __forceinline__ long long top_first(long long q) const { return top_last ? q * top_k : at(q, positions * top_k, 1); }
+    __device__ __forceinline__ long long top_step() const { return top_last ? 1 : positions; }
 };
 
 // What a position's answers go to; any may be null but stats and the others together.  stats: m, log S, H, each of all positions; where no class can
@@ -181,7 +194,14 @@ __device__ __forceinline__ void write_position(const Logits& g, const Answers<T>
     }
 }
 
-constexpr int kAhead = 8;        // loads that a lane has under way
+// 16 bytes a load where classes lie side by side
+template <typename T> struct Bytes16;
+template <> struct Bytes16<float> { using type = float4; };
+template <> struct Bytes16<double> { using type = double2; };
+template <typename T> constexpr int kWide = 16 / sizeof(T);
+
+template <typename T>
+__device__ __forceinline__ int in_front(const T* x) { return int(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T)); }
 
 // ---------------------------------------------------------------------------------------------------- a lane a position
 // For maps, whose positions lie side by side, and for rows of so few classes that a warp's rows are a few lines of memory.  Where there
@@ -217,49 +237,103 @@ __device__ __forceinline__ long long lane_position(const Logits& g, bool* mine) 
     *mine = q < n;
     return q < n ? q : n - 1;
 }
-// the classes [begin, end) of a warp
-__device__ __forceinline__ void warp_classes(const Logits& g, int* begin, int* end) {
-    const int share = (g.classes + int(blockDim.y) - 1) / int(blockDim.y);
-    *begin = min(g.classes, int(threadIdx.y) * share);
-    *end = min(g.classes, *begin + share);
-}
 
-// kAhead classes from `at` on, which moves behind them; `left` of them are there
-template <typename T>
-__device__ __forceinline__ void load_classes(T (&v)[kAhead], const T*& at, long long stride, int left) {
-    if (left >= kAhead) {
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) { v[u] = *at; at += stride; }
-    } else {
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) { v[u] = u < left ? *at : -infinity<T>(); at += u < left ? stride : 0; }
+// Classes that a lane loads at a time, the next ones on their way meanwhile.
+constexpr int kLaneAhead = 8;
+
+// The run [begin, end) of a position's classes that a warp has, U at a time from c on.  SIDE: classes lie side by side, and c is counted from the
+// 16-byte boundary in front of the run, which may be in front of it.
+template <typename T, bool SIDE>
+struct Run {
+    static_assert(kLaneAhead % kWide<T> == 0, "chunks start at 16-byte addresses");
+    int begin, end, c;
+    long long step;
+    __device__ __forceinline__ explicit Run(const Logits& g, const T* x) {
+        const int share = (g.classes + int(blockDim.y) - 1) / int(blockDim.y);
+        begin = min(g.classes, int(threadIdx.y) * share);
+        end = min(g.classes, begin + share);
+        c = begin - (SIDE ? in_front(x + begin) : 0);
+        step = g.stride_class;
     }
-}
+    // the same for all lanes of a warp
+    __device__ __forceinline__ int chunks(int u) const { return (end - begin + (SIDE ? kWide<T> - 1 : 0) + u - 1) / u; }
+    // x: class c
+    template <int U>
+    __device__ __forceinline__ void load(T (&v)[U], const T* x) const {
+        if (SIDE) {
+#pragma unroll
+            for (int j = 0; j < U; j += kWide<T>) {
+                if (c + j >= begin && c + j + kWide<T> <= end) {
+                    *reinterpret_cast<typename Bytes16<T>::type*>(v + j) = *reinterpret_cast<const typename Bytes16<T>::type*>(x + j);
+                } else {
+#pragma unroll
+                    for (int e = j; e < j + kWide<T>; ++e) v[e] = c + e >= begin && c + e < end ? x[e] : -infinity<T>();
+                }
+            }
+        } else if (c + U <= end) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) { v[u] = *x; x += step; }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                v[u] = c + u < end ? *x : -infinity<T>();
+                if (c + u < end) x += step;
+            }
+        }
+    }
+    // to: class c, which `aligned` says lies to 16 bytes as the logits do
+    template <int U>
+    __device__ __forceinline__ void store(const T (&v)[U], T* to, long long to_step, bool aligned) const {
+        if (SIDE) {
+#pragma unroll
+            for (int j = 0; j < U; j += kWide<T>) {
+                if (aligned && c + j >= begin && c + j + kWide<T> <= end) {
+                    *reinterpret_cast<typename Bytes16<T>::type*>(to + j) = *reinterpret_cast<const typename Bytes16<T>::type*>(v + j);
+                } else {
+#pragma unroll
+                    for (int e = j; e < j + kWide<T>; ++e)
+                        if (c + e >= begin && c + e < end) to[e] = v[e];
+                }
+            }
+        } else if (c + U <= end) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) { *to = v[u]; to += to_step; }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (c + u < end) { *to = v[u]; to += to_step; }
+        }
+    }
+};
 
-template <typename T, int TOP>
-__global__ void __launch_bounds__(512) answer_lanes(Logits g, Answers<T> a) {
+template <typename T, int TOP, bool SIDE>
+__global__ void __launch_bounds__(512, sizeof(T) == 4 && TOP <= 4 ? 2 : 1) answer_lanes(Logits g, Answers<T> a) {
+    constexpr int U = kLaneAhead;
     stream_order();
     extern __shared__ __align__(16) char room[];
     bool mine;
     const long long q = lane_position(g, &mine);
     const T* x = a.logits + g.at(q);
+    Run<T, SIDE> run(g, x);
+    const T* from = x + run.c * run.step;
+    T v[U];
+    run.load(v, from);
     const long long label = a.label && threadIdx.y == 0 ? a.labels[q] : -1;
     const bool labelled = label >= 0 && label < g.classes;
     const T of_label = labelled ? x[label * g.stride_class] : T(0);
     Found<T, TOP> f;
     f.sums.clear();
     f.top.clear();
-    int begin, end;
-    warp_classes(g, &begin, &end);
-    const T* at_class = x + begin * g.stride_class;
-    for (int c = begin; c < end; c += kAhead) {
-        T v[kAhead];
-        load_classes(v, at_class, g.stride_class, end - c);
+    for (int n = run.chunks(U); n > 0; --n) {
+        const int c = run.c;
+        run.c += U;
+        from += U * run.step;
+        T next[U];
+        if (n > 1) run.load(next, from);
         const T hi = f.sums.add(v);
-        if (TOP > 0 && __any_sync(0xffffffffu, hi > f.top.v[TOP > 0 ? TOP - 1 : 0])) {
+        f.top.offer(v, hi, c);
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) f.top.offer(v[u], c + u);
-        }
+        for (int u = 0; u < U; ++u) v[u] = next[u];
     }
     char* at = room + (threadIdx.z * blockDim.y + threadIdx.y) * Found<T, TOP>::kBytes;
     for (int d = 1; d < int(blockDim.y); d *= 2) {
@@ -270,24 +344,18 @@ __global__ void __launch_bounds__(512) answer_lanes(Logits g, Answers<T> a) {
     if (threadIdx.y != 0 || !mine) return;
     const Answer<T> w(f.sums);
     write_position(g, a, q, of_label, labelled, w);
+    long long to = TOP > 0 ? g.top_first(q) : 0;
 #pragma unroll
     for (int j = 0; j < TOP; ++j) {
         if (j >= g.top_k) break;
-        a.top_index[g.top_at(q, j)] = f.top.i[j];
-        a.top[g.top_at(q, j)] = f.top.i[j] < 0 ? -infinity<T>() : w.of(f.top.v[j]);
+        a.top_index[to] = f.top.i[j];
+        a.top[to] = f.top.i[j] < 0 ? -infinity<T>() : w.of(f.top.v[j]);
+        to += g.top_step();
     }
 }
 
 // ----------------------------------------------------------------------------------------------- several lanes a position
-// For rows, whose classes lie side by side: a warp, a CTA or a cluster of CTAs a row, 16 bytes a load.  Rows start anywhere: chunks are counted from
-// the 16-byte boundary in front of a row.
-template <typename T> struct Bytes16;
-template <> struct Bytes16<float> { using type = float4; };
-template <> struct Bytes16<double> { using type = double2; };
-template <typename T> constexpr int kWide = 16 / sizeof(T);
-
-template <typename T>
-__device__ __forceinline__ int in_front(const T* x) { return int(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T)); }
+// For rows, whose classes lie side by side, 16 bytes a load.  Rows start anywhere: chunks are counted from the 16-byte boundary in front of a row.
 
 // The share of thread `tid` of THREADS in the U * THREADS classes from `first` on; value u is class first + class_in_chunk(tid, u).
 template <typename T, int THREADS>
@@ -322,20 +390,27 @@ __device__ __forceinline__ void store_chunk(const T (&v)[U], T* x, bool aligned,
     }
 }
 
-// Numbers as unsigned ones in the same order (-0 as 0)
+// float32 numbers as unsigned ones in the same order (-0 as 0), of which a warp finds the largest in one instruction
 __device__ __forceinline__ unsigned ordered(float v) {
     const unsigned b = __float_as_uint(v + 0.f);
     return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
 }
 __device__ __forceinline__ float number(unsigned k) { return __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xffffffffu)); }
-__device__ __forceinline__ unsigned long long ordered(double v) {
-    const unsigned long long b = (unsigned long long)__double_as_longlong(v + 0.0);
-    return b ^ (b >> 63 ? ~0ULL : 1ULL << 63);
+
+// the best of the lanes' values, the lowest index of equal ones
+__device__ __forceinline__ void warp_best(float& v, int& i) {
+    const unsigned key = ordered(v), best = __reduce_max_sync(0xffffffffu, key);
+    i = int(__reduce_min_sync(0xffffffffu, key == best ? unsigned(i) : 0xffffffffu));
+    v = number(best);
 }
-__device__ __forceinline__ double number(unsigned long long k) { return __longlong_as_double((long long)(k ^ (k >> 63 ? 1ULL << 63 : ~0ULL))); }
-template <typename T> struct KeyOf;
-template <> struct KeyOf<float> { using type = unsigned; };
-template <> struct KeyOf<double> { using type = unsigned long long; };
+__device__ __forceinline__ void warp_best(double& v, int& i) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        const double ov = __shfl_xor_sync(0xffffffffu, v, d);
+        const int oi = __shfl_xor_sync(0xffffffffu, i, d);
+        if (ov > v || (ov == v && unsigned(oi) < unsigned(i))) { v = ov; i = oi; }
+    }
+}
 
 __device__ __forceinline__ float warp_max(float v) { return number(__reduce_max_sync(0xffffffffu, ordered(v))); }
 __device__ __forceinline__ double warp_max(double v) {
@@ -343,18 +418,6 @@ __device__ __forceinline__ double warp_max(double v) {
     for (int d = 16; d > 0; d >>= 1) v = larger(v, __shfl_xor_sync(0xffffffffu, v, d));
     return v;
 }
-// the k-th largest of the lanes' values
-template <typename T>
-__device__ __forceinline__ T warp_largest(T v, int k) {
-    T best = -infinity<T>();
-    for (int j = 0; j < k; ++j) {
-        best = warp_max(v);
-        const unsigned who = __ballot_sync(0xffffffffu, v == best);
-        if (int(threadIdx.x % 32) == __ffs(who) - 1) v = -infinity<T>();
-    }
-    return best;
-}
-
 // The largest so far as a list of the warp, the j-th of them in lane j.  A class is compared with the last one that counts, and only one above it moves
 // the list: a row of n classes in any order moves it about top_k log(n / top_k) times.
 template <typename T>
@@ -376,18 +439,34 @@ struct WarpList {
     template <int THREADS, int U>
     __device__ __forceinline__ void offer(const T (&x)[U], T hi, T bound, long long first, int top_k) {
         if (!__any_sync(0xffffffffu, hi > last && hi >= bound)) return;
+        const int tid = THREADS == 32 ? int(threadIdx.x % 32) : int(threadIdx.x);
         unsigned mine = 0;
 #pragma unroll
         for (int u = 0; u < U; ++u) mine |= x[u] > last && x[u] >= bound ? 1u << u : 0u;
-        while (const unsigned who = __ballot_sync(0xffffffffu, mine)) {
-            const int from = __ffs(who) - 1, u = __shfl_sync(0xffffffffu, __ffs(mine) - 1, from);
+        // one of each lane's at a time
+        while (unsigned who = __ballot_sync(0xffffffffu, mine)) {
+            const int u = __ffs(mine) - 1, c = int(first + class_in_chunk<T, THREADS>(tid, u));
             T xu = x[0];
 #pragma unroll
             for (int w = 1; w < U; ++w) xu = u == w ? x[w] : xu;
-            xu = __shfl_sync(0xffffffffu, xu, from);
-            if (xu >= last) insert(xu, int(first + class_in_chunk<T, THREADS>((THREADS == 32 ? 0 : int(threadIdx.x) / 32 * 32) + from, u)), top_k);
-            if (int(threadIdx.x % 32) == from) mine &= mine - 1;
+            mine &= mine - 1;
+            for (; who; who &= who - 1) {
+                const T best = __shfl_sync(0xffffffffu, xu, __ffs(who) - 1);
+                if (best >= last) insert(best, __shfl_sync(0xffffffffu, c, __ffs(who) - 1), top_k);
+            }
         }
+    }
+    // the first chunk: at least top_k of its classes are not below the k-th largest of the lanes' largest
+    template <int THREADS, int U>
+    __device__ __forceinline__ void start(const T (&x)[U], T hi, long long first, int top_k) {
+        clear();
+        T rest = hi == hi ? hi : -infinity<T>(), bound = rest;             // (a lane all of whose classes are NaN)
+        for (int j = 0; j < top_k; ++j) {
+            bound = warp_max(rest);
+            const unsigned who = __ballot_sync(0xffffffffu, rest == bound);
+            if (int(threadIdx.x % 32) == __ffs(who) - 1) rest = -infinity<T>();
+        }
+        offer<THREADS>(x, hi, bound, first, top_k);
     }
 };
 
@@ -399,20 +478,6 @@ struct RowFound {
     int top_index[16];
 };
 
-// the best of the lanes' values, the lowest index of equal ones
-__device__ __forceinline__ void warp_best(float& v, int& i) {
-    const unsigned key = ordered(v), best = __reduce_max_sync(0xffffffffu, key);
-    i = int(__reduce_min_sync(0xffffffffu, key == best ? unsigned(i) : 0xffffffffu));
-    v = number(best);
-}
-__device__ __forceinline__ void warp_best(double& v, int& i) {
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-        const double ov = __shfl_xor_sync(0xffffffffu, v, d);
-        const int oi = __shfl_xor_sync(0xffffffffu, i, d);
-        if (ov > v || (ov == v && unsigned(oi) < unsigned(i))) { v = ov; i = oi; }
-    }
-}
 // the lists of `count` rows of `found` (32 at most) as one: each lane looks at the front of one of them, and the best of these goes into the list
 template <typename T>
 __device__ __forceinline__ void join_lists(WarpList<T>& list, const RowFound<T>* found, int count, int top_k) {
@@ -437,108 +502,363 @@ __device__ __forceinline__ void join_lists(WarpList<T>& list, const RowFound<T>*
 
 template <typename T>
 __device__ __forceinline__ Sums<T> over_warp(Sums<T> a) {
+    const T m = warp_max(a.m);                      // (no NaN among them)
+    if (m > -infinity<T>()) a.raise(m);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) {
-        const Sums<T> o = {__shfl_xor_sync(0xffffffffu, a.m, d), __shfl_xor_sync(0xffffffffu, a.s, d), __shfl_xor_sync(0xffffffffu, a.t, d)};
-        a.join(o);
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, d);
+        a.t += __shfl_xor_sync(0xffffffffu, a.t, d);
     }
+    a.m = m;
     return a;
 }
 
-// WARPS = 1: a warp a row, kRowWarps rows a CTA; else a cluster of gridDim.y CTAs of WARPS warps a row
-constexpr int kRowWarps = 8;
-template <int WARPS> constexpr int kRowAhead = WARPS == 1 ? 4 : 8;
-template <typename T, bool TOP, int WARPS>
-__global__ void __launch_bounds__(32 * (WARPS == 1 ? kRowWarps : WARPS)) answer_rows(Logits g, Answers<T> a) {
-    using Key = typename KeyOf<T>::type;
-    stream_order();
-    __shared__ RowFound<T> found[WARPS == 1 ? 1 : WARPS];
-    __shared__ Key shared_bound;            // the largest value that a warp's list ends with
-    constexpr int U = kRowAhead<WARPS>, kThreads = 32 * WARPS;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, tid = WARPS == 1 ? lane : int(threadIdx.x);
-    const long long q = WARPS == 1 ? (long long)blockIdx.x * kRowWarps + warp : blockIdx.x;
-    if (WARPS == 1 && q >= g.count()) return;
-    const T* x = a.logits + g.at(q);
-    const bool writes = lane == 0 && (WARPS == 1 || (warp == 0 && blockIdx.y == 0));
-    const long long label = a.label && writes ? a.labels[q] : -1;
-    const bool labelled = label >= 0 && label < g.classes;
-    const T of_label = labelled ? x[label] : T(0);
-    Sums<T> sums;
-    WarpList<T> list;
-    sums.clear();
-    list.clear();
-    if (TOP && WARPS > 1) {
-        if (threadIdx.x == 0) shared_bound = ordered(-infinity<T>());
-        __syncthreads();
-    }
-    const long long step = (long long)kThreads * U * (WARPS == 1 ? 1 : gridDim.y);
-    long long first = (WARPS == 1 ? 0LL : (long long)blockIdx.y * kThreads * U) - in_front(x);
-    T v[U];
-    if (first < g.classes) load_chunk<T, U, kThreads>(v, x, first, g.classes, tid);
-    for (bool start = true; first < g.classes; first += step, start = false) {
-        T next[U];
-        if (first + step < g.classes) load_chunk<T, U, kThreads>(next, x, first + step, g.classes, tid);
-        const T hi = sums.add(v);
-        if (TOP) {
-            // at the start at least top_k of the warp's classes are not below the k-th largest of the lanes' largest
-            // (of a lane all of whose classes are NaN, hi is one too)
-            T bound = start ? warp_largest(hi == hi ? hi : -infinity<T>(), g.top_k) : -infinity<T>();
-            if (WARPS > 1) {
-                if (start && lane == 0) atomicMax(&shared_bound, ordered(bound));
-                bound = larger(bound, number(*static_cast<volatile Key*>(&shared_bound)));
-            }
-            const T before = list.last;
-            list.template offer<kThreads>(v, hi, bound, first, g.top_k);
-            if (WARPS > 1 && lane == 0 && list.last > before) atomicMax(&shared_bound, ordered(list.last));
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = next[u];
-    }
-    sums = over_warp(sums);
-    if (WARPS > 1) {
-        // the warps of the CTA, then the CTAs of the cluster, into the first of them
-        if (lane == 0) found[warp].sums = sums;
-        if (TOP && lane < 16) { found[warp].top[lane] = list.v; found[warp].top_index[lane] = list.i; }
-        __syncthreads();
-        if (warp == 0) {
-            sums.clear();
-            if (lane < WARPS) sums = found[lane].sums;
-            sums = over_warp(sums);
-            if (TOP) join_lists(list, found, WARPS, g.top_k);
-        }
-        if (gridDim.y > 1) {
-            const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
-            __syncwarp();
-            if (warp == 0 && lane == 0) found[0].sums = sums;
-            if (TOP && warp == 0 && lane < 16) { found[0].top[lane] = list.v; found[0].top_index[lane] = list.i; }
-            cluster.sync();
-            if (warp == 0 && blockIdx.y == 0) {
-                const int others = int(gridDim.y);
-                sums.clear();
-                if (lane < others) sums = cluster.map_shared_rank(found, lane)->sums;
-                sums = over_warp(sums);
-                if (TOP) {
-                    // (one list a warp of this CTA was joined already: their places take the other CTAs' lists)
-                    for (int e = lane; e < others * 16; e += 32) {
-                        const RowFound<T>* other = cluster.map_shared_rank(found, e / 16);
-                        const T top = other->top[e % 16];
-                        const int index = other->top_index[e % 16];
-                        if (e >= 16) { found[e / 16].top[e % 16] = top; found[e / 16].top_index[e % 16] = index; }
-                    }
-                    __syncwarp();
-                    join_lists(list, found, others, g.top_k);
-                }
-            }
-            cluster.sync();
-        }
-        if (warp != 0 || blockIdx.y != 0) return;
-    }
+// the answers of position q by a whole warp, from what its label's logit is in lane 0
+template <typename T, bool TOP>
+__device__ __forceinline__ void write_row(const Logits& g, const Answers<T>& a, long long q, T of_label, bool labelled, const Sums<T>& sums, const WarpList<T>& list) {
+    const int lane = threadIdx.x % 32;
     const Answer<T> w(sums);
     if (lane == 0) write_position(g, a, q, of_label, labelled, w);
     if (TOP && lane < g.top_k) {
-        a.top_index[g.top_at(q, lane)] = list.i;
-        a.top[g.top_at(q, lane)] = list.i < 0 ? -infinity<T>() : w.of(list.v);
+        const long long to = g.top_first(q) + lane * g.top_step();
+        a.top_index[to] = list.i;
+        a.top[to] = list.i < 0 ? -infinity<T>() : w.of(list.v);
     }
+}
+// the label's logit of position q, in lane 0
+template <typename T>
+__device__ __forceinline__ T logit_of_label(const Logits& g, const Answers<T>& a, long long q, const T* x, bool* labelled) {
+    const long long label = a.label && threadIdx.x % 32 == 0 ? a.labels[q] : -1;
+    *labelled = label >= 0 && label < g.classes;
+    return *labelled ? x[label] : T(0);
+}
+
+// A warp a row, kRowWarps of them a CTA, U classes a lane and chunk.
+constexpr int kRowWarps = 8;
+template <typename T, bool TOP, int U>
+__global__ void __launch_bounds__(32 * kRowWarps) answer_rows(Logits g, Answers<T> a) {
+    stream_order();
+    const int lane = threadIdx.x % 32;
+    const long long q = (long long)blockIdx.x * kRowWarps + threadIdx.x / 32;
+    if (q >= g.count()) return;
+    const T* x = a.logits + g.at(q);
+    int first = -in_front(x);
+    T v[U];
+    load_chunk<T, U, 32>(v, x, first, g.classes, lane);
+    bool labelled;
+    const T of_label = logit_of_label(g, a, q, x, &labelled);
+    Sums<T> sums;
+    WarpList<T> list;
+    sums.clear();
+    T hi = sums.add(v);
+    if (TOP) list.template start<32>(v, hi, first, g.top_k);
+    for (first += 32 * U; first < g.classes; first += 32 * U) {
+        load_chunk<T, U, 32>(v, x, first, g.classes, lane);
+        hi = sums.add(v);
+        if (TOP) list.template offer<32>(v, hi, -infinity<T>(), first, g.top_k);
+    }
+    write_row<T, TOP>(g, a, q, of_label, labelled, over_warp(sums), list);
+}
+
+// Long rows: all rows' chunks in their order, in equal runs for the CTAs of one wave, which have the next ones on their way all the time, those of the
+// next row as well: every thread copies what it reads itself into shared memory (cp.async), kStages - 1 chunks ahead, and waits for nobody else.
+// More on the way at once is slower (2048 rows of 65537 classes with 5 alternatives / of 32000 without, us: 2 CTAs a multiprocessor with 2, 3, 4
+// stages 121 / 55, 104 / 46, 110 / 46, 3 CTAs with 2, 3, 4 stages 105 / 47, 116 / 47, 121 / 51, 4 with 3 132 / 51; the memory's floor 82 / 40).
+//
+// The likeliest classes cost the streaming warps a comparison a chunk.  Every thread keeps the largest of its classes and the chunk in which it came up
+// first.  Of the threads by their largest, equal ones by its first class, the first top_k have all of the row's top_k: every other thread's classes have at
+// least top_k in front of them.  Another warp, while the others go on, picks these threads and reads their classes again, a few hundred.
+//
+// A run that has all of a row answers it; of others what it found goes to `parts`, two places a CTA (0: with its first chunk, 1: without), where join_parts
+// finds it.
+constexpr int kStreamWarps = 8, kStreamThreads = 32 * kStreamWarps, kStages = 3, kStreamCtas = 2;
+template <typename T> constexpr int kStreamAhead = 64 / sizeof(T);
+template <typename T> constexpr int kStreamChunk = kStreamThreads * kStreamAhead<T>;
+constexpr int kStreamBytes = kStages * kStreamThreads * 64;
+
+struct Runs {
+    long long chunks;                               // of all rows
+    int of_row, ctas;
+    __host__ __device__ long long begin(int cta) const { return chunks / ctas * cta + (chunks % ctas) * cta / ctas; }
+};
+
+// 16 bytes from class c of row x on their way into shared memory, what is not of the row as classes that cannot be
+template <typename T>
+__device__ __forceinline__ void copy_wide(char* to, const T* x, long long c, bool inside, int classes) {
+    constexpr int kBytes = int(sizeof(T));
+    const unsigned at = unsigned(__cvta_generic_to_shared(to));
+    if (inside || (c >= 0 && c + kWide<T> <= classes)) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(x + c) : "memory");
+    } else {
+#pragma unroll
+        for (int e = 0; e < kWide<T>; ++e) {
+            if (c + e >= 0 && c + e < classes) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at + e * kBytes), "l"(x + c + e), "n"(kBytes) : "memory");
+            else reinterpret_cast<T*>(to)[e] = -infinity<T>();
+        }
+    }
+}
+// a thread's share of the chunk from `first` on: value u is class_in_chunk(threadIdx.x, u), 16 bytes of every kStreamThreads * 16
+template <typename T>
+__device__ __forceinline__ void copy_chunk(char* to, const T* x, long long first, int classes) {
+    const bool inside = first >= 0 && first + kStreamChunk<T> <= classes;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        copy_wide(to + (j * kStreamThreads + threadIdx.x) * 16, x, first + class_in_chunk<T, kStreamThreads>(threadIdx.x, j * kWide<T>), inside, classes);
+}
+
+// What the streaming warps leave of (their part of) a row.
+template <typename T>
+struct Streamed {
+    Sums<T> sums[kStreamWarps];
+    T largest[kStreamThreads];
+    int chunk[kStreamThreads];              // where it came up
+};
+
+// All warps but the waiting one come and go on (bar.arrive), or wait for it: 32 more threads than stream take part.
+__device__ __forceinline__ void barrier_arrive(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kStreamThreads + 32) : "memory"); }
+__device__ __forceinline__ void barrier_wait(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kStreamThreads + 32) : "memory"); }
+
+// where the j-th 16 bytes of thread `tid` in the chunk from `first` on are
+template <typename T>
+__device__ __forceinline__ long long share_of(long long first, int tid, int j) { return first + class_in_chunk<T, kStreamThreads>(tid, j * kWide<T>); }
+
+// Room for picking: classes on their way, and those that may be among the likeliest.
+constexpr int kAgain = 12;
+template <typename T>
+struct Above {
+    __align__(16) char again[kAgain][32 * 16];
+    T top[32];
+    int top_index[32];
+};
+
+// The top_k largest of the classes in chunks [begin, end) of row x, from what the threads kept of them; by one warp.
+template <typename T>
+__device__ __forceinline__ void pick(WarpList<T>& list, const Streamed<T>& kept, Above<T>& room, const T* x, int begin, int end, int classes, int top_k) {
+    const int lane = threadIdx.x % 32, front = in_front(x);
+    T rest[kStreamWarps], bound = -infinity<T>();
+#pragma unroll
+    for (int w = 0; w < kStreamWarps; ++w) rest[w] = kept.largest[w * 32 + lane];
+    int picked = -1, n = 0;                                 // (lane j: the j-th thread)
+#pragma unroll 1
+    for (; n < top_k; ++n) {
+        T most = rest[0];
+#pragma unroll
+        for (int w = 1; w < kStreamWarps; ++w) most = larger(most, rest[w]);
+        const T best = warp_max(most);
+        if (best == -infinity<T>()) break;
+        bound = best;
+        int equal = 0, place = 0;
+#pragma unroll
+        for (int w = kStreamWarps - 1; w >= 0; --w) {
+            equal += rest[w] == best;
+            place = rest[w] == best ? w : place;
+        }
+        unsigned who = __ballot_sync(0xffffffffu, equal > 0);
+        if (__reduce_add_sync(0xffffffffu, equal) > 1) {
+            // the first class of equal ones decides
+            unsigned at = 0xffffffffu;
+#pragma unroll 1
+            for (int w = 0; w < kStreamWarps; ++w) {
+                T r = rest[0];
+#pragma unroll
+                for (int i = 1; i < kStreamWarps; ++i) r = i == w ? rest[i] : r;
+                if (r != best) continue;
+                const int tid = w * 32 + lane;
+#pragma unroll 1
+                for (int u = kStreamAhead<T> - 1; u >= 0; --u) {
+                    const long long c = (long long)kept.chunk[tid] * kStreamChunk<T> - front + class_in_chunk<T, kStreamThreads>(tid, u);
+                    if (c >= 0 && c < classes && x[c] == best && unsigned(c) < at) { at = unsigned(c); place = w; }
+                }
+            }
+            who = __ballot_sync(0xffffffffu, at == __reduce_min_sync(0xffffffffu, at));
+        }
+        const int from = __ffs(who) - 1, tid = __shfl_sync(0xffffffffu, place * 32 + lane, from);
+        if (lane == n) picked = tid;
+#pragma unroll
+        for (int w = 0; w < kStreamWarps; ++w)
+            if (w * 32 + lane == tid) rest[w] = -infinity<T>();
+    }
+    if (n < top_k) bound = -infinity<T>();                  // (all of the classes that can be are theirs)
+    // Their classes, up to kAgain * 32 times 16 bytes at a time.  Those not below the bound are hardly ever more than the lanes of a warp: the best of
+    // these again and again; more, equal ones, are put in one by one.  (Loops that are not unrolled: the code runs once a row, and would
+    // wait for its instructions.)
+    list.clear();
+    const int each = 4 * (end - begin), total = n * each;
+    int count = 0;
+    for (int from = 0; from < total; from += kAgain * 32) {
+#pragma unroll 1
+        for (int i = 0; i < kAgain && from + i * 32 < total; ++i) {
+            const int at = min(from + i * 32 + lane, total - 1), j = at / each, tid = __shfl_sync(0xffffffffu, picked, j), place = begin * 4 + at - j * each;
+            copy_wide(room.again[i] + lane * 16, x, share_of<T>((long long)(place / 4) * kStreamChunk<T> - front, tid, place % 4), false, classes);
+        }
+        asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+#pragma unroll 1
+        for (int i = 0; i < kAgain && from + i * 32 < total; ++i) {
+            T v[kWide<T>];
+            *reinterpret_cast<typename Bytes16<T>::type*>(v) = *reinterpret_cast<const typename Bytes16<T>::type*>(room.again[i] + lane * 16);
+            const int at = from + i * 32 + lane, j = min(at, total - 1) / each, tid = __shfl_sync(0xffffffffu, picked, j), place = begin * 4 + at - j * each;
+            unsigned mine = 0;
+#pragma unroll
+            for (int e = 0; e < kWide<T>; ++e) mine |= at < total && v[e] > -infinity<T>() && v[e] >= bound ? 1u << e : 0u;
+#pragma unroll 1
+            while (unsigned who = __ballot_sync(0xffffffffu, mine)) {
+                const int e = __ffs(mine) - 1, left = 32 - count, to = count + __popc(who & ((1u << lane) - 1));
+                const int c = int(share_of<T>((long long)(place / 4) * kStreamChunk<T> - front, tid, place % 4)) + e;
+                T w = v[0];
+#pragma unroll
+                for (int k = 1; k < kWide<T>; ++k) w = e == k ? v[k] : w;
+                if (mine && to < 32) { room.top[to] = w; room.top_index[to] = c; }
+                mine &= mine - 1;
+                count += __popc(who);
+                if (count > 32) {
+                    who = left <= 0 ? who : who & ~((2u << __fns(who, 0, left)) - 1);
+                    const unsigned last_i = unsigned(__shfl_sync(0xffffffffu, list.i, top_k - 1));
+#pragma unroll 1
+                    for (who &= __ballot_sync(0xffffffffu, w > list.last || (w == list.last && unsigned(c) < last_i)); who; who &= who - 1)
+                        list.insert(__shfl_sync(0xffffffffu, w, __ffs(who) - 1), __shfl_sync(0xffffffffu, c, __ffs(who) - 1), top_k);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    T mine = lane < count ? room.top[lane] : -infinity<T>();
+    int mine_i = lane < count ? room.top_index[lane] : -1;
+    if (count > 32) {
+#pragma unroll 1
+        for (int j = 0; j < 32; ++j) list.insert(__shfl_sync(0xffffffffu, mine, j), __shfl_sync(0xffffffffu, mine_i, j), top_k);
+    } else {
+#pragma unroll 1
+        for (int j = 0; j < top_k; ++j) {
+            T best = mine;
+            int at = mine_i;
+            warp_best(best, at);
+            if (at < 0) break;
+            if (lane == j) { list.v = best; list.i = at; }
+            if (at == mine_i) { mine = -infinity<T>(); mine_i = -1; }
+        }
+    }
+    __syncwarp();
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kStreamThreads + 32, kStreamCtas) answer_stream(Logits g, Answers<T> a, Runs runs, RowFound<T>* parts) {
+    stream_order();
+    constexpr int U = kStreamAhead<T>;
+    extern __shared__ __align__(16) char stages[];
+    __shared__ Streamed<T> kept[2];                         // (the warps that stream are at the next row meanwhile)
+    __shared__ Above<T> above;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const long long begin = runs.begin(blockIdx.x), end = runs.begin(blockIdx.x + 1);
+    if (begin >= end) return;
+    long long q = begin / runs.of_row;
+    int chunk = int(begin - q * runs.of_row), turn = 0;
+    const T* x = a.logits + g.at(q);
+    // barriers 1 and 2: a row is streamed, into kept[0] and kept[1]; 3 and 4: it is answered, and kept may be written again
+    if (warp == kStreamWarps) {
+        bool first_part = true;
+        for (long long at = begin; at < end; turn ^= 1, ++q, chunk = 0, first_part = false) {
+            const int last = int(min((long long)runs.of_row, chunk + (end - at)));
+            const bool whole = chunk == 0 && last == runs.of_row;
+            x = a.logits + g.at(q);
+            bool labelled = false;
+            const T of_label = whole ? logit_of_label(g, a, q, x, &labelled) : T(0);
+            barrier_wait(1 + turn);
+            Sums<T> sums;
+            sums.clear();
+            if (lane < kStreamWarps) sums = kept[turn].sums[lane];
+            sums = over_warp(sums);
+            WarpList<T> list;
+            list.clear();
+            if (TOP) pick(list, kept[turn], above, x, chunk, last, g.classes, g.top_k);
+            at += last - chunk;
+            // (the next row but one is there: who waits is sure to come)
+            __threadfence_block();
+            if (end - at > runs.of_row) barrier_arrive(3 + turn);
+            if (whole) {
+                write_row<T, TOP>(g, a, q, of_label, labelled, sums, list);
+            } else {
+                RowFound<T>* const to = parts + 2 * blockIdx.x + (first_part ? 0 : 1);
+                if (lane == 0) to->sums = sums;
+                if (TOP && lane < 16) { to->top[lane] = list.v; to->top_index[lane] = list.i; }
+            }
+        }
+        return;
+    }
+    // what is on its way
+    long long q_ahead = q, ahead = begin;
+    int chunk_ahead = chunk, stage = 0, stage_ahead = 0, rows = 0;
+    const T* x_ahead = x;
+    auto copy_next = [&] {
+        if (ahead < end) {
+            copy_chunk(stages + stage_ahead * (kStreamThreads * 64), x_ahead, (long long)chunk_ahead * kStreamChunk<T> - in_front(x_ahead), g.classes);
+            ++ahead;
+            if (++chunk_ahead == runs.of_row && ahead < end) {
+                chunk_ahead = 0;
+                x_ahead = a.logits + g.at(++q_ahead);
+            }
+        }
+        stage_ahead = stage_ahead + 1 == kStages ? 0 : stage_ahead + 1;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int s = 0; s + 1 < kStages; ++s) copy_next();
+    Sums<T> sums;
+    sums.clear();
+    T largest = -infinity<T>();
+    int largest_chunk = 0;
+    for (long long at = begin; at < end; ++at) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        T v[U];
+        const char* here = stages + stage * (kStreamThreads * 64) + threadIdx.x * 16;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<typename Bytes16<T>::type*>(v + j * kWide<T>) = *reinterpret_cast<const typename Bytes16<T>::type*>(here + j * kStreamThreads * 16);
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+        copy_next();                                        // (into what was read an iteration ago)
+        const T hi = sums.add(v);
+        if (TOP && hi > largest) { largest = hi; largest_chunk = chunk; }
+        const bool ends = ++chunk == runs.of_row;
+        if (ends || at + 1 == end) {
+            sums = over_warp(sums);
+            if (rows >= 2) barrier_wait(3 + turn);          // (the row before the last one has been answered)
+            if (lane == 0) kept[turn].sums[warp] = sums;
+            if (TOP) { kept[turn].largest[threadIdx.x] = largest; kept[turn].chunk[threadIdx.x] = largest_chunk; }
+            __threadfence_block();
+            barrier_arrive(1 + turn);
+            ++rows;
+            turn ^= 1;
+            chunk = 0;
+            sums.clear();
+            largest = -infinity<T>();
+        }
+    }
+}
+
+// A warp for every border between two runs that is inside a row and the first one there: the row's parts, up to 32.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(32) join_parts(Logits g, Answers<T> a, Runs runs, const RowFound<T>* parts) {
+    stream_order();
+    __shared__ RowFound<T> found[32];
+    const int lane = threadIdx.x, cta = int(blockIdx.x) + 1;
+    const long long border = runs.begin(cta), q = border / runs.of_row, row = q * runs.of_row;
+    if (border == row || runs.begin(cta - 1) > row) return;
+    bool labelled;
+    const T of_label = logit_of_label(g, a, q, a.logits + g.at(q), &labelled);
+    // the run in front of the border has the row's first part, behind other rows' unless it starts with it
+    const int mine = cta - 1 + lane;
+    const bool has = mine < runs.ctas && (lane == 0 || runs.begin(mine) < row + runs.of_row);
+    Sums<T> sums;
+    sums.clear();
+    if (has) {
+        const RowFound<T>& part = parts[2 * mine + (lane == 0 && runs.begin(mine) < row ? 1 : 0)];
+        sums = part.sums;
+        if (TOP)
+            for (int j = 0; j < g.top_k; ++j) { found[lane].top[j] = part.top[j]; found[lane].top_index[j] = part.top_index[j]; }
+    }
+    __syncwarp();
+    WarpList<T> list;
+    list.clear();
+    if (TOP) join_lists(list, found, __popc(__ballot_sync(0xffffffffu, has)), g.top_k);
+    write_row<T, TOP>(g, a, q, of_label, labelled, over_warp(sums), list);
 }
 
 // ----------------------------------------------------------------------------------------------------------- the gradient
@@ -558,23 +878,18 @@ struct Gradients {
 template <typename T>
 struct Share {
     T m, log_s, fixed, by_log, g_label;
-    long long label;
+    int label;
     bool nothing;
-    __device__ __forceinline__ Share(const Logits& g, const Gradients<T>& a, long long q) {
-        const long long n = g.count();
+    // top: the sum of the gradients of the alternatives
+    __device__ __forceinline__ Share(const Logits& g, const Gradients<T>& a, long long q, T top) {
+        const long long n = g.count(), at = a.label ? a.labels[q] : -1;
+        const T log_nats = a.stats[n + q], entropy = a.stats[2 * n + q], g_entropy = a.entropy ? a.entropy[q] : T(0), given = a.label ? a.label[q] : T(0);
         m = a.stats[q];
-        const T log_nats = a.stats[n + q];
         nothing = m == infinity<T>() && log_nats == T(0);
         log_s = log_nats * Unit<T>::per_nat();
-        label = a.label ? a.labels[q] : -1;
-        if (label < 0 || label >= g.classes || nothing) label = -1;
-        g_label = label >= 0 ? a.label[q] : T(0);
-        T taken = g_label;
-        if (a.top)
-            for (int j = 0; j < g.top_k; ++j)
-                if (a.top_index[g.top_at(q, j)] >= 0) taken += a.top[g.top_at(q, j)];
-        const T g_entropy = a.entropy ? a.entropy[q] : T(0);
-        fixed = nothing ? T(0) : -(taken + g_entropy * a.stats[2 * n + q]);
+        label = at < 0 || at >= g.classes || nothing ? -1 : int(at);
+        g_label = label >= 0 ? given : T(0);
+        fixed = nothing ? T(0) : -(g_label + top + g_entropy * entropy);
         by_log = nothing ? T(0) : -g_entropy * Unit<T>::nats();
     }
     __device__ __forceinline__ Pair<T> of(Pair<T> x) const {
@@ -592,74 +907,94 @@ struct Share {
     }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(512) gradient_lanes(Logits g, Gradients<T> a) {
+template <typename T, bool SIDE>
+__global__ void __launch_bounds__(512, sizeof(T) == 4 ? 2 : 1) gradient_lanes(Logits g, Gradients<T> a) {
+    constexpr int U = kLaneAhead;
     stream_order();
     bool mine;
     const long long q = lane_position(g, &mine);
     if (!mine) return;
-    T* dx = a.dlogits + (q / g.positions) * a.out_batch + (q % g.positions) * a.out_position;
-    const Share<T> share(g, a, q);
-    int begin, end;
-    warp_classes(g, &begin, &end);
-    const T* at_class = a.logits + g.at(q) + begin * g.stride_class;
-    T* to = dx + begin * a.out_class;
-    for (int c = begin; c < end; c += kAhead) {
-        T v[kAhead];
-        load_classes(v, at_class, g.stride_class, end - c);
-        share.of(v);
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-            if (u < end - c) { *to = v[u]; to += a.out_class; }
+    const T* x = a.logits + g.at(q);
+    T* dx = a.dlogits + g.at(q, a.out_batch, a.out_position);
+    Run<T, SIDE> run(g, x), out = run;
+    const T* from = x + run.c * run.step;
+    T* to = dx + run.c * a.out_class;
+    const bool aligned = in_front(x) == in_front(dx);
+    T v[U], top = T(0);
+    run.load(v, from);
+    if (a.top) {
+        long long at = g.top_first(q);
+        for (int j = 0; j < g.top_k; ++j, at += g.top_step()) top += a.top_index[at] >= 0 ? a.top[at] : T(0);
     }
-    if (share.label >= begin && share.label < end) dx[share.label * a.out_class] += share.g_label;
-    if (a.top && !share.nothing)
-        for (int j = 0; j < g.top_k; ++j) {
-            const int c = a.top_index[g.top_at(q, j)];
-            if (c >= begin && c < end) dx[c * a.out_class] += a.top[g.top_at(q, j)];
+    const Share<T> share(g, a, q, top);
+    for (int n = run.chunks(U); n > 0; --n) {
+        run.c += U;
+        from += U * run.step;
+        T next[U];
+        if (n > 1) run.load(next, from);
+        share.of(v);
+        out.store(v, to, a.out_class, aligned);
+        out.c += U;
+        to += U * a.out_class;
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = next[u];
+    }
+    if (share.label >= run.begin && share.label < run.end) dx[share.label * a.out_class] += share.g_label;
+    if (a.top && !share.nothing) {
+        long long at = g.top_first(q);
+        for (int j = 0; j < g.top_k; ++j, at += g.top_step()) {
+            const int c = a.top_index[at];
+            if (c >= run.begin && c < run.end) dx[c * a.out_class] += a.top[at];
         }
+    }
 }
 
-// WARPS = 1: a warp a row; else gridDim.y CTAs of WARPS warps share a row, a run of its classes each
-template <typename T, int WARPS>
+// WARPS = 1: a warp a row, kRowWarps of them a CTA; else gridDim.y CTAs of WARPS warps share a row, a run of its chunks each.  U classes a thread and chunk.
+template <typename T, int WARPS, int U>
 __global__ void __launch_bounds__(32 * (WARPS == 1 ? kRowWarps : WARPS)) gradient_rows(Logits g, Gradients<T> a) {
     stream_order();
-    constexpr int U = kRowAhead<WARPS>, kThreads = 32 * WARPS;
+    constexpr int kThreads = 32 * WARPS;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, tid = WARPS == 1 ? lane : int(threadIdx.x);
     const long long q = WARPS == 1 ? (long long)blockIdx.x * kRowWarps + warp : blockIdx.x;
     if (WARPS == 1 && q >= g.count()) return;
     const T* x = a.logits + g.at(q);
-    T* dx = a.dlogits + (q / g.positions) * a.out_batch + (q % g.positions) * a.out_position;
-    const Share<T> share(g, a, q);
+    T* dx = a.dlogits + g.at(q, a.out_batch, a.out_position);
     const int skip = in_front(x);
     const bool aligned = in_front(dx) == skip;
-    // whole chunks a CTA
-    const long long chunks = (g.classes + skip + kThreads * U - 1) / (kThreads * U), each = (chunks + gridDim.y - 1) / gridDim.y;
-    const long long begin = blockIdx.y * each * kThreads * U - skip, end = begin + each * kThreads * U;
-    // single classes, which get more: written once the others have been
-    const int place = WARPS == 1 || warp == 0 ? lane : 32;
-    long long single = -1;
-    T add = T(0);
-    if (place < 32) {
-        const int c = place < g.top_k && a.top ? a.top_index[g.top_at(q, place)] : -1;
-        const bool both_ways = __any_sync(0xffffffffu, c >= 0 && c == share.label);
-        if (c >= 0) { single = c; add = (c == share.label ? share.g_label : T(0)); }
-        if (place == 31 && share.label >= 0 && !both_ways) { single = share.label; add = share.g_label; }
-        if (share.nothing || single >= g.classes || single < begin || single >= end) single = -1;
-        if (single >= 0) {
-            add += share.of(Pair<T>{x[single], x[single]}).x;
-            if (c >= 0) add += a.top[g.top_at(q, place)];
-        }
+    const long long chunks = ((long long)g.classes + skip + kThreads * U - 1) / (kThreads * U), each = WARPS == 1 ? chunks : (chunks + gridDim.y - 1) / gridDim.y;
+    const long long begin = (WARPS == 1 ? 0 : blockIdx.y) * each * kThreads * U - skip;
+    const int end = int(min((long long)g.classes, begin + each * kThreads * U));
+    T v[U];
+    if (begin < end) load_chunk<T, U, kThreads>(v, x, begin, g.classes, tid);
+    // lane j of every warp has the j-th alternative
+    int single = -1;
+    T more = T(0), top = T(0);
+    if (a.top) {
+        const long long at = g.top_first(q) + lane * g.top_step();
+        if (lane < g.top_k) { single = a.top_index[at]; more = a.top[at]; }
+        top = single >= 0 ? more : T(0);
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) top += __shfl_xor_sync(0xffffffffu, top, d);
+        top = __shfl_sync(0xffffffffu, top, 0);
     }
-    for (long long first = begin; first < end && first < g.classes; first += kThreads * U) {
-        T v[U];
-        load_chunk<T, U, kThreads>(v, x, first, g.classes, tid);
+    const Share<T> share(g, a, q, top);
+    // single classes get more than the others: the alternatives, and by lane 31 the label unless it is one of them
+    const bool is_label = single >= 0 && single == share.label;
+    T more_label = is_label ? share.g_label : T(0), single_x = T(0);
+    if (!__any_sync(0xffffffffu, is_label) && lane == 31) { single = share.label; more_label = share.g_label; }
+    if (share.nothing || single < begin || single >= end || (WARPS > 1 && warp > 0)) single = -1;
+    if (single >= 0) single_x = x[single];
+    for (long long first = begin; first < end; first += kThreads * U) {
+        T next[U];
+        if (first + kThreads * U < end) load_chunk<T, U, kThreads>(next, x, first + kThreads * U, g.classes, tid);
         share.of(v);
         store_chunk<T, U, kThreads>(v, dx, aligned, first, g.classes, tid);
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = next[u];
     }
     if (WARPS == 1) __syncwarp();
     else __syncthreads();
-    if (single >= 0) dx[single] = add;
+    if (single >= 0) dx[single] = share.of(Pair<T>{single_x, single_x}).x + more_label + more;
 }
 
 // --------------------------------------------------------------------------------------------------------------- launches
@@ -667,14 +1002,15 @@ Logits logits_of(const simnets_likelihood_desc& d) {
     return {d.batch, d.positions, d.stride_batch, d.stride_class, d.stride_position, d.classes, d.top_k, d.top_last};
 }
 
-// rows of more classes than this are read by several lanes
-bool by_rows(const Logits& g) { return g.stride_class == 1 && g.classes > 32; }
+// Classes that lie side by side are read by several lanes where they are more than this: below, a lane's loads of 16 bytes are a few lines of memory for
+// the whole warp, and joining what lanes found costs more than the classes.
+bool by_rows(const Logits& g) { return g.stride_class == 1 && g.classes > 128; }
 
 // warps that share 32 positions
 int warps_of_lanes(const Logits& g, size_t bytes_a_warp) {
     const long long tiles = (g.count() + 31) / 32;
     int w = 1;
-    while (w < 16 && tiles * w < 32LL * device_sm_count() && g.classes >= 2 * w * kAhead && 2 * w * bytes_a_warp <= 48 * 1024) w *= 2;
+    while (w < 16 && tiles * w < 16LL * device_sm_count() && g.classes >= 2 * w * kLaneAhead && 2 * w * bytes_a_warp <= 48 * 1024) w *= 2;
     return w;
 }
 
@@ -689,27 +1025,52 @@ cudaError_t launch_lanes(Kernel* kernel, const Logits& g, const A& a, int warps,
 
 template <typename T, int TOP>
 cudaError_t answer_lanes_of(const Logits& g, const Answers<T>& a, cudaStream_t s) {
-    return launch_lanes(answer_lanes<T, TOP>, g, a, warps_of_lanes(g, Found<T, TOP>::kBytes), Found<T, TOP>::kBytes, s);
+    constexpr size_t kBytes = Found<T, TOP>::kBytes;
+    return launch_lanes(g.stride_class == 1 ? answer_lanes<T, TOP, true> : answer_lanes<T, TOP, false>, g, a, warps_of_lanes(g, kBytes), kBytes, s);
+}
+
+// A warp a row where a row is one chunk, or where rows are enough to fill the multiprocessors and not so long that a warp's is late.
+bool by_warps(const Logits& g) { return g.classes <= 512 || (g.classes <= 8192 && g.count() >= 16LL * device_sm_count()); }
+
+// runs of one wave, but a row no more than 32 parts (30 runs a row have 31 borders in it at most)
+template <typename T>
+Runs runs_of(const Logits& g) {
+    Runs r;
+    r.of_row = int(((long long)g.classes + kWide<T> - 1 + kStreamChunk<T> - 1) / kStreamChunk<T>);
+    r.chunks = r.of_row * g.count();
+    r.ctas = int(std::min({r.chunks, (long long)kStreamCtas * device_sm_count(), 30 * g.count()}));
+    return r;
+}
+
+template <typename T, bool TOP, int U>
+cudaError_t answer_rows_of(const Logits& g, const Answers<T>& a, cudaStream_t s) {
+    in_stream_order(answer_rows<T, TOP, U>, unsigned((g.count() + kRowWarps - 1) / kRowWarps), 32 * kRowWarps, 0, s)(g, a);
+    count_launch();
+    return cudaGetLastError();
 }
 
 template <typename T, bool TOP>
-cudaError_t answer_rows_of(const Logits& g, const Answers<T>& a, cudaStream_t s) {
-    if (g.classes <= 1024) {
-        in_stream_order(answer_rows<T, TOP, 1>, unsigned((g.count() + kRowWarps - 1) / kRowWarps), 32 * kRowWarps, 0, s)(g, a);
-    } else {
-        int cluster = 1;
-        while (cluster < 8 && g.count() * cluster < 2LL * device_sm_count() && g.classes > 2048 * cluster) cluster *= 2;
-        const dim3 grid(unsigned(g.count()), cluster);
-        if (cluster > 1) in_stream_order(answer_rows<T, TOP, 32>, grid, 1024, 0, s, cluster)(g, a);
-        else in_stream_order(answer_rows<T, TOP, 8>, grid, 256, 0, s)(g, a);
-    }
+cudaError_t answer_stream_of(const Logits& g, const Answers<T>& a, void* ws, cudaStream_t s) {
+    const Runs runs = runs_of<T>(g);
+    RowFound<T>* parts = static_cast<RowFound<T>*>(ws);
+    static SmemLimit limit;
+    cudaError_t e = limit.raise(answer_stream<T, TOP>, kStreamBytes);
+    if (e != cudaSuccess) return e;
+    in_stream_order(answer_stream<T, TOP>, runs.ctas, kStreamThreads + 32, kStreamBytes, s)(g, a, runs, parts);
+    count_launch();
+    e = cudaGetLastError();
+    if (e != cudaSuccess || runs.ctas == 1 || runs.chunks % runs.ctas == 0 && runs.chunks / runs.ctas % runs.of_row == 0) return e;     // (whole rows)
+    in_stream_order(join_parts<T, TOP>, runs.ctas - 1, 32, 0, s)(g, a, runs, (const RowFound<T>*)parts);
     count_launch();
     return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t answer_as(const Logits& g, const Answers<T>& a, cudaStream_t s) {
-    if (by_rows(g)) return g.top_k > 0 ? answer_rows_of<T, true>(g, a, s) : answer_rows_of<T, false>(g, a, s);
+cudaError_t answer_as(const Logits& g, const Answers<T>& a, void* ws, cudaStream_t s) {
+    if (by_rows(g)) {
+        if (!by_warps(g)) return g.top_k > 0 ? answer_stream_of<T, true>(g, a, ws, s) : answer_stream_of<T, false>(g, a, ws, s);
+        return g.top_k > 0 ? answer_rows_of<T, true, kStreamAhead<T>>(g, a, s) : answer_rows_of<T, false, kStreamAhead<T>>(g, a, s);
+    }
     if (g.top_k == 0) return answer_lanes_of<T, 0>(g, a, s);
     if (g.top_k == 1) return answer_lanes_of<T, 1>(g, a, s);
     if (g.top_k <= 4) return answer_lanes_of<T, 4>(g, a, s);
@@ -719,12 +1080,13 @@ cudaError_t answer_as(const Logits& g, const Answers<T>& a, cudaStream_t s) {
 
 template <typename T>
 cudaError_t gradient_as(const Logits& g, const Gradients<T>& a, cudaStream_t s) {
-    if (!by_rows(g)) return launch_lanes(gradient_lanes<T>, g, a, warps_of_lanes(g, 0), 0, s);
+    if (!by_rows(g))
+        return launch_lanes(g.stride_class == 1 ? gradient_lanes<T, true> : gradient_lanes<T, false>, g, a, warps_of_lanes(g, 0), 0, s);
     if (g.classes <= 1024) {
-        in_stream_order(gradient_rows<T, 1>, unsigned((g.count() + kRowWarps - 1) / kRowWarps), 32 * kRowWarps, 0, s)(g, a);
+        in_stream_order(gradient_rows<T, 1, 4>, unsigned((g.count() + kRowWarps - 1) / kRowWarps), 32 * kRowWarps, 0, s)(g, a);
     } else {
-        const dim3 grid(unsigned(g.count()), std::min((g.classes + 8191) / 8192, 65535));
-        in_stream_order(gradient_rows<T, 8>, grid, 256, 0, s)(g, a);
+        const dim3 grid(unsigned(g.count()), std::min((g.classes + 16383) / 16384, 65535));
+        in_stream_order(gradient_rows<T, 8, kStreamAhead<T>>, grid, 256, 0, s)(g, a);
     }
     count_launch();
     return cudaGetLastError();
@@ -733,12 +1095,18 @@ cudaError_t gradient_as(const Logits& g, const Gradients<T>& a, cudaStream_t s) 
 }  // namespace
 
 cudaError_t launch_log_probabilities(const simnets_likelihood_desc& d, const void* logits, const long long* labels, void* label, void* entropy, int* top_index,
-                                     void* top, void* stats, cudaStream_t s) {
+                                     void* top, void* stats, void* ws, cudaStream_t s) {
     const Logits g = logits_of(d);
     if (g.count() == 0) return cudaSuccess;
     if (d.dtype == SIMNETS_F64)
-        return answer_as<double>(g, {(const double*)logits, labels, (double*)label, (double*)entropy, (double*)top, (double*)stats, top_index}, s);
-    return answer_as<float>(g, {(const float*)logits, labels, (float*)label, (float*)entropy, (float*)top, (float*)stats, top_index}, s);
+        return answer_as<double>(g, {(const double*)logits, labels, (double*)label, (double*)entropy, (double*)top, (double*)stats, top_index}, ws, s);
+    return answer_as<float>(g, {(const float*)logits, labels, (float*)label, (float*)entropy, (float*)top, (float*)stats, top_index}, ws, s);
+}
+
+size_t log_probabilities_workspace_bytes(const simnets_likelihood_desc& d) {
+    const Logits g = logits_of(d);
+    if (g.count() == 0 || !by_rows(g) || by_warps(g)) return 0;
+    return d.dtype == SIMNETS_F64 ? 2 * sizeof(RowFound<double>) * runs_of<double>(g).ctas : 2 * sizeof(RowFound<float>) * runs_of<float>(g).ctas;
 }
 
 cudaError_t launch_log_probabilities_gradient(const simnets_likelihood_desc& d, const void* logits, const long long* labels, const void* stats, const int* top_index,

@@ -33,7 +33,7 @@ def test_the_c_entry_points_check_before_they_launch(cuda_lib):
 
     def both(logits=one, labels=one, label=one, index=one, top=one, stats=one, **kw):
         d = abi.LikelihoodDesc(**dict(dict(dtype=abi.F32, classes=12, top_k=2, batch=2, positions=9, stride_batch=108, stride_class=9, stride_position=1), **kw))
-        return (cuda_lib.simnets_log_probabilities(C.byref(d), logits, labels, label, None, index, top, stats, None),
+        return (cuda_lib.simnets_log_probabilities(C.byref(d), logits, labels, label, None, index, top, stats, None, 0, None),
                 cuda_lib.simnets_log_probabilities_gradient(C.byref(d), logits, labels, stats, index, label, None, top, one, None))
     assert C.sizeof(abi.LikelihoodDesc) == 56
     assert both(dtype=2) == (abi.E_DTYPE,) * 2
@@ -46,7 +46,12 @@ def test_the_c_entry_points_check_before_they_launch(cuda_lib):
         assert both(**kw) == (abi.E_NULL,) * 2, kw
     assert both(stats=None)[1] == abi.E_NULL
     assert both(batch=0, logits=None) == (0, 0) and both(positions=0, logits=None) == (0, 0)
-    assert cuda_lib.simnets_log_probabilities(None, *[one] * 7, None) == abi.E_NULL
+    # one long row is shared by several CTAs, which leave what they find in a workspace
+    long_row = dict(classes=100000, batch=1, positions=1, stride_class=1)
+    assert both(**long_row)[0] == abi.E_WORKSPACE
+    d = abi.LikelihoodDesc(dtype=abi.F32, top_k=2, **long_row)
+    assert cuda_lib.simnets_log_probabilities_workspace_bytes(C.byref(d)) > 0 == cuda_lib.simnets_log_probabilities_workspace_bytes(None)
+    assert cuda_lib.simnets_log_probabilities(None, *[one] * 8, 0, None) == abi.E_NULL
     assert cuda_lib.simnets_log_probabilities_gradient(None, *[one] * 8, None) == abi.E_NULL
 
 
