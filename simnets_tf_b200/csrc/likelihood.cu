@@ -126,23 +126,20 @@ struct Largest {
 #pragma unroll
         for (int j = 0; j < N; ++j) { v[j] = -infinity<T>(); i[j] = -1; }
     }
-    __device__ __forceinline__ void offer(T x, int c) {
+    __device__ __forceinline__ void offer(T x, int c) { put<false>(x, c); }
+    // in any order: of equal ones the lowest index is the first (a free place has -1, the largest of unsigned ones)
+    __device__ __forceinline__ void offer_any(T x, int c) { put<true>(x, c); }
+    template <bool ANY>
+    __device__ __forceinline__ void put(T x, int c) {
         bool above = false;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            above = above || x > v[j];
+            above = above || x > v[j] || (ANY && x == v[j] && x > -infinity<T>() && unsigned(c) < unsigned(i[j]));
             const T ov = v[j];
             const int oi = i[j];
             v[j] = above ? x : ov; i[j] = above ? c : oi;
             x = above ? ov : x; c = above ? oi : c;
         }
-    }
-    // U more classes from c on, `hi` the largest of them
-    template <int U>
-    __device__ __forceinline__ void offer(const T (&x)[U], T hi, int c) {
-        if (!__any_sync(0xffffffffu, hi > v[N - 1])) return;
-#pragma unroll
-        for (int u = 0; u < U; ++u) offer(x[u], c + u);
     }
 };
 template <typename T>
@@ -151,7 +148,6 @@ struct Largest<T, 0> {
     int i[1];
     __device__ __forceinline__ void clear() {}
     __device__ __forceinline__ void offer(T, int) {}
-    template <int U> __device__ __forceinline__ void offer(const T (&)[U], T, int) {}
 };
 
 struct Logits {
@@ -248,9 +244,9 @@ struct Run {
     static_assert(kLaneAhead % kWide<T> == 0, "chunks start at 16-byte addresses");
     int begin, end, c;
     long long step;
-    __device__ __forceinline__ explicit Run(const Logits& g, const T* x) {
+    __device__ __forceinline__ Run(const Logits& g, const T* x, int warp) {
         const int share = (g.classes + int(blockDim.y) - 1) / int(blockDim.y);
-        begin = min(g.classes, int(threadIdx.y) * share);
+        begin = min(g.classes, warp * share);
         end = min(g.classes, begin + share);
         c = begin - (SIDE ? in_front(x + begin) : 0);
         step = g.stride_class;
@@ -306,50 +302,109 @@ struct Run {
     }
 };
 
-template <typename T, int TOP, bool SIDE>
-__global__ void __launch_bounds__(512, sizeof(T) == 4 && TOP <= 4 ? 2 : 1) answer_lanes(Logits g, Answers<T> a) {
+// The likeliest classes: a list takes as many comparisons and choices a class as it has places, times five.  So what is listed are chunks by their largest,
+// equal ones by their order (warp << kWarpShift | chunk of its run): the first top_k of them have the top_k largest classes, and only these
+// are read again for it.
+constexpr int kWarpShift = 27;          // (2^30 classes are 2^27 chunks)
+
+// what a lane finds in its run; DIRECT: classes are listed, not chunks
+template <typename T, int TOP, bool SIDE, bool DIRECT>
+__device__ __forceinline__ Found<T, TOP> found_in_run(const Logits& g, const T* x) {
+    constexpr int U = kLaneAhead;
+    Run<T, SIDE> run(g, x, threadIdx.y);
+    const T* from = x + run.c * run.step;
+    T v[U];
+    run.load(v, from);
+    Found<T, TOP> f;
+    f.sums.clear();
+    f.top.clear();
+    for (int n = run.chunks(U), i = int(threadIdx.y) << kWarpShift; n > 0; --n, ++i) {
+        run.c += U;
+        from += U * run.step;
+        T next[U];
+        if (n > 1) run.load(next, from);
+        const T hi = f.sums.add(v);
+        if (TOP > 0 && __any_sync(0xffffffffu, hi > f.top.v[TOP > 0 ? TOP - 1 : 0])) {
+            if (DIRECT) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) f.top.offer(v[u], run.c - U + u);
+            } else {
+                f.top.offer(hi, i);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = next[u];
+    }
+    return f;
+}
+// a listed chunk of the logits x
+template <typename T, bool SIDE>
+__device__ __forceinline__ Run<T, SIDE> listed_chunk(const Logits& g, const T* x, int i) {
+    Run<T, SIDE> chunk(g, x, i >> kWarpShift);
+    chunk.c += (i & ((1 << kWarpShift) - 1)) * kLaneAhead;
+    return chunk;
+}
+
+template <typename T, int TOP, bool SIDE, bool DIRECT>
+__global__ void __launch_bounds__(128, sizeof(T) == 4 && TOP <= 4 ? 8 : 1) answer_lanes(Logits g, Answers<T> a) {
     constexpr int U = kLaneAhead;
     stream_order();
     extern __shared__ __align__(16) char room[];
     bool mine;
     const long long q = lane_position(g, &mine);
     const T* x = a.logits + g.at(q);
-    Run<T, SIDE> run(g, x);
-    const T* from = x + run.c * run.step;
-    T v[U];
-    run.load(v, from);
     const long long label = a.label && threadIdx.y == 0 ? a.labels[q] : -1;
+    Found<T, TOP> f = found_in_run<T, TOP, SIDE, DIRECT>(g, x);
     const bool labelled = label >= 0 && label < g.classes;
     const T of_label = labelled ? x[label * g.stride_class] : T(0);
-    Found<T, TOP> f;
-    f.sums.clear();
-    f.top.clear();
-    for (int n = run.chunks(U); n > 0; --n) {
-        const int c = run.c;
-        run.c += U;
-        from += U * run.step;
-        T next[U];
-        if (n > 1) run.load(next, from);
-        const T hi = f.sums.add(v);
-        f.top.offer(v, hi, c);
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = next[u];
-    }
     char* at = room + (threadIdx.z * blockDim.y + threadIdx.y) * Found<T, TOP>::kBytes;
     for (int d = 1; d < int(blockDim.y); d *= 2) {
         if (threadIdx.y % (2 * d) == d) f.put(at, threadIdx.x);
         __syncthreads();
         if (threadIdx.y % (2 * d) == 0 && threadIdx.y + d < blockDim.y) f.join(at + d * Found<T, TOP>::kBytes, threadIdx.x);
     }
-    if (threadIdx.y != 0 || !mine) return;
+    if (threadIdx.y != 0) return;
+    Largest<T, TOP> top = f.top;
+    if constexpr (TOP > 0 && !DIRECT) {
+        // the chunks in the order of the list, and every lane's classes not below its last chunk's largest one after the other
+        top.clear();
+        T bound = f.top.v[0];
+#pragma unroll
+        for (int j = 1; j < TOP; ++j) bound = j < g.top_k ? f.top.v[j] : bound;
+#pragma unroll
+        for (int j = 0; j < TOP; ++j) {
+            const int i = f.top.i[j];
+            const bool has = j < g.top_k && i >= 0;
+            if (!__any_sync(0xffffffffu, has)) break;
+            unsigned above = 0;
+            int c = 0;
+            T v[U];
+            if (has) {
+                const Run<T, SIDE> chunk = listed_chunk<T, SIDE>(g, x, i);
+                c = chunk.c;
+                chunk.load(v, x + chunk.c * chunk.step);
+#pragma unroll
+                for (int u = 0; u < U; ++u) above |= v[u] >= bound && v[u] > -infinity<T>() ? 1u << u : 0u;
+            }
+            while (__any_sync(0xffffffffu, above)) {
+                const int u = __ffs(above) - 1;
+                T xu = -infinity<T>();
+#pragma unroll
+                for (int w = 0; w < U; ++w) xu = u == w ? v[w] : xu;
+                top.offer_any(xu, c + u);
+                above &= above - 1;
+            }
+        }
+    }
+    if (!mine) return;
     const Answer<T> w(f.sums);
     write_position(g, a, q, of_label, labelled, w);
     long long to = TOP > 0 ? g.top_first(q) : 0;
 #pragma unroll
     for (int j = 0; j < TOP; ++j) {
         if (j >= g.top_k) break;
-        a.top_index[to] = f.top.i[j];
-        a.top[to] = f.top.i[j] < 0 ? -infinity<T>() : w.of(f.top.v[j]);
+        a.top_index[to] = top.i[j];
+        a.top[to] = top.i[j] < 0 ? -infinity<T>() : w.of(top.v[j]);
         to += g.top_step();
     }
 }
@@ -418,6 +473,28 @@ __device__ __forceinline__ double warp_max(double v) {
     for (int d = 16; d > 0; d >>= 1) v = larger(v, __shfl_xor_sync(0xffffffffu, v, d));
     return v;
 }
+// take(j, value, index) of the top_k best of all lanes' values, by falling value, equal ones by index; NaN and -infinity are none
+template <typename T, int N, class Take>
+__device__ __forceinline__ void best_of_lanes(T (&v)[N], int (&i)[N], int top_k, Take take) {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+        if (!(v[e] > -infinity<T>())) { v[e] = -infinity<T>(); i[e] = -1; }
+#pragma unroll 1
+    for (int j = 0; j < top_k; ++j) {
+        T best = v[0];
+        int at = i[0];
+#pragma unroll
+        for (int e = 1; e < N; ++e)
+            if (v[e] > best || (v[e] == best && unsigned(i[e]) < unsigned(at))) { best = v[e]; at = i[e]; }
+        warp_best(best, at);
+        if (at < 0) break;
+        take(j, best, at);
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (i[e] == at) { v[e] = -infinity<T>(); i[e] = -1; }
+    }
+}
+
 // The largest so far as a list of the warp, the j-th of them in lane j.  A class is compared with the last one that counts, and only one above it moves
 // the list: a row of n classes in any order moves it about top_k log(n / top_k) times.
 template <typename T>
@@ -531,6 +608,70 @@ __device__ __forceinline__ T logit_of_label(const Logits& g, const Answers<T>& a
     const long long label = a.label && threadIdx.x % 32 == 0 ? a.labels[q] : -1;
     *labelled = label >= 0 && label < g.classes;
     return *labelled ? x[label] : T(0);
+}
+
+// Few positions whose classes are apart, by kGroupWarps warps a tile of 32: what the warps found is joined position by position, a warp each, its lanes
+// over the listed chunks and then over their classes.
+constexpr int kGroupWarps = 16;
+// (the entries of a position lie in as many banks)
+template <typename T, int TOP> constexpr size_t kGroupBytes = Found<T, TOP>::kBytes + 8;
+template <typename T, int TOP, bool SIDE>
+__global__ void __launch_bounds__(32 * kGroupWarps, sizeof(T) == 4 ? 2 : 1) answer_groups(Logits g, Answers<T> a) {
+    stream_order();
+    extern __shared__ __align__(16) char room[];
+    const int lane = threadIdx.x;
+    bool mine;
+    {
+        const T* x = a.logits + g.at(lane_position(g, &mine));
+        const Found<T, TOP> f = found_in_run<T, TOP, SIDE, false>(g, x);
+        f.put(room + threadIdx.y * kGroupBytes<T, TOP>, lane);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int p = threadIdx.y; p < 32; p += kGroupWarps) {
+        const long long q = (long long)blockIdx.x * 32 + p;
+        if (q >= g.count()) break;
+        const T* x = a.logits + g.at(q);
+        const long long label = a.label && lane == 0 ? a.labels[q] : -1;
+        const bool labelled = label >= 0 && label < g.classes;
+        const T of_label = labelled ? x[label * g.stride_class] : T(0);
+        auto values = [&](int warp) { return reinterpret_cast<const T*>(room + warp * kGroupBytes<T, TOP>) + p; };
+        Sums<T> sums;
+        sums.clear();
+        if (lane < kGroupWarps) sums = {values(lane)[0], values(lane)[32], values(lane)[64]};
+        sums = over_warp(sums);
+        WarpList<T> list;
+        list.clear();
+        if constexpr (TOP > 0) {
+            // (kGroupWarps * TOP entries, and then 8 classes of each chunk that is taken)
+            constexpr int kEntries = (kGroupWarps * TOP + 31) / 32, kClasses = (TOP * kLaneAhead + 31) / 32;
+            T v[kEntries];
+            int i[kEntries], taken = -1;
+#pragma unroll
+            for (int e = 0; e < kEntries; ++e) {
+                const int entry = e * 32 + lane, warp = entry % kGroupWarps, j = entry / kGroupWarps;
+                const bool there = j < TOP;
+                v[e] = there ? values(warp)[32 * (3 + j)] : -infinity<T>();
+                i[e] = there ? reinterpret_cast<const int*>(values(warp) - p + 32 * (3 + TOP))[32 * j + p] : -1;
+            }
+            best_of_lanes(v, i, g.top_k, [&](int j, T, int at) { if (lane == j) taken = at; });
+            T w[kClasses];
+            int c[kClasses];
+#pragma unroll
+            for (int e = 0; e < kClasses; ++e) {
+                const int entry = e * 32 + lane, j = entry / kLaneAhead, at = __shfl_sync(0xffffffffu, taken, j < 16 ? j : 0);
+                w[e] = -infinity<T>();
+                c[e] = -1;
+                if (j < g.top_k && at >= 0) {
+                    const Run<T, SIDE> chunk = listed_chunk<T, SIDE>(g, x, at);
+                    const int here = chunk.c + entry % kLaneAhead;
+                    if (here >= chunk.begin && here < chunk.end) { w[e] = x[here * chunk.step]; c[e] = here; }
+                }
+            }
+            best_of_lanes(w, c, g.top_k, [&](int j, T best, int at) { if (lane == j) { list.v = best; list.i = at; } });
+        }
+        write_row<T, (TOP > 0)>(g, a, q, of_label, labelled, sums, list);
+    }
 }
 
 // A warp a row, kRowWarps of them a CTA, U classes a lane and chunk.
@@ -916,7 +1057,7 @@ __global__ void __launch_bounds__(512, sizeof(T) == 4 ? 2 : 1) gradient_lanes(Lo
     if (!mine) return;
     const T* x = a.logits + g.at(q);
     T* dx = a.dlogits + g.at(q, a.out_batch, a.out_position);
-    Run<T, SIDE> run(g, x), out = run;
+    Run<T, SIDE> run(g, x, threadIdx.y), out = run;
     const T* from = x + run.c * run.step;
     T* to = dx + run.c * a.out_class;
     const bool aligned = in_front(x) == in_front(dx);
@@ -1006,27 +1147,37 @@ Logits logits_of(const simnets_likelihood_desc& d) {
 // the whole warp, and joining what lanes found costs more than the classes.
 bool by_rows(const Logits& g) { return g.stride_class == 1 && g.classes > 128; }
 
-// warps that share 32 positions
-int warps_of_lanes(const Logits& g, size_t bytes_a_warp) {
-    const long long tiles = (g.count() + 31) / 32;
-    int w = 1;
-    while (w < 16 && tiles * w < 16LL * device_sm_count() && g.classes >= 2 * w * kLaneAhead && 2 * w * bytes_a_warp <= 48 * 1024) w *= 2;
-    return w;
+// warps that share 32 positions: 1, 2, 4 or kGroupWarps
+int warps_of_lanes(const Logits& g) {
+    const long long tiles = (g.count() + 31) / 32, enough = 16LL * device_sm_count();
+    if (tiles * 4 < enough && g.classes >= 8 * kLaneAhead) return kGroupWarps;
+    return tiles * 2 < enough && g.classes >= 4 * kLaneAhead ? 4 : tiles < enough && g.classes >= 2 * kLaneAhead ? 2 : 1;
 }
 
 template <class Kernel, class A>
-cudaError_t launch_lanes(Kernel* kernel, const Logits& g, const A& a, int warps, size_t bytes_a_warp, cudaStream_t s) {
+cudaError_t launch_lanes(Kernel* kernel, const Logits& g, const A& a, int warps, size_t bytes, cudaStream_t s) {
     const int tiles = warps < 4 ? 4 / warps : 1;
     const unsigned grid = unsigned((g.count() + 32 * tiles - 1) / (32 * tiles));
-    in_stream_order(kernel, grid, dim3(32, warps, tiles), warps > 1 ? bytes_a_warp * warps * tiles : 0, s)(g, a);
+    in_stream_order(kernel, grid, dim3(32, warps, tiles), bytes, s)(g, a);
     count_launch();
     return cudaGetLastError();
 }
 
-template <typename T, int TOP>
+template <typename T, int TOP, bool SIDE>
 cudaError_t answer_lanes_of(const Logits& g, const Answers<T>& a, cudaStream_t s) {
-    constexpr size_t kBytes = Found<T, TOP>::kBytes;
-    return launch_lanes(g.stride_class == 1 ? answer_lanes<T, TOP, true> : answer_lanes<T, TOP, false>, g, a, warps_of_lanes(g, kBytes), kBytes, s);
+    const int warps = warps_of_lanes(g);
+    // a run of hardly more chunks than the list has places would be read twice (us, classes / chunks listed: 65536 rows of 10, three alternatives 4.4 / 7.6,
+    // float64 maps of 37, four alternatives 7.3 / 9.5, 100000 rows of 100, three alternatives 20.7 / 16.9, a map of 150 36 / 27)
+    const bool direct = g.classes <= 16 * TOP * warps;
+    if (warps < kGroupWarps)
+        return launch_lanes(direct || TOP == 0 ? answer_lanes<T, TOP, SIDE, true> : answer_lanes<T, TOP, SIDE, TOP == 0>, g, a, warps, warps > 1 ? 4 * Found<T, TOP>::kBytes : 0, s);
+    constexpr int kBytes = int(kGroupWarps * kGroupBytes<T, TOP>);
+    if (kBytes > 48 * 1024) {
+        static SmemLimit limit;
+        const cudaError_t e = limit.raise(answer_groups<T, TOP, SIDE>, kBytes);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_lanes(answer_groups<T, TOP, SIDE>, g, a, kGroupWarps, kBytes, s);
 }
 
 // A warp a row where a row is one chunk, or where rows are enough to fill the multiprocessors and not so long that a warp's is late.
@@ -1065,23 +1216,28 @@ cudaError_t answer_stream_of(const Logits& g, const Answers<T>& a, void* ws, cud
     return cudaGetLastError();
 }
 
+template <typename T, bool SIDE>
+cudaError_t answer_by_lanes(const Logits& g, const Answers<T>& a, cudaStream_t s) {
+    if (g.top_k == 0) return answer_lanes_of<T, 0, SIDE>(g, a, s);
+    if (g.top_k == 1) return answer_lanes_of<T, 1, SIDE>(g, a, s);
+    if (g.top_k <= 4) return answer_lanes_of<T, 4, SIDE>(g, a, s);
+    if (g.top_k <= 8) return answer_lanes_of<T, 8, SIDE>(g, a, s);
+    return answer_lanes_of<T, 16, SIDE>(g, a, s);
+}
+
 template <typename T>
 cudaError_t answer_as(const Logits& g, const Answers<T>& a, void* ws, cudaStream_t s) {
     if (by_rows(g)) {
         if (!by_warps(g)) return g.top_k > 0 ? answer_stream_of<T, true>(g, a, ws, s) : answer_stream_of<T, false>(g, a, ws, s);
         return g.top_k > 0 ? answer_rows_of<T, true, kStreamAhead<T>>(g, a, s) : answer_rows_of<T, false, kStreamAhead<T>>(g, a, s);
     }
-    if (g.top_k == 0) return answer_lanes_of<T, 0>(g, a, s);
-    if (g.top_k == 1) return answer_lanes_of<T, 1>(g, a, s);
-    if (g.top_k <= 4) return answer_lanes_of<T, 4>(g, a, s);
-    if (g.top_k <= 8) return answer_lanes_of<T, 8>(g, a, s);
-    return answer_lanes_of<T, 16>(g, a, s);
+    return g.stride_class == 1 ? answer_by_lanes<T, true>(g, a, s) : answer_by_lanes<T, false>(g, a, s);
 }
 
 template <typename T>
 cudaError_t gradient_as(const Logits& g, const Gradients<T>& a, cudaStream_t s) {
     if (!by_rows(g))
-        return launch_lanes(g.stride_class == 1 ? gradient_lanes<T, true> : gradient_lanes<T, false>, g, a, warps_of_lanes(g, 0), 0, s);
+        return launch_lanes(g.stride_class == 1 ? gradient_lanes<T, true> : gradient_lanes<T, false>, g, a, warps_of_lanes(g), 0, s);
     if (g.classes <= 1024) {
         in_stream_order(gradient_rows<T, 1, 4>, unsigned((g.count() + kRowWarps - 1) / kRowWarps), 32 * kRowWarps, 0, s)(g, a);
     } else {
