@@ -1143,9 +1143,11 @@ Logits logits_of(const simnets_likelihood_desc& d) {
     return {d.batch, d.positions, d.stride_batch, d.stride_class, d.stride_position, d.classes, d.top_k, d.top_last};
 }
 
-// Classes that lie side by side are read by several lanes where they are more than this: below, a lane's loads of 16 bytes are a few lines of memory for
-// the whole warp, and joining what lanes found costs more than the classes.
-bool by_rows(const Logits& g) { return g.stride_class == 1 && g.classes > 128; }
+// Classes that lie side by side are read by several lanes where they are many or the rows are few.  Else a lane's loads of 16 bytes are a few lines of
+// memory for the whole warp, and joining what lanes found costs more than the classes (lanes / warps of rows, us: 100000 rows of 100 with three
+// alternatives 18 / 64 and their gradient 39 / 42, 60000 of 200 20 / 38 and 50 / 35, 3000 of 100 6.0 / 4.5 and 6.0 / 4.3).
+bool by_rows(const Logits& g, int most) { return g.stride_class == 1 && (g.classes > most || (g.classes > 32 && g.count() < 16384)); }
+constexpr int kMostByLanes = 256, kMostGradientByLanes = 128;
 
 // warps that share 32 positions: 1, 2, 4 or kGroupWarps
 int warps_of_lanes(const Logits& g) {
@@ -1227,23 +1229,28 @@ cudaError_t answer_by_lanes(const Logits& g, const Answers<T>& a, cudaStream_t s
 
 template <typename T>
 cudaError_t answer_as(const Logits& g, const Answers<T>& a, void* ws, cudaStream_t s) {
-    if (by_rows(g)) {
+    if (by_rows(g, kMostByLanes)) {
         if (!by_warps(g)) return g.top_k > 0 ? answer_stream_of<T, true>(g, a, ws, s) : answer_stream_of<T, false>(g, a, ws, s);
-        return g.top_k > 0 ? answer_rows_of<T, true, kStreamAhead<T>>(g, a, s) : answer_rows_of<T, false, kStreamAhead<T>>(g, a, s);
+        // (60000 rows of 200 classes with three alternatives 38 us with 8 a lane, 49 with 16, 20000 of 500 20 and 18; float64 3000 of 1500 24 with 4, 32 with 8)
+        constexpr int kFew = sizeof(T) == 4 ? 8 : 4, kMany = sizeof(T) == 4 ? 16 : 4;
+        if (g.classes <= 32 * kFew) return g.top_k > 0 ? answer_rows_of<T, true, kFew>(g, a, s) : answer_rows_of<T, false, kFew>(g, a, s);
+        return g.top_k > 0 ? answer_rows_of<T, true, kMany>(g, a, s) : answer_rows_of<T, false, kMany>(g, a, s);
     }
     return g.stride_class == 1 ? answer_by_lanes<T, true>(g, a, s) : answer_by_lanes<T, false>(g, a, s);
 }
 
 template <typename T>
 cudaError_t gradient_as(const Logits& g, const Gradients<T>& a, cudaStream_t s) {
-    if (!by_rows(g))
+    if (!by_rows(g, kMostGradientByLanes))
         return launch_lanes(g.stride_class == 1 ? gradient_lanes<T, true> : gradient_lanes<T, false>, g, a, warps_of_lanes(g), 0, s);
-    if (g.classes <= 1024) {
-        in_stream_order(gradient_rows<T, 1, 4>, unsigned((g.count() + kRowWarps - 1) / kRowWarps), 32 * kRowWarps, 0, s)(g, a);
-    } else {
-        const dim3 grid(unsigned(g.count()), std::min((g.classes + 16383) / 16384, 65535));
-        in_stream_order(gradient_rows<T, 8, kStreamAhead<T>>, grid, 256, 0, s)(g, a);
-    }
+    // A chunk should be no more than a row, and a row a few chunks (us, 3000 rows of 1000 with 4 classes a lane / 16 9.3 / 6.8, 60000 of 200 34 / 45;
+    // 4096 rows of 2000 by a warp / 8 13.7 / 23.4; 3000 of 6000 by 4 warps / 8 26.9 / 31.0, 2048 of 32000 86.0 / 83.5).
+    constexpr int U = kStreamAhead<T>;
+    const unsigned rows = unsigned(g.count()), ctas = unsigned((g.count() + kRowWarps - 1) / kRowWarps);
+    if (g.classes <= 512) in_stream_order(gradient_rows<T, 1, 4>, ctas, 32 * kRowWarps, 0, s)(g, a);
+    else if (g.classes <= 4096) in_stream_order(gradient_rows<T, 1, U>, ctas, 32 * kRowWarps, 0, s)(g, a);
+    else if (g.classes <= 16384) in_stream_order(gradient_rows<T, 4, U>, rows, 128, 0, s)(g, a);
+    else in_stream_order(gradient_rows<T, 8, U>, dim3(rows, std::min((g.classes + 16383) / 16384, 65535)), 256, 0, s)(g, a);
     count_launch();
     return cudaGetLastError();
 }
@@ -1261,7 +1268,7 @@ cudaError_t launch_log_probabilities(const simnets_likelihood_desc& d, const voi
 
 size_t log_probabilities_workspace_bytes(const simnets_likelihood_desc& d) {
     const Logits g = logits_of(d);
-    if (g.count() == 0 || !by_rows(g) || by_warps(g)) return 0;
+    if (g.count() == 0 || !by_rows(g, kMostByLanes) || by_warps(g)) return 0;
     return d.dtype == SIMNETS_F64 ? 2 * sizeof(RowFound<double>) * runs_of<double>(g).ctas : 2 * sizeof(RowFound<float>) * runs_of<float>(g).ctas;
 }
 
