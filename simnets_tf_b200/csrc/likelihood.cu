@@ -706,9 +706,10 @@ __global__ void __launch_bounds__(32 * kRowWarps) answer_rows(Logits g, Answers<
 // More on the way at once is slower (2048 rows of 65537 classes with 5 alternatives / of 32000 without, us: 2 CTAs a multiprocessor with 2, 3, 4
 // stages 121 / 55, 104 / 46, 110 / 46, 3 CTAs with 2, 3, 4 stages 105 / 47, 116 / 47, 121 / 51, 4 with 3 132 / 51; the memory's floor 82 / 40).
 //
-// The likeliest classes cost the streaming warps a comparison a chunk.  Every thread keeps the largest of its classes and the chunk in which it came up
-// first.  Of the threads by their largest, equal ones by its first class, the first top_k have all of the row's top_k: every other thread's classes have at
-// least top_k in front of them.  Another warp, while the others go on, picks these threads and reads their classes again, a few hundred.
+// The likeliest classes cost the streaming warps a few comparisons a chunk.  Every thread keeps the largest of its classes, the chunk in which it came up
+// first, and the largest of its other chunks.  Of the threads by their largest, equal ones by its first class, the first top_k have all of the row's
+// top_k: every other thread's classes have at least top_k in front of them.  Another warp, while the others go on, picks these threads and reads the
+// chunks of theirs again that may have one, seldom more than one a thread.
 //
 // A run that has all of a row answers it; of others what it found goes to `parts`, two places a CTA (0: with its first chunk, 1: without), where join_parts
 // finds it.
@@ -751,8 +752,8 @@ __device__ __forceinline__ void copy_chunk(char* to, const T* x, long long first
 template <typename T>
 struct Streamed {
     Sums<T> sums[kStreamWarps];
-    T largest[kStreamThreads];
-    int chunk[kStreamThreads];              // where it came up
+    T largest[kStreamThreads], second[kStreamThreads];          // (second: of the chunks' largest)
+    int chunk[kStreamThreads];                                  // where the largest came up
 };
 
 // All warps but the waiting one come and go on (bar.arrive), or wait for it: 32 more threads than stream take part.
@@ -763,11 +764,9 @@ __device__ __forceinline__ void barrier_wait(int id) { asm volatile("bar.sync %0
 template <typename T>
 __device__ __forceinline__ long long share_of(long long first, int tid, int j) { return first + class_in_chunk<T, kStreamThreads>(tid, j * kWide<T>); }
 
-// Room for picking: classes on their way, and those that may be among the likeliest.
-constexpr int kAgain = 12;
+// classes that may be among the likeliest
 template <typename T>
 struct Above {
-    __align__(16) char again[kAgain][32 * 16];
     T top[32];
     int top_index[32];
 };
@@ -820,31 +819,29 @@ __device__ __forceinline__ void pick(WarpList<T>& list, const Streamed<T>& kept,
             if (w * 32 + lane == tid) rest[w] = -infinity<T>();
     }
     if (n < top_k) bound = -infinity<T>();                  // (all of the classes that can be are theirs)
-    // Their classes, up to kAgain * 32 times 16 bytes at a time.  Those not below the bound are hardly ever more than the lanes of a warp: the best of
-    // these again and again; more, equal ones, are put in one by one.  (Loops that are not unrolled: the code runs once a row, and would
-    // wait for its instructions.)
+    // First the chunks in which their largest came up, then all others of a thread whose second largest is not below the bound.  The classes that are
+    // not are hardly ever more than the lanes of a warp: the best of these again and again; more, equal ones, are put in one by one.  (Loops
+    // that are not unrolled: the code runs once a row, and would wait for its instructions.)
     list.clear();
-    const int each = 4 * (end - begin), total = n * each;
     int count = 0;
-    for (int from = 0; from < total; from += kAgain * 32) {
+    const bool more = lane < n && kept.second[picked] >= bound && kept.second[picked] > -infinity<T>();
+    unsigned passes = __ballot_sync(0xffffffffu, more);
 #pragma unroll 1
-        for (int i = 0; i < kAgain && from + i * 32 < total; ++i) {
-            const int at = min(from + i * 32 + lane, total - 1), j = at / each, tid = __shfl_sync(0xffffffffu, picked, j), place = begin * 4 + at - j * each;
-            copy_wide(room.again[i] + lane * 16, x, share_of<T>((long long)(place / 4) * kStreamChunk<T> - front, tid, place % 4), false, classes);
-        }
-        asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+    for (int pass = -1;;) {
+        const int total = pass < 0 ? 4 * n : 4 * (end - begin);
 #pragma unroll 1
-        for (int i = 0; i < kAgain && from + i * 32 < total; ++i) {
+        for (int from = 0; from < total; from += 32) {
+            const int at = from + lane, tid = __shfl_sync(0xffffffffu, picked, pass < 0 ? min(at, total - 1) / 4 : pass), first = kept.chunk[tid], chunk = pass < 0 ? first : begin + at / 4;
+            const long long c0 = share_of<T>((long long)chunk * kStreamChunk<T> - front, tid, at % 4);
             T v[kWide<T>];
-            *reinterpret_cast<typename Bytes16<T>::type*>(v) = *reinterpret_cast<const typename Bytes16<T>::type*>(room.again[i] + lane * 16);
-            const int at = from + i * 32 + lane, j = min(at, total - 1) / each, tid = __shfl_sync(0xffffffffu, picked, j), place = begin * 4 + at - j * each;
+#pragma unroll
+            for (int e = 0; e < kWide<T>; ++e) v[e] = at < total && (pass < 0 || chunk != first) && c0 + e >= 0 && c0 + e < classes ? x[c0 + e] : -infinity<T>();
             unsigned mine = 0;
 #pragma unroll
-            for (int e = 0; e < kWide<T>; ++e) mine |= at < total && v[e] > -infinity<T>() && v[e] >= bound ? 1u << e : 0u;
+            for (int e = 0; e < kWide<T>; ++e) mine |= v[e] > -infinity<T>() && v[e] >= bound ? 1u << e : 0u;
 #pragma unroll 1
             while (unsigned who = __ballot_sync(0xffffffffu, mine)) {
-                const int e = __ffs(mine) - 1, left = 32 - count, to = count + __popc(who & ((1u << lane) - 1));
-                const int c = int(share_of<T>((long long)(place / 4) * kStreamChunk<T> - front, tid, place % 4)) + e;
+                const int e = __ffs(mine) - 1, left = 32 - count, to = count + __popc(who & ((1u << lane) - 1)), c = int(c0) + e;
                 T w = v[0];
 #pragma unroll
                 for (int k = 1; k < kWide<T>; ++k) w = e == k ? v[k] : w;
@@ -860,6 +857,9 @@ __device__ __forceinline__ void pick(WarpList<T>& list, const Streamed<T>& kept,
                 }
             }
         }
+        if (!passes) break;
+        pass = __ffs(passes) - 1;
+        passes &= passes - 1;
     }
     __syncwarp();
     T mine = lane < count ? room.top[lane] : -infinity<T>();
@@ -945,7 +945,7 @@ __global__ void __launch_bounds__(kStreamThreads + 32, kStreamCtas) answer_strea
     for (int s = 0; s + 1 < kStages; ++s) copy_next();
     Sums<T> sums;
     sums.clear();
-    T largest = -infinity<T>();
+    T largest = -infinity<T>(), second = largest;
     int largest_chunk = 0;
     for (long long at = begin; at < end; ++at) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
@@ -956,20 +956,23 @@ __global__ void __launch_bounds__(kStreamThreads + 32, kStreamCtas) answer_strea
         stage = stage + 1 == kStages ? 0 : stage + 1;
         copy_next();                                        // (into what was read an iteration ago)
         const T hi = sums.add(v);
-        if (TOP && hi > largest) { largest = hi; largest_chunk = chunk; }
+        if (TOP) {
+            second = larger(second, hi > largest ? largest : hi);
+            if (hi > largest) { largest = hi; largest_chunk = chunk; }
+        }
         const bool ends = ++chunk == runs.of_row;
         if (ends || at + 1 == end) {
             sums = over_warp(sums);
             if (rows >= 2) barrier_wait(3 + turn);          // (the row before the last one has been answered)
             if (lane == 0) kept[turn].sums[warp] = sums;
-            if (TOP) { kept[turn].largest[threadIdx.x] = largest; kept[turn].chunk[threadIdx.x] = largest_chunk; }
+            if (TOP) { kept[turn].largest[threadIdx.x] = largest; kept[turn].second[threadIdx.x] = second; kept[turn].chunk[threadIdx.x] = largest_chunk; }
             __threadfence_block();
             barrier_arrive(1 + turn);
             ++rows;
             turn ^= 1;
             chunk = 0;
             sums.clear();
-            largest = -infinity<T>();
+            largest = second = -infinity<T>();
         }
     }
 }
