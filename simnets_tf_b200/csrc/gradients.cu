@@ -15,7 +15,7 @@ namespace simnets {
 namespace {
 
 constexpr int kThreads = 256, kItemBytes = 16 * 1024;       // a CTA takes 16 KB of one tensor at a time
-constexpr int kMostTensors = 384, kFew = 24;                // of a launch: their table is the kernel's argument
+constexpr int kMostTensors = 1088, kFew = 24;                // of a launch: their table is the kernel's argument
 
 struct Partial { double mid, big, small; };
 __host__ __device__ constexpr double up600() { return 0x1p600; }

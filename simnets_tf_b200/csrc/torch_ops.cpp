@@ -1067,20 +1067,22 @@ Tensor gradients_impl(const py::object& given_in, int64_t order, bool scaled, do
     if (out && out->tensors.size() != n) throw std::invalid_argument("out must have one tensor for each gradient, got " + std::to_string(out->tensors.size()) + " for " + std::to_string(n));
     const Tensor* first = nullptr;
     bool f64 = false;
+    const bool grad_mode = at::GradMode::is_enabled();
     for (size_t i = 0; i < n; ++i) {
         const Tensor* const p = given.tensors[i];
         if (!p) continue;
-        const Tensor& t = *p;
+        const at::TensorImpl& t = *p->unsafeGetTensorImpl();
         if (t.layout() != at::kStrided) throw py::type_error("gradients must be dense tensors");
-        if (t.scalar_type() != at::kFloat && t.scalar_type() != at::kDouble) throw py::type_error("simnets ops are registered for float32 and float64 only");
+        const at::ScalarType type = p->scalar_type();
+        if (type != at::kFloat && type != at::kDouble) throw py::type_error("simnets ops are registered for float32 and float64 only");
         if (!t.is_cuda()) throw std::runtime_error("simnets_b200 has no CPU kernels: every tensor must live on a CUDA device");
         if (!first) first = p;
         if (t.device() != first->device()) throw std::runtime_error("all tensors of one op call must be on the same device");
         const Tensor* const q = out ? out->tensors[i] : p;
-        if (at::GradMode::is_enabled() && (t.requires_grad() || (q && q->requires_grad()))) throw std::invalid_argument("the norm of gradients has no gradient itself: detach them");
-        f64 = f64 || t.scalar_type() == at::kDouble;
+        if (grad_mode && (t.requires_grad() || (q && q->requires_grad()))) throw std::invalid_argument("the norm of gradients has no gradient itself: detach them");
+        f64 = f64 || type == at::kDouble;
         if (!scaled) continue;
-        if (!q || q->layout() != at::kStrided || q->sizes() != t.sizes() || q->scalar_type() != t.scalar_type() || q->device() != t.device())
+        if (!q || q->layout() != at::kStrided || q->sizes() != t.sizes() || q->scalar_type() != type || q->device() != t.device())
             throw std::invalid_argument("out must have the shapes, types and device of the gradients");
         if (!elements_apart(*q)) throw std::invalid_argument("a tensor that is written has elements that share memory");
     }

@@ -41,7 +41,7 @@ def agree(norm, got, want_norm, want, arrays, limit):
 
 @pytest.mark.parametrize("order", [2, INF])
 @pytest.mark.parametrize("kinds", [[np.float32], [np.float64], [np.float32, np.float64]], ids=["f32", "f64", "both"])
-@pytest.mark.parametrize("count", [1, 4, 11, 30, 1000])
+@pytest.mark.parametrize("count", [1, 4, 11, 30, 1000, 2500])
 def test_norm_and_clipping(count, kinds, order):
     sizes = [SIZES[i % len(SIZES)] if count <= 30 else (1 + i % 37,) for i in range(count)]
     arrays = make(sizes, kinds)
