@@ -123,10 +123,13 @@ int likelihood_check(const simnets_likelihood_desc* d) {
     if (d->dtype != SIMNETS_F32 && d->dtype != SIMNETS_F64) return SIMNETS_E_DTYPE;
     if (d->classes < 1 || d->batch < 0 || d->positions < 0 || d->top_k < 0 || d->top_k > d->classes || d->stride_batch < 0 || d->stride_class < 0 || d->stride_position < 0)
         return SIMNETS_E_DESC;
-    // (places of classes are counted in 32 bits, CTAs of positions as well)
-    if (d->top_k > 16 || d->classes > (1 << 30) || (d->batch > 0 && d->positions > (1LL << 36) / d->batch)) return SIMNETS_E_UNSUPPORTED;
+    // (classes are counted in 32 bits, CTAs of positions as well: eight positions each at least, or 4096 classes)
+    if (d->top_k > 16 || d->classes > (1 << 30) || (d->batch > 0 && d->positions > std::min(1LL << 33, (1LL << 43) / d->classes) / d->batch)) return SIMNETS_E_UNSUPPORTED;
     return SIMNETS_OK;
 }
+
+// whether a place cannot hold values of the type
+bool misplaced(const void* p, int32_t dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype == SIMNETS_F64 ? 8 : 4) != 0; }
 
 int gradients_check(int32_t order, int32_t tensors, const int32_t* dtypes, const int64_t* counts, const void* const* in, const void* norm, const void* ws, size_t ws_bytes) {
     if ((order != 0 && order != 2) || tensors < 0) return SIMNETS_E_DESC;
@@ -136,6 +139,7 @@ int gradients_check(int32_t order, int32_t tensors, const int32_t* dtypes, const
         if (dtypes && dtypes[i] != SIMNETS_F32 && dtypes[i] != SIMNETS_F64) return SIMNETS_E_DTYPE;
         if (counts[i] < 0) return SIMNETS_E_DESC;
         if (counts[i] > 0 && !in[i]) return SIMNETS_E_NULL;
+        if (counts[i] > 0 && misplaced(in[i], dtypes ? dtypes[i] : SIMNETS_F32)) return SIMNETS_E_UNSUPPORTED;
         if (counts[i] > (1LL << 40) - total) return SIMNETS_E_UNSUPPORTED;          // (pieces of 16 KB are counted in 32 bits)
         total += counts[i];
     }
@@ -569,6 +573,7 @@ int simnets_log_probabilities(const simnets_likelihood_desc* d, const void* logi
     if (d->batch == 0 || d->positions == 0) return SIMNETS_OK;
     if (!logits || (label && !labels) || (top == nullptr) != (top_index == nullptr)) return SIMNETS_E_NULL;
     if ((d->top_k > 0) != (top != nullptr)) return SIMNETS_E_DESC;
+    if (misplaced(logits, d->dtype)) return SIMNETS_E_UNSUPPORTED;
     if (const size_t need = log_probabilities_workspace_bytes(*d); need > 0 && (!ws || ws_bytes < need)) return SIMNETS_E_WORKSPACE;
     return from_cuda(launch_log_probabilities(*d, logits, reinterpret_cast<const long long*>(labels), label, entropy, top_index, top, stats, ws, as_stream(stream)));
 }
@@ -580,6 +585,7 @@ int simnets_log_probabilities_gradient(const simnets_likelihood_desc* d, const v
     if (d->batch == 0 || d->positions == 0) return SIMNETS_OK;
     if (!logits || !stats || !dlogits || (g_label && !labels) || (g_top && !top_index)) return SIMNETS_E_NULL;
     if ((d->top_k > 0) != (g_top != nullptr)) return SIMNETS_E_DESC;
+    if (misplaced(logits, d->dtype) || misplaced(dlogits, d->dtype)) return SIMNETS_E_UNSUPPORTED;
     return from_cuda(launch_log_probabilities_gradient(*d, logits, reinterpret_cast<const long long*>(labels), stats, top_index, g_label, g_entropy, g_top, dlogits,
                                                        as_stream(stream)));
 }
@@ -598,8 +604,10 @@ int simnets_clip_gradients(int32_t order, double max_norm, int32_t tensors, cons
     if (tensors > 0 && !out) return SIMNETS_E_NULL;
     const int rc = gradients_check(order, tensors, dtypes, counts, in, norm, ws, ws_bytes);
     if (rc) return rc;
-    for (int i = 0; i < tensors; ++i)
+    for (int i = 0; i < tensors; ++i) {
         if (counts[i] > 0 && !out[i]) return SIMNETS_E_NULL;
+        if (counts[i] > 0 && misplaced(out[i], dtypes ? dtypes[i] : SIMNETS_F32)) return SIMNETS_E_UNSUPPORTED;
+    }
     return gradients(order, max_norm, tensors, dtypes, counts, in, out, norm, ws, stream);
 }
 

@@ -925,7 +925,7 @@ Likelihood likelihood_impl(const Tensor& logits_in, const OptTensor& labels_in, 
     auto at_or_null = [](const Tensor& t) { return t.defined() ? ptr(t) : nullptr; };
     Tensor ws;
     if (const size_t need = simnets_log_probabilities_workspace_bytes(&d)) ws = scratch(logits, need);
-    if (d.batch * d.positions > 0)
+    if (d.batch * d.positions > 0 && (labels || entropy || top_k > 0))
         check(simnets_log_probabilities(&d, ptr(logits), labels ? labels->data_ptr<int64_t>() : nullptr, at_or_null(r.label), at_or_null(r.entropy),
                                         r.top_index.defined() ? r.top_index.data_ptr<int32_t>() : nullptr, at_or_null(r.top), at_or_null(r.stats),
                                         at_or_null(ws), ws.defined() ? ws.numel() : 0, stream_of(logits)));

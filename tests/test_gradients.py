@@ -50,7 +50,8 @@ def test_the_c_entry_points_check_before_they_launch(cuda_lib):
     assert both(dtypes=(0, 2)) == (abi.E_DTYPE,) * 2
     assert both(counts=None) == both(tensors=None) == both(norm=None) == both(tensors=(256, None)) == (abi.E_NULL,) * 2
     assert both(w=None) == both(size=ws - 1) == (abi.E_WORKSPACE,) * 2
-    assert both(counts=(1 << 40, 1)) == (abi.E_UNSUPPORTED,) * 2
+    assert both(counts=(1 << 40, 1)) == both(tensors=(257, 512)) == both(tensors=(256, 516)) == (abi.E_UNSUPPORTED,) * 2
+    assert both(out=(256, 516))[1] == abi.E_UNSUPPORTED
     assert both(size=ws - 1, limit=-1.0)[1] == both(size=ws - 1, limit=math.nan)[1] == abi.E_DESC
     assert both(size=ws - 1, out=None)[1] == abi.E_NULL
 

@@ -40,8 +40,9 @@ def test_the_c_entry_points_check_before_they_launch(cuda_lib):
     for kw in (dict(classes=0), dict(batch=-1), dict(positions=-1), dict(top_k=-1), dict(top_k=13), dict(stride_batch=-1), dict(stride_class=-9), dict(stride_position=-1),
                dict(top_k=0), dict(top=None, index=None)):
         assert both(**kw) == (abi.E_DESC,) * 2, kw
-    for kw in (dict(classes=40, top_k=17), dict(classes=(1 << 30) + 1), dict(batch=1 << 20, positions=1 << 20)):
+    for kw in (dict(classes=40, top_k=17), dict(classes=(1 << 30) + 1), dict(batch=1 << 17, positions=1 << 17), dict(classes=1 << 20, batch=1 << 12, positions=1 << 12)):
         assert both(**kw) == (abi.E_UNSUPPORTED,) * 2, kw
+    assert both(logits=C.c_void_p(258)) == (abi.E_UNSUPPORTED,) * 2 and both(logits=C.c_void_p(260), dtype=abi.F64) == (abi.E_UNSUPPORTED,) * 2
     for kw in (dict(logits=None), dict(labels=None), dict(index=None)):
         assert both(**kw) == (abi.E_NULL,) * 2, kw
     assert both(stats=None)[1] == abi.E_NULL
