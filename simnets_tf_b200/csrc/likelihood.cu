@@ -474,25 +474,36 @@ __device__ __forceinline__ double warp_max(double v) {
     for (int d = 16; d > 0; d >>= 1) v = larger(v, __shfl_xor_sync(0xffffffffu, v, d));
     return v;
 }
-// take(j, value, index) of the top_k best of all lanes' values, by falling value, equal ones by index; NaN and -infinity are none
+// take(j, value, index) of the top_k best of all lanes' values, by falling value, equal ones by index; NaN and -infinity are none.  Every lane puts its own
+// in order, and the best of the lanes' first ones is taken away again and again.
 template <typename T, int N, class Take>
 __device__ __forceinline__ void best_of_lanes(T (&v)[N], int (&i)[N], int top_k, Take take) {
 #pragma unroll
     for (int e = 0; e < N; ++e)
         if (!(v[e] > -infinity<T>())) { v[e] = -infinity<T>(); i[e] = -1; }
+#pragma unroll
+    for (int n = N - 1; n > 0; --n)
+#pragma unroll
+        for (int e = 0; e < n; ++e) {
+            const bool swap = v[e + 1] > v[e] || (v[e + 1] == v[e] && unsigned(i[e + 1]) < unsigned(i[e]));
+            const T ov = v[e];
+            const int oi = i[e];
+            v[e] = swap ? v[e + 1] : ov; i[e] = swap ? i[e + 1] : oi;
+            v[e + 1] = swap ? ov : v[e + 1]; i[e + 1] = swap ? oi : i[e + 1];
+        }
 #pragma unroll 1
     for (int j = 0; j < top_k; ++j) {
         T best = v[0];
         int at = i[0];
-#pragma unroll
-        for (int e = 1; e < N; ++e)
-            if (v[e] > best || (v[e] == best && unsigned(i[e]) < unsigned(at))) { best = v[e]; at = i[e]; }
         warp_best(best, at);
         if (at < 0) break;
         take(j, best, at);
+        const bool mine = i[0] == at;
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-            if (i[e] == at) { v[e] = -infinity<T>(); i[e] = -1; }
+        for (int e = 0; e < N; ++e) {
+            v[e] = mine ? (e + 1 < N ? v[e + 1 < N ? e + 1 : e] : -infinity<T>()) : v[e];
+            i[e] = mine ? (e + 1 < N ? i[e + 1 < N ? e + 1 : e] : -1) : i[e];
+        }
     }
 }
 
