@@ -507,15 +507,15 @@ __device__ __forceinline__ void best_of_lanes(T (&v)[N], int (&i)[N], int top_k,
     }
 }
 
-// The largest so far as a list of the warp, the j-th of them in lane j.  A class is compared with the last one that counts, and only one above it moves
-// the list: a row of n classes in any order moves it about top_k log(n / top_k) times.
+// The largest so far as a list of the warp, the j-th of them in lane j.  A class is compared with the last one that counts, and only one in front of it
+// moves the list: a row of n classes in any order moves it about top_k log(n / top_k) times.
 template <typename T>
 struct WarpList {
-    T v, last;               // this lane's value; the value of place top_k - 1
-    int i;
+    T v, last;               // this lane's value; that of place top_k - 1
+    int i;                   // (a free place is -infinity and -1, the largest of unsigned indices)
     __device__ __forceinline__ void clear() { v = last = -infinity<T>(); i = -1; }
+    __device__ __forceinline__ unsigned last_i(int top_k) const { return unsigned(__shfl_sync(0xffffffffu, i, top_k - 1)); }
     __device__ __forceinline__ void insert(T x, int c, int top_k) {
-        // (a free place is -infinity and -1, the largest of unsigned indices)
         const unsigned behind = __ballot_sync(0xffffffffu, x > v || (x == v && unsigned(c) < unsigned(i)));
         const T up = __shfl_up_sync(0xffffffffu, v, 1);
         const int up_i = __shfl_up_sync(0xffffffffu, i, 1);
@@ -523,39 +523,56 @@ struct WarpList {
         if (behind && lane >= place) { v = lane == place ? x : up; i = lane == place ? c : up_i; }
         last = __shfl_sync(0xffffffffu, v, top_k - 1);
     }
-    // The classes of a chunk (see load_chunk), all behind those that were offered before, `hi` the lane's largest.  Those below `bound` are known not
-    // to be among the top_k.
-    template <int THREADS, int U>
-    __device__ __forceinline__ void offer(const T (&x)[U], T hi, T bound, long long first, int top_k) {
-        if (!__any_sync(0xffffffffu, hi > last && hi >= bound)) return;
-        const int tid = THREADS == 32 ? int(threadIdx.x % 32) : int(threadIdx.x);
+    // one value of each lane that is in `who`.  (Where they are many most are not in front of the last any more: equal classes, 20000 rows of 500 zeros 361 us
+    // if all are put in, 65 so.)
+    __device__ __forceinline__ void insert_lanes(unsigned who, T x, int c, int top_k) {
+        if (__popc(who) > 8) {
+            const unsigned behind = last_i(top_k);
+            who &= __ballot_sync(0xffffffffu, x > last || (x == last && x > -infinity<T>() && unsigned(c) < behind));
+        }
+        for (; who; who &= who - 1) {
+            const T best = __shfl_sync(0xffffffffu, x, __ffs(who) - 1);
+            if (best >= last) insert(best, __shfl_sync(0xffffffffu, c, __ffs(who) - 1), top_k);
+        }
+    }
+    // The classes of a warp's chunk (see load_chunk) that are not below `bound`, all behind those that were offered before.
+    template <int U>
+    __device__ __forceinline__ void offer_above(const T (&x)[U], T bound, long long first, int top_k) {
         unsigned mine = 0;
 #pragma unroll
         for (int u = 0; u < U; ++u) mine |= x[u] > last && x[u] >= bound ? 1u << u : 0u;
         // one of each lane's at a time
-        while (unsigned who = __ballot_sync(0xffffffffu, mine)) {
-            const int u = __ffs(mine) - 1, c = int(first + class_in_chunk<T, THREADS>(tid, u));
+        while (const unsigned who = __ballot_sync(0xffffffffu, mine)) {
+            const int u = __ffs(mine) - 1, c = int(first + class_in_chunk<T, 32>(threadIdx.x % 32, u));
             T xu = x[0];
 #pragma unroll
             for (int w = 1; w < U; ++w) xu = u == w ? x[w] : xu;
             mine &= mine - 1;
-            for (; who; who &= who - 1) {
-                const T best = __shfl_sync(0xffffffffu, xu, __ffs(who) - 1);
-                if (best >= last) insert(best, __shfl_sync(0xffffffffu, c, __ffs(who) - 1), top_k);
-            }
+            insert_lanes(who, xu, c, top_k);
         }
     }
-    // the first chunk: at least top_k of its classes are not below the k-th largest of the lanes' largest
-    template <int THREADS, int U>
-    __device__ __forceinline__ void start(const T (&x)[U], T hi, long long first, int top_k) {
-        clear();
-        T rest = hi == hi ? hi : -infinity<T>(), bound = rest;             // (a lane all of whose classes are NaN)
+    // the top_k-th largest of the lanes' values, of which none is NaN
+    static __device__ __forceinline__ T bound_of(T rest, int top_k) {
+        T bound = rest;
         for (int j = 0; j < top_k; ++j) {
             bound = warp_max(rest);
             const unsigned who = __ballot_sync(0xffffffffu, rest == bound);
             if (int(threadIdx.x % 32) == __ffs(who) - 1) rest = -infinity<T>();
         }
-        offer<THREADS>(x, hi, bound, first, top_k);
+        return bound;
+    }
+    // the first chunk, `hi` the lane's largest: at least top_k classes are not below the top_k-th largest of these
+    template <int U>
+    __device__ __forceinline__ void start(const T (&x)[U], T hi, long long first, int top_k) {
+        clear();
+        offer_above(x, bound_of(hi == hi ? hi : -infinity<T>(), top_k), first, top_k);           // (a lane all of whose classes are NaN)
+    }
+    // a further one; a bound is worth its search where most lanes have a candidate (classes in rising order: 4096 rows of 2000 187 us without, 38 with)
+    template <int U>
+    __device__ __forceinline__ void offer(const T (&x)[U], T hi, long long first, int top_k) {
+        const unsigned lanes = __ballot_sync(0xffffffffu, hi > last);
+        if (!lanes) return;
+        offer_above(x, __popc(lanes) > 16 ? bound_of(hi > last ? hi : -infinity<T>(), top_k) : -infinity<T>(), first, top_k);
     }
 };
 
@@ -704,11 +721,11 @@ __global__ void __launch_bounds__(32 * kRowWarps) answer_rows(Logits g, Answers<
     WarpList<T> list;
     sums.clear();
     T hi = sums.add(v);
-    if (TOP) list.template start<32>(v, hi, first, g.top_k);
+    if (TOP) list.start(v, hi, first, g.top_k);
     for (first += 32 * U; first < g.classes; first += 32 * U) {
         load_chunk<T, U, 32>(v, x, first, g.classes, lane);
         hi = sums.add(v);
-        if (TOP) list.template offer<32>(v, hi, -infinity<T>(), first, g.top_k);
+        if (TOP) list.offer(v, hi, first, g.top_k);
     }
     write_row<T, TOP>(g, a, q, of_label, labelled, over_warp(sums), list);
 }
@@ -776,6 +793,17 @@ __device__ __forceinline__ void barrier_wait(int id) { asm volatile("bar.sync %0
 template <typename T>
 __device__ __forceinline__ long long share_of(long long first, int tid, int j) { return first + class_in_chunk<T, kStreamThreads>(tid, j * kWide<T>); }
 
+// the first class of thread `tid` in the chunk from `first` on that is `value` (there is one)
+template <typename T>
+__device__ __noinline__ int first_equal(const T* x, T value, long long first, int tid, int classes) {
+#pragma unroll 1
+    for (int u = 0; u < kStreamAhead<T>; ++u) {
+        const long long c = first + class_in_chunk<T, kStreamThreads>(tid, u);
+        if (c >= 0 && c < classes && x[c] == value) return int(c);
+    }
+    return 0x7fffffff;
+}
+
 // classes that may be among the likeliest
 template <typename T>
 struct Above {
@@ -788,9 +816,14 @@ template <typename T>
 __device__ __forceinline__ void pick(WarpList<T>& list, const Streamed<T>& kept, Above<T>& room, const T* x, int begin, int end, int classes, int top_k) {
     const int lane = threadIdx.x % 32, front = in_front(x);
     T rest[kStreamWarps], bound = -infinity<T>();
+    int chunk[kStreamWarps], front_class[kStreamWarps];     // (front_class: the first class that is the thread's largest, where it was looked up)
 #pragma unroll
-    for (int w = 0; w < kStreamWarps; ++w) rest[w] = kept.largest[w * 32 + lane];
-    int picked = -1, n = 0;                                 // (lane j: the j-th thread)
+    for (int w = 0; w < kStreamWarps; ++w) {
+        rest[w] = kept.largest[w * 32 + lane];
+        chunk[w] = kept.chunk[w * 32 + lane];
+        front_class[w] = -1;
+    }
+    int picked = -1, last_chunk = -1, n = 0;                // lane j: the j-th thread; the last chunk of those picked for the same value
 #pragma unroll 1
     for (; n < top_k; ++n) {
         T most = rest[0];
@@ -798,49 +831,51 @@ __device__ __forceinline__ void pick(WarpList<T>& list, const Streamed<T>& kept,
         for (int w = 1; w < kStreamWarps; ++w) most = larger(most, rest[w]);
         const T best = warp_max(most);
         if (best == -infinity<T>()) break;
+        if (best != bound) last_chunk = -1;
         bound = best;
         int equal = 0, place = 0;
+        unsigned soonest = 0xffffffffu;
 #pragma unroll
         for (int w = kStreamWarps - 1; w >= 0; --w) {
-            equal += rest[w] == best;
-            place = rest[w] == best ? w : place;
+            const bool is = rest[w] == best;
+            equal += is;
+            place = is ? w : place;
+            soonest = is ? min(soonest, unsigned(chunk[w])) : soonest;
         }
         unsigned who = __ballot_sync(0xffffffffu, equal > 0);
         if (__reduce_add_sync(0xffffffffu, equal) > 1) {
-            // the first class of equal ones decides
+            // of equal ones the first class decides, which is of those in the first chunk
+            soonest = __reduce_min_sync(0xffffffffu, soonest);
             unsigned at = 0xffffffffu;
-#pragma unroll 1
-            for (int w = 0; w < kStreamWarps; ++w) {
-                T r = rest[0];
 #pragma unroll
-                for (int i = 1; i < kStreamWarps; ++i) r = i == w ? rest[i] : r;
-                if (r != best) continue;
-                const int tid = w * 32 + lane;
-#pragma unroll 1
-                for (int u = kStreamAhead<T> - 1; u >= 0; --u) {
-                    const long long c = (long long)kept.chunk[tid] * kStreamChunk<T> - front + class_in_chunk<T, kStreamThreads>(tid, u);
-                    if (c >= 0 && c < classes && x[c] == best && unsigned(c) < at) { at = unsigned(c); place = w; }
+            for (int w = 0; w < kStreamWarps; ++w) {
+                if (rest[w] == best && unsigned(chunk[w]) == soonest) {
+                    if (front_class[w] < 0) front_class[w] = first_equal(x, best, (long long)chunk[w] * kStreamChunk<T> - front, w * 32 + lane, classes);
+                    if (unsigned(front_class[w]) < at) { at = unsigned(front_class[w]); place = w; }
                 }
             }
             who = __ballot_sync(0xffffffffu, at == __reduce_min_sync(0xffffffffu, at));
         }
         const int from = __ffs(who) - 1, tid = __shfl_sync(0xffffffffu, place * 32 + lane, from);
         if (lane == n) picked = tid;
+        last_chunk = max(last_chunk, kept.chunk[tid]);
 #pragma unroll
         for (int w = 0; w < kStreamWarps; ++w)
             if (w * 32 + lane == tid) rest[w] = -infinity<T>();
     }
     if (n < top_k) bound = -infinity<T>();                  // (all of the classes that can be are theirs)
-    // First the chunks in which their largest came up, then all others of a thread whose second largest is not below the bound.  The classes that are
-    // not are hardly ever more than the lanes of a warp: the best of these again and again; more, equal ones, are put in one by one.  (Loops
-    // that are not unrolled: the code runs once a row, and would wait for its instructions.)
+    // First the chunks in which their largest came up, then all others of a thread whose second largest is above the bound, or those up to last_chunk where it is
+    // the bound: of equal classes, those picked come before what is behind.  The classes that are not below the bound are hardly ever more
+    // than the lanes of a warp: the best of these again and again; more, equal ones, are put in one by one.  (Loops that are not unrolled:
+    // the code runs once a row, and would wait for its instructions.)
     list.clear();
     int count = 0;
-    const bool more = lane < n && kept.second[picked] >= bound && kept.second[picked] > -infinity<T>();
-    unsigned passes = __ballot_sync(0xffffffffu, more);
+    const T second = lane < n ? kept.second[picked] : -infinity<T>();
+    const unsigned all = __ballot_sync(0xffffffffu, second > bound);
+    unsigned passes = all | __ballot_sync(0xffffffffu, second == bound && second > -infinity<T>());
 #pragma unroll 1
     for (int pass = -1;;) {
-        const int total = pass < 0 ? 4 * n : 4 * (end - begin);
+        const int total = pass < 0 ? 4 * n : 4 * ((all >> pass & 1 ? end : min(end, last_chunk + 1)) - begin);
 #pragma unroll 1
         for (int from = 0; from < total; from += 32) {
             const int at = from + lane, tid = __shfl_sync(0xffffffffu, picked, pass < 0 ? min(at, total - 1) / 4 : pass), first = kept.chunk[tid], chunk = pass < 0 ? first : begin + at / 4;
@@ -852,7 +887,7 @@ __device__ __forceinline__ void pick(WarpList<T>& list, const Streamed<T>& kept,
 #pragma unroll
             for (int e = 0; e < kWide<T>; ++e) mine |= v[e] > -infinity<T>() && v[e] >= bound ? 1u << e : 0u;
 #pragma unroll 1
-            while (unsigned who = __ballot_sync(0xffffffffu, mine)) {
+            while (const unsigned who = __ballot_sync(0xffffffffu, mine)) {
                 const int e = __ffs(mine) - 1, left = 32 - count, to = count + __popc(who & ((1u << lane) - 1)), c = int(c0) + e;
                 T w = v[0];
 #pragma unroll
@@ -860,13 +895,8 @@ __device__ __forceinline__ void pick(WarpList<T>& list, const Streamed<T>& kept,
                 if (mine && to < 32) { room.top[to] = w; room.top_index[to] = c; }
                 mine &= mine - 1;
                 count += __popc(who);
-                if (count > 32) {
-                    who = left <= 0 ? who : who & ~((2u << __fns(who, 0, left)) - 1);
-                    const unsigned last_i = unsigned(__shfl_sync(0xffffffffu, list.i, top_k - 1));
-#pragma unroll 1
-                    for (who &= __ballot_sync(0xffffffffu, w > list.last || (w == list.last && unsigned(c) < last_i)); who; who &= who - 1)
-                        list.insert(__shfl_sync(0xffffffffu, w, __ffs(who) - 1), __shfl_sync(0xffffffffu, c, __ffs(who) - 1), top_k);
-                }
+                // (what has no room)
+                if (count > 32) list.insert_lanes(left <= 0 ? who : who & ~((2u << __fns(who, 0, left)) - 1), w, c, top_k);
             }
         }
         if (!passes) break;
@@ -877,8 +907,7 @@ __device__ __forceinline__ void pick(WarpList<T>& list, const Streamed<T>& kept,
     T mine = lane < count ? room.top[lane] : -infinity<T>();
     int mine_i = lane < count ? room.top_index[lane] : -1;
     if (count > 32) {
-#pragma unroll 1
-        for (int j = 0; j < 32; ++j) list.insert(__shfl_sync(0xffffffffu, mine, j), __shfl_sync(0xffffffffu, mine_i, j), top_k);
+        list.insert_lanes(0xffffffffu, mine, mine_i, top_k);
     } else {
 #pragma unroll 1
         for (int j = 0; j < top_k; ++j) {
