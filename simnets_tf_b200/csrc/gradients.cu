@@ -42,12 +42,12 @@ struct Vector {
     T v[kWidth];
 };
 
-// [begin, end) of an item inside its tensor; begin may be below 0 and end beyond its last value
+// an item of a tensor: the values from `begin` on, which may be below 0, and there may be fewer than an item has
 template <typename T>
 struct Item {
     const T* in;
     T* out;
-    long long begin, end, values;
+    long long begin, values;
     bool aligned;                                           // the 16-byte pieces of `in` from `begin` on are pieces of `out` as well
     template <int N>
     __device__ __forceinline__ Item(const Table<N>& t, int item) {
@@ -61,7 +61,6 @@ struct Item {
         values = t.values[lo];
         const int skip = int(reinterpret_cast<uintptr_t>(in) % 16 / sizeof(T));
         begin = (long long)(item - t.first[lo]) * (kItemBytes / sizeof(T)) - skip;
-        end = begin + kItemBytes / (long long)sizeof(T);
         aligned = (reinterpret_cast<uintptr_t>(in) - reinterpret_cast<uintptr_t>(out)) % 16 == 0;
     }
     __device__ __forceinline__ Vector<T> load(long long at) const {
@@ -228,7 +227,8 @@ long long items_of(const void* in, long long values, int size) {
     return values > 0 ? (skip + values + kItemBytes / size - 1) / (kItemBytes / size) : 0;
 }
 int grid_of(long long items, int a_multiprocessor) { return int(std::min<long long>(items, (long long)a_multiprocessor * device_sm_count())); }
-// body(dtype, table, items, last) for every launch
+
+// body(dtype, table) for every launch
 template <int N, class Body>
 cudaError_t each_table(const Call& c, Body body) {
     Table<N> t;

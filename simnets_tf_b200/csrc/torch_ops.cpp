@@ -882,7 +882,8 @@ bool likelihood_desc(const Tensor& x, int64_t axis, int64_t top_k, simnets_likel
 struct Likelihood { Tensor label, entropy, top_index, top, stats; };
 
 // logits as the library reads them
-Tensor likelihood_logits(const Tensor& x, int64_t axis, int64_t top_k, simnets_likelihood_desc* d) {
+Tensor likelihood_logits(const Tensor& given, int64_t axis, int64_t top_k, simnets_likelihood_desc* d) {
+    const Tensor x = given.is_neg() ? given.resolve_neg() : given;              // (a view that stands for the negated values)
     if (likelihood_desc(x, axis, top_k, d)) return x;
     const Tensor dense = x.contiguous();
     likelihood_desc(dense, axis, top_k, d);
@@ -1103,7 +1104,7 @@ Tensor gradients_impl(const py::object& given_in, int64_t order, bool scaled, do
         const Tensor* const p = given.tensors[i];
         if (!p) continue;
         Tensor copy;
-        if (!p->is_non_overlapping_and_dense()) copies.push_back(copy = p->contiguous());
+        if (!p->is_non_overlapping_and_dense() || p->is_neg()) copies.push_back(copy = p->is_neg() ? p->resolve_neg().contiguous() : p->contiguous());
         const Tensor& in = copy.defined() ? copy : *p;
         dtypes.push_back(in.scalar_type() == at::kDouble ? SIMNETS_F64 : SIMNETS_F32);
         counts.push_back(in.numel());
@@ -1111,7 +1112,7 @@ Tensor gradients_impl(const py::object& given_in, int64_t order, bool scaled, do
         if (!scaled) continue;
         const Tensor& to = out ? *out->tensors[i] : *p;
         const size_t bytes = in.nbytes();
-        void* dst = to.is_non_overlapping_and_dense() && (to.strides() == in.strides() || in.numel() < 2) ? ptr(to) : nullptr;
+        void* dst = to.is_non_overlapping_and_dense() && !to.is_neg() && (to.strides() == in.strides() || in.numel() < 2) ? ptr(to) : nullptr;
         if (!dst) {
             if (!copy.defined()) copies.push_back(copy = at::empty_strided(in.sizes(), in.strides(), in.options()));
             back.emplace_back(&to, copies.size() - 1);

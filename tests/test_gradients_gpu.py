@@ -227,3 +227,26 @@ def test_a_bucket():
     assert abs(float(bucket.norm()) / want - 1) < 1e-6 and float(bucket.norm(order=INF)) == 4.0
     assert abs(float(bucket.clip(1.0)) / want - 1) < 1e-6
     assert abs(float(a.grad[0, 0]) * want / 2 - 1) < 1e-6 and abs(float(b.grad[0]) * want / 4 - 1) < 1e-6
+
+
+def test_views_that_stand_for_negated_values():
+    z = torch.randn(5000, dtype=torch.complex64, device="cuda")
+    x, want = z.conj().imag, (-z.imag).contiguous()
+    assert x.is_neg()
+    out = torch.zeros(5000, device="cuda")
+    n = clip_gradients([x], 1.0, out=[out])
+    clip_gradients([want], 1.0)
+    assert bool((out == want).all()) and bool(n == gradient_norm([(-z.imag).contiguous()]))
+    clip_gradients([x], 1.0)
+    assert bool((x == want).all()) and bool((z.imag == -want).all())
+
+
+def test_nothing_to_take_the_norm_of():
+    """Through Python tensors without values, through the C entry point none at all."""
+    assert float(gradient_norm([torch.zeros(0, device="cuda"), torch.zeros(3, 0, device="cuda")])) == 0.0
+    assert float(clip_gradients([torch.zeros(0, device="cuda", dtype=torch.float64)], 1.0)) == 0.0
+    lib = _lib.lib()
+    size = lib.simnets_gradient_norm_workspace_bytes(0)
+    ws, norm = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.full((3,), 7.0, device="cuda")
+    _lib.check(lib.simnets_gradient_norm(2, 0, None, None, None, norm.data_ptr() + 4, ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream))
+    assert norm.tolist() == [7.0, 0.0, 7.0]

@@ -309,3 +309,60 @@ def test_memory_in_front_of_and_behind_the_outputs_stays():
         assert bool((t[:pad] == 77).all()) and bool((t[-pad:] == 77).all()), n
     got = log_probabilities(dev, lab, top, True)
     assert bool((bufs["label"][pad:-pad].view(b, p) == got.label).all()) and bool((bufs["top"][pad:-pad].view(b, top, p) == got.top).all())
+
+
+def test_what_is_refused():
+    x = torch.zeros(3, 7, 5, device="cuda")
+    for bad in (torch.zeros(3, 7, dtype=torch.int64, device="cuda"), torch.zeros(3, 5, 1, dtype=torch.int64, device="cuda"), torch.zeros(15, dtype=torch.int64, device="cuda")):
+        with pytest.raises(ValueError, match="labels must have shape"):
+            log_probabilities(x, bad)
+    with pytest.raises(TypeError, match="int64"):
+        log_probabilities(x, torch.zeros(3, 5, dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError, match="labels must live"):
+        log_probabilities(x, torch.zeros(3, 5, dtype=torch.int64))
+    with pytest.raises(TypeError, match="float32 and float64"):
+        log_probabilities(x.half())
+    with pytest.raises(ValueError, match="at most the number of classes"):
+        log_probabilities(x, top_k=8)
+
+
+def test_autograd_sees_what_changes_between_the_passes():
+    for change in ("logits", "labels", "index"):
+        x, labels = torch.randn(3, 9, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+        leaf = x.clone().requires_grad_()
+        mid = leaf * 1.0
+        got = log_probabilities(mid, labels, 2)
+        with torch.no_grad():
+            dict(logits=mid, labels=labels, index=got.top_index)[change].fill_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            (got.label.sum() + got.top.sum()).backward()
+
+
+def test_kept_graphs_shared_and_broadcast_logits():
+    x = torch.randn(1, 40, 6, device="cuda", dtype=torch.float64, requires_grad=True)
+    wide = x.expand(4, 40, 6)
+    labels = torch.randint(0, 40, (4, 6), device="cuda")
+    got = log_probabilities(wide, labels, entropy=True)
+    total = got.label.sum() - 0.3 * got.entropy.sum()
+    a, = torch.autograd.grad(total, x, retain_graph=True)
+    b, = torch.autograd.grad(total, x)
+    assert bool((a == b).all())
+    r = plain.Rows(rows_of(x.detach().expand(4, 40, 6).cpu().numpy(), 1), labels.cpu().numpy().reshape(-1), 0, 64)
+    want, off = r.gradient(np.ones(24), np.full(24, -0.3))
+    want, off = want.reshape(4, 6, 40).sum(0), off.reshape(4, 6, 40).sum(0)
+    # a sum of four, each within its bound, and three additions of numbers below 2.5 (the label's 1 - p and 0.3 p (log p + H), of which the latter is
+    # at most 0.3 (1 / e + log 40) = 1.2), whose sums are below four times that
+    assert (abs(rows_of(a.cpu().numpy(), 1) - want) <= off + 3 * 4 * 2.5 * np.finfo(np.float64).eps).all()
+    # two calls on the same logits: their gradients add up
+    y = torch.randn(5, 30, device="cuda", requires_grad=True)
+    one, = torch.autograd.grad(log_probabilities(y, entropy=True).entropy.sum(), y)
+    two, = torch.autograd.grad(log_probabilities(y, entropy=True).entropy.sum() + log_probabilities(y, entropy=True).entropy.sum(), y)
+    assert bool((two == 2 * one).all())
+
+
+def test_views_that_stand_for_negated_values():
+    z = torch.randn(4, 300, dtype=torch.complex64, device="cuda")
+    x = z.conj().imag
+    assert x.is_neg()
+    a, b = log_probabilities(x, top_k=3, entropy=True), log_probabilities((-z.imag).contiguous(), top_k=3, entropy=True)
+    assert all(u is v is None or bool((u == v).all()) for u, v in zip(a, b))
