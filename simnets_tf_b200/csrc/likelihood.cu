@@ -113,7 +113,8 @@ struct Answer {
         nothing = a.m == -infinity<T>() && a.s == T(0);
         m = a.m;
         log_s = log_of(a.s);
-        entropy = nothing ? T(0) : log_s - Unit<T>::nats() * (a.t / a.s);
+        entropy = log_s - Unit<T>::nats() * (a.t / a.s);
+        if (nothing || entropy < T(0)) entropy = T(0);                // (of one class that is nearly sure, by rounding)
     }
     __device__ __forceinline__ T of(T x) const { return nothing ? -infinity<T>() : (x - m) - log_s; }
 };

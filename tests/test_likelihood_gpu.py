@@ -311,6 +311,17 @@ def test_memory_in_front_of_and_behind_the_outputs_stays():
     assert bool((bufs["label"][pad:-pad].view(b, p) == got.label).all()) and bool((bufs["top"][pad:-pad].view(b, top, p) == got.top).all())
 
 
+@pytest.mark.parametrize("kind", KINDS, ids=["f32", "f64"])
+def test_positions_that_are_nearly_sure(kind):
+    """Log probabilities are at most 0 and entropies at least, whatever rounding does."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for shape in ((4000, 10), (300, 700), (3, 20000), (5, 30, 500)):
+        x = torch.randn(shape, generator=gen, device="cuda", dtype=kind)
+        x[:, 0] += torch.linspace(0, 40, x[:, 0].numel(), device="cuda", dtype=kind).view(x[:, 0].shape)
+        got = log_probabilities(x, top_k=2, entropy=True)
+        assert bool((got.entropy >= 0).all()) and bool((got.top <= 0).all())
+
+
 def test_what_is_refused():
     x = torch.zeros(3, 7, 5, device="cuda")
     for bad in (torch.zeros(3, 7, dtype=torch.int64, device="cuda"), torch.zeros(3, 5, 1, dtype=torch.int64, device="cuda"), torch.zeros(15, dtype=torch.int64, device="cuda")):
