@@ -1123,6 +1123,11 @@ Tensor gradients_impl(const py::object& given_in, int64_t order, bool scaled, do
         const uintptr_t a = reinterpret_cast<uintptr_t>(dst), b = reinterpret_cast<uintptr_t>(from.back());
         ranges.push_back({a, a + bytes, true});
         if (a != b) ranges.push_back({b, b + bytes, false});
+        // (those that are copied may lie between one another: their first elements alone)
+        if (const uintptr_t to_at = reinterpret_cast<uintptr_t>(ptr(to)), in_at = reinterpret_cast<uintptr_t>(ptr(*p)); to_at != a || in_at != b) {
+            if (to_at != a) ranges.push_back({to_at, to_at + in.element_size(), true});
+            if (in_at != b && in_at != to_at) ranges.push_back({in_at, in_at + in.element_size(), false});
+        }
     }
     if (scaled) {
         refuse_overlaps(ranges);

@@ -134,6 +134,21 @@ def test_tensors_that_are_not_dense():
     assert abs(float(gradient_norm([e])) - math.sqrt(160)) < 1e-5           # (every element counts)
 
 
+def test_a_tensor_that_is_not_dense_is_given_once_too():
+    a = torch.ones(10, 6, device="cuda")
+    for bad in ([a[:, :3], a[:, :3]], [a[:, ::2], a], [a[:, :3], a[:4, :2]], [a[3, 2:], a[3:, 2:4]]):
+        with pytest.raises(ValueError, match="share memory"):
+            clip_gradients(bad, 1.0)
+    to = torch.zeros(10, 6, device="cuda")
+    with pytest.raises(ValueError, match="share memory"):
+        clip_gradients([a[:, :3], a[:, 3:]], 1.0, out=[to[:, :3], to[:, :3]])
+    assert bool((a == 1).all()) and bool((to == 0).all())
+    assert abs(float(gradient_norm([a[:, :3], a[:, :3]])) - math.sqrt(60)) < 1e-5
+    # into itself, and into the other's place
+    n = clip_gradients([a[:, :3], a[:, 3:]], 1.0, out=[a[:, :3], to[:, 3:]])
+    assert torch.allclose(a[:, :3], 1 / n, rtol=1e-6, atol=0) and bool((a[:, 3:] == 1).all()) and torch.allclose(to[:, 3:], 1 / n, rtol=1e-6, atol=0)
+
+
 def test_what_is_refused():
     a = torch.ones(10, device="cuda")
     for bad in ([a, a], [a, a[2:5]], [a[:6], a[5:]]):
