@@ -30,6 +30,12 @@ def require_cuda(*tensors):
     return dev
 
 
+def plain(t):
+    """`t` with its values in memory one after the other (a view can stand for the negated values of its memory, and contiguous() leaves
+    it one)."""
+    return t.resolve_neg().contiguous()
+
+
 def stream_ptr(dev):
     return torch.cuda.current_stream(dev).cuda_stream
 

@@ -113,6 +113,9 @@ void refuse_tangents(std::initializer_list<const Tensor*> inputs) {
             throw py::error_already_set();
         }
 }
+// A tensor whose values lie in memory one after the other.  (A view can stand for the negated values of its memory, and contiguous() leaves it one: logits
+// that are the imaginary part of a conjugate, say, and the gradient that the conjugate's backward pass hands to a node.)
+Tensor plain(const Tensor& t) { return (t.is_neg() ? t.resolve_neg() : t).contiguous(); }
 inline cudaStream_t stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 inline void* ptr(const Tensor& t) { return t.data_ptr(); }
 
@@ -219,7 +222,7 @@ std::pair<Tensor, Tensor> mex_forward_impl(const MexPlan& p, const Tensor& x_in,
     require_cuda_all(x_in, off_in);
     p.check_input(x_in);
     p.check_offsets(off_in);
-    const Tensor x = x_in.contiguous(), off = off_in.contiguous();
+    const Tensor x = plain(x_in), off = plain(off_in);
     const c10::cuda::CUDAGuard guard(x.device());
     const cudaStream_t s = stream_of(x);
     const simnets_mex_desc d = p.with(flags);
@@ -256,7 +259,7 @@ std::pair<Tensor, Tensor> mex_forward_pool2(const MexPlanPtr& p, const Tensor& x
 
 Tensor grad_target(const Tensor& like, const OptTensor& out) {
     if (!out) return at::empty(like.sizes(), like.options());
-    TORCH_CHECK(out->is_contiguous() && out->numel() == like.numel() && out->scalar_type() == like.scalar_type(), "out: need a contiguous tensor of the gradient's size and dtype");
+    TORCH_CHECK(out->is_contiguous() && !out->is_neg() && out->numel() == like.numel() && out->scalar_type() == like.scalar_type(), "out: need a contiguous tensor of the gradient's size and dtype");
     return *out;
 }
 
@@ -268,7 +271,7 @@ std::pair<Tensor, Tensor> mex_grads(const MexPlan& p, const Tensor& x_in, const 
     p.check_offsets(off_in);
     p.check_dy(dy_in, pooled);
     flags |= (pooled ? SIMNETS_FLAG_MEX_DY_POOLED2 : 0u) | (primed ? SIMNETS_FLAG_MEX_WORKSPACE_PRIMED : 0u);
-    const Tensor x = x_in.contiguous(), off = off_in.contiguous(), y = y_in.contiguous(), dy = dy_in.contiguous();
+    const Tensor x = plain(x_in), off = plain(off_in), y = plain(y_in), dy = plain(dy_in);
     const c10::cuda::CUDAGuard guard(x.device());
     const cudaStream_t s = stream_of(x);
     const simnets_mex_desc d = p.with(flags);
@@ -362,7 +365,7 @@ Tensor sim_workspace(const simnets_sim_desc& d, const Tensor& x) { return scratc
 Tensor sim_forward(const SimPlanPtr& p, const Tensor& x_in, const Tensor& t_in, const Tensor& w_in, uint32_t flags, uint64_t ch_max, uint64_t ch_min) {
     require_cuda_all(x_in, t_in, w_in);
     p->check_tensors(x_in, t_in, w_in);
-    const Tensor x = x_in.contiguous(), t = t_in.contiguous(), w = w_in.contiguous();
+    const Tensor x = plain(x_in), t = plain(t_in), w = plain(w_in);
     const c10::cuda::CUDAGuard guard(x.device());
     const cudaStream_t s = stream_of(x);
     const simnets_sim_desc d = p->with(flags);
@@ -381,7 +384,7 @@ Tensor sim_input_grad(const SimPlanPtr& p, const Tensor& x_in, const Tensor& t_i
     require_cuda_all(x_in, t_in, w_in, dy_in);
     p->check_tensors(x_in, t_in, w_in);
     p->check_dy(dy_in);
-    const Tensor x = x_in.contiguous(), t = t_in.contiguous(), w = w_in.contiguous(), dy = dy_in.contiguous();
+    const Tensor x = plain(x_in), t = plain(t_in), w = plain(w_in), dy = plain(dy_in);
     const c10::cuda::CUDAGuard guard(x.device());
     const cudaStream_t s = stream_of(x);
     const simnets_sim_desc d = p->with(flags);
@@ -398,7 +401,7 @@ std::pair<Tensor, Tensor> sim_params_grad(const SimPlanPtr& p, const Tensor& x_i
     require_cuda_all(x_in, t_in, w_in, dy_in);
     p->check_tensors(x_in, t_in, w_in);
     p->check_dy(dy_in);
-    const Tensor x = x_in.contiguous(), t = t_in.contiguous(), w = w_in.contiguous(), dy = dy_in.contiguous();
+    const Tensor x = plain(x_in), t = plain(t_in), w = plain(w_in), dy = plain(dy_in);
     const c10::cuda::CUDAGuard guard(x.device());
     const cudaStream_t s = stream_of(x);
     const simnets_sim_desc d = p->with(flags);
@@ -464,7 +467,7 @@ OptTensor mixture_statistics(const SimPlanPtr& p, const Tensor& x_in, const Tens
     p->check_tensors(x_in, means_in, covs_in);
     const size_t n = simnets_mixture_workspace_bytes(&p->d);
     if (n == 0) return std::nullopt;
-    const Tensor x = x_in.contiguous(), means = means_in.contiguous(), covs = covs_in.contiguous();
+    const Tensor x = plain(x_in), means = plain(means_in), covs = plain(covs_in);
     const c10::cuda::CUDAGuard guard(x.device());
     Tensor stats = at::empty({2 * means.numel() + means.size(0)}, means.options());
     const Tensor ws = scratch(x, n);
@@ -474,7 +477,7 @@ OptTensor mixture_statistics(const SimPlanPtr& p, const Tensor& x_in, const Tens
 
 std::pair<Tensor, Tensor> mixture_parameters(const Tensor& stats, const Tensor& means_in, double min_var) {
     require_cuda_all(stats, means_in);
-    const Tensor means = means_in.contiguous();
+    const Tensor means = plain(means_in);
     TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == 2 * means.numel() + means.size(0), "stats do not belong to these means");
     const c10::cuda::CUDAGuard guard(means.device());
     Tensor new_means = at::empty(means.sizes(), means.options()), new_covs = at::empty(means.sizes(), means.options());
@@ -491,7 +494,7 @@ Kept checkpoint_pack(const Tensor& x_in, int64_t group) {
     require_cuda_all(x_in);
     refuse_tangents({&x_in});
     const at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor x = x_in.contiguous();
+    const Tensor x = plain(x_in);
     const c10::cuda::CUDAGuard guard(x.device());
     Kept kept{at::empty({x.numel()}, x.options().dtype(at::kByte)), at::empty({simnets_checkpoint_groups(x.numel(), int32_t(group)), 2}, x.options())};
     check(simnets_checkpoint_pack(x.scalar_type() == at::kDouble, x.numel(), int32_t(group), ptr(x), ptr(kept.codes), ptr(kept.ranges), stream_of(x)));
@@ -523,7 +526,7 @@ std::pair<Tensor, Tensor> mex_checkpoint_grads(const MexPlan& p, const Tensor& c
     const Tensor ranges = reinterpret_cast<uintptr_t>(ranges_in.data_ptr()) % 8 ? ranges_in.clone() : ranges_in;        // (read as pairs)
     p.check_offsets(off_in);
     p.check_dy(dy_in, pooled);
-    const Tensor off = off_in.contiguous(), dy = dy_in.contiguous();
+    const Tensor off = plain(off_in), dy = plain(dy_in);
     const c10::cuda::CUDAGuard guard(ranges.device());
     const cudaStream_t s = stream_of(ranges);
     const simnets_mex_desc d = p.with(flags | (pooled ? SIMNETS_FLAG_MEX_DY_POOLED2 : 0u));
@@ -550,7 +553,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> sim_checkpoint_grads(const SimPlan& 
     if ((ranges.scalar_type() == at::kDouble) != (p.d.dtype == SIMNETS_F64)) throw py::type_error("input does not have the planned dtype");
     p.check_params(t_in, w_in);
     p.check_dy(dy_in);
-    const Tensor t = t_in.contiguous(), w = w_in.contiguous(), dy = dy_in.contiguous();
+    const Tensor t = plain(t_in), w = plain(w_in), dy = plain(dy_in);
     const c10::cuda::CUDAGuard guard(ranges.device());
     const cudaStream_t s = stream_of(ranges);
     const simnets_sim_desc d = p.with(flags);
@@ -718,7 +721,7 @@ OptTensor per_component(const Tensor& scores, const OptTensor& v, const char* wh
     if (!v) return std::nullopt;
     require_cuda(scores, *v);
     if (v->dim() != 1 || v->size(0) != scores.size(1)) throw std::invalid_argument(std::string(what) + " must hold one value per component");
-    return v->contiguous();
+    return plain(*v);
 }
 
 struct Routed { Tensor index, weights, dense, load, mass; };
@@ -726,7 +729,7 @@ struct Routed { Tensor index, weights, dense, load, mass; };
 Routed route_impl(const Tensor& scores_in, const OptTensor& prior_in, const OptTensor& bias_in, const simnets_route_desc& d, bool dense) {
     require_cuda_all(scores_in);
     const OptTensor prior = per_component(scores_in, prior_in, "prior"), bias = per_component(scores_in, bias_in, "bias");
-    const Tensor scores = scores_in.contiguous();
+    const Tensor scores = plain(scores_in);
     const c10::cuda::CUDAGuard guard(scores.device());
     const size_t need = simnets_route_workspace_bytes(&d);
     std::vector<int64_t> shape = scores.sizes().vec();
@@ -757,7 +760,7 @@ struct RouteNode : torch::autograd::Node {
         std::lock_guard<std::mutex> lock(mutex_);
         variable_list out(1);
         if (!grads[0].defined() || !task_should_compute_output(0)) return out;
-        const Tensor iv = index.unpack(), wv = weights.unpack(shared_from_this()), sv = d.sigmoid ? scores.unpack().contiguous() : Tensor(), g = grads[0].contiguous();
+        const Tensor iv = index.unpack(), wv = weights.unpack(shared_from_this()), sv = d.sigmoid ? plain(scores.unpack()) : Tensor(), g = plain(grads[0]);
         require_cuda_all(wv, g);
         if (g.sizes() != wv.sizes()) throw std::invalid_argument("route: gradient must have shape " + shape_text(wv.sizes()) + ", got " + shape_text(g.sizes()));
         const c10::cuda::CUDAGuard guard(wv.device());
@@ -812,7 +815,7 @@ std::pair<Tensor, Tensor> xent_with_grad(const Tensor& logits_in, const Tensor& 
     if (!labels_in.is_cuda() || labels_in.device() != logits_in.device()) throw std::runtime_error("labels must live on the device of the logits");
     if (logits_in.scalar_type() != at::kFloat || labels_in.scalar_type() != at::kLong || logits_in.dim() != 2 || labels_in.dim() != 1 || labels_in.size(0) != logits_in.size(0))
         throw std::invalid_argument("logits must be float32 [batch, classes] and labels int64 [batch]");
-    const Tensor logits = logits_in.contiguous(), labels = labels_in.contiguous();
+    const Tensor logits = plain(logits_in), labels = plain(labels_in);
     const c10::cuda::CUDAGuard guard(logits.device());
     Tensor loss = at::empty({}, logits.options()), dlogits = at::empty(logits.sizes(), logits.options());
     const Tensor ws = scratch(logits, std::max<size_t>(simnets_softmax_cross_entropy_workspace_bytes(int32_t(logits.size(0))), 256));
@@ -883,7 +886,7 @@ struct Likelihood { Tensor label, entropy, top_index, top, stats; };
 
 // logits as the library reads them
 Tensor likelihood_logits(const Tensor& given, int64_t axis, int64_t top_k, simnets_likelihood_desc* d) {
-    const Tensor x = given.is_neg() ? given.resolve_neg() : given;              // (a view that stands for the negated values)
+    const Tensor x = given.is_neg() ? given.resolve_neg() : given;
     if (likelihood_desc(x, axis, top_k, d)) return x;
     const Tensor dense = x.contiguous();
     likelihood_desc(dense, axis, top_k, d);
@@ -910,7 +913,7 @@ Likelihood likelihood_impl(const Tensor& logits_in, const OptTensor& labels_in, 
     const c10::cuda::CUDAGuard guard(logits_in.device());
     const Tensor logits = likelihood_logits(logits_in, axis, top_k, &d);
     OptTensor labels;
-    if (labels_in) labels = labels_in->contiguous();
+    if (labels_in) labels = plain(*labels_in);
     std::vector<int64_t> shape = logits.sizes().vec(), top_shape = shape;
     shape.erase(shape.begin() + axis);
     top_shape[axis] = top_k;
@@ -941,7 +944,7 @@ struct LikelihoodNode : torch::autograd::Node {
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
         variable_list out(1);
-        auto given = [&](int i) { return i >= 0 && grads[i].defined() ? OptTensor(grads[i].contiguous()) : OptTensor(); };
+        auto given = [&](int i) { return i >= 0 && grads[i].defined() ? OptTensor(plain(grads[i])) : OptTensor(); };
         const OptTensor gl = given(label_at), ge = given(entropy_at), gt = given(top_at);
         if ((!gl && !ge && !gt) || !task_should_compute_output(0)) return out;
         const Tensor xv = logits.unpack(), lv = labels.unpack(), sv = stats.unpack(), iv = top_index.unpack();
@@ -995,7 +998,7 @@ LikelihoodOut log_probabilities_apply(const Tensor& logits, const OptTensor& lab
         node->axis = axis;
         node->top_k = top_k;
         node->logits = SavedVariable(logits, false);
-        if (labels) node->labels = SavedVariable(labels->contiguous(), false);
+        if (labels) node->labels = SavedVariable(plain(*labels), false);
         node->stats = SavedVariable(r.stats, false);
         if (r.top_index.defined()) node->top_index = SavedVariable(r.top_index, false);
         int n = 0;
@@ -1104,7 +1107,7 @@ Tensor gradients_impl(const py::object& given_in, int64_t order, bool scaled, do
         const Tensor* const p = given.tensors[i];
         if (!p) continue;
         Tensor copy;
-        if (!p->is_non_overlapping_and_dense() || p->is_neg()) copies.push_back(copy = p->is_neg() ? p->resolve_neg().contiguous() : p->contiguous());
+        if (!p->is_non_overlapping_and_dense() || p->is_neg()) copies.push_back(copy = plain(*p));
         const Tensor& in = copy.defined() ? copy : *p;
         dtypes.push_back(in.scalar_type() == at::kDouble ? SIMNETS_F64 : SIMNETS_F32);
         counts.push_back(in.numel());

@@ -213,8 +213,8 @@ class _NormalizeOffsets(torch.autograd.Function):
     @staticmethod
     def forward(ctx, offsets):
         from . import _lib
-        from ._torch_glue import stream_ptr
-        off = offsets.contiguous()
+        from ._torch_glue import plain, stream_ptr
+        off = plain(offsets)
         rows, k = off.shape[0] * off.shape[1], int(math.prod(off.shape[2:]))
         out = torch.empty_like(off)
         with torch.cuda.device(off.device):
@@ -225,9 +225,9 @@ class _NormalizeOffsets(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         from . import _lib
-        from ._torch_glue import stream_ptr
+        from ._torch_glue import plain, stream_ptr
         off, = ctx.saved_tensors
-        grad = grad.contiguous()
+        grad = plain(grad)
         rows, k = off.shape[0] * off.shape[1], int(math.prod(off.shape[2:]))
         doff = torch.empty_like(off)
         with torch.cuda.device(off.device):

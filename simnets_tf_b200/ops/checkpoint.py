@@ -45,7 +45,7 @@ class Checkpoint(object):
                              % (self.shape, self.group, n, -(-n // self.group), codes.numel(), tuple(ranges.shape)))
         if codes.device != ranges.device:
             raise RuntimeError("codes and ranges must be on the same device")
-        self.codes, self.ranges = codes.contiguous(), ranges.contiguous()
+        self.codes, self.ranges = _torch_glue.plain(codes), _torch_glue.plain(ranges)
 
     @classmethod
     def _packed(cls, codes, ranges, shape, group):

@@ -150,7 +150,7 @@ def mex_backward(input, offsets, orig_output, output_grad, num_instances, flags=
 def sum_pool2x2(y):
     """2x2 / stride-2 sum pooling of a float32 CUDA tensor [B, C, H, W] with even H and W (the library's kernel)."""
     dev = require_cuda(y)
-    y = y.contiguous()
+    y = _torch_glue.plain(y)
     out = torch.empty(y.shape[:2] + (y.shape[2] // 2, y.shape[3] // 2), dtype=y.dtype, device=dev)
     with torch.cuda.device(dev):
         _lib.check(_lib.lib().simnets_sum_pool2x2_forward(y.shape[0] * y.shape[1], y.shape[2], y.shape[3], y.data_ptr(), out.data_ptr(),
