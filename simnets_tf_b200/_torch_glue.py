@@ -32,7 +32,11 @@ def require_cuda(*tensors):
 
 def plain(t):
     """`t` with its values in memory one after the other (a view can stand for the negated values of its memory, and contiguous() leaves
-    it one)."""
+    it one; zeros can have no memory)."""
+    if t._is_zerotensor():
+        return t.clone()
+    if t.numel() and not t.data_ptr():
+        raise RuntimeError("a tensor of %d values has no memory" % t.numel())
     return t.resolve_neg().contiguous()
 
 

@@ -113,11 +113,25 @@ void refuse_tangents(std::initializer_list<const Tensor*> inputs) {
             throw py::error_already_set();
         }
 }
-// A tensor whose values lie in memory one after the other.  (A view can stand for the negated values of its memory, and contiguous() leaves it one: logits
-// that are the imaginary part of a conjugate, say, and the gradient that the conjugate's backward pass hands to a node.)
-Tensor plain(const Tensor& t) { return (t.is_neg() ? t.resolve_neg() : t).contiguous(); }
 inline cudaStream_t stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
-inline void* ptr(const Tensor& t) { return t.data_ptr(); }
+// (a tensor whose storage has been given back, as sharded training does between its uses, has an address of null)
+inline void* ptr(const Tensor& t) {
+    void* const p = t.data_ptr();
+    if (!p && t.numel() > 0) throw std::runtime_error("a tensor of " + std::to_string(t.numel()) + " values has no memory");
+    return p;
+}
+template <typename T>
+T* ptr(const Tensor& t) {
+    ptr(t);
+    return t.data_ptr<T>();
+}
+// A tensor whose values lie in memory one after the other.  (A view can stand for the negated values of its memory, and contiguous() leaves it one: logits
+// that are the imaginary part of a conjugate, say, and the gradient that the conjugate's backward pass hands to a node.  Zeros can have no memory.)
+Tensor plain(const Tensor& t) {
+    if (t._is_zerotensor()) return t.clone(at::MemoryFormat::Contiguous);
+    ptr(t);
+    return (t.is_neg() ? t.resolve_neg() : t).contiguous();
+}
 
 // ------------------------------------------------------------------------------------------------------------------- plans
 // The descriptor of one (shape, type, attributes) combination, checked once.
@@ -481,7 +495,7 @@ std::pair<Tensor, Tensor> mixture_parameters(const Tensor& stats, const Tensor& 
     TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == 2 * means.numel() + means.size(0), "stats do not belong to these means");
     const c10::cuda::CUDAGuard guard(means.device());
     Tensor new_means = at::empty(means.sizes(), means.options()), new_covs = at::empty(means.sizes(), means.options());
-    check(simnets_mixture_parameters(int32_t(means.size(0)), int32_t(means.numel() / means.size(0)), float(min_var), stats.data_ptr<float>(), means.data_ptr<float>(),
+    check(simnets_mixture_parameters(int32_t(means.size(0)), int32_t(means.numel() / means.size(0)), float(min_var), ptr<float>(stats), ptr<float>(means),
                                      new_means.data_ptr<float>(), new_covs.data_ptr<float>(), stream_of(means)));
     return {new_means, new_covs};
 }
@@ -744,8 +758,8 @@ Routed route_impl(const Tensor& scores_in, const OptTensor& prior_in, const OptT
     }
     r.load = at::empty({scores.size(1)}, scores.options().dtype(at::kLong));
     const Tensor ws = scratch(scores, std::max<size_t>(need, 256));
-    check(simnets_route(&d, ptr(scores), prior ? ptr(*prior) : nullptr, bias ? ptr(*bias) : nullptr, dense ? nullptr : r.index.data_ptr<int32_t>(), dense ? nullptr : ptr(r.weights),
-                        dense ? ptr(r.dense) : nullptr, r.load.data_ptr<int64_t>(), dense ? ptr(r.mass) : nullptr, ptr(ws), ws.numel(), stream_of(scores)));
+    check(simnets_route(&d, ptr(scores), prior ? ptr(*prior) : nullptr, bias ? ptr(*bias) : nullptr, dense ? nullptr : ptr<int32_t>(r.index), dense ? nullptr : ptr(r.weights),
+                        dense ? ptr(r.dense) : nullptr, ptr<int64_t>(r.load), dense ? ptr(r.mass) : nullptr, ptr(ws), ws.numel(), stream_of(scores)));
     return r;
 }
 
@@ -765,7 +779,7 @@ struct RouteNode : torch::autograd::Node {
         if (g.sizes() != wv.sizes()) throw std::invalid_argument("route: gradient must have shape " + shape_text(wv.sizes()) + ", got " + shape_text(g.sizes()));
         const c10::cuda::CUDAGuard guard(wv.device());
         Tensor ds = at::empty(shape, wv.options());
-        check(simnets_route_gradient(&d, d.sigmoid ? ptr(sv) : nullptr, prior ? ptr(*prior) : nullptr, iv.data_ptr<int32_t>(), ptr(wv), ptr(g), ptr(ds), stream_of(wv)));
+        check(simnets_route_gradient(&d, d.sigmoid ? ptr(sv) : nullptr, prior ? ptr(*prior) : nullptr, ptr<int32_t>(iv), ptr(wv), ptr(g), ptr(ds), stream_of(wv)));
         out[0] = ds;
         return once(*this, grads, std::move(out));
     }
@@ -819,7 +833,7 @@ std::pair<Tensor, Tensor> xent_with_grad(const Tensor& logits_in, const Tensor& 
     const c10::cuda::CUDAGuard guard(logits.device());
     Tensor loss = at::empty({}, logits.options()), dlogits = at::empty(logits.sizes(), logits.options());
     const Tensor ws = scratch(logits, std::max<size_t>(simnets_softmax_cross_entropy_workspace_bytes(int32_t(logits.size(0))), 256));
-    check(simnets_softmax_cross_entropy(int32_t(logits.size(0)), int32_t(logits.size(1)), float(scale), logits.data_ptr<float>(), labels.data_ptr<int64_t>(),
+    check(simnets_softmax_cross_entropy(int32_t(logits.size(0)), int32_t(logits.size(1)), float(scale), ptr<float>(logits), ptr<int64_t>(labels),
                                         loss.data_ptr<float>(), dlogits.data_ptr<float>(), ptr(ws), ws.numel(), stream_of(logits)));
     return {loss, dlogits};
 }
@@ -886,9 +900,9 @@ struct Likelihood { Tensor label, entropy, top_index, top, stats; };
 
 // logits as the library reads them
 Tensor likelihood_logits(const Tensor& given, int64_t axis, int64_t top_k, simnets_likelihood_desc* d) {
-    const Tensor x = given.is_neg() ? given.resolve_neg() : given;
+    const Tensor x = given.is_neg() || given._is_zerotensor() ? plain(given) : given;
     if (likelihood_desc(x, axis, top_k, d)) return x;
-    const Tensor dense = x.contiguous();
+    const Tensor dense = plain(x);
     likelihood_desc(dense, axis, top_k, d);
     return dense;
 }
@@ -930,8 +944,8 @@ Likelihood likelihood_impl(const Tensor& logits_in, const OptTensor& labels_in, 
     Tensor ws;
     if (const size_t need = simnets_log_probabilities_workspace_bytes(&d)) ws = scratch(logits, need);
     if (d.batch * d.positions > 0 && (labels || entropy || top_k > 0))
-        check(simnets_log_probabilities(&d, ptr(logits), labels ? labels->data_ptr<int64_t>() : nullptr, at_or_null(r.label), at_or_null(r.entropy),
-                                        r.top_index.defined() ? r.top_index.data_ptr<int32_t>() : nullptr, at_or_null(r.top), at_or_null(r.stats),
+        check(simnets_log_probabilities(&d, ptr(logits), labels ? ptr<int64_t>(*labels) : nullptr, at_or_null(r.label), at_or_null(r.entropy),
+                                        r.top_index.defined() ? ptr<int32_t>(r.top_index) : nullptr, at_or_null(r.top), at_or_null(r.stats),
                                         at_or_null(ws), ws.defined() ? ws.numel() : 0, stream_of(logits)));
     return r;
 }
@@ -961,7 +975,7 @@ struct LikelihoodNode : torch::autograd::Node {
         }
         Tensor dx = empty_in_order(x, d);
         if (x.numel() > 0)
-            check(simnets_log_probabilities_gradient(&d, ptr(x), lv.defined() ? lv.data_ptr<int64_t>() : nullptr, ptr(sv), gt ? iv.data_ptr<int32_t>() : nullptr,
+            check(simnets_log_probabilities_gradient(&d, ptr(x), lv.defined() ? ptr<int64_t>(lv) : nullptr, ptr(sv), gt ? ptr<int32_t>(iv) : nullptr,
                                                      gl ? ptr(*gl) : nullptr, ge ? ptr(*ge) : nullptr, gt ? ptr(*gt) : nullptr, ptr(dx), stream_of(x)));
         out[0] = dx;
         return once(*this, grads, std::move(out));
@@ -1088,6 +1102,7 @@ Tensor gradients_impl(const py::object& given_in, int64_t order, bool scaled, do
         if (!scaled) continue;
         if (!q || q->layout() != at::kStrided || q->sizes() != t.sizes() || q->scalar_type() != type || q->device() != t.device())
             throw std::invalid_argument("out must have the shapes, types and device of the gradients");
+        if (q->_is_zerotensor()) throw std::invalid_argument("a tensor that is written has no memory");
         if (!elements_apart(*q)) throw std::invalid_argument("a tensor that is written has elements that share memory");
     }
     if (!first) throw std::invalid_argument("gradients: no tensors");
@@ -1107,7 +1122,7 @@ Tensor gradients_impl(const py::object& given_in, int64_t order, bool scaled, do
         const Tensor* const p = given.tensors[i];
         if (!p) continue;
         Tensor copy;
-        if (!p->is_non_overlapping_and_dense() || p->is_neg()) copies.push_back(copy = plain(*p));
+        if (!p->is_non_overlapping_and_dense() || p->is_neg() || p->_is_zerotensor()) copies.push_back(copy = plain(*p));
         const Tensor& in = copy.defined() ? copy : *p;
         dtypes.push_back(in.scalar_type() == at::kDouble ? SIMNETS_F64 : SIMNETS_F32);
         counts.push_back(in.numel());
@@ -1127,7 +1142,7 @@ Tensor gradients_impl(const py::object& given_in, int64_t order, bool scaled, do
         ranges.push_back({a, a + bytes, true});
         if (a != b) ranges.push_back({b, b + bytes, false});
         // (those that are copied may lie between one another: their first elements alone)
-        if (const uintptr_t to_at = reinterpret_cast<uintptr_t>(ptr(to)), in_at = reinterpret_cast<uintptr_t>(ptr(*p)); to_at != a || in_at != b) {
+        if (const uintptr_t to_at = reinterpret_cast<uintptr_t>(ptr(to)), in_at = p->_is_zerotensor() ? b : reinterpret_cast<uintptr_t>(ptr(*p)); to_at != a || in_at != b) {
             if (to_at != a) ranges.push_back({to_at, to_at + in.element_size(), true});
             if (in_at != b && in_at != to_at) ranges.push_back({in_at, in_at + in.element_size(), false});
         }
