@@ -133,6 +133,14 @@ Tensor plain(const Tensor& t) {
     return (t.is_neg() ? t.resolve_neg() : t).contiguous();
 }
 
+// What a node has kept, as the hooks on saved tensors (torch.autograd.graph.saved_tensors_hooks) give it back: `values` of its type on the device of `first`.
+Tensor given_back(const Tensor& t, const Tensor& first, at::ScalarType type, int64_t values) {
+    if (t.device() != first.device() || t.scalar_type() != type || t.numel() != values)
+        throw std::runtime_error("a hook on saved tensors gave back another tensor than was saved: " + std::to_string(t.numel()) + " values on " + t.device().str() + " for " +
+                                 std::to_string(values) + " on " + first.device().str());
+    return plain(t);
+}
+
 // ------------------------------------------------------------------------------------------------------------------- plans
 // The descriptor of one (shape, type, attributes) combination, checked once.
 struct MexPlan {
@@ -774,10 +782,14 @@ struct RouteNode : torch::autograd::Node {
         std::lock_guard<std::mutex> lock(mutex_);
         variable_list out(1);
         if (!grads[0].defined() || !task_should_compute_output(0)) return out;
-        const Tensor iv = index.unpack(), wv = weights.unpack(shared_from_this()), sv = d.sigmoid ? plain(scores.unpack()) : Tensor(), g = plain(grads[0]);
-        require_cuda_all(wv, g);
-        if (g.sizes() != wv.sizes()) throw std::invalid_argument("route: gradient must have shape " + shape_text(wv.sizes()) + ", got " + shape_text(g.sizes()));
-        const c10::cuda::CUDAGuard guard(wv.device());
+        const Tensor g = plain(grads[0]), wu = weights.unpack(shared_from_this());
+        require_cuda_all(g, wu);
+        if (g.sizes() != wu.sizes()) throw std::invalid_argument("route: gradient must have shape " + shape_text(wu.sizes()) + ", got " + shape_text(g.sizes()));
+        const c10::cuda::CUDAGuard guard(g.device());
+        const int64_t places = int64_t(d.batch) * d.positions;
+        const at::ScalarType type = d.dtype == SIMNETS_F64 ? at::kDouble : at::kFloat;
+        const Tensor wv = given_back(wu, g, type, places * d.top_k), iv = given_back(index.unpack(), g, at::kInt, places * d.top_k);
+        const Tensor sv = d.sigmoid ? given_back(scores.unpack(), g, type, places * d.components) : Tensor();
         Tensor ds = at::empty(shape, wv.options());
         check(simnets_route_gradient(&d, d.sigmoid ? ptr(sv) : nullptr, prior ? ptr(*prior) : nullptr, ptr<int32_t>(iv), ptr(wv), ptr(g), ptr(ds), stream_of(wv)));
         out[0] = ds;
@@ -961,12 +973,16 @@ struct LikelihoodNode : torch::autograd::Node {
         auto given = [&](int i) { return i >= 0 && grads[i].defined() ? OptTensor(plain(grads[i])) : OptTensor(); };
         const OptTensor gl = given(label_at), ge = given(entropy_at), gt = given(top_at);
         if ((!gl && !ge && !gt) || !task_should_compute_output(0)) return out;
-        const Tensor xv = logits.unpack(), lv = labels.unpack(), sv = stats.unpack(), iv = top_index.unpack();
+        const Tensor xv = logits.unpack();
+        check_likelihood(xv, std::nullopt, top_k, axis);
         simnets_likelihood_desc d;
         const c10::cuda::CUDAGuard guard(xv.device());
         const Tensor x = likelihood_logits(xv, axis, gt ? top_k : 0, &d);
         std::vector<int64_t> shape = x.sizes().vec();
         shape.erase(shape.begin() + axis);
+        const int64_t places = x.numel() / x.size(axis);
+        const Tensor sv = given_back(stats.unpack(), x, x.scalar_type(), 3 * places);
+        const Tensor lv = gl ? given_back(labels.unpack(), x, at::kLong, places) : Tensor(), iv = gt ? given_back(top_index.unpack(), x, at::kInt, places * top_k) : Tensor();
         for (const OptTensor* g : {&gl, &ge, &gt}) {
             if (!*g) continue;
             require_cuda(x, **g);
