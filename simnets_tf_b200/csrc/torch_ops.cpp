@@ -182,6 +182,12 @@ struct MexPlan {
         if (off.sizes() != at::IntArrayRef(want, 5))
             throw std::invalid_argument("offsets must have shape " + shape_text(at::IntArrayRef(want, 5)) + ", got " + shape_text(off.sizes()));
     }
+    // (only its values count, whatever its shape)
+    void check_output(const Tensor& y) const {
+        const auto want = out_shape();
+        if (y.numel() != want[0] * want[1] * want[2] * want[3])
+            throw std::invalid_argument("orig_output must have shape " + shape_text(want) + ", got " + shape_text(y.sizes()));
+    }
     void check_dy(const Tensor& dy, bool pooled) const {
         const auto want = out_shape(pooled ? 2 : 1);
         if (dy.sizes() != at::IntArrayRef(want))
@@ -292,6 +298,7 @@ std::pair<Tensor, Tensor> mex_grads(const MexPlan& p, const Tensor& x_in, const 
     p.check_input(x_in);
     p.check_offsets(off_in);
     p.check_dy(dy_in, pooled);
+    p.check_output(y_in);
     flags |= (pooled ? SIMNETS_FLAG_MEX_DY_POOLED2 : 0u) | (primed ? SIMNETS_FLAG_MEX_WORKSPACE_PRIMED : 0u);
     const Tensor x = plain(x_in), off = plain(off_in), y = plain(y_in), dy = plain(dy_in);
     const c10::cuda::CUDAGuard guard(x.device());
