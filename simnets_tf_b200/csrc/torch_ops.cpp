@@ -18,6 +18,7 @@
 #include <limits>
 #include <memory>
 #include <mutex>
+#include <numeric>
 #include <string>
 #include <vector>
 #include "simnets_b200.h"
@@ -1065,15 +1066,84 @@ bool elements_apart(const Tensor& t) {
     return true;
 }
 
+// The bytes of a tensor: those at begin + any sum of i * stride, i < size, over its dimensions by falling stride, of which a run of bytes side by side is the last.
+struct Bytes {
+    struct Dim { int64_t stride, size, span; };               // (span: from the first to behind the last byte of this dimension and those inside it)
+    uintptr_t begin = 0;
+    std::vector<Dim> dims;
+    bool written = false;
+    Bytes(const Tensor& t, bool written_) : begin(reinterpret_cast<uintptr_t>(ptr(t))), written(written_) {
+        dims.push_back({1, int64_t(t.element_size()), 0});
+        std::vector<std::pair<int64_t, int64_t>> sorted;
+        for (int64_t i = 0; i < t.dim(); ++i)
+            if (t.size(i) > 1 && t.stride(i) > 0) sorted.emplace_back(t.stride(i) * int64_t(t.element_size()), t.size(i));
+        std::sort(sorted.begin(), sorted.end());
+        for (const auto& [stride, size] : sorted) {
+            if (stride == dims.back().stride * dims.back().size) dims.back().size *= size;
+            else dims.push_back({stride, size, 0});
+        }
+        int64_t span = 1;
+        for (Dim& d : dims) d.span = span += d.stride * (d.size - 1);
+        std::reverse(dims.begin(), dims.end());
+    }
+    Bytes(uintptr_t from, uintptr_t to, bool written_) : begin(from), dims{{1, int64_t(to - from), int64_t(to - from)}}, written(written_) {}
+};
+
+int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }
+
+// Whether boxes a and b, of which b begins `apart` bytes behind a, have a byte in common: the steps of the longer stride at which their spans meet, each without
+// that dimension; steps of the same stride by their difference.  (Out of `tries`, after some milliseconds, they count as if they had.)
+bool meet(const Bytes::Dim* a, const Bytes::Dim* b, int64_t apart, int64_t& tries) {
+    if (apart >= a->span || -apart >= b->span) return false;
+    if (--tries < 0 || (a->stride == 1 && b->stride == 1)) return true;
+    const int64_t s = std::max(a->stride, b->stride);
+    const bool of_a = a->stride == s, of_b = b->stride == s;
+    const Bytes::Dim *in_a = a + of_a, *in_b = b + of_b;
+    const int64_t lowest = std::max(of_b ? 1 - b->size : 0, floor_div(apart - in_a->span, s) + 1), highest = std::min(of_a ? a->size - 1 : 0, floor_div(apart + in_b->span - 1, s));
+    for (int64_t i = lowest; i <= highest; ++i)
+        if (meet(in_a, in_b, apart - i * s, tries)) return true;
+    return false;
+}
+bool meet(const Bytes& a, const Bytes& b) {
+    const int64_t apart = int64_t(b.begin - a.begin);
+    if (apart >= a.dims[0].span || -apart >= b.dims[0].span) return false;
+    // (columns of one matrix, every second value and those between: runs that never meet, counted from multiples of what divides all strides)
+    int64_t common = 0;
+    for (const Bytes* x : {&a, &b})
+        for (size_t i = 0; i + 1 < x->dims.size(); ++i) common = std::gcd(common, x->dims[i].stride);
+    if (common > 0) {
+        const int64_t place = apart - floor_div(apart, common) * common;
+        if (place >= a.dims.back().size && place + b.dims.back().size <= common) return false;
+    }
+    int64_t tries = 1 << 20;
+    return meet(a.dims.data(), b.dims.data(), apart, tries);
+}
+
+[[noreturn]] void refuse_shared() { throw std::invalid_argument("two of the tensors share memory: each must be given once"); }
+
+// Whether two tensors of the same sizes have every element in the same place.
+bool lies_alike(const Tensor& a, const Tensor& b) {
+    bool alike = ptr(a) == ptr(b);
+    for (int64_t i = 0; i < a.dim() && alike; ++i) alike = a.size(i) == 1 || a.stride(i) == b.stride(i);
+    return alike;
+}
+
 struct Range { uintptr_t begin, end; bool written; };
-// Refuses ranges of memory of which one that is written overlaps another.
-void refuse_overlaps(std::vector<Range>& ranges) {
+// Refuses tensors of which one that is written has memory in common with another: ranges, of those that have all bytes of theirs, and others.
+void refuse_overlaps(std::vector<Range>& ranges, const std::vector<Bytes>& others) {
     auto in_front = [](const Range& x, const Range& y) { return x.begin < y.begin; };
     if (!std::is_sorted(ranges.begin(), ranges.end(), in_front)) std::sort(ranges.begin(), ranges.end(), in_front);
     uintptr_t read = 0, written = 0;
     for (const Range& r : ranges) {
-        if (r.begin < written || (r.written && r.begin < read)) throw std::invalid_argument("two of the tensors share memory: each must be given once");
+        if (r.begin < written || (r.written && r.begin < read)) refuse_shared();
         (r.written ? written : read) = std::max(r.written ? written : read, r.end);
+    }
+    for (size_t i = 0; i < others.size(); ++i) {
+        const Bytes& x = others[i];
+        for (size_t j = 0; j < i; ++j)
+            if ((x.written || others[j].written) && meet(x, others[j])) refuse_shared();
+        for (const Range& r : ranges)
+            if ((x.written || r.written) && r.begin < x.begin + x.dims[0].span && x.begin < r.end && meet(x, Bytes(r.begin, r.end, r.written))) refuse_shared();
     }
 }
 
@@ -1135,6 +1205,7 @@ Tensor gradients_impl(const py::object& given_in, int64_t order, bool scaled, do
     std::vector<Tensor> copies;
     std::vector<std::pair<const Tensor*, size_t>> back;                     // a destination, and the copy that goes there
     std::vector<Range> ranges;
+    std::vector<Bytes> others;
     std::vector<int32_t> dtypes;
     std::vector<int64_t> counts;
     std::vector<const void*> from;
@@ -1161,17 +1232,17 @@ Tensor gradients_impl(const py::object& given_in, int64_t order, bool scaled, do
         }
         into.push_back(dst);
         if (bytes == 0) continue;
-        const uintptr_t a = reinterpret_cast<uintptr_t>(dst), b = reinterpret_cast<uintptr_t>(from.back());
-        ranges.push_back({a, a + bytes, true});
-        if (a != b) ranges.push_back({b, b + bytes, false});
-        // (those that are copied may lie between one another: their first elements alone)
-        if (const uintptr_t to_at = reinterpret_cast<uintptr_t>(ptr(to)), in_at = p->_is_zerotensor() ? b : reinterpret_cast<uintptr_t>(ptr(*p)); to_at != a || in_at != b) {
-            if (to_at != a) ranges.push_back({to_at, to_at + in.element_size(), true});
-            if (in_at != b && in_at != to_at) ranges.push_back({in_at, in_at + in.element_size(), false});
-        }
+        // what is read and written of the caller's memory (a copy is nobody else's); a tensor may be its own destination if it lies there as it does
+        auto take = [&](const Tensor& t, bool written) {
+            const uintptr_t at = reinterpret_cast<uintptr_t>(ptr(t));
+            if (t.is_non_overlapping_and_dense()) ranges.push_back({at, at + bytes, written});
+            else others.emplace_back(t, written);
+        };
+        take(to, true);
+        if (&to != p && !p->_is_zerotensor() && !lies_alike(*p, to)) take(*p, false);
     }
     if (scaled) {
-        refuse_overlaps(ranges);
+        refuse_overlaps(ranges, others);
         for (size_t i = 0; i < n; ++i)
             if (given.tensors[i]) torch::autograd::impl::bump_version(out ? *out->tensors[i] : *given.tensors[i]);
     }
@@ -1240,6 +1311,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("xent_with_grad", &xent_with_grad);
     m.def("xent_apply", &xent_apply);
     m.def("log_probabilities", &log_probabilities_apply);
+    m.def("share_memory", [](const Tensor& a, const Tensor& b) { return a.numel() > 0 && b.numel() > 0 && meet(Bytes(a, false), Bytes(b, false)); });
     m.def("gradient_norm", [](const py::object& tensors, int64_t order) { return gradients_impl(tensors, order, false, 0.0, py::none()); });
     m.def("clip_gradients", [](const py::object& tensors, double max_norm, int64_t order, const py::object& out) { return gradients_impl(tensors, order, true, max_norm, out); });
     m.def("profile_start", [] { py::list dropped = profile_take(); g_profiling = true; });

@@ -25,7 +25,7 @@ def clip_gradients(tensors, max_norm, order=2, out=None):
     """Scales `tensors` in place by max_norm / norm where their norm (see `gradient_norm`) is above `max_norm`, and returns the norm before.
     out: a list of tensors alike that the result goes to instead (a bucket that is added to further keeps its sums).  A norm that is NaN or
     infinite changes nothing: the norm that is returned tells.  The host waits for nothing, so a call can be part of a CUDA graph.
-    A tensor may be given once only."""
+    No tensor that is written may share memory with another one that is given, as a slice of it, say; a tensor may be its own destination."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError("max_norm must not be negative, got %r" % max_norm)
