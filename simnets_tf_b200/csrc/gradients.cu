@@ -66,7 +66,8 @@ struct Item {
     __device__ __forceinline__ Vector<T> load(long long at) const {
         Vector<T> x;
         if (at >= 0 && at + Vector<T>::kWidth <= values) {
-            *reinterpret_cast<typename Four<T>::type*>(x.v) = *reinterpret_cast<const typename Four<T>::type*>(in + at);
+            const typename Four<T>::type w = *reinterpret_cast<const typename Four<T>::type*>(in + at);
+            memcpy(x.v, &w, 16);                            // (an array that is not in registers lies at a multiple of its values' size only)
         } else {
 #pragma unroll
             for (int i = 0; i < Vector<T>::kWidth; ++i) x.v[i] = at + i >= 0 && at + i < values ? in[at + i] : T(0);
@@ -75,7 +76,9 @@ struct Item {
     }
     __device__ __forceinline__ void store(long long at, const Vector<T>& x) const {
         if (aligned && at >= 0 && at + Vector<T>::kWidth <= values) {
-            *reinterpret_cast<typename Four<T>::type*>(out + at) = *reinterpret_cast<const typename Four<T>::type*>(x.v);
+            typename Four<T>::type w;
+            memcpy(&w, x.v, 16);
+            *reinterpret_cast<typename Four<T>::type*>(out + at) = w;
         } else {
 #pragma unroll
             for (int i = 0; i < Vector<T>::kWidth; ++i)

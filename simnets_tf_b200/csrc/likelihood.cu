@@ -197,6 +197,18 @@ template <typename T> struct Bytes16;
 template <> struct Bytes16<float> { using type = float4; };
 template <> struct Bytes16<double> { using type = double2; };
 template <typename T> constexpr int kWide = 16 / sizeof(T);
+// (What they go to and come from is an array of T, which is bound to a multiple of its own size only wherever it is not in registers.)
+template <typename T>
+__device__ __forceinline__ void load_wide(T* v, const void* from) {
+    const typename Bytes16<T>::type w = *static_cast<const typename Bytes16<T>::type*>(from);
+    memcpy(v, &w, 16);
+}
+template <typename T>
+__device__ __forceinline__ void store_wide(T* to, const T* v) {
+    typename Bytes16<T>::type w;
+    memcpy(&w, v, 16);
+    *reinterpret_cast<typename Bytes16<T>::type*>(to) = w;
+}
 
 template <typename T>
 __device__ __forceinline__ int in_front(const T* x) { return int(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T)); }
@@ -262,7 +274,7 @@ struct Run {
 #pragma unroll
             for (int j = 0; j < U; j += kWide<T>) {
                 if (c + j >= begin && c + j + kWide<T> <= end) {
-                    *reinterpret_cast<typename Bytes16<T>::type*>(v + j) = *reinterpret_cast<const typename Bytes16<T>::type*>(x + j);
+                    load_wide(v + j, x + j);
                 } else {
 #pragma unroll
                     for (int e = j; e < j + kWide<T>; ++e) v[e] = c + e >= begin && c + e < end ? x[e] : -infinity<T>();
@@ -286,7 +298,7 @@ struct Run {
 #pragma unroll
             for (int j = 0; j < U; j += kWide<T>) {
                 if (aligned && c + j >= begin && c + j + kWide<T> <= end) {
-                    *reinterpret_cast<typename Bytes16<T>::type*>(to + j) = *reinterpret_cast<const typename Bytes16<T>::type*>(v + j);
+                    store_wide(to + j, v + j);
                 } else {
 #pragma unroll
                     for (int e = j; e < j + kWide<T>; ++e)
@@ -424,7 +436,7 @@ __device__ __forceinline__ void load_chunk(T (&v)[U], const T* x, long long firs
     for (int j = 0; j < U; j += kWide<T>) {
         const long long c = first + class_in_chunk<T, THREADS>(tid, j);
         if (inside || (c >= 0 && c + kWide<T> <= classes)) {
-            *reinterpret_cast<typename Bytes16<T>::type*>(v + j) = *reinterpret_cast<const typename Bytes16<T>::type*>(x + c);
+            load_wide(v + j, x + c);
         } else {
 #pragma unroll
             for (int e = 0; e < kWide<T>; ++e) v[j + e] = c + e >= 0 && c + e < classes ? x[c + e] : -infinity<T>();
@@ -438,7 +450,7 @@ __device__ __forceinline__ void store_chunk(const T (&v)[U], T* x, bool aligned,
     for (int j = 0; j < U; j += kWide<T>) {
         const long long c = first + class_in_chunk<T, THREADS>(tid, j);
         if (inside || (aligned && c >= 0 && c + kWide<T> <= classes)) {
-            *reinterpret_cast<typename Bytes16<T>::type*>(x + c) = *reinterpret_cast<const typename Bytes16<T>::type*>(v + j);
+            store_wide(x + c, v + j);
         } else {
 #pragma unroll
             for (int e = 0; e < kWide<T>; ++e)
@@ -996,7 +1008,7 @@ __global__ void __launch_bounds__(kStreamThreads + 32, kStreamCtas) answer_strea
         T v[U];
         const char* here = stages + stage * (kStreamThreads * 64) + threadIdx.x * 16;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<typename Bytes16<T>::type*>(v + j * kWide<T>) = *reinterpret_cast<const typename Bytes16<T>::type*>(here + j * kStreamThreads * 16);
+        for (int j = 0; j < 4; ++j) load_wide(v + j * kWide<T>, here + j * kStreamThreads * 16);
         stage = stage + 1 == kStages ? 0 : stage + 1;
         copy_next();                                        // (into what was read an iteration ago)
         const T hi = sums.add(v);
