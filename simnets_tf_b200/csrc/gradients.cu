@@ -147,9 +147,9 @@ __global__ void __launch_bounds__(kThreads) norm_partials(const __grid_constant_
     }
     p = over_cta<MAX>(p, room);
     if (threadIdx.x == 0) {
-        // (a sum of float32 squares is a number between 2^-298 and 2^319, which stays one when it is scaled the first way; the second
-        // is looked at only where the sum is far smaller)
-        if (!MAX && sizeof(T) == 4) { p.big = p.mid * down600() * down600(); p.small = p.mid * up600() * up600(); }
+        // (A finite sum of float32 squares other than 0 is between 2^-298 and 2^319.  `big` is taken where all sums together are above 2^1000, of which that
+        // is nothing, and `small` where they are below 2^-900, which it is not: both are 0.  Only an infinity counts in `big`.)
+        if (!MAX && sizeof(T) == 4) p.big = p.mid == double(CUDART_INF) ? p.mid : 0.0;
         partials[blockIdx.x] = p;
     }
 }
