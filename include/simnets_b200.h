@@ -491,8 +491,9 @@ SIMNETS_API int simnets_softmax_cross_entropy(int32_t batch, int32_t classes, fl
  * simnets_log_probabilities_gradient: the gradient of all logits for the gradients g_label, g_entropy and g_top (each may be NULL) of the outputs,
  *   dlogits_c = -p_c (g_label + sum g_top + g_entropy (log p_c + entropy)) + g_label [c = labels] + sum over g_top [c = top_index],
  * 0 where no class can be; a label or an alternative that is none adds nothing.  dlogits is dense, [batch, positions, classes] if
- * stride_class is 1, else [batch, classes, positions], and must not overlap the logits.  Logits and dlogits may start at any multiple of the
- * value's size; at other addresses, and beyond 2^30 classes, 2^33 positions or 2^43 logits, the call is SIMNETS_E_UNSUPPORTED.
+ * stride_class is 1, else [batch, classes, positions], and must not overlap the logits.  Every array may start at any multiple of its
+ * values' size, the workspace of 8 bytes; at other addresses, and beyond 2^30 classes, 2^33 positions or 2^43 logits, the call is
+ * SIMNETS_E_UNSUPPORTED.
  * The reference has softmax and cross-entropy of its framework only (README.md:108-111). */
 typedef struct simnets_likelihood_desc {
     int32_t dtype;
@@ -514,7 +515,8 @@ SIMNETS_API int simnets_log_probabilities_gradient(const simnets_likelihood_desc
  * if a tensor is, else float32.  Sums are in 64 bits and of a fixed order; float64 squares neither overflow nor vanish.
  * simnets_clip_gradients also writes out[i] = tensors[i] * (max_norm / norm where norm > max_norm, else 1), the product rounded once; a norm that is
  * NaN or, as returned, infinite leaves the values as they are.  out[i] may be tensors[i]; otherwise no two of the tensors written and read may
- * overlap (not checked here).  Tensors start at any multiple of their value's size (else, and beyond 2^40 values, SIMNETS_E_UNSUPPORTED).
+ * overlap (not checked here).  Tensors and norm start at any multiple of their values' size, the workspace at one of 8 bytes (else, and beyond
+ * 2^40 values, SIMNETS_E_UNSUPPORTED).
  * max_norm: at least 0, infinity for no limit.  The reference leaves its gradients to its framework's optimisers. */
 SIMNETS_API size_t simnets_gradient_norm_workspace_bytes(int32_t num_tensors);
 SIMNETS_API int simnets_gradient_norm(int32_t order, int32_t num_tensors, const int32_t* dtypes, const int64_t* counts, const void* const* tensors,

@@ -128,13 +128,15 @@ int likelihood_check(const simnets_likelihood_desc* d) {
     return SIMNETS_OK;
 }
 
-// whether a place cannot hold values of the type
+// whether a place cannot hold values of the type, or whole numbers and workspaces of 64 bits
 bool misplaced(const void* p, int32_t dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype == SIMNETS_F64 ? 8 : 4) != 0; }
+bool misplaced64(const void* p) { return reinterpret_cast<uintptr_t>(p) % 8 != 0; }
 
 int gradients_check(int32_t order, int32_t tensors, const int32_t* dtypes, const int64_t* counts, const void* const* in, const void* norm, const void* ws, size_t ws_bytes) {
     if ((order != 0 && order != 2) || tensors < 0) return SIMNETS_E_DESC;
     if (!norm || (tensors > 0 && (!counts || !in))) return SIMNETS_E_NULL;
     long long total = 0;
+    bool f64 = false;
     for (int i = 0; i < tensors; ++i) {
         if (dtypes && dtypes[i] != SIMNETS_F32 && dtypes[i] != SIMNETS_F64) return SIMNETS_E_DTYPE;
         if (counts[i] < 0) return SIMNETS_E_DESC;
@@ -142,7 +144,9 @@ int gradients_check(int32_t order, int32_t tensors, const int32_t* dtypes, const
         if (counts[i] > 0 && misplaced(in[i], dtypes ? dtypes[i] : SIMNETS_F32)) return SIMNETS_E_UNSUPPORTED;
         if (counts[i] > (1LL << 40) - total) return SIMNETS_E_UNSUPPORTED;          // (pieces of 16 KB are counted in 32 bits)
         total += counts[i];
+        f64 = f64 || (dtypes && dtypes[i] == SIMNETS_F64);
     }
+    if (misplaced(norm, f64 ? SIMNETS_F64 : SIMNETS_F32) || misplaced64(ws)) return SIMNETS_E_UNSUPPORTED;
     return !ws || ws_bytes < gradient_norm_workspace_bytes(tensors) ? SIMNETS_E_WORKSPACE : SIMNETS_OK;
 }
 
@@ -573,7 +577,9 @@ int simnets_log_probabilities(const simnets_likelihood_desc* d, const void* logi
     if (d->batch == 0 || d->positions == 0) return SIMNETS_OK;
     if (!logits || (label && !labels) || (top == nullptr) != (top_index == nullptr)) return SIMNETS_E_NULL;
     if ((d->top_k > 0) != (top != nullptr)) return SIMNETS_E_DESC;
-    if (misplaced(logits, d->dtype)) return SIMNETS_E_UNSUPPORTED;
+    for (const void* p : {logits, (const void*)label, (const void*)entropy, (const void*)top, (const void*)stats})
+        if (misplaced(p, d->dtype)) return SIMNETS_E_UNSUPPORTED;
+    if (misplaced64(labels) || misplaced(top_index, SIMNETS_F32) || misplaced64(ws)) return SIMNETS_E_UNSUPPORTED;
     if (const size_t need = log_probabilities_workspace_bytes(*d); need > 0 && (!ws || ws_bytes < need)) return SIMNETS_E_WORKSPACE;
     return from_cuda(launch_log_probabilities(*d, logits, reinterpret_cast<const long long*>(labels), label, entropy, top_index, top, stats, ws, as_stream(stream)));
 }
@@ -585,7 +591,9 @@ int simnets_log_probabilities_gradient(const simnets_likelihood_desc* d, const v
     if (d->batch == 0 || d->positions == 0) return SIMNETS_OK;
     if (!logits || !stats || !dlogits || (g_label && !labels) || (g_top && !top_index)) return SIMNETS_E_NULL;
     if ((d->top_k > 0) != (g_top != nullptr)) return SIMNETS_E_DESC;
-    if (misplaced(logits, d->dtype) || misplaced(dlogits, d->dtype)) return SIMNETS_E_UNSUPPORTED;
+    for (const void* p : {logits, stats, g_label, g_entropy, g_top, (const void*)dlogits})
+        if (misplaced(p, d->dtype)) return SIMNETS_E_UNSUPPORTED;
+    if (misplaced64(labels) || misplaced(top_index, SIMNETS_F32)) return SIMNETS_E_UNSUPPORTED;
     return from_cuda(launch_log_probabilities_gradient(*d, logits, reinterpret_cast<const long long*>(labels), stats, top_index, g_label, g_entropy, g_top, dlogits,
                                                        as_stream(stream)));
 }
