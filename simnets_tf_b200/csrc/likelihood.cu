@@ -657,7 +657,7 @@ __device__ __forceinline__ T logit_of_label(const Logits& g, const Answers<T>& a
 constexpr int kGroupWarps = 16;
 // (the entries of a position lie in as many banks)
 template <typename T, int TOP> constexpr size_t kGroupBytes = Found<T, TOP>::kBytes + 8;
-template <typename T, int TOP, bool SIDE>
+template <typename T, int TOP>
 __global__ void __launch_bounds__(32 * kGroupWarps, sizeof(T) == 4 ? 2 : 1) answer_groups(Logits g, Answers<T> a) {
     stream_order();
     extern __shared__ __align__(16) char room[];
@@ -665,7 +665,7 @@ __global__ void __launch_bounds__(32 * kGroupWarps, sizeof(T) == 4 ? 2 : 1) answ
     bool mine;
     {
         const T* x = a.logits + g.at(lane_position(g, &mine));
-        const Found<T, TOP> f = found_in_run<T, TOP, SIDE, false>(g, x);
+        const Found<T, TOP> f = found_in_run<T, TOP, false, false>(g, x);
         f.put(room + threadIdx.y * kGroupBytes<T, TOP>, lane);
     }
     __syncthreads();
@@ -705,7 +705,7 @@ __global__ void __launch_bounds__(32 * kGroupWarps, sizeof(T) == 4 ? 2 : 1) answ
                 w[e] = -infinity<T>();
                 c[e] = -1;
                 if (j < g.top_k && at >= 0) {
-                    const Run<T, SIDE> chunk = listed_chunk<T, SIDE>(g, x, at);
+                    const Run<T, false> chunk = listed_chunk<T, false>(g, x, at);
                     const int here = chunk.c + entry % kLaneAhead;
                     if (here >= chunk.begin && here < chunk.end) { w[e] = x[here * chunk.step]; c[e] = here; }
                 }
@@ -1210,11 +1210,27 @@ Logits logits_of(const simnets_likelihood_desc& d) {
 bool by_rows(const Logits& g, int most) { return g.stride_class == 1 && (g.classes > most || (g.classes > 32 && g.count() < 16384)); }
 constexpr int kMostByLanes = 256, kMostGradientByLanes = 128;
 
-// warps that share 32 positions: 1, 2, 4 or kGroupWarps
+// Warps that share 32 positions: 4 or 2 where the tiles are then there all at once (by the CTAs of 4 warps that registers let be on a multiprocessor), and
+// kGroupWarps where that many are as well and runs of so many classes are worth the join; of more classes two rounds of them are.  float64 answers of many
+// classes are shared by 2 beyond that, and by 4 where those 2 would be a few more CTAs than are there at once.
+// All sides, maps with four alternatives, us:
+//     1 / 2 / 4 warps: 32768 positions of 150 classes 18.2 / 13.1 / 12.9, 49152 20.4 / 15.4 / 18.3, 98304 26.5 / 29.3 / 31.5, their gradients 20.5 / 14.2 / 11.4,
+//         23.1 / 17.7 / 18.4, 34.8 / 34.1 / 32.7; float64 12288 of 64 12.6 / 8.8 / 7.4, 24576 15.1 / 11.1 / 13.8, 49152 18.6 / 20.1 / 24.0, 65536 29.2 / 26.5 /
+//         30.4, of 32 15.6 / 16.3 / 21.5, 32768 of 300 62 / 66 / 60, the gradients of 64 10.2 / 7.5 / 5.9, 12.0 / 9.1 / 9.9, 15.9 / 17.5 / 16.3, 19.1 / 20.1 / 21.6
+//     4 / 16: 8192 of 150 6.0 / 9.1, of 256 9.8 / 9.7, of 512 16.3 / 11.8, 16384 of 512 18.5 / 22.7, of 1000 33 / 31, gradients of 96 4.2 / 4.2, of 100 5.0 / 4.3, of
+//         150 6.7 / 5.6, 16384 of 150 8.2 / 9.8, of 512 21.2 / 18.8; float64 4096 of 256 14.0 / 13.6, of 512 25 / 18, 8192 of 512 29 / 35, of 2000 97 / 79,
+//         gradients of 64 4.6 / 4.9, of 100 5.6 / 4.9, 8192 of 256 13 / 13.6, of 512 22.0 / 20.5
+// Rows, whose classes lie side by side, come here in such numbers only that 16 warps lose: 17500 of 128 8.4 / 16.9, of 256 12.6 / 20.5, the gradient of
+// 128 10.7 / 16.0.
+template <typename T, bool GRADIENT>
 int warps_of_lanes(const Logits& g) {
-    const long long tiles = (g.count() + 31) / 32, enough = 16LL * device_sm_count();
-    if (tiles * 4 < enough && g.classes >= 8 * kLaneAhead) return kGroupWarps;
-    return tiles * 2 < enough && g.classes >= 4 * kLaneAhead ? 4 : tiles < enough && g.classes >= 2 * kLaneAhead ? 2 : 1;
+    constexpr bool kDouble = sizeof(T) == 8, kAnswer64 = kDouble && !GRADIENT;
+    constexpr int kCtas = !kDouble ? 8 : GRADIENT ? 4 : 3, kSixteen = GRADIENT ? 97 : 256, kSixteenTwice = GRADIENT ? (kDouble ? 512 : 256) : kDouble ? 1024 : 768;
+    const long long tiles = (g.count() + 31) / 32, sms = device_sm_count(), groups = (kDouble ? 1 : 2) * sms;
+    if (g.stride_class != 1 && g.classes >= kSixteen && tiles <= (g.classes >= kSixteenTwice ? 2 * groups : groups)) return kGroupWarps;
+    if (g.classes >= 4 * kLaneAhead && tiles < kCtas * sms) return 4;
+    if (kAnswer64 && g.classes >= 16 * kLaneAhead && tiles >= 2 * kCtas * sms && tiles < 8 * sms) return 4;
+    return g.classes >= 2 * kLaneAhead && tiles < (kAnswer64 && g.classes >= 8 * kLaneAhead ? 16 : 2 * kCtas) * sms ? 2 : 1;
 }
 
 template <class Kernel, class A>
@@ -1228,19 +1244,23 @@ cudaError_t launch_lanes(Kernel* kernel, const Logits& g, const A& a, int warps,
 
 template <typename T, int TOP, bool SIDE>
 cudaError_t answer_lanes_of(const Logits& g, const Answers<T>& a, cudaStream_t s) {
-    const int warps = warps_of_lanes(g);
+    const int warps = warps_of_lanes<T, false>(g);
     // a run of hardly more chunks than the list has places would be read twice (us, classes / chunks listed: 65536 rows of 10, three alternatives 4.4 / 7.6,
     // float64 maps of 37, four alternatives 7.3 / 9.5, 100000 rows of 100, three alternatives 20.7 / 16.9, a map of 150 36 / 27)
     const bool direct = g.classes <= 16 * TOP * warps;
     if (warps < kGroupWarps)
         return launch_lanes(direct || TOP == 0 ? answer_lanes<T, TOP, SIDE, true> : answer_lanes<T, TOP, SIDE, TOP == 0>, g, a, warps, warps > 1 ? 4 * Found<T, TOP>::kBytes : 0, s);
-    constexpr int kBytes = int(kGroupWarps * kGroupBytes<T, TOP>);
-    if (kBytes > 48 * 1024) {
-        static SmemLimit limit;
-        const cudaError_t e = limit.raise(answer_groups<T, TOP, SIDE>, kBytes);
-        if (e != cudaSuccess) return e;
+    if constexpr (SIDE) {
+        return cudaErrorInvalidValue;                       // (not reached: warps_of_lanes)
+    } else {
+        constexpr int kBytes = int(kGroupWarps * kGroupBytes<T, TOP>);
+        if (kBytes > 48 * 1024) {
+            static SmemLimit limit;
+            const cudaError_t e = limit.raise(answer_groups<T, TOP>, kBytes);
+            if (e != cudaSuccess) return e;
+        }
+        return launch_lanes(answer_groups<T, TOP>, g, a, kGroupWarps, kBytes, s);
     }
-    return launch_lanes(answer_groups<T, TOP, SIDE>, g, a, kGroupWarps, kBytes, s);
 }
 
 // A warp a row where a row is one chunk, or where rows are so many that their number hides how long a warp is at one; else streams (four alternatives,
@@ -1305,7 +1325,7 @@ cudaError_t answer_as(const Logits& g, const Answers<T>& a, void* ws, cudaStream
 template <typename T>
 cudaError_t gradient_as(const Logits& g, const Gradients<T>& a, cudaStream_t s) {
     if (!by_rows(g, kMostGradientByLanes))
-        return launch_lanes(g.stride_class == 1 ? gradient_lanes<T, true> : gradient_lanes<T, false>, g, a, warps_of_lanes(g), 0, s);
+        return launch_lanes(g.stride_class == 1 ? gradient_lanes<T, true> : gradient_lanes<T, false>, g, a, warps_of_lanes<T, true>(g), 0, s);
     // A chunk should be no more than a row, and a row a few chunks (us, 3000 rows of 1000 with 4 classes a lane / 16 9.3 / 6.8, 60000 of 200 34 / 45;
     // 4096 rows of 2000 by a warp / 8 13.7 / 23.4; 3000 of 6000 by 4 warps / 8 26.9 / 31.0, 2048 of 32000 86.0 / 83.5).
     constexpr int U = kStreamAhead<T>;
