@@ -1263,10 +1263,16 @@ cudaError_t answer_lanes_of(const Logits& g, const Answers<T>& a, cudaStream_t s
     }
 }
 
-// A warp a row where a row is one chunk, or where rows are so many that their number hides how long a warp is at one; else streams (four alternatives,
-// warps / streams, us: 100 rows of 2000 classes 6.7 / 4.5, 500 7.1 / 9.4, 1000 8.5 / 15; 500 of 8000 20 / 15, 1000 21 / 19, 2000 24 / 30; 10000 of
-// 16000 116 / 133; 2048 of 32000 59 / 47).
-bool by_warps(const Logits& g) { return g.classes <= 512 || 4 * g.count() >= g.classes; }
+// A warp a row where a row is a chunk or two, or where rows are so many that their number hides how long a warp is at one; else streams.  (Four alternatives,
+// warps / streams, us: 100 rows of 2000 classes 7.5 / 4.6, 500 8.0 / 9.5, 1000 9.3 / 15.4; 500 of 8000 21.5 / 14.7, 1000 22.8 / 19.1, 2000 26.1 / 30.5; 10000 of
+// 16000 120 / 137; 2048 of 32000 72 / 52, 8000 187 / 169.  float64, whose warps are longer at a row, unless there are 2^24 logits: 200 of 1000 12.6 /
+// 8.4, 400 12.9 / 15.2; 500 of 2000 24.4 / 15.3, 1000 24.5 / 26.1; 1500 of 4000 47 / 45, 2000 48 / 55; 2000 of 8000 82 / 75, 3000 99 / 104; 4000 of 16000 221 /
+// 230; 2048 of 32000 270 / 227.)
+template <typename T>
+bool by_warps(const Logits& g) {
+    const long long rows = g.count();
+    return g.classes <= 512 || 2 * rows >= g.classes || (4 * rows >= g.classes && (sizeof(T) == 4 || rows >= (1 << 24) / g.classes));
+}
 
 // runs of one wave, but a row no more than 32 parts (30 runs a row have 31 borders in it at most)
 template <typename T>
@@ -1313,7 +1319,7 @@ cudaError_t answer_by_lanes(const Logits& g, const Answers<T>& a, cudaStream_t s
 template <typename T>
 cudaError_t answer_as(const Logits& g, const Answers<T>& a, void* ws, cudaStream_t s) {
     if (by_rows(g, kMostByLanes)) {
-        if (!by_warps(g)) return g.top_k > 0 ? answer_stream_of<T, true>(g, a, ws, s) : answer_stream_of<T, false>(g, a, ws, s);
+        if (!by_warps<T>(g)) return g.top_k > 0 ? answer_stream_of<T, true>(g, a, ws, s) : answer_stream_of<T, false>(g, a, ws, s);
         // (60000 rows of 200 classes with three alternatives 38 us with 8 a lane, 49 with 16, 20000 of 500 20 and 18; float64 3000 of 1500 24 with 4, 32 with 8)
         constexpr int kFew = sizeof(T) == 4 ? 8 : 4, kMany = sizeof(T) == 4 ? 16 : 4;
         if (g.classes <= 32 * kFew) return g.top_k > 0 ? answer_rows_of<T, true, kFew>(g, a, s) : answer_rows_of<T, false, kFew>(g, a, s);
@@ -1351,8 +1357,9 @@ cudaError_t launch_log_probabilities(const simnets_likelihood_desc& d, const voi
 
 size_t log_probabilities_workspace_bytes(const simnets_likelihood_desc& d) {
     const Logits g = logits_of(d);
-    if (g.count() == 0 || !by_rows(g, kMostByLanes) || by_warps(g)) return 0;
-    return d.dtype == SIMNETS_F64 ? 2 * sizeof(RowFound<double>) * runs_of<double>(g).ctas : 2 * sizeof(RowFound<float>) * runs_of<float>(g).ctas;
+    if (g.count() == 0 || !by_rows(g, kMostByLanes)) return 0;
+    if (d.dtype == SIMNETS_F64) return by_warps<double>(g) ? 0 : 2 * sizeof(RowFound<double>) * runs_of<double>(g).ctas;
+    return by_warps<float>(g) ? 0 : 2 * sizeof(RowFound<float>) * runs_of<float>(g).ctas;
 }
 
 cudaError_t launch_log_probabilities_gradient(const simnets_likelihood_desc& d, const void* logits, const long long* labels, const void* stats, const int* top_index,

@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 import torch
 
+from simnets_tf_b200.ops.likelihood import log_probabilities
 from test_likelihood_gpu import KINDS, make, verify
 
 pytestmark = pytest.mark.gpu
@@ -51,3 +52,29 @@ def test_one_two_and_four_warps_a_tile(classes, kind):
 def test_rows_of_some_classes_in_great_numbers(rows, classes, top_k, kind):
     x, labels = make((rows, classes), 1, "plain", kind, seed=rows)
     verify(x, labels, 1, top_k, True, torch.from_numpy(x).cuda())
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=["f32", "f64"])
+@pytest.mark.parametrize("top_k", [0, 5])
+def test_rows_by_warps_and_by_streams(top_k, kind):
+    """As many rows as are just enough for a warp each, and one fewer."""
+    for classes in (513, 700, 2000, 4099):
+        for of in (4,) if kind == torch.float32 else (2, 4):
+            for rows in (-(-classes // of), -(-classes // of) - 1):
+                x, labels = make((rows, classes), 1, "plain", kind, seed=rows)
+                verify(x, labels, 1, top_k, True, torch.from_numpy(x).cuda())
+
+
+def test_rows_of_two_to_the_24_logits():
+    """float64 beyond the one border that counts logits: the answers of 2100 rows of 8000 by warps are those of half of them by streams."""
+    x = torch.randn(2100, 8000, device="cuda", dtype=torch.float64, generator=torch.Generator(device="cuda").manual_seed(0))
+    labels = torch.arange(2100, device="cuda")
+    whole = log_probabilities(x, labels, 3, True)
+    for at in (slice(0, 1050), slice(1050, 2100)):
+        half = log_probabilities(x[at], labels[at], 3, True)
+        assert bool((half.top_index == whole.top_index[at]).all())
+        # log S of 8000 numbers, added up in two orders of chains of at most 8000 / 32 and what joins them: 300 units of S each, which are 300 of its logarithm,
+        # and the same of the entropy's second sum, whose terms are below 8
+        eps = torch.finfo(torch.float64).eps
+        assert float((half.label - whole.label[at]).abs().max()) <= 600 * eps and float((half.top - whole.top[at]).abs().max()) <= 600 * eps
+        assert float((half.entropy - whole.entropy[at]).abs().max()) <= 600 * 9 * eps
