@@ -38,7 +38,8 @@ template <> struct Unit<double> {
 };
 
 // Two values that one instruction adds, multiplies, or multiplies and adds (float32; float64 in two).  With / without, us: 2048 rows of 65537 classes with
-// five alternatives 141 / 147, the gradient of 20000 rows of 500 20.2 / 22.6.
+// five alternatives 96 / 100, the gradient of 20000 rows of 500 20.3 / 22.9.  (Times here are of kernels back to back for some milliseconds, at 1.97 GHz; under the
+// power limit, after some hundred milliseconds, the clock is 1.63 GHz and these 96 are 108.)
 template <typename T> struct Pair { T x, y; };
 __device__ __forceinline__ unsigned long long bits(Pair<float> p) { unsigned long long r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(p.x), "f"(p.y)); return r; }
 __device__ __forceinline__ Pair<float> pair(unsigned long long b) { Pair<float> p; asm("mov.b64 {%0, %1}, %2;" : "=f"(p.x), "=f"(p.y) : "l"(b)); return p; }
@@ -746,7 +747,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) answer_rows(Logits g, Answers<
 // Long rows: all rows' chunks in their order, in equal runs for the CTAs of one wave, which have the next ones on their way all the time, those of the
 // next row as well: every thread copies what it reads itself into shared memory (cp.async), kStages - 1 chunks ahead, and waits for nobody else.
 // More on the way at once is slower (2048 rows of 65537 classes with 5 alternatives / of 32000 without, us: 2 CTAs a multiprocessor with 2, 3, 4
-// stages 121 / 55, 104 / 46, 110 / 46, 3 CTAs with 2, 3, 4 stages 105 / 47, 116 / 47, 121 / 51, 4 with 3 132 / 51; the memory's floor 82 / 40).
+// stages 116 / 55, 96 / 46, 101 / 47, 3 CTAs with 2, 3, 4 stages 97 / 47, 105 / 47, 109 / 51, 4 with 3 112 / 52; the memory's floor 82 / 40).
 //
 // The likeliest classes cost the streaming warps a few comparisons a chunk.  Every thread keeps the largest of its classes, the chunk in which it came up
 // first, and the largest of its other chunks.  Of the threads by their largest, equal ones by its first class, the first top_k have all of the row's
