@@ -35,7 +35,7 @@ def plain(t):
     it one; zeros can have no memory)."""
     if t._is_zerotensor():
         return t.clone()
-    if t.numel() and not t.data_ptr():
+    if not t.data_ptr() and t.numel():
         raise RuntimeError("a tensor of %d values has no memory" % t.numel())
     return t.resolve_neg().contiguous()
 

@@ -1249,26 +1249,25 @@ cudaError_t answer_lanes_of(const Logits& g, const Answers<T>& a, cudaStream_t s
     // a run of hardly more chunks than the list has places would be read twice (us, classes / chunks listed: 65536 rows of 10, three alternatives 4.4 / 7.6,
     // float64 maps of 37, four alternatives 7.3 / 9.5, 100000 rows of 100, three alternatives 20.7 / 16.9, a map of 150 36 / 27)
     const bool direct = g.classes <= 16 * TOP * warps;
-    if (warps < kGroupWarps)
-        return launch_lanes(direct || TOP == 0 ? answer_lanes<T, TOP, SIDE, true> : answer_lanes<T, TOP, SIDE, TOP == 0>, g, a, warps, warps > 1 ? 4 * Found<T, TOP>::kBytes : 0, s);
-    if constexpr (SIDE) {
-        return cudaErrorInvalidValue;                       // (not reached: warps_of_lanes)
-    } else {
-        constexpr int kBytes = int(kGroupWarps * kGroupBytes<T, TOP>);
-        if (kBytes > 48 * 1024) {
-            static SmemLimit limit;
-            const cudaError_t e = limit.raise(answer_groups<T, TOP>, kBytes);
-            if (e != cudaSuccess) return e;
+    if constexpr (!SIDE) {
+        if (warps == kGroupWarps) {
+            constexpr int kBytes = int(kGroupWarps * kGroupBytes<T, TOP>);
+            if (kBytes > 48 * 1024) {
+                static SmemLimit limit;
+                const cudaError_t e = limit.raise(answer_groups<T, TOP>, kBytes);
+                if (e != cudaSuccess) return e;
+            }
+            return launch_lanes(answer_groups<T, TOP>, g, a, kGroupWarps, kBytes, s);
         }
-        return launch_lanes(answer_groups<T, TOP>, g, a, kGroupWarps, kBytes, s);
     }
+    return launch_lanes(direct || TOP == 0 ? answer_lanes<T, TOP, SIDE, true> : answer_lanes<T, TOP, SIDE, TOP == 0>, g, a, warps, warps > 1 ? 4 * Found<T, TOP>::kBytes : 0, s);
 }
 
-// A warp a row where a row is a chunk or two, or where rows are so many that their number hides how long a warp is at one; else streams.  (Four alternatives,
-// warps / streams, us: 100 rows of 2000 classes 7.5 / 4.6, 500 8.0 / 9.5, 1000 9.3 / 15.4; 500 of 8000 21.5 / 14.7, 1000 22.8 / 19.1, 2000 26.1 / 30.5; 10000 of
-// 16000 120 / 137; 2048 of 32000 72 / 52, 8000 187 / 169.  float64, whose warps are longer at a row, unless there are 2^24 logits: 200 of 1000 12.6 /
-// 8.4, 400 12.9 / 15.2; 500 of 2000 24.4 / 15.3, 1000 24.5 / 26.1; 1500 of 4000 47 / 45, 2000 48 / 55; 2000 of 8000 82 / 75, 3000 99 / 104; 4000 of 16000 221 /
-// 230; 2048 of 32000 270 / 227.)
+// A warp a row where a row is a chunk or two, or where rows are so many that their number hides how long a warp is at one, a quarter as many as classes;
+// else streams.  float64 warps are longer at a row: half as many, or a quarter where they have 2^24 logits or more.  (Four alternatives, warps / streams,
+// us: 100 rows of 2000 classes 7.5 / 4.6, 500 8.0 / 9.5, 1000 9.3 / 15.4; 500 of 8000 21.5 / 14.7, 1000 22.8 / 19.1, 2000 26.1 / 30.5; 10000 of 16000 120
+// / 137; 2048 of 32000 72 / 52, 8000 187 / 169.  float64: 200 of 1000 12.6 / 8.4, 400 12.9 / 15.2; 500 of 2000 24.4 / 15.3, 1000 24.5 / 26.1; 1500 of 4000
+// 47 / 45, 2000 48 / 55; 2000 of 8000 82 / 75, 3000 99 / 104; 4000 of 16000 221 / 230; 2048 of 32000 270 / 227.)
 template <typename T>
 bool by_warps(const Logits& g) {
     const long long rows = g.count();
